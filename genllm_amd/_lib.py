@@ -107,6 +107,12 @@ SIGNATURES = {
     "genllm_flash_attention": (_int, [_P, _P, _P, _P, _i32, _i32, _i32, _i32, _i32, _i32, _f, _i32, _P]),
     "genllm_linear_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "genllm_linear": (_int, [_P, _P, _P, _P, _i64, _i64, _i64, _P, _sz, _P]),
+    "genllm_gated_delta_workspace_bytes": (_sz, [_i32] * 6),
+    "genllm_gated_delta_rule": (_int, [_P, _i64, _i64, _i64] * 3 + [_P, _i64, _i64] * 2 + [_P, _P, _P, _i32, _P, _P]
+                                + [_P, _i64, _i64, _i64] + [_i32] * 7 + [_f, _f, _P, _sz, _P]),
+    "genllm_causal_conv": (_int, [_P, _i64, _i64, _P, _P, _P, _i64, _i64, _P, _i32, _P, _P] + [_i32] * 6 + [_P]),
+    "genllm_qk_norm_rope_axes": (_int, [_P, _i64, _i64, _P, _i64, _i64, _P, _i32] * 2
+                                 + [_f, _P, _P, _i32, _i32, _P, _i64, _i32, _P, _i32, _i32, _i32, _i32, _P]),
     "genllm_fill_normal_bf16": (_int, [_P, _sz, _u64, _u64, _P]),
     "genllm_fill_normal_f16": (_int, [_P, _sz, _u64, _u64, _P]),
     "genllm_selftest_mfma": (_int, [_i32, _P, _P, _P, _P]),

@@ -415,6 +415,160 @@ def linear(x, w, out, bias=None, workspace=None, stream=None):
          _stream(stream))
 
 
+# ----------------------------------------------------------- hybrid layers
+_ELEMENT_CODES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
+
+
+def _need(op, name, t, shape, dtype, device):
+    """t is a tensor of that shape, type and device whose last dim is dense."""
+    if t.shape != shape or t.dtype != dtype or t.device != device or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        raise ValueError(f"{op}: {name} must be {dtype} {tuple(shape)} on {device}, the last dim dense; got "
+                         f"{t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
+
+
+def _call_on(device, name, *args, stream=None):
+    """call() with `device` current, on `stream` or that device's current stream."""
+    if _current_device is None or device.index != _current_device():
+        with torch.cuda.device(device):
+            return call(name, *args, _stream(stream))
+    return call(name, *args, _stream(stream))
+
+
+def _element_code(op, t):
+    code = _ELEMENT_CODES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{op}: bf16 or float16 elements, got {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError("expected a GPU tensor")
+    return code
+
+
+def gated_delta_workspace_bytes(batch: int, seq_len: int, n_k_heads: int, n_v_heads: int, k_dim: int, v_dim: int) -> int:
+    return lib().genllm_gated_delta_workspace_bytes(batch, seq_len, n_k_heads, n_v_heads, k_dim, v_dim)
+
+
+def gated_delta_rule(q, k, v, a, b, state, out, scale: float, a_log=None, dt_bias=None, l2_eps=None, seq_lens=None,
+                     state_ids=None, workspace=None, stream=None):
+    """genllm_gated_delta_rule: out = the gated delta rule over a padded batch, the state replaced.
+
+    q, k [B, S, Hk, Dk], v, out [B, S, Hv, Dv], bf16 or float16, any strides
+    that keep rows dense and 16-byte aligned; state [n, Hv, Dk, Dv] float32,
+    contiguous.  a_log, dt_bias [Hv] float32 with a, b [B, S, Hv] elements: decay
+    exp(-exp(a_log) softplus(a + dt_bias)), beta sigmoid(b); without them a is
+    the log decay and b beta, float32.  l2_eps: normalise q and k rows with it
+    (None: take them as they are).  seq_lens, state_ids [B] int32 on the
+    GPU.  workspace: a device buffer of at least gated_delta_workspace_bytes(...)
+    bytes when that is non-zero; None allocates one for this call."""
+    op = "gated_delta_rule"
+    code = _element_code(op, q)
+    B, S, Hk, Dk = q.shape
+    Hv, Dv = v.shape[2:]
+    dt, dev = q.dtype, q.device
+    gate = torch.float32 if a_log is None else dt
+    _need(op, "k", k, (B, S, Hk, Dk), dt, dev)
+    _need(op, "v", v, (B, S, Hv, Dv), dt, dev)
+    _need(op, "out", out, (B, S, Hv, Dv), dt, dev)
+    _need(op, "a", a, (B, S, Hv), gate, dev)
+    _need(op, "b", b, (B, S, Hv), gate, dev)
+    if q.stride(3) != 1:
+        raise ValueError(f"{op}: the last dim of q must be dense")
+    if state.shape[1:] != (Hv, Dk, Dv) or state.dtype != torch.float32 or state.device != dev or not state.is_contiguous():
+        raise ValueError(f"{op}: state must be contiguous float32 [n, {Hv}, {Dk}, {Dv}] on {dev}")
+    if (a_log is None) != (dt_bias is None):
+        raise ValueError(f"{op}: a_log and dt_bias go together")
+    if a_log is not None:
+        _need(op, "a_log", a_log, (Hv,), torch.float32, dev)
+        _need(op, "dt_bias", dt_bias, (Hv,), torch.float32, dev)
+    if seq_lens is not None:
+        _need(op, "seq_lens", seq_lens, (B,), torch.int32, dev)
+    if state_ids is not None:
+        _need(op, "state_ids", state_ids, (B,), torch.int32, dev)
+    need = lib().genllm_gated_delta_workspace_bytes(B, S, Hk, Hv, Dk, Dv)
+    if need and workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        if stream is not None:  # freed into the current stream's pool while `stream` still uses it
+            handle = stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream), device=dev)
+            workspace.record_stream(handle)
+    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    qs, ks, vs, os_, as_, bs = q.stride(), k.stride(), v.stride(), out.stride(), a.stride(), b.stride()
+    _call_on(dev, "genllm_gated_delta_rule", q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2],
+             v.data_ptr(), vs[0], vs[1], vs[2], a.data_ptr(), as_[0], as_[1], b.data_ptr(), bs[0], bs[1], _ptr(a_log),
+             _ptr(dt_bias), state.data_ptr(), state.shape[0], _ptr(state_ids), _ptr(seq_lens), out.data_ptr(), os_[0],
+             os_[1], os_[2], B, S, Hk, Hv, Dk, Dv, code, scale, -1.0 if l2_eps is None else l2_eps, _ptr(workspace),
+             ws_bytes, stream=stream)
+
+
+def causal_conv(x, weight, out, state=None, bias=None, silu: bool = True, seq_lens=None, state_ids=None, stream=None):
+    """genllm_causal_conv: causal depthwise convolution with the last inputs as state.
+
+    x, out [B, S, C] (any batch and token strides; out apart from x), weight
+    [C, W] with W 2 to 4, bias [C] or None, state [n, W - 1, C] or None (zeros
+    before each sequence, none kept), all bf16 or all float16.  seq_lens,
+    state_ids [B] int32 on the GPU."""
+    op = "causal_conv"
+    code = _element_code(op, x)
+    B, S, Ch = x.shape
+    W = weight.shape[1]
+    dt, dev = x.dtype, x.device
+    _need(op, "out", out, (B, S, Ch), dt, dev)
+    if weight.shape != (Ch, W) or weight.dtype != dt or weight.device != dev or not weight.is_contiguous():
+        raise ValueError(f"{op}: weight must be contiguous {dt} [{Ch}, W] on {dev}")
+    if x.stride(2) != 1 and Ch > 1:
+        raise ValueError(f"{op}: the channels of x must be dense")
+    if bias is not None:
+        _need(op, "bias", bias, (Ch,), dt, dev)
+    n = 0
+    if state is not None:
+        n = state.shape[0]
+        if state.shape != (n, W - 1, Ch) or state.dtype != dt or state.device != dev or not state.is_contiguous():
+            raise ValueError(f"{op}: state must be contiguous {dt} [n, {W - 1}, {Ch}] on {dev}")
+    if seq_lens is not None:
+        _need(op, "seq_lens", seq_lens, (B,), torch.int32, dev)
+    if state_ids is not None:
+        _need(op, "state_ids", state_ids, (B,), torch.int32, dev)
+    xs, os_ = x.stride(), out.stride()
+    _call_on(dev, "genllm_causal_conv", x.data_ptr(), xs[0], xs[1], weight.data_ptr(), _ptr(bias), out.data_ptr(), os_[0],
+             os_[1], _ptr(state), n, _ptr(state_ids), _ptr(seq_lens), B, S, Ch, W, code, int(silu), stream=stream)
+
+
+def qk_norm_rope_axes(q, k, q_out, k_out, gamma_q, gamma_k, eps: float, cos, sin, positions, sections,
+                      interleaved: bool = False, stream=None):
+    """genllm_qk_norm_rope_axes: per-head RMSNorm and the rotation by positions on several axes, in one pass.
+
+    q, q_out [S, Hq, D] and k, k_out [S, Hk, D] with any token and head strides
+    (a head-major tensor comes in transposed); k and k_out may be None.
+    gamma_q, gamma_k [D] float32 or None (no norm).  cos, sin [max_seq, rope_dim]
+    float32, contiguous, as rope_cache makes them; positions [n_axes, S] int32 on
+    the GPU; sections: the pairs of each axis, on the host."""
+    op = "qk_norm_rope_axes"
+    code = _element_code(op, q)
+    S, Hq, D = q.shape
+    dt, dev = q.dtype, q.device
+    n_axes = len(sections)
+    if q.stride(2) != 1:
+        raise ValueError(f"{op}: the last dim of q must be dense")
+    _need(op, "q_out", q_out, (S, Hq, D), dt, dev)
+    Hk, kp, ks, kop, kos = 0, None, (0, 0), None, (0, 0)
+    if k is not None:
+        Hk = k.shape[1]
+        _need(op, "k", k, (S, Hk, D), dt, dev)
+        _need(op, "k_out", k_out, (S, Hk, D), dt, dev)
+        kp, ks, kop, kos = k.data_ptr(), k.stride(), k_out.data_ptr(), k_out.stride()
+    for gamma in (gamma_q, gamma_k):
+        if gamma is not None:
+            _need(op, "gamma", gamma, (D,), torch.float32, dev)
+    max_seq, rope_dim = cos.shape
+    for t in (cos, sin):
+        if t.shape != (max_seq, rope_dim) or t.dtype != torch.float32 or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{op}: cos and sin must be contiguous float32 [max_seq, rope_dim] on {dev}")
+    _need(op, "positions", positions, (n_axes, S), torch.int32, dev)
+    qs, qos = q.stride(), q_out.stride()
+    _call_on(dev, "genllm_qk_norm_rope_axes", q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), qos[0], qos[1], _ptr(gamma_q),
+             Hq, kp, ks[0], ks[1], kop, kos[0], kos[1], _ptr(gamma_k), Hk, eps, cos.data_ptr(), sin.data_ptr(), max_seq,
+             rope_dim, positions.data_ptr(), positions.stride(0), n_axes, (C.c_int32 * n_axes)(*sections),
+             int(interleaved), S, D, code, stream=stream)
+
+
 def fill_normal_bf16(t: torch.Tensor, seed: int, offset: int = 0, stream=None):
     call("genllm_fill_normal_bf16", _ptr(t), t.numel(), seed, offset, _stream(stream))
 
@@ -445,8 +599,8 @@ def to_host_bits(t: torch.Tensor) -> np.ndarray:
 
 __all__ = [
     "PagedAttentionManager", "paged_attention", "qk_norm_rope_append", "rms_norm", "apply_rope", "rope_cache",
-    "kv_scatter", "paged_decode", "paged_decode_noalloc", "paged_prefill", "flash_attention", "decode_workspace_bytes", "fill_normal_bf16",
-    "fill_normal_f16",
+    "kv_scatter", "paged_decode", "paged_decode_noalloc", "paged_prefill", "flash_attention", "decode_workspace_bytes", "gated_delta_rule",
+    "gated_delta_workspace_bytes", "causal_conv", "qk_norm_rope_axes", "fill_normal_bf16", "fill_normal_f16",
     "selftest_mfma", "device_view", "to_device_bf16", "to_device_f16", "to_host_bits", "GenllmError", "PAGE",
     "DTYPE_BF16", "DTYPE_F16",
 ]

@@ -340,6 +340,82 @@ size_t genllm_linear_workspace_bytes(int64_t rows, int64_t common, int64_t cols)
 int genllm_linear(const void *x, const void *w, const void *bias, void *out, int64_t rows, int64_t common,
                   int64_t cols, void *workspace, size_t workspace_bytes, void *stream);
 
+/* -------------------------------------------------------- hybrid layers
+ * What a hybrid model (Qwen3.5) needs beside the paged attention: layers whose
+ * memory is one matrix per head instead of a KV cache, the short convolution
+ * in front of them (op types CAUSAL_CONV1D and SSM_SCAN of the reference's
+ * graph, include/utils/utils.hpp), and q/k rotations by positions on several
+ * axes for prompts with images.  Elements are bf16 or fp16 (dtype), strides in
+ * elements, the innermost dim dense.  No call allocates, copies or
+ * synchronises; all of them are kernel launches that a graph may capture.
+ *
+ * Calls with a state per sequence take a padded batch: entry b has seq_lens[b]
+ * tokens (device; null: all have seq_len; values are clamped to 0..seq_len) and
+ * the state state_ids[b] (device; null: state b).  Rows of out behind an
+ * entry's last token are left as they were.  An entry with a negative id or no
+ * tokens reads and writes nothing.  An id past the states, or one that an
+ * earlier entry of the batch has, gives NaN in the entry's rows of out and
+ * leaves the states alone.
+ *
+ * genllm_gated_delta_rule: per entry and value head h (key head h / (n_v_heads /
+ * n_k_heads)) the state S [k_dim][v_dim], fp32, takes token after token:
+ *     S <- exp(g) S;  u = beta (v - S^T k);  S <- S + k u^T;  out = scale S^T q
+ * with q, k the given rows or, where l2_eps >= 0, x / sqrt(sum x^2 + l2_eps)
+ * (l2_eps < 0: as given; |k| should then be about 1 or less, as the rule itself
+ * asks for).  a_log, dt_bias [n_v_heads] fp32: g = -exp(a_log) softplus(a +
+ * dt_bias) and beta = sigmoid(b), a and b elements; both null: a is g and b is
+ * beta, fp32.  g must be <= 0 (-inf clears the state).  q, k [batch][seq_len]
+ * [n_k_heads][k_dim]; v, out [batch][seq_len][n_v_heads][v_dim]; a, b [batch]
+ * [seq_len][n_v_heads]; state [n_states][n_v_heads][k_dim][v_dim], read and
+ * replaced.  k_dim and v_dim 64 or 128, rows 16-byte aligned.  A token or a few
+ * run token by token; longer calls run in chunks and need a workspace of
+ * genllm_gated_delta_workspace_bytes (0 where none is needed), whose contents
+ * do not matter before or after the call; calls that share one must be
+ * ordered. */
+size_t genllm_gated_delta_workspace_bytes(int32_t batch, int32_t seq_len, int32_t n_k_heads, int32_t n_v_heads,
+                                          int32_t k_dim, int32_t v_dim);
+int genllm_gated_delta_rule(const void *q, int64_t q_batch_stride, int64_t q_tok_stride, int64_t q_head_stride,
+                            const void *k, int64_t k_batch_stride, int64_t k_tok_stride, int64_t k_head_stride,
+                            const void *v, int64_t v_batch_stride, int64_t v_tok_stride, int64_t v_head_stride,
+                            const void *a, int64_t a_batch_stride, int64_t a_tok_stride, const void *b,
+                            int64_t b_batch_stride, int64_t b_tok_stride, const float *a_log, const float *dt_bias,
+                            float *state, int32_t n_states, const int32_t *state_ids, const int32_t *seq_lens,
+                            void *out, int64_t o_batch_stride, int64_t o_tok_stride, int64_t o_head_stride,
+                            int32_t batch, int32_t seq_len, int32_t n_k_heads, int32_t n_v_heads, int32_t k_dim,
+                            int32_t v_dim, int32_t dtype, float scale, float l2_eps, void *workspace,
+                            size_t workspace_bytes, void *stream);
+
+/* Causal depthwise convolution of width 2, 3 or 4 over the tokens, per channel:
+ *     y[t] = bias + sum_j weight[j] x[t - (width-1) + j],  out = y or silu(y)
+ * (silu != 0), fp32, rounded once.  x, out [batch][seq_len][channels]; out
+ * must not overlap x; weight [channels][width]; bias [channels] or null; state
+ * [n_states][width-1][channels]: the sequence's inputs before x[0], replaced by
+ * its last width-1 inputs; null: zeros, and none are kept. */
+int genllm_causal_conv(const void *x, int64_t x_batch_stride, int64_t x_tok_stride, const void *weight,
+                       const void *bias, void *out, int64_t o_batch_stride, int64_t o_tok_stride, void *state,
+                       int32_t n_states, const int32_t *state_ids, const int32_t *seq_lens, int32_t batch,
+                       int32_t seq_len, int32_t channels, int32_t width, int32_t dtype, int32_t silu, void *stream);
+
+/* Per-head RMSNorm of q and k (gamma null: none; x / sqrt(mean x^2 + eps) *
+ * gamma), then the rotation by positions on n_axes axes (1 to 4), in one pass,
+ * fp32, rounded once.  q, k and their outputs are rows of head_dim (64, 128 or
+ * 256) at tok and head strides of their own, 16-byte aligned (an output may be
+ * its input, with the same strides); a head count of 0 leaves that part out.
+ * The first rope_dim dims (a multiple of 16) rotate in pairs (i, i + rope_dim/2)
+ * by row positions[axis * pos_stride + token] (device) of the tables
+ * [max_seq][rope_dim] that genllm_rope_cache makes, the others pass through.
+ * sections (host): the pairs of each axis, summing to rope_dim/2, one axis
+ * after another or, interleaved, pair i to axis i % n_axes while i / n_axes <
+ * sections[that axis], else to axis 0.  A position outside the tables gives NaN
+ * in the pairs of its axis. */
+int genllm_qk_norm_rope_axes(const void *q, int64_t q_tok_stride, int64_t q_head_stride, void *q_out,
+                             int64_t qo_tok_stride, int64_t qo_head_stride, const float *gamma_q, int32_t n_q_heads,
+                             const void *k, int64_t k_tok_stride, int64_t k_head_stride, void *k_out,
+                             int64_t ko_tok_stride, int64_t ko_head_stride, const float *gamma_k, int32_t n_k_heads,
+                             float eps, const float *cos_tab, const float *sin_tab, int32_t max_seq, int32_t rope_dim,
+                             const int32_t *positions, int64_t pos_stride, int32_t n_axes, const int32_t *sections,
+                             int32_t interleaved, int32_t seq_len, int32_t head_dim, int32_t dtype, void *stream);
+
 /* ------------------------------------------------------------ utilities
  * No counterpart in the reference: synthetic seeded inputs for tests and the
  * benchmark (counter-based hash -> Box-Muller -> RNE bf16, or RNE fp16 with
