@@ -13,6 +13,23 @@
 // elements of a row, so that products with them have one exact operand.
 //
 // delta_recurrent_kernel runs the rule as written, the state in registers.
+//
+// Longer calls run in chunks of C = 64 tokens.  With G the running sum of g in a
+// chunk, S0 the state before it and U the chunk's rows u:
+//
+//   (1 + L) U = diag(beta) (V - diag(e^G) K S0)      L_ij = beta_i e^(G_i - G_j) k_i.k_j, j < i
+//   O  = scale (diag(e^G) Q S0 + P U)                P_ij = e^(G_i - G_j) q_i.k_j, j <= i
+//   S1 = e^(G_last) S0 + K^T diag(e^(G_last - G)) U
+//
+// delta_chunk_prepare_kernel forms T = (1 + L)^-1 diag(beta), P and the factors
+// of every chunk and head at once; delta_chunk_scan_kernel takes 16 columns of
+// a head's state from chunk to chunk through the matrix cores.  The state and
+// everything that enters it keep 24 bits there: an fp32 value is the exact sum
+// of three bf16 parts (24 = 3 x 8 bits), k is one part (fp16: two, 11 bits), and
+// the products of parts below 2^-24 are left out.  What enters out only (Q, P,
+// and S and U beside them) takes two parts, 2^-17 of a term, against out's own
+// rounding of 2^-8 (fp16: 2^-11).  One part would be 2^-9 of every term.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -89,39 +106,21 @@ __device__ __forceinline__ float l2_factor(float sum, float eps) {
     return eps < 0.0f ? 1.0f : 1.0f / __builtin_sqrtf(sum + eps);
 }
 
-// One wave per 4 CQ columns of a head's state, whole tokens in its registers:
-// lane (rg, cq) = (lane / CQ, lane % CQ) holds rows rg NR .. + NR - 1 of columns
-// 4 cq .. + 3.  S^T k and S^T q of the state before the token are summed in one
-// pass over the registers and one reduction over the row groups; then
+// Tokens t0 .. t1 - 1 through 4 CQ columns of a head's state in one wave's
+// registers: lane (rg, cq) = (lane / CQ, lane % CQ) holds rows rg NR .. + NR - 1
+// of columns col .. + 3.  S^T k and S^T q of the state before the token are summed
+// in one pass over the registers and one reduction over the row groups; then
 //   u = beta (v - alpha S^T k),  o = scale (alpha S^T q + (k.q) u),
 // and the state is updated.
 template <int DK, int CQ, bool F16>
-__global__ __launch_bounds__(256) void delta_recurrent_kernel(DeltaParams p, int64_t units) {
-    constexpr int RG = 64 / CQ, NR = DK / RG;
-    const int64_t unit = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (unit >= units) return;
-    const int lane = threadIdx.x & 63, cq = lane % CQ, rg = lane / CQ;
-    const int slices = p.Dv / (4 * CQ);
-    const int64_t bh = unit / slices;
-    const int col = int(unit - bh * slices) * 4 * CQ + 4 * cq;
-    const int b = int(bh / p.Hv), h = int(bh - int64_t(b) * p.Hv);
-    const int slot = entry_state(p.seq, b), len = entry_len(p.seq, b);
-    if (slot == kEntryEmpty || len == 0) return;
-    uint16_t* const out = p.out + b * p.o_batch + h * p.o_head + col;
-    if (slot == kEntryBad) {
-        const uint32_t nan2 = Elem<F16>::pack_p(__builtin_nanf(""), __builtin_nanf(""));
-        for (int t = rg; t < len; t += RG) *reinterpret_cast<uint2*>(out + t * p.o_tok) = make_uint2(nan2, nan2);
-        return;
-    }
-    float* const st = p.state + ((int64_t(slot) * p.Hv + h) * DK + rg * NR) * p.Dv + col;
-    f32x4_t s[NR];
-#pragma unroll
-    for (int i = 0; i < NR; ++i) s[i] = *reinterpret_cast<const f32x4_t*>(st + int64_t(i) * p.Dv);
-    const int hk = h / p.G;
+__device__ __forceinline__ void recur(const DeltaParams& p, f32x4_t (&s)[DK * CQ / 64], int b, int h, int col, int t0, int t1) {
+    constexpr int NR = DK * CQ / 64;
+    const int rg = int(threadIdx.x & 63) / CQ, hk = h / p.G;
     const uint16_t* const q = p.q.p + b * p.q.batch + hk * p.q.head + rg * NR;
     const uint16_t* const k = p.k.p + b * p.k.batch + hk * p.k.head + rg * NR;
     const uint16_t* const v = p.v.p + b * p.v.batch + h * p.v.head + col;
-    for (int t = 0; t < len; ++t) {
+    uint16_t* const out = p.out + b * p.o_batch + h * p.o_head + col;
+    for (int t = t0; t < t1; ++t) {
         float kf[NR], qf[NR], vf[4], g, beta;
         load_elems<F16>(k + t * p.k.tok, kf);
         load_elems<F16>(q + t * p.q.tok, qf);
@@ -159,8 +158,595 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(DeltaParams p, int
             *reinterpret_cast<uint2*>(out + t * p.o_tok) =
                 make_uint2(Elem<F16>::pack_p(o[0], o[1]), Elem<F16>::pack_p(o[2], o[3]));
     }
+}
+
+// NaN in four columns of an entry's rows, one row per lane group of CQ lanes
+template <int CQ, bool F16>
+__device__ __forceinline__ void nan_rows(const DeltaParams& p, int b, int h, int col, int t0, int t1) {
+    const uint32_t nan2 = Elem<F16>::pack_p(__builtin_nanf(""), __builtin_nanf(""));
+    uint16_t* const out = p.out + b * p.o_batch + h * p.o_head + col;
+    for (int t = t0 + int(threadIdx.x & 63) / CQ; t < t1; t += 64 / CQ)
+        *reinterpret_cast<uint2*>(out + t * p.o_tok) = make_uint2(nan2, nan2);
+}
+
+// One wave per 4 CQ columns of a head's state, token after token.
+template <int DK, int CQ, bool F16>
+__global__ __launch_bounds__(256) void delta_recurrent_kernel(DeltaParams p, int64_t units) {
+    constexpr int NR = DK * CQ / 64;
+    const int64_t unit = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (unit >= units) return;
+    const int lane = threadIdx.x & 63, rg = lane / CQ;
+    const int slices = p.Dv / (4 * CQ);
+    const int64_t bh = unit / slices;
+    const int col = int(unit - bh * slices) * 4 * CQ + 4 * (lane % CQ);
+    const int b = int(bh / p.Hv), h = int(bh - int64_t(b) * p.Hv);
+    const int slot = entry_state(p.seq, b), len = entry_len(p.seq, b);
+    if (slot == kEntryEmpty || len == 0) return;
+    if (slot == kEntryBad) {
+        nan_rows<CQ, F16>(p, b, h, col, 0, len);
+        return;
+    }
+    float* const st = p.state + ((int64_t(slot) * p.Hv + h) * DK + rg * NR) * p.Dv + col;
+    f32x4_t s[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) s[i] = *reinterpret_cast<const f32x4_t*>(st + int64_t(i) * p.Dv);
+    recur<DK, CQ, F16>(p, s, b, h, col, 0, len);
 #pragma unroll
     for (int i = 0; i < NR; ++i) *reinterpret_cast<f32x4_t*>(st + int64_t(i) * p.Dv) = s[i];
+}
+
+// ------------------------------------------------------------------ chunks
+constexpr int kChunk = 64;
+constexpr int kScanCols = 16;  // columns of the state per workgroup of the scan
+
+// What the scan needs of one chunk and value head, in the order its lanes read
+// it: operand fragments of 64 lanes x 16 bytes.  Of the 64 x 64 triangles only
+// the six fragments (row tile, 32 columns) on and below the diagonal are kept:
+// row tiles 0 and 1 have one, 2 and 3 two.
+constexpr int kFrag = 64 * 8;                    // elements of a fragment
+constexpr int kTriFrags = 6;
+constexpr int kTPart = kTriFrags * kFrag;        // elements of one part of T or P
+constexpr int kUnitT = 0, kUnitP = 3 * kTPart;   // T in three parts, P in two
+constexpr int kUnitVec = 5 * kTPart;             // floats: see kVec*
+constexpr int kVecC = 0, kVecD = 64, kVecE = 128, kVecLast = 192, kVecBad = 193, kVecFloats = 256;
+constexpr int kUnitElems = kUnitVec + 2 * kVecFloats;
+__device__ __forceinline__ constexpr int tri_frag(int tile, int ks) { return tile < 2 ? tile : 2 * tile - 2 + ks; }
+
+struct ChunkPlan {
+    uint16_t* units = nullptr;  // [batch][chunk][Hv][kUnitElems]
+    uint16_t* kt = nullptr;     // [batch][chunk][Hk][Dk / 16][2] fragments of K^T
+    int32_t first = 0, count = 0;  // chunks of this launch
+};
+
+// the top 16 bits of an fp32 value are a bf16 value; two of them in one word
+__device__ __forceinline__ uint32_t top2(float lo, float hi) {
+    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+__device__ __forceinline__ float top(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); }
+
+// (lo, hi) in three bf16 parts each, exactly: 8 + 8 + 8 bits
+__device__ __forceinline__ void split3(float lo, float hi, uint32_t& a, uint32_t& b, uint32_t& c) {
+    a = top2(lo, hi);
+    lo -= top(lo), hi -= top(hi);
+    b = top2(lo, hi);
+    lo -= top(lo), hi -= top(hi);
+    c = top2(lo, hi);
+}
+// in two parts, the second rounded: 2^-17
+__device__ __forceinline__ void split2(float lo, float hi, uint32_t& a, uint32_t& b) {
+    a = top2(lo, hi);
+    b = Elem<false>::pack_p(lo - top(lo), hi - top(hi));
+}
+// eight fp16 elements in two bf16 parts each, exactly (11 bits)
+__device__ __forceinline__ void split_f16(const uint4& x, uint4& a, uint4& b) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    uint32_t p[4], r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split2(Elem<true>::lo(w[i]), Elem<true>::hi(w[i]), p[i], r[i]);
+    a = make_uint4(p[0], p[1], p[2], p[3]);
+    b = make_uint4(r[0], r[1], r[2], r[3]);
+}
+__device__ __forceinline__ f32x4_t mma(const uint4& a, const uint4& b, const f32x4_t& c) { return Elem<false>::mma32(a, b, c); }
+
+// acc += A B for 16 x 16 fp32 matrices, A given as row (lane % 16), columns 4 (lane
+// / 16) .. + 3, B and acc as the products leave them (rows 4 (lane / 16) + i, column
+// lane % 16): step i contracts the columns 4 j + i of A with those rows of B
+__device__ __forceinline__ f32x4_t mm16(const f32x4_t& a, const f32x4_t& b, f32x4_t acc) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], acc, 0, 0, 0);
+    return acc;
+}
+
+// LDS written before it is seen after it; loads from memory stay in flight (a
+// __syncthreads would wait for them too)
+__device__ __forceinline__ void lds_barrier() {
+    __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __asm__ volatile("" ::: "memory");
+}
+
+// Four waves per chunk and value head; wave w has row tile w of the 64 x 64
+// matrices.  (1 + L)^-1 by halves: the four diagonal 16 x 16 blocks by
+// substitution, a lane per column; then T10 = -T11 (L10 T00) for 16- and for
+// 32-wide blocks, as fp32 matrix products.
+template <int DK, bool F16>
+__global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p, ChunkPlan c) {
+    constexpr int KS = DK / 32, LD = 68, LK = DK + 8;
+    __shared__ __attribute__((aligned(16))) float s_l[64 * LD];   // L, then the products M in its upper blocks
+    __shared__ __attribute__((aligned(16))) float s_t[64 * LD];   // P, then the inverse
+    __shared__ __attribute__((aligned(16))) uint16_t s_k[64 * LK];
+    __shared__ double s_g[64];
+    __shared__ float s_beta[64], s_rk[64], s_rq[64];
+    const int h = int(blockIdx.x % uint32_t(p.Hv)), rest = int(blockIdx.x / uint32_t(p.Hv));
+    const int n = rest % c.count, b = rest / c.count;
+    const int t0 = (c.first + n) * kChunk;
+    const int slot = entry_state(p.seq, b), len = entry_len(p.seq, b);
+    if (slot < 0 || t0 >= len) return;
+    const int left = len - t0;  // tokens of this chunk and behind it
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g4 = lane >> 4;
+    const int hk = h / p.G;
+    const bool writes_kt = h % p.G == 0;
+    uint16_t* const unit = c.units + ((int64_t(b) * c.count + n) * p.Hv + h) * kUnitElems;
+    float* const vec = reinterpret_cast<float*>(unit + kUnitVec);
+
+    // rows of K (tiles 0 .. w) and Q (tile w); rows behind the end are zeros
+    uint4 kf[4][KS], qf[KS];
+    const uint16_t* const kp = p.k.p + b * p.k.batch + hk * p.k.head + 8 * g4;
+    const uint16_t* const qp = p.q.p + b * p.q.batch + hk * p.q.head + 8 * g4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            kf[j][ks] = make_uint4(0, 0, 0, 0);
+            if (j <= w && 16 * j + r < left) kf[j][ks] = *reinterpret_cast<const uint4*>(kp + (t0 + 16 * j + r) * p.k.tok + 32 * ks);
+        }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        qf[ks] = make_uint4(0, 0, 0, 0);
+        if (16 * w + r < left) qf[ks] = *reinterpret_cast<const uint4*>(qp + (t0 + 16 * w + r) * p.q.tok + 32 * ks);
+    }
+    // gates of token `lane`, the running sum in 64 bits (differences of far sums
+    // enter the exponents); exp(-2000) is 0 in either precision
+    float g = 0.0f, beta = 0.0f;
+    if (lane < left) gates<F16>(p, b, t0 + lane, h, g, beta);
+    g = g < -2000.0f ? -2000.0f : g;
+    double sum = g;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const double up = __shfl_up(sum, m);
+        if (lane >= m) sum += up;
+    }
+    float kk = 0.0f, qq = 0.0f;
+    uint4 own[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        own[ks] = w == 0 ? kf[0][ks] : w == 1 ? kf[1][ks] : w == 2 ? kf[2][ks] : kf[3][ks];
+        const uint32_t a[4] = {own[ks].x, own[ks].y, own[ks].z, own[ks].w};
+        const uint32_t d[4] = {qf[ks].x, qf[ks].y, qf[ks].z, qf[ks].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            kk = __builtin_fmaf(Elem<F16>::lo(a[i]), Elem<F16>::lo(a[i]), kk);
+            kk = __builtin_fmaf(Elem<F16>::hi(a[i]), Elem<F16>::hi(a[i]), kk);
+            qq = __builtin_fmaf(Elem<F16>::lo(d[i]), Elem<F16>::lo(d[i]), qq);
+            qq = __builtin_fmaf(Elem<F16>::hi(d[i]), Elem<F16>::hi(d[i]), qq);
+        }
+        *reinterpret_cast<uint4*>(s_k + (16 * w + r) * LK + 32 * ks + 8 * g4) = own[ks];
+    }
+    kk += __shfl_xor(kk, 16);
+    qq += __shfl_xor(qq, 16);
+    kk += __shfl_xor(kk, 32);
+    qq += __shfl_xor(qq, 32);
+    const bool there = 16 * w + r < left;
+    const float rk = there ? l2_factor(kk, p.l2_eps) : 0.0f;
+    const float rq = there ? p.scale * l2_factor(qq, p.l2_eps) : 0.0f;
+    if (g4 == 0) s_rk[16 * w + r] = rk, s_rq[16 * w + r] = rq;
+    if (w == 0) s_g[lane] = sum, s_beta[lane] = beta;
+    // what is not finite (or an infinite factor) would reach earlier tokens
+    // through the zeros of T: the scan runs such a chunk token by token
+    const bool odd = !(fabsf(rk) < INFINITY) || !(fabsf(kk) < INFINITY) || !(fabsf(g) < INFINITY) || !(fabsf(beta) < INFINITY);
+    const int bad = __syncthreads_or(odd);
+
+    // L below and P on and below the diagonal, tile (w, j)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (j > w) continue;
+        f32x4_t ak = {0.0f, 0.0f, 0.0f, 0.0f}, aq = ak;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            ak = Elem<F16>::mma32(own[ks], kf[j][ks], ak);
+            aq = Elem<F16>::mma32(qf[ks], kf[j][ks], aq);
+        }
+        const int col = 16 * j + r;
+        const double gc = s_g[col];
+        const float rc = s_rk[col];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = 16 * w + 4 * g4 + i;
+            const float e = row >= col ? expf(float(s_g[row] - gc)) * rc : 0.0f;
+            s_l[row * LD + col] = row > col ? s_beta[row] * s_rk[row] * e * ak[i] : 0.0f;
+            s_t[row * LD + col] = row >= col ? s_rq[row] * e * aq[i] : 0.0f;
+        }
+    }
+    __syncthreads();
+
+    // P's fragments of row tile w, the vectors, K^T
+    for (int ks = 0; ks <= w >> 1; ++ks) {
+        const float* const src = s_t + (16 * w + r) * LD + 32 * ks + 8 * g4;
+        uint32_t a[4], d[4];
+        const bool zero = 32 * ks + 8 * g4 >= 16 * (w + 1);  // a block right of the diagonal's
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split2(zero ? 0.0f : src[2 * i], zero ? 0.0f : src[2 * i + 1], a[i], d[i]);
+        uint16_t* const to = unit + kUnitP + tri_frag(w, ks) * kFrag + 8 * lane;
+        *reinterpret_cast<uint4*>(to) = make_uint4(a[0], a[1], a[2], a[3]);
+        *reinterpret_cast<uint4*>(to + kTPart) = make_uint4(d[0], d[1], d[2], d[3]);
+    }
+    if (w == 3) {
+        const double last = s_g[63];
+        vec[kVecC + lane] = s_rk[lane] * expf(float(s_g[lane]));
+        vec[kVecD + lane] = s_rk[lane] * expf(float(last - s_g[lane]));
+        vec[kVecE + lane] = s_rq[lane] * expf(float(s_g[lane]));
+        if (lane == 0) vec[kVecLast] = expf(float(last)), vec[kVecBad] = bad ? 1.0f : 0.0f;
+    }
+    if (writes_kt) {
+        uint16_t* const kt = c.kt + ((int64_t(b) * c.count + n) * p.Hk + hk) * (DK * kChunk);
+#pragma unroll
+        for (int m = w; m < DK / 16; m += 4)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                const uint16_t* const src = s_k + (32 * ks + 8 * g4) * LK + 16 * m + r;
+                uint32_t a[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a[i] = pack2(src[2 * i * LK], src[(2 * i + 1) * LK]);
+                *reinterpret_cast<uint4*>(kt + (2 * m + ks) * kFrag + 8 * lane) = make_uint4(a[0], a[1], a[2], a[3]);
+            }
+    }
+    // the inverse of diagonal block w: column r in every lane group, by substitution
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float* const row = s_l + (16 * w + i) * LD + 16 * w;
+        float a = i == r ? 1.0f : 0.0f;
+#pragma unroll
+        for (int m = 0; m < i; ++m) a = __builtin_fmaf(-row[m], x[m], a);
+        x[i] = a;
+    }
+    __syncthreads();  // P has been read
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (i / 4 == g4) s_t[(16 * w + i) * LD + 16 * w + r] = x[i];
+    __syncthreads();
+    const auto row_of = [&](const float* m, int i, int j) {  // block (i, j) as the left operand
+        return *reinterpret_cast<const f32x4_t*>(m + (16 * i + r) * LD + 16 * j + 4 * g4);
+    };
+    const auto col_of = [&](const float* m, int i, int j) {  // block (i, j) as the right operand
+        f32x4_t v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = m[(16 * i + 4 * g4 + e) * LD + 16 * j + r];
+        return v;
+    };
+    const auto put = [&](float* m, int i, int j, const f32x4_t& v, float sign) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m[(16 * i + 4 * g4 + e) * LD + 16 * j + r] = sign * v[e];
+    };
+    const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    if ((w & 1) == 0) {  // blocks (1, 0) and (3, 2)
+        const f32x4_t m = mm16(row_of(s_l, w + 1, w), col_of(s_t, w, w), zero);
+        put(s_t, w + 1, w, mm16(row_of(s_t, w + 1, w + 1), m, zero), -1.0f);
+    }
+    __syncthreads();
+    const int bi = 2 + (w >> 1), bj = w & 1;  // the lower left half: M = L T, then -T M
+    {
+        f32x4_t m = zero;
+        for (int e = bj; e < 2; ++e) m = mm16(row_of(s_l, bi, e), col_of(s_t, e, bj), m);
+        put(s_l, bj, bi, m, 1.0f);  // an upper block of L
+    }
+    __syncthreads();
+    {
+        f32x4_t m = zero;
+        for (int e = 2; e <= bi; ++e) m = mm16(row_of(s_t, bi, e), col_of(s_l, bj, e), m);
+        put(s_t, bi, bj, m, -1.0f);
+    }
+    __syncthreads();
+    for (int ks = 0; ks <= w >> 1; ++ks) {
+        const int col = 32 * ks + 8 * g4;
+        const float* const src = s_t + (16 * w + r) * LD + col;
+        uint32_t a[4], d[4], e[4];
+        const bool none = col >= 16 * (w + 1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            split3(none ? 0.0f : src[2 * i] * s_beta[col + 2 * i], none ? 0.0f : src[2 * i + 1] * s_beta[col + 2 * i + 1], a[i],
+                   d[i], e[i]);
+        uint16_t* const to = unit + kUnitT + tri_frag(w, ks) * kFrag + 8 * lane;
+        *reinterpret_cast<uint4*>(to) = make_uint4(a[0], a[1], a[2], a[3]);
+        *reinterpret_cast<uint4*>(to + kTPart) = make_uint4(d[0], d[1], d[2], d[3]);
+        *reinterpret_cast<uint4*>(to + 2 * kTPart) = make_uint4(e[0], e[1], e[2], e[3]);
+    }
+}
+
+// 16 columns of one head's state from chunk to chunk.  Waves 0 to 3 keep the
+// state: wave w its rows w DK/4 .. in fp32, as the products leave them, and
+// all of it in LDS as the bf16 parts that are the right operand of K S and Q S.
+// Per chunk: (1) wave w forms rows 16 w .. of Y = V - diag(e^G) K S0 while wave
+// 4 + w forms them of Q S0; (2) wave w its rows of U = T Y; (3) wave w its rows
+// of the new state while wave 4 + w adds P U to its rows of out and stores them.
+// What a stage needs from memory was loaded a chunk before.
+template <int DK, bool F16>
+__global__ __launch_bounds__(512) void delta_chunk_scan_kernel(DeltaParams p, ChunkPlan c) {
+    constexpr int KS = DK / 32, MT = DK / 64;  // MT: 16-row tiles of the state per wave
+    constexpr int LS = DK + 8, LU = kChunk + 8, LW = 20;
+    constexpr int NS = kScanCols * LS, NU = kScanCols * LU;
+    __shared__ __attribute__((aligned(16))) uint16_t s_s[3 * NS];  // state parts [part][column][row]
+    __shared__ __attribute__((aligned(16))) uint16_t s_y[3 * NU];  // Y parts [part][column][token]
+    __shared__ __attribute__((aligned(16))) uint16_t s_d[3 * NU];  // diag(e^(G_last - G)) U in three parts
+    __shared__ __attribute__((aligned(16))) uint16_t s_u[2 * NU];  // U in two
+    __shared__ __attribute__((aligned(16))) float s_w[DK * LW];    // the state of a chunk that runs token by token
+    __shared__ int s_bad[2];
+    const int heads = p.B * p.Hv;
+    const int bh = int(blockIdx.x) % heads, col0 = int(blockIdx.x) / heads * kScanCols;
+    const int b = bh / p.Hv, h = bh - b * p.Hv, hk = h / p.G;
+    const int slot = entry_state(p.seq, b), len = entry_len(p.seq, b);
+    const int begin = c.first * kChunk;
+    if (slot == kEntryEmpty || begin >= len) return;
+    const int end = min(len, begin + c.count * kChunk);
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g4 = lane >> 4;
+    if (slot == kEntryBad) {
+        if (w == 0) nan_rows<4, F16>(p, b, h, col0 + 4 * (lane & 3), begin, end);
+        return;
+    }
+    const bool keeps = w < 4;
+    const int tile = w & 3;
+    const int chunks = (end - begin + kChunk - 1) / kChunk;
+    const uint16_t* unit = c.units + (int64_t(b) * c.count * p.Hv + h) * kUnitElems;
+    const int64_t unit_step = int64_t(p.Hv) * kUnitElems;
+    const uint16_t* kt = c.kt + (int64_t(b) * c.count * p.Hk + hk) * (DK * kChunk) + tile * MT * 2 * kFrag + 8 * lane;
+    const int64_t kt_step = int64_t(p.Hk) * (DK * kChunk);
+    const uint16_t* const rows = keeps ? p.k.p + b * p.k.batch + hk * p.k.head : p.q.p + b * p.q.batch + hk * p.q.head;
+    const int64_t rows_tok = keeps ? p.k.tok : p.q.tok;
+    const uint16_t* const v = p.v.p + b * p.v.batch + h * p.v.head + col0 + r;
+    uint16_t* const out = p.out + b * p.o_batch + h * p.o_head + col0 + r;
+    float* const st = p.state + ((int64_t(slot) * p.Hv + h) * DK + tile * (DK / 4)) * p.Dv + col0 + r;
+
+    f32x4_t s[MT];
+    const auto put_state = [&]() {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            uint32_t a[2], d[2], e[2];
+            split3(s[m][0], s[m][1], a[0], d[0], e[0]);
+            split3(s[m][2], s[m][3], a[1], d[1], e[1]);
+            uint16_t* const to = s_s + r * LS + tile * (DK / 4) + 16 * m + 4 * g4;
+            *reinterpret_cast<uint2*>(to) = make_uint2(a[0], a[1]);
+            *reinterpret_cast<uint2*>(to + NS) = make_uint2(d[0], d[1]);
+            *reinterpret_cast<uint2*>(to + 2 * NS) = make_uint2(e[0], e[1]);
+        }
+    };
+    uint4 fx[KS], ft[2][3], fk[2 * MT];  // rows of K or Q; parts of T or P; K^T
+    float vv[4], ve[4], vd[4], vlast = 0.0f, vbad = 0.0f;
+    const auto load_rows = [&](int t0) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            fx[ks] = make_uint4(0, 0, 0, 0);
+            const int t = t0 + 16 * tile + r;
+            if (t < end) fx[ks] = *reinterpret_cast<const uint4*>(rows + t * rows_tok + 32 * ks + 8 * g4);
+        }
+        if (keeps)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = t0 + 16 * tile + 4 * g4 + i;
+                vv[i] = t < end ? Elem<F16>::lo(v[t * p.v.tok]) : 0.0f;
+            }
+    };
+    const auto load_unit = [&](const uint16_t* u, const uint16_t* k) {
+        const float* const vec = reinterpret_cast<const float*>(u + kUnitVec);
+        const f32x4_t e = *reinterpret_cast<const f32x4_t*>(vec + (keeps ? kVecC : kVecE) + 16 * tile + 4 * g4);
+        const f32x4_t d = *reinterpret_cast<const f32x4_t*>(vec + kVecD + 16 * tile + 4 * g4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ve[i] = e[i], vd[i] = d[i];
+        vlast = vec[kVecLast], vbad = vec[kVecBad];
+        const uint16_t* const tri = u + (keeps ? kUnitT : kUnitP) + 8 * lane;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int q = 0; q < 3; ++q)
+                if (ks <= tile >> 1 && (keeps || q < 2))
+                    ft[ks][q] = *reinterpret_cast<const uint4*>(tri + q * kTPart + tri_frag(tile, ks) * kFrag);
+        if (keeps)
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i) fk[i] = *reinterpret_cast<const uint4*>(k + i * kFrag);
+    };
+    const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (keeps) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[m][i] = st[int64_t(16 * m + 4 * g4 + i) * p.Dv];
+        put_state();
+    }
+    if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
+    load_rows(begin);
+    load_unit(unit, kt);
+    lds_barrier();
+
+    for (int n = 0; n < chunks; ++n) {
+        const int t0 = begin + n * kChunk;
+        f32x4_t z = zero;
+        // (1) rows of K S0 or Q S0
+        {
+            f32x4_t a0 = zero, a1 = zero, a2 = zero;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const uint16_t* const src = s_s + r * LS + 32 * ks + 8 * g4;
+                const uint4 s0 = *reinterpret_cast<const uint4*>(src), s1 = *reinterpret_cast<const uint4*>(src + NS);
+                uint4 x0 = fx[ks], x1;
+                if constexpr (F16) split_f16(fx[ks], x0, x1);
+                a0 = mma(x0, s0, a0);
+                a1 = mma(x0, s1, a1);
+                if constexpr (F16) a1 = mma(x1, s0, a1);
+                if (keeps) {
+                    const uint4 s2 = *reinterpret_cast<const uint4*>(src + 2 * NS);
+                    a2 = mma(x0, s2, a2);
+                    if constexpr (F16) a2 = mma(x1, s1, a2);
+                }
+            }
+            z = a0 + (a1 + a2);
+        }
+        if (keeps) {
+            float y[4];
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                y[i] = vv[i] - ve[i] * z[i];
+                odd |= !(fabsf(y[i]) < INFINITY);
+            }
+            uint32_t a[2], d[2], e[2];
+            split3(y[0], y[1], a[0], d[0], e[0]);
+            split3(y[2], y[3], a[1], d[1], e[1]);
+            uint16_t* const to = s_y + r * LU + 16 * tile + 4 * g4;
+            *reinterpret_cast<uint2*>(to) = make_uint2(a[0], a[1]);
+            *reinterpret_cast<uint2*>(to + NU) = make_uint2(d[0], d[1]);
+            *reinterpret_cast<uint2*>(to + 2 * NU) = make_uint2(e[0], e[1]);
+            if (odd || vbad != 0.0f) s_bad[n & 1] = 1;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[i] *= ve[i];
+        }
+        if (n + 1 < chunks) load_rows(t0 + kChunk);
+        lds_barrier();
+        const bool slow = __builtin_amdgcn_readfirstlane(s_bad[n & 1]) != 0;
+        if (threadIdx.x == 0) s_bad[(n + 1) & 1] = 0;  // read last a chunk ago, set next after two barriers
+        if (slow) {
+            if (keeps)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s_w[(tile * (DK / 4) + 16 * m + 4 * g4 + i) * LW + r] = s[m][i];
+            lds_barrier();
+            if (w == 0) {
+                constexpr int NR = DK / 16;
+                f32x4_t sr[NR];
+#pragma unroll
+                for (int i = 0; i < NR; ++i) sr[i] = *reinterpret_cast<const f32x4_t*>(s_w + (lane / 4 * NR + i) * LW + 4 * (lane & 3));
+                recur<DK, 4, F16>(p, sr, b, h, col0 + 4 * (lane & 3), t0, min(end, t0 + kChunk));
+#pragma unroll
+                for (int i = 0; i < NR; ++i) *reinterpret_cast<f32x4_t*>(s_w + (lane / 4 * NR + i) * LW + 4 * (lane & 3)) = sr[i];
+            }
+            lds_barrier();
+            if (keeps) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[m][i] = s_w[(tile * (DK / 4) + 16 * m + 4 * g4 + i) * LW + r];
+                put_state();
+            }
+        } else {
+            if (keeps) {  // (2) rows of U
+                f32x4_t a0 = zero, a1 = zero, a2 = zero;
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    if (ks > tile >> 1) continue;
+                    const uint16_t* const src = s_y + r * LU + 32 * ks + 8 * g4;
+                    const uint4 y0 = *reinterpret_cast<const uint4*>(src), y1 = *reinterpret_cast<const uint4*>(src + NU),
+                                y2 = *reinterpret_cast<const uint4*>(src + 2 * NU);
+                    a0 = mma(ft[ks][0], y0, a0);
+                    a1 = mma(ft[ks][0], y1, a1);
+                    a2 = mma(ft[ks][0], y2, a2);
+                    a1 = mma(ft[ks][1], y0, a1);
+                    a2 = mma(ft[ks][1], y1, a2);
+                    a2 = mma(ft[ks][2], y0, a2);
+                }
+                const f32x4_t u = a0 + (a1 + a2);
+                uint32_t a[2], d[2], e[2];
+                uint16_t* to = s_u + r * LU + 16 * tile + 4 * g4;
+                split2(u[0], u[1], a[0], d[0]);
+                split2(u[2], u[3], a[1], d[1]);
+                *reinterpret_cast<uint2*>(to) = make_uint2(a[0], a[1]);
+                *reinterpret_cast<uint2*>(to + NU) = make_uint2(d[0], d[1]);
+                to = s_d + r * LU + 16 * tile + 4 * g4;
+                split3(vd[0] * u[0], vd[1] * u[1], a[0], d[0], e[0]);
+                split3(vd[2] * u[2], vd[3] * u[3], a[1], d[1], e[1]);
+                *reinterpret_cast<uint2*>(to) = make_uint2(a[0], a[1]);
+                *reinterpret_cast<uint2*>(to + NU) = make_uint2(d[0], d[1]);
+                *reinterpret_cast<uint2*>(to + 2 * NU) = make_uint2(e[0], e[1]);
+            }
+            lds_barrier();
+            if (keeps) {  // (3) rows of the new state
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    f32x4_t a0 = s[m] * vlast, a1 = zero, a2 = zero;
+#pragma unroll
+                    for (int ks = 0; ks < 2; ++ks) {
+                        const uint16_t* const src = s_d + r * LU + 32 * ks + 8 * g4;
+                        const uint4 d0 = *reinterpret_cast<const uint4*>(src), d1 = *reinterpret_cast<const uint4*>(src + NU),
+                                    d2 = *reinterpret_cast<const uint4*>(src + 2 * NU);
+                        uint4 k0 = fk[2 * m + ks], k1;
+                        if constexpr (F16) split_f16(fk[2 * m + ks], k0, k1);
+                        a0 = mma(k0, d0, a0);
+                        a1 = mma(k0, d1, a1);
+                        a2 = mma(k0, d2, a2);
+                        if constexpr (F16) a1 = mma(k1, d0, a1), a2 = mma(k1, d1, a2);
+                    }
+                    s[m] = a0 + (a1 + a2);
+                }
+                put_state();
+            } else {  // rows of out
+                f32x4_t a0 = z, a1 = zero;
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    if (ks > tile >> 1) continue;
+                    const uint16_t* const src = s_u + r * LU + 32 * ks + 8 * g4;
+                    const uint4 u0 = *reinterpret_cast<const uint4*>(src), u1 = *reinterpret_cast<const uint4*>(src + NU);
+                    a0 = mma(ft[ks][0], u0, a0);
+                    a1 = mma(ft[ks][0], u1, a1);
+                    a1 = mma(ft[ks][1], u0, a1);
+                }
+                a0 += a1;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int t = t0 + 16 * tile + 4 * g4 + i;
+                    if (t < end) out[t * p.o_tok] = uint16_t(Elem<F16>::pack_p(a0[i], 0.0f));
+                }
+            }
+        }
+        unit += unit_step;
+        kt += kt_step;
+        if (n + 1 < chunks) load_unit(unit, kt);
+        lds_barrier();
+    }
+    if (keeps)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st[int64_t(16 * m + 4 * g4 + i) * p.Dv] = s[m][i];
+}
+
+// Chunks of one pair of launches: their units stay near 128 MB, within the
+// 256 MB cache between the two kernels, however long the sequence is.
+constexpr size_t kUnitBytes = kUnitElems * 2;
+int64_t chunks_per_launch(int64_t B, int64_t S, int64_t Hv) {
+    const int64_t all = (S + kChunk - 1) / kChunk;
+    const int64_t fit = int64_t((size_t(128) << 20) / kUnitBytes) / (B * Hv);
+    return std::min(all, std::max<int64_t>(fit, 1));
+}
+
+// Up to this many tokens per entry the rule runs token by token.
+constexpr int kRecurrentTokens = 16;
+bool in_chunks(int64_t S) { return S > kRecurrentTokens; }
+
+template <bool F16>
+int launch_chunks(const DeltaParams& p, void* ws, hipStream_t stream) {
+    const int64_t per = chunks_per_launch(p.B, p.seq.S, p.Hv), all = (int64_t(p.seq.S) + kChunk - 1) / kChunk;
+    ChunkPlan c;
+    c.units = static_cast<uint16_t*>(ws);
+    c.kt = c.units + size_t(p.B) * per * p.Hv * kUnitElems;
+    auto* prepare = p.Dk == 128 ? delta_chunk_prepare_kernel<128, F16> : delta_chunk_prepare_kernel<64, F16>;
+    auto* scan = p.Dk == 128 ? delta_chunk_scan_kernel<128, F16> : delta_chunk_scan_kernel<64, F16>;
+    for (int64_t first = 0; first < all; first += per) {
+        c.first = int32_t(first), c.count = int32_t(std::min(per, all - first));
+        hipLaunchKernelGGL(prepare, dim3(unsigned(int64_t(p.B) * c.count * p.Hv)), dim3(256), 0, stream, p, c);
+        GENLLM_LAUNCH_CHECK("delta_chunk_prepare_kernel");
+        hipLaunchKernelGGL(scan, dim3(unsigned(p.B * p.Hv * (p.Dv / kScanCols))), dim3(512), 0, stream, p, c);
+        GENLLM_LAUNCH_CHECK("delta_chunk_scan_kernel");
+    }
+    return GENLLM_OK;
 }
 
 template <bool F16>
@@ -183,7 +769,10 @@ using namespace genllm;
 
 extern "C" size_t genllm_gated_delta_workspace_bytes(int32_t batch, int32_t seq_len, int32_t n_k_heads, int32_t n_v_heads,
                                                      int32_t k_dim, int32_t v_dim) {
-    return 0;
+    if (batch <= 0 || seq_len <= 0 || n_k_heads <= 0 || n_v_heads <= 0 || k_dim <= 0 || v_dim <= 0 || !in_chunks(seq_len))
+        return 0;
+    const size_t n = size_t(batch) * size_t(chunks_per_launch(batch, seq_len, n_v_heads));
+    return n * (size_t(n_v_heads) * kUnitBytes + size_t(n_k_heads) * k_dim * kChunk * 2);
 }
 
 extern "C" int genllm_gated_delta_rule(const void* q, int64_t q_batch_stride, int64_t q_tok_stride, int64_t q_head_stride,
@@ -233,12 +822,20 @@ extern "C" int genllm_gated_delta_rule(const void* q, int64_t q_batch_stride, in
     if (!aligned_to(a, gate_align) || !aligned_to(b, gate_align) || !aligned_to(a_log, 4) || !aligned_to(dt_bias, 4) ||
         !aligned_to(state_ids, 4) || !aligned_to(seq_lens, 4))
         return fail(GENLLM_ERR_INVALID, "gated_delta_rule: a pointer is not aligned to its type");
-    if (int64_t(batch) * n_v_heads > (int64_t(1) << 26))
-        return fail(GENLLM_ERR_INVALID, "gated_delta_rule: batch * n_v_heads must be at most 2^26");
+    if (int64_t(batch) * n_v_heads > (int64_t(1) << 19))  // a grid has at most 2^32 threads
+        return fail(GENLLM_ERR_INVALID, "gated_delta_rule: batch * n_v_heads must be at most 2^19");
     p.a = a, p.b = b, p.a_batch = a_batch_stride, p.a_tok = a_tok_stride, p.b_batch = b_batch_stride, p.b_tok = b_tok_stride;
     p.a_log = a_log, p.dt_bias = dt_bias, p.state = state;
     p.seq.ids = state_ids, p.seq.lens = seq_lens, p.seq.n_states = n_states, p.seq.S = seq_len;
     p.B = batch, p.Hk = n_k_heads, p.Hv = n_v_heads, p.G = n_v_heads / n_k_heads, p.Dk = k_dim, p.Dv = v_dim;
     p.scale = scale, p.l2_eps = l2_eps < 0.0f ? -1.0f : l2_eps;
+    if (in_chunks(seq_len)) {
+        const size_t need = genllm_gated_delta_workspace_bytes(batch, seq_len, n_k_heads, n_v_heads, k_dim, v_dim);
+        if (!workspace || workspace_bytes < need || !aligned_to(workspace, 16))
+            return fail(GENLLM_ERR_INVALID, "gated_delta_rule: a workspace of " + std::to_string(need) +
+                                                " bytes, 16-byte aligned, is needed (have " +
+                                                std::to_string(workspace_bytes) + ")");
+        return f16 ? launch_chunks<true>(p, workspace, as_stream(stream)) : launch_chunks<false>(p, workspace, as_stream(stream));
+    }
     return f16 ? launch_recurrent<true>(p, as_stream(stream)) : launch_recurrent<false>(p, as_stream(stream));
 }
