@@ -32,6 +32,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "common.hpp"
 #include "kernels.hpp"
@@ -283,27 +284,23 @@ __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p,
     const int slot = entry_state(p.seq, b), len = entry_len(p.seq, b);
     if (slot < 0 || t0 >= len) return;
     const int left = len - t0;  // tokens of this chunk and behind it
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g4 = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g4 = lane >> 4;
     const int hk = h / p.G;
     const bool writes_kt = h % p.G == 0;
     uint16_t* const unit = c.units + ((int64_t(b) * c.count + n) * p.Hv + h) * kUnitElems;
     float* const vec = reinterpret_cast<float*>(unit + kUnitVec);
 
-    // rows of K (tiles 0 .. w) and Q (tile w); rows behind the end are zeros
-    uint4 kf[4][KS], qf[KS];
+    // rows of K and Q of tile w; rows behind the end are zeros
+    uint4 own[KS], qf[KS];
     const uint16_t* const kp = p.k.p + b * p.k.batch + hk * p.k.head + 8 * g4;
     const uint16_t* const qp = p.q.p + b * p.q.batch + hk * p.q.head + 8 * g4;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            kf[j][ks] = make_uint4(0, 0, 0, 0);
-            if (j <= w && 16 * j + r < left) kf[j][ks] = *reinterpret_cast<const uint4*>(kp + (t0 + 16 * j + r) * p.k.tok + 32 * ks);
-        }
-#pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-        qf[ks] = make_uint4(0, 0, 0, 0);
-        if (16 * w + r < left) qf[ks] = *reinterpret_cast<const uint4*>(qp + (t0 + 16 * w + r) * p.q.tok + 32 * ks);
+        own[ks] = qf[ks] = make_uint4(0, 0, 0, 0);
+        if (16 * w + r < left) {
+            own[ks] = *reinterpret_cast<const uint4*>(kp + (t0 + 16 * w + r) * p.k.tok + 32 * ks);
+            qf[ks] = *reinterpret_cast<const uint4*>(qp + (t0 + 16 * w + r) * p.q.tok + 32 * ks);
+        }
     }
     // gates of token `lane`, the running sum in 64 bits (differences of far sums
     // enter the exponents); exp(-2000) is 0 in either precision
@@ -317,10 +314,8 @@ __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p,
         if (lane >= m) sum += up;
     }
     float kk = 0.0f, qq = 0.0f;
-    uint4 own[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-        own[ks] = w == 0 ? kf[0][ks] : w == 1 ? kf[1][ks] : w == 2 ? kf[2][ks] : kf[3][ks];
         const uint32_t a[4] = {own[ks].x, own[ks].y, own[ks].z, own[ks].w};
         const uint32_t d[4] = {qf[ks].x, qf[ks].y, qf[ks].z, qf[ks].w};
 #pragma unroll
@@ -353,8 +348,9 @@ __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p,
         f32x4_t ak = {0.0f, 0.0f, 0.0f, 0.0f}, aq = ak;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            ak = Elem<F16>::mma32(own[ks], kf[j][ks], ak);
-            aq = Elem<F16>::mma32(qf[ks], kf[j][ks], aq);
+            const uint4 kj = *reinterpret_cast<const uint4*>(s_k + (16 * j + r) * LK + 32 * ks + 8 * g4);
+            ak = Elem<F16>::mma32(own[ks], kj, ak);
+            aq = Elem<F16>::mma32(qf[ks], kj, aq);
         }
         const int col = 16 * j + r;
         const double gc = s_g[col];
@@ -463,18 +459,32 @@ __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p,
     }
 }
 
+// What one wave of the scan needs from memory for one chunk.
+template <int KS, int MT>
+struct ScanLoad {
+    uint4 x[KS];         // a row of K (waves that keep the state) or Q
+    uint4 tri[2][3];     // fragments of T or P
+    uint4 kt[2 * MT];    // fragments of K^T
+    uint16_t v[4];
+    f32x4_t e, d;        // e^G and e^(G_last - G) with the norms of the rows
+    float last, bad;
+};
+
 // 16 columns of one head's state from chunk to chunk.  Waves 0 to 3 keep the
 // state: wave w its rows w DK/4 .. in fp32, as the products leave them, and
 // all of it in LDS as the bf16 parts that are the right operand of K S and Q S.
-// Per chunk: (1) wave w forms rows 16 w .. of Y = V - diag(e^G) K S0 while wave
-// 4 + w forms them of Q S0; (2) wave w its rows of U = T Y; (3) wave w its rows
-// of the new state while wave 4 + w adds P U to its rows of out and stores them.
-// What a stage needs from memory was loaded a chunk before.
+// Per chunk: (1) wave w forms rows 16 w .. of Y = V - diag(e^G) K S0; (2) its
+// rows of U = T Y, while wave 4 + w forms rows of Q S0; (3) its rows of the new
+// state, while wave 4 + w adds P U to its rows of out and stores them.  The two
+// kinds of waves run loops of their own that meet at the same barriers.  What
+// a chunk needs from memory is loaded a chunk before, into the registers that
+// this chunk's use of them has just freed.
 template <int DK, bool F16>
 __global__ __launch_bounds__(512) void delta_chunk_scan_kernel(DeltaParams p, ChunkPlan c) {
     constexpr int KS = DK / 32, MT = DK / 64;  // MT: 16-row tiles of the state per wave
     constexpr int LS = DK + 8, LU = kChunk + 8, LW = 20;
     constexpr int NS = kScanCols * LS, NU = kScanCols * LU;
+    using Load = ScanLoad<KS, MT>;
     __shared__ __attribute__((aligned(16))) uint16_t s_s[3 * NS];  // state parts [part][column][row]
     __shared__ __attribute__((aligned(16))) uint16_t s_y[3 * NU];  // Y parts [part][column][token]
     __shared__ __attribute__((aligned(16))) uint16_t s_d[3 * NU];  // diag(e^(G_last - G)) U in three parts
@@ -488,7 +498,7 @@ __global__ __launch_bounds__(512) void delta_chunk_scan_kernel(DeltaParams p, Ch
     const int begin = c.first * kChunk;
     if (slot == kEntryEmpty || begin >= len) return;
     const int end = min(len, begin + c.count * kChunk);
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g4 = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g4 = lane >> 4;
     if (slot == kEntryBad) {
         if (w == 0) nan_rows<4, F16>(p, b, h, col0 + 4 * (lane & 3), begin, end);
         return;
@@ -496,132 +506,166 @@ __global__ __launch_bounds__(512) void delta_chunk_scan_kernel(DeltaParams p, Ch
     const bool keeps = w < 4;
     const int tile = w & 3;
     const int chunks = (end - begin + kChunk - 1) / kChunk;
-    const uint16_t* unit = c.units + (int64_t(b) * c.count * p.Hv + h) * kUnitElems;
-    const int64_t unit_step = int64_t(p.Hv) * kUnitElems;
-    const uint16_t* kt = c.kt + (int64_t(b) * c.count * p.Hk + hk) * (DK * kChunk) + tile * MT * 2 * kFrag + 8 * lane;
-    const int64_t kt_step = int64_t(p.Hk) * (DK * kChunk);
-    const uint16_t* const rows = keeps ? p.k.p + b * p.k.batch + hk * p.k.head : p.q.p + b * p.q.batch + hk * p.q.head;
+    const uint16_t* const units = c.units + (int64_t(b) * c.count * p.Hv + h) * kUnitElems;
+    const uint16_t* const kts = c.kt + (int64_t(b) * c.count * p.Hk + hk) * (DK * kChunk) + tile * MT * 2 * kFrag + 8 * lane;
+    const uint16_t* const rows = (keeps ? p.k.p + b * p.k.batch + hk * p.k.head : p.q.p + b * p.q.batch + hk * p.q.head) + 8 * g4;
     const int64_t rows_tok = keeps ? p.k.tok : p.q.tok;
     const uint16_t* const v = p.v.p + b * p.v.batch + h * p.v.head + col0 + r;
-    uint16_t* const out = p.out + b * p.o_batch + h * p.o_head + col0 + r;
-    float* const st = p.state + ((int64_t(slot) * p.Hv + h) * DK + tile * (DK / 4)) * p.Dv + col0 + r;
-
-    f32x4_t s[MT];
-    const auto put_state = [&]() {
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            uint32_t a[2], d[2], e[2];
-            split3(s[m][0], s[m][1], a[0], d[0], e[0]);
-            split3(s[m][2], s[m][3], a[1], d[1], e[1]);
-            uint16_t* const to = s_s + r * LS + tile * (DK / 4) + 16 * m + 4 * g4;
-            *reinterpret_cast<uint2*>(to) = make_uint2(a[0], a[1]);
-            *reinterpret_cast<uint2*>(to + NS) = make_uint2(d[0], d[1]);
-            *reinterpret_cast<uint2*>(to + 2 * NS) = make_uint2(e[0], e[1]);
-        }
-    };
-    uint4 fx[KS], ft[2][3], fk[2 * MT];  // rows of K or Q; parts of T or P; K^T
-    float vv[4], ve[4], vd[4], vlast = 0.0f, vbad = 0.0f;
-    const auto load_rows = [&](int t0) {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            fx[ks] = make_uint4(0, 0, 0, 0);
-            const int t = t0 + 16 * tile + r;
-            if (t < end) fx[ks] = *reinterpret_cast<const uint4*>(rows + t * rows_tok + 32 * ks + 8 * g4);
-        }
-        if (keeps)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = t0 + 16 * tile + 4 * g4 + i;
-                vv[i] = t < end ? Elem<F16>::lo(v[t * p.v.tok]) : 0.0f;
-            }
-    };
-    const auto load_unit = [&](const uint16_t* u, const uint16_t* k) {
-        const float* const vec = reinterpret_cast<const float*>(u + kUnitVec);
-        const f32x4_t e = *reinterpret_cast<const f32x4_t*>(vec + (keeps ? kVecC : kVecE) + 16 * tile + 4 * g4);
-        const f32x4_t d = *reinterpret_cast<const f32x4_t*>(vec + kVecD + 16 * tile + 4 * g4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ve[i] = e[i], vd[i] = d[i];
-        vlast = vec[kVecLast], vbad = vec[kVecBad];
-        const uint16_t* const tri = u + (keeps ? kUnitT : kUnitP) + 8 * lane;
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-            for (int q = 0; q < 3; ++q)
-                if (ks <= tile >> 1 && (keeps || q < 2))
-                    ft[ks][q] = *reinterpret_cast<const uint4*>(tri + q * kTPart + tri_frag(tile, ks) * kFrag);
-        if (keeps)
-#pragma unroll
-            for (int i = 0; i < 2 * MT; ++i) fk[i] = *reinterpret_cast<const uint4*>(k + i * kFrag);
-    };
+    const int tri0 = tri_frag(tile, 0) * kFrag + 8 * lane, tri1 = tri_frag(tile, tile >> 1) * kFrag + 8 * lane;
     const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (keeps) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[m][i] = st[int64_t(16 * m + 4 * g4 + i) * p.Dv];
-        put_state();
-    }
-    if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
-    load_rows(begin);
-    load_unit(unit, kt);
-    lds_barrier();
 
-    for (int n = 0; n < chunks; ++n) {
-        const int t0 = begin + n * kChunk;
-        f32x4_t z = zero;
-        // (1) rows of K S0 or Q S0
-        {
-            f32x4_t a0 = zero, a1 = zero, a2 = zero;
+    // the rows of chunk n, or the last one's again; rows behind the end are read
+    // as the last row
+    const auto load_rows = [&](Load& x, int n, auto state) {
+        n = min(n, chunks - 1);
+        const int t0 = begin + n * kChunk + 16 * tile;
+        const uint16_t* const row = rows + min(t0 + r, end - 1) * rows_tok;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) x.x[ks] = *reinterpret_cast<const uint4*>(row + 32 * ks);
+        const float* const vec = reinterpret_cast<const float*>(units + int64_t(n) * p.Hv * kUnitElems + kUnitVec);
+        x.e = *reinterpret_cast<const f32x4_t*>(vec + (state.value ? kVecC : kVecE) + 16 * tile + 4 * g4);
+        if constexpr (state.value) {
+            x.bad = vec[kVecBad];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x.v[i] = v[min(t0 + 4 * g4 + i, end - 1) * p.v.tok];
+        }
+    };
+    const auto load_tri = [&](Load& x, int n, auto state) {
+        const uint16_t* const u = units + int64_t(min(n, chunks - 1)) * p.Hv * kUnitElems;
+        if constexpr (state.value) x.d = *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(u + kUnitVec) + kVecD + 16 * tile + 4 * g4);
+#pragma unroll
+        for (int q = 0; q < (state.value ? 3 : 2); ++q) {
+            const uint16_t* const part = u + (state.value ? kUnitT : kUnitP) + q * kTPart;
+            x.tri[0][q] = *reinterpret_cast<const uint4*>(part + tri0);
+            x.tri[1][q] = *reinterpret_cast<const uint4*>(part + tri1);
+        }
+    };
+    const auto load_kt = [&](Load& x, int n) {
+        n = min(n, chunks - 1);
+        x.last = reinterpret_cast<const float*>(units + int64_t(n) * p.Hv * kUnitElems + kUnitVec)[kVecLast];
+        const uint16_t* const k = kts + int64_t(n) * p.Hk * (DK * kChunk);
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i) x.kt[i] = *reinterpret_cast<const uint4*>(k + i * kFrag);
+    };
+    const auto s_part = [&](int ks, int q) { return *reinterpret_cast<const uint4*>(s_s + q * NS + r * LS + 32 * ks + 8 * g4); };
+    const auto u_part = [&](const uint16_t* m, int ks, int q) {
+        return *reinterpret_cast<const uint4*>(m + q * NU + r * LU + 32 * ks + 8 * g4);
+    };
+    const auto put3 = [&](uint16_t* to, int step, float x0, float x1, float x2, float x3) {
+        uint32_t a[2], d[2], e[2];
+        split3(x0, x1, a[0], d[0], e[0]);
+        split3(x2, x3, a[1], d[1], e[1]);
+        *reinterpret_cast<uint2*>(to) = make_uint2(a[0], a[1]);
+        *reinterpret_cast<uint2*>(to + step) = make_uint2(d[0], d[1]);
+        *reinterpret_cast<uint2*>(to + 2 * step) = make_uint2(e[0], e[1]);
+    };
+    Load x;
+
+    if (!keeps) {  // rows of out
+        uint16_t* const out = p.out + b * p.o_batch + h * p.o_head + col0 + r;
+        constexpr std::false_type outs;
+        load_rows(x, 0, outs);
+        load_tri(x, 0, outs);
+        lds_barrier();
+        for (int n = 0; n < chunks; ++n) {
+            lds_barrier();
+            if (__builtin_amdgcn_readfirstlane(s_bad[n & 1]) != 0) {
+                load_rows(x, n + 1, outs);
+                load_tri(x, n + 1, outs);
+                lds_barrier();
+                lds_barrier();
+                lds_barrier();
+                continue;
+            }
+            f32x4_t a0 = zero, a1 = zero;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const uint16_t* const src = s_s + r * LS + 32 * ks + 8 * g4;
-                const uint4 s0 = *reinterpret_cast<const uint4*>(src), s1 = *reinterpret_cast<const uint4*>(src + NS);
-                uint4 x0 = fx[ks], x1;
-                if constexpr (F16) split_f16(fx[ks], x0, x1);
+                const uint4 s0 = s_part(ks, 0), s1 = s_part(ks, 1);
+                uint4 x0 = x.x[ks], x1;
+                if constexpr (F16) split_f16(x.x[ks], x0, x1);
                 a0 = mma(x0, s0, a0);
                 a1 = mma(x0, s1, a1);
                 if constexpr (F16) a1 = mma(x1, s0, a1);
-                if (keeps) {
-                    const uint4 s2 = *reinterpret_cast<const uint4*>(src + 2 * NS);
-                    a2 = mma(x0, s2, a2);
-                    if constexpr (F16) a2 = mma(x1, s1, a2);
-                }
             }
-            z = a0 + (a1 + a2);
+            a0 = (a0 + a1) * x.e;
+            a1 = zero;
+            load_rows(x, n + 1, outs);
+            lds_barrier();
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                if (ks > tile >> 1) continue;
+                const uint4 u0 = u_part(s_u, ks, 0), u1 = u_part(s_u, ks, 1);
+                a0 = mma(x.tri[ks][0], u0, a0);
+                a1 = mma(x.tri[ks][0], u1, a1);
+                a1 = mma(x.tri[ks][1], u0, a1);
+            }
+            a0 += a1;
+            load_tri(x, n + 1, outs);
+            const int t = begin + n * kChunk + 16 * tile + 4 * g4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (t + i < end) out[(t + i) * p.o_tok] = uint16_t(Elem<F16>::pack_p(a0[i], 0.0f));
+            lds_barrier();
         }
-        if (keeps) {
+        return;
+    }
+
+    float* const st = p.state + ((int64_t(slot) * p.Hv + h) * DK + tile * (DK / 4)) * p.Dv + col0 + r;
+    f32x4_t s[MT];
+    const auto put_state = [&]() {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+            put3(s_s + r * LS + tile * (DK / 4) + 16 * m + 4 * g4, NS, s[m][0], s[m][1], s[m][2], s[m][3]);
+    };
+    constexpr std::true_type keep;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[m][i] = st[int64_t(16 * m + 4 * g4 + i) * p.Dv];
+    put_state();
+    if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
+    load_rows(x, 0, keep);
+    load_tri(x, 0, keep);
+    load_kt(x, 0);
+    lds_barrier();
+    for (int n = 0; n < chunks; ++n) {
+        {  // (1) rows of Y
+            f32x4_t a0 = zero, a1 = zero, a2 = zero;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const uint4 s0 = s_part(ks, 0), s1 = s_part(ks, 1), s2 = s_part(ks, 2);
+                uint4 x0 = x.x[ks], x1;
+                if constexpr (F16) split_f16(x.x[ks], x0, x1);
+                a0 = mma(x0, s0, a0);
+                a1 = mma(x0, s1, a1);
+                a2 = mma(x0, s2, a2);
+                if constexpr (F16) a1 = mma(x1, s0, a1), a2 = mma(x1, s1, a2);
+            }
+            const f32x4_t z = a0 + (a1 + a2);
+            const int t = begin + n * kChunk + 16 * tile + 4 * g4;
             float y[4];
-            bool odd = false;
+            bool odd = x.bad != 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                y[i] = vv[i] - ve[i] * z[i];
+                y[i] = t + i < end ? Elem<F16>::lo(x.v[i]) - x.e[i] * z[i] : 0.0f;
                 odd |= !(fabsf(y[i]) < INFINITY);
             }
-            uint32_t a[2], d[2], e[2];
-            split3(y[0], y[1], a[0], d[0], e[0]);
-            split3(y[2], y[3], a[1], d[1], e[1]);
-            uint16_t* const to = s_y + r * LU + 16 * tile + 4 * g4;
-            *reinterpret_cast<uint2*>(to) = make_uint2(a[0], a[1]);
-            *reinterpret_cast<uint2*>(to + NU) = make_uint2(d[0], d[1]);
-            *reinterpret_cast<uint2*>(to + 2 * NU) = make_uint2(e[0], e[1]);
-            if (odd || vbad != 0.0f) s_bad[n & 1] = 1;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) z[i] *= ve[i];
+            put3(s_y + r * LU + 16 * tile + 4 * g4, NU, y[0], y[1], y[2], y[3]);
+            if (odd) s_bad[n & 1] = 1;
+            load_rows(x, n + 1, keep);
         }
-        if (n + 1 < chunks) load_rows(t0 + kChunk);
         lds_barrier();
         const bool slow = __builtin_amdgcn_readfirstlane(s_bad[n & 1]) != 0;
-        if (threadIdx.x == 0) s_bad[(n + 1) & 1] = 0;  // read last a chunk ago, set next after two barriers
+        if (threadIdx.x == 0) s_bad[(n + 1) & 1] = 0;  // read last a chunk ago, set next after more barriers
         if (slow) {
-            if (keeps)
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s_w[(tile * (DK / 4) + 16 * m + 4 * g4 + i) * LW + r] = s[m][i];
+                for (int i = 0; i < 4; ++i) s_w[(tile * (DK / 4) + 16 * m + 4 * g4 + i) * LW + r] = s[m][i];
             lds_barrier();
             if (w == 0) {
                 constexpr int NR = DK / 16;
+                const int t0 = begin + n * kChunk;
                 f32x4_t sr[NR];
 #pragma unroll
                 for (int i = 0; i < NR; ++i) sr[i] = *reinterpret_cast<const f32x4_t*>(s_w + (lane / 4 * NR + i) * LW + 4 * (lane & 3));
@@ -630,92 +674,64 @@ __global__ __launch_bounds__(512) void delta_chunk_scan_kernel(DeltaParams p, Ch
                 for (int i = 0; i < NR; ++i) *reinterpret_cast<f32x4_t*>(s_w + (lane / 4 * NR + i) * LW + 4 * (lane & 3)) = sr[i];
             }
             lds_barrier();
-            if (keeps) {
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[m][i] = s_w[(tile * (DK / 4) + 16 * m + 4 * g4 + i) * LW + r];
-                put_state();
-            }
-        } else {
-            if (keeps) {  // (2) rows of U
-                f32x4_t a0 = zero, a1 = zero, a2 = zero;
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    if (ks > tile >> 1) continue;
-                    const uint16_t* const src = s_y + r * LU + 32 * ks + 8 * g4;
-                    const uint4 y0 = *reinterpret_cast<const uint4*>(src), y1 = *reinterpret_cast<const uint4*>(src + NU),
-                                y2 = *reinterpret_cast<const uint4*>(src + 2 * NU);
-                    a0 = mma(ft[ks][0], y0, a0);
-                    a1 = mma(ft[ks][0], y1, a1);
-                    a2 = mma(ft[ks][0], y2, a2);
-                    a1 = mma(ft[ks][1], y0, a1);
-                    a2 = mma(ft[ks][1], y1, a2);
-                    a2 = mma(ft[ks][2], y0, a2);
-                }
-                const f32x4_t u = a0 + (a1 + a2);
-                uint32_t a[2], d[2], e[2];
-                uint16_t* to = s_u + r * LU + 16 * tile + 4 * g4;
-                split2(u[0], u[1], a[0], d[0]);
-                split2(u[2], u[3], a[1], d[1]);
-                *reinterpret_cast<uint2*>(to) = make_uint2(a[0], a[1]);
-                *reinterpret_cast<uint2*>(to + NU) = make_uint2(d[0], d[1]);
-                to = s_d + r * LU + 16 * tile + 4 * g4;
-                split3(vd[0] * u[0], vd[1] * u[1], a[0], d[0], e[0]);
-                split3(vd[2] * u[2], vd[3] * u[3], a[1], d[1], e[1]);
-                *reinterpret_cast<uint2*>(to) = make_uint2(a[0], a[1]);
-                *reinterpret_cast<uint2*>(to + NU) = make_uint2(d[0], d[1]);
-                *reinterpret_cast<uint2*>(to + 2 * NU) = make_uint2(e[0], e[1]);
-            }
+                for (int i = 0; i < 4; ++i) s[m][i] = s_w[(tile * (DK / 4) + 16 * m + 4 * g4 + i) * LW + r];
+            put_state();
+            load_tri(x, n + 1, keep);
+            load_kt(x, n + 1);
             lds_barrier();
-            if (keeps) {  // (3) rows of the new state
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    f32x4_t a0 = s[m] * vlast, a1 = zero, a2 = zero;
-#pragma unroll
-                    for (int ks = 0; ks < 2; ++ks) {
-                        const uint16_t* const src = s_d + r * LU + 32 * ks + 8 * g4;
-                        const uint4 d0 = *reinterpret_cast<const uint4*>(src), d1 = *reinterpret_cast<const uint4*>(src + NU),
-                                    d2 = *reinterpret_cast<const uint4*>(src + 2 * NU);
-                        uint4 k0 = fk[2 * m + ks], k1;
-                        if constexpr (F16) split_f16(fk[2 * m + ks], k0, k1);
-                        a0 = mma(k0, d0, a0);
-                        a1 = mma(k0, d1, a1);
-                        a2 = mma(k0, d2, a2);
-                        if constexpr (F16) a1 = mma(k1, d0, a1), a2 = mma(k1, d1, a2);
-                    }
-                    s[m] = a0 + (a1 + a2);
-                }
-                put_state();
-            } else {  // rows of out
-                f32x4_t a0 = z, a1 = zero;
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    if (ks > tile >> 1) continue;
-                    const uint16_t* const src = s_u + r * LU + 32 * ks + 8 * g4;
-                    const uint4 u0 = *reinterpret_cast<const uint4*>(src), u1 = *reinterpret_cast<const uint4*>(src + NU);
-                    a0 = mma(ft[ks][0], u0, a0);
-                    a1 = mma(ft[ks][0], u1, a1);
-                    a1 = mma(ft[ks][1], u0, a1);
-                }
-                a0 += a1;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int t = t0 + 16 * tile + 4 * g4 + i;
-                    if (t < end) out[t * p.o_tok] = uint16_t(Elem<F16>::pack_p(a0[i], 0.0f));
-                }
-            }
+            continue;
         }
-        unit += unit_step;
-        kt += kt_step;
-        if (n + 1 < chunks) load_unit(unit, kt);
+        {  // (2) rows of U
+            f32x4_t a0 = zero, a1 = zero, a2 = zero;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                if (ks > tile >> 1) continue;
+                const uint4 y0 = u_part(s_y, ks, 0), y1 = u_part(s_y, ks, 1), y2 = u_part(s_y, ks, 2);
+                a0 = mma(x.tri[ks][0], y0, a0);
+                a1 = mma(x.tri[ks][0], y1, a1);
+                a2 = mma(x.tri[ks][0], y2, a2);
+                a1 = mma(x.tri[ks][1], y0, a1);
+                a2 = mma(x.tri[ks][1], y1, a2);
+                a2 = mma(x.tri[ks][2], y0, a2);
+            }
+            const f32x4_t u = a0 + (a1 + a2);
+            put3(s_d + r * LU + 16 * tile + 4 * g4, NU, x.d[0] * u[0], x.d[1] * u[1], x.d[2] * u[2], x.d[3] * u[3]);
+            uint32_t a[2], d[2];
+            split2(u[0], u[1], a[0], d[0]);
+            split2(u[2], u[3], a[1], d[1]);
+            uint16_t* const to = s_u + r * LU + 16 * tile + 4 * g4;
+            *reinterpret_cast<uint2*>(to) = make_uint2(a[0], a[1]);
+            *reinterpret_cast<uint2*>(to + NU) = make_uint2(d[0], d[1]);
+            load_tri(x, n + 1, keep);
+        }
+        lds_barrier();
+        // (3) rows of the new state
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            f32x4_t a0 = s[m] * x.last, a1 = zero, a2 = zero;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                const uint4 d0 = u_part(s_d, ks, 0), d1 = u_part(s_d, ks, 1), d2 = u_part(s_d, ks, 2);
+                uint4 k0 = x.kt[2 * m + ks], k1;
+                if constexpr (F16) split_f16(x.kt[2 * m + ks], k0, k1);
+                a0 = mma(k0, d0, a0);
+                a1 = mma(k0, d1, a1);
+                a2 = mma(k0, d2, a2);
+                if constexpr (F16) a1 = mma(k1, d0, a1), a2 = mma(k1, d1, a2);
+            }
+            s[m] = a0 + (a1 + a2);
+        }
+        load_kt(x, n + 1);
+        put_state();
         lds_barrier();
     }
-    if (keeps)
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) st[int64_t(16 * m + 4 * g4 + i) * p.Dv] = s[m][i];
+        for (int i = 0; i < 4; ++i) st[int64_t(16 * m + 4 * g4 + i) * p.Dv] = s[m][i];
 }
 
 // Chunks of one pair of launches: their units stay near 128 MB, within the
