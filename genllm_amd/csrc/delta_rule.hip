@@ -198,6 +198,7 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(DeltaParams p, int
 
 // ------------------------------------------------------------------ chunks
 constexpr int kChunk = 64;
+constexpr int kScanThreads = 768;
 constexpr int kScanCols = 16;  // columns of the state per workgroup of the scan
 
 // What the scan needs of one chunk and value head, in the order its lanes read
@@ -212,6 +213,14 @@ constexpr int kUnitVec = 5 * kTPart;             // floats: see kVec*
 constexpr int kVecC = 0, kVecD = 64, kVecE = 128, kVecLast = 192, kVecBad = 193, kVecFloats = 256;
 constexpr int kUnitElems = kUnitVec + 2 * kVecFloats;
 __device__ __forceinline__ constexpr int tri_frag(int tile, int ks) { return tile < 2 ? tile : 2 * tile - 2 + ks; }
+
+// Row rho of 16-row tile t, for tokens and for the state's rows.  A product
+// leaves rows 4 j + i, i < 4, of a tile in lane group j; as the right operand of the
+// next product the group holds 8 consecutive ones of 32.  With this order of
+// the rows its rows of two tiles are those eight: no lane needs another's.
+__device__ __forceinline__ constexpr int tile_row(int t, int rho) {
+    return 32 * (t >> 1) + 8 * (rho >> 2) + 4 * (t & 1) + (rho & 3);
+}
 
 struct ChunkPlan {
     uint16_t* units = nullptr;  // [batch][chunk][Hv][kUnitElems]
@@ -264,6 +273,12 @@ __device__ __forceinline__ void lds_barrier() {
     __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     __asm__ volatile("" ::: "memory");
+}
+
+// 16 bytes per lane from memory into LDS at `to` + 16 lane, `to` uniform
+__device__ __forceinline__ void load_lds(const void* from, void* to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)from,
+                                     (__attribute__((address_space(3))) uint32_t*)to, 16, 0, 0);
 }
 
 // Four waves per chunk and value head; wave w has row tile w of the 64 x 64
@@ -367,11 +382,12 @@ __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p,
 
     // P's fragments of row tile w, the vectors, K^T
     for (int ks = 0; ks <= w >> 1; ++ks) {
-        const float* const src = s_t + (16 * w + r) * LD + 32 * ks + 8 * g4;
+        const int row = tile_row(w, r), col = 32 * ks + 8 * g4;
+        const float* const src = s_t + row * LD + col;
         uint32_t a[4], d[4];
-        const bool zero = 32 * ks + 8 * g4 >= 16 * (w + 1);  // a block right of the diagonal's
 #pragma unroll
-        for (int i = 0; i < 4; ++i) split2(zero ? 0.0f : src[2 * i], zero ? 0.0f : src[2 * i + 1], a[i], d[i]);
+        for (int i = 0; i < 4; ++i)
+            split2(col + 2 * i > row ? 0.0f : src[2 * i], col + 2 * i + 1 > row ? 0.0f : src[2 * i + 1], a[i], d[i]);
         uint16_t* const to = unit + kUnitP + tri_frag(w, ks) * kFrag + 8 * lane;
         *reinterpret_cast<uint4*>(to) = make_uint4(a[0], a[1], a[2], a[3]);
         *reinterpret_cast<uint4*>(to + kTPart) = make_uint4(d[0], d[1], d[2], d[3]);
@@ -389,7 +405,7 @@ __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p,
         for (int m = w; m < DK / 16; m += 4)
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-                const uint16_t* const src = s_k + (32 * ks + 8 * g4) * LK + 16 * m + r;
+                const uint16_t* const src = s_k + (32 * ks + 8 * g4) * LK + tile_row(m, r);
                 uint32_t a[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) a[i] = pack2(src[2 * i * LK], src[(2 * i + 1) * LK]);
@@ -444,14 +460,13 @@ __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p,
     }
     __syncthreads();
     for (int ks = 0; ks <= w >> 1; ++ks) {
-        const int col = 32 * ks + 8 * g4;
-        const float* const src = s_t + (16 * w + r) * LD + col;
+        const int row = tile_row(w, r), col = 32 * ks + 8 * g4;
+        const float* const src = s_t + row * LD + col;
         uint32_t a[4], d[4], e[4];
-        const bool none = col >= 16 * (w + 1);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            split3(none ? 0.0f : src[2 * i] * s_beta[col + 2 * i], none ? 0.0f : src[2 * i + 1] * s_beta[col + 2 * i + 1], a[i],
-                   d[i], e[i]);
+            split3(col + 2 * i > row ? 0.0f : src[2 * i] * s_beta[col + 2 * i],
+                   col + 2 * i + 1 > row ? 0.0f : src[2 * i + 1] * s_beta[col + 2 * i + 1], a[i], d[i], e[i]);
         uint16_t* const to = unit + kUnitT + tri_frag(w, ks) * kFrag + 8 * lane;
         *reinterpret_cast<uint4*>(to) = make_uint4(a[0], a[1], a[2], a[3]);
         *reinterpret_cast<uint4*>(to + kTPart) = make_uint4(d[0], d[1], d[2], d[3]);
@@ -459,38 +474,58 @@ __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p,
     }
 }
 
-// What one wave of the scan needs from memory for one chunk.
-template <int KS, int MT>
-struct ScanLoad {
-    uint4 x[KS];         // a row of K (waves that keep the state) or Q
-    uint4 tri[2][3];     // fragments of T or P
-    uint4 kt[2 * MT];    // fragments of K^T
-    uint16_t v[4];
-    f32x4_t e, d;        // e^G and e^(G_last - G) with the norms of the rows
-    float last, bad;
+// A right operand of MT tiles' rows in lane order: 8 (MT = 2, a step of 32) or 4
+// values (MT = 1, a step of 16) per lane.
+template <int MT>
+struct Operand {
+    uint32_t w[2 * MT];
 };
+template <int MT>
+__device__ __forceinline__ f32x4_t mma_step(const Operand<MT>& a, const Operand<MT>& b, const f32x4_t& c) {
+    if constexpr (MT == 2)
+        return Elem<false>::mma32(make_uint4(a.w[0], a.w[1], a.w[2], a.w[3]), make_uint4(b.w[0], b.w[1], b.w[2], b.w[3]), c);
+    else
+        return Elem<false>::mma16(make_uint2(a.w[0], a.w[1]), make_uint2(b.w[0], b.w[1]), c);
+}
+// fp16 elements in two bf16 parts
+template <int MT>
+__device__ __forceinline__ void split_f16(const Operand<MT>& x, Operand<MT>& a, Operand<MT>& b) {
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) split2(Elem<true>::lo(x.w[i]), Elem<true>::hi(x.w[i]), a.w[i], b.w[i]);
+}
 
-// 16 columns of one head's state from chunk to chunk.  Waves 0 to 3 keep the
-// state: wave w its rows w DK/4 .. in fp32, as the products leave them, and
-// all of it in LDS as the bf16 parts that are the right operand of K S and Q S.
-// Per chunk: (1) wave w forms rows 16 w .. of Y = V - diag(e^G) K S0; (2) its
-// rows of U = T Y, while wave 4 + w forms rows of Q S0; (3) its rows of the new
-// state, while wave 4 + w adds P U to its rows of out and stores them.  The two
-// kinds of waves run loops of their own that meet at the same barriers.  What
-// a chunk needs from memory is loaded a chunk before, into the registers that
-// this chunk's use of them has just freed.
+// 16 columns of one head's state from chunk to chunk, in twelve waves.  Waves 0
+// to 3 keep the state: wave w its rows of the tiles MT w .. in fp32, as the
+// products leave them, which is also how the next product takes them.  Per chunk:
+//   (1) wave w: its rows' share of K S0 for all tokens; (2) wave w: the sum of the
+//   shares and Y = V - diag(e^G) K S0 for token tile w; (3) wave w: tile w of U = T Y;
+//   (4) wave w: its rows of the new state, S <- e^(G_last) S + K^T diag(e^(G_last - G)) U.
+// Waves 4 to 7 have the state and U from LDS and form out, tile w - 4: Q S0
+// during (2), P U during (4).  Waves 8 to 11 load what waves 0 to 3 need straight
+// into LDS, two chunks ahead: the chain (1) to (4) is bound by the instructions
+// that one wave can issue, and 53 KB a chunk keep the memory pipe busy.  Rows
+// behind the end come as copies of the last row; T has zeros in their place.
 template <int DK, bool F16>
-__global__ __launch_bounds__(512) void delta_chunk_scan_kernel(DeltaParams p, ChunkPlan c) {
+__global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaParams p, ChunkPlan c) {
     constexpr int KS = DK / 32, MT = DK / 64;  // MT: 16-row tiles of the state per wave
-    constexpr int LS = DK + 8, LU = kChunk + 8, LW = 20;
-    constexpr int NS = kScanCols * LS, NU = kScanCols * LU;
-    using Load = ScanLoad<KS, MT>;
-    __shared__ __attribute__((aligned(16))) uint16_t s_s[3 * NS];  // state parts [part][column][row]
-    __shared__ __attribute__((aligned(16))) uint16_t s_y[3 * NU];  // Y parts [part][column][token]
-    __shared__ __attribute__((aligned(16))) uint16_t s_d[3 * NU];  // diag(e^(G_last - G)) U in three parts
-    __shared__ __attribute__((aligned(16))) uint16_t s_u[2 * NU];  // U in two
-    __shared__ __attribute__((aligned(16))) float s_w[DK * LW];    // the state of a chunk that runs token by token
+    constexpr int LW = 20;
+    using Op = Operand<MT>;
+    struct Stage {
+        uint4 k[4 * KS * 64];                      // [token tile][step][lane]
+        uint4 t[3 * kTriFrags * 64];               // [part][fragment][lane]
+        uint4 kt[DK / 16 * 2 * 64];                // [state tile][step][lane]
+        uint16_t v[kChunk * kScanCols];
+        float vec[kVecFloats];
+    };
+    __shared__ __attribute__((aligned(16))) Stage s_in[2];
+    __shared__ f32x4_t s_x[4 * 4 * 64];     // shares of K S0 [wave][token tile][lane]
+    __shared__ uint4 s_s[2 * KS * 64];      // the state in two parts [part][step][lane]
+    __shared__ uint4 s_y[3 * 2 * 64];       // Y in three parts [part][step][lane], a tile's half of each
+    __shared__ uint4 s_d[3 * 2 * 64];       // diag(e^(G_last - G)) U in three parts
+    __shared__ uint4 s_u[2 * 2 * 64];       // U in two
     __shared__ int s_bad[2];
+    float* const s_w = reinterpret_cast<float*>(s_x);  // the state of a chunk that runs token by token
+    static_assert(DK * LW * sizeof(float) <= sizeof(s_x), "s_w lies in s_x");
     const int heads = p.B * p.Hv;
     const int bh = int(blockIdx.x) % heads, col0 = int(blockIdx.x) / heads * kScanCols;
     const int b = bh / p.Hv, h = bh - b * p.Hv, hk = h / p.G;
@@ -503,165 +538,272 @@ __global__ __launch_bounds__(512) void delta_chunk_scan_kernel(DeltaParams p, Ch
         if (w == 0) nan_rows<4, F16>(p, b, h, col0 + 4 * (lane & 3), begin, end);
         return;
     }
-    const bool keeps = w < 4;
     const int tile = w & 3;
     const int chunks = (end - begin + kChunk - 1) / kChunk;
-    const uint16_t* const units = c.units + (int64_t(b) * c.count * p.Hv + h) * kUnitElems;
-    const uint16_t* const kts = c.kt + (int64_t(b) * c.count * p.Hk + hk) * (DK * kChunk) + tile * MT * 2 * kFrag + 8 * lane;
-    const uint16_t* const rows = (keeps ? p.k.p + b * p.k.batch + hk * p.k.head : p.q.p + b * p.q.batch + hk * p.q.head) + 8 * g4;
-    const int64_t rows_tok = keeps ? p.k.tok : p.q.tok;
-    const uint16_t* const v = p.v.p + b * p.v.batch + h * p.v.head + col0 + r;
-    const int tri0 = tri_frag(tile, 0) * kFrag + 8 * lane, tri1 = tri_frag(tile, tile >> 1) * kFrag + 8 * lane;
+    const int tok0 = tile_row(tile, 4 * g4);  // the lane's four tokens of tile `tile`
     const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int half = 2 * ((tile >> 1) * 64 + lane) + (tile & 1);  // the lane's half of an operand, in uint2
+    constexpr int kPart = 2 * 2 * 64;                             // uint2 per part of s_y, s_d, s_u
 
-    // the rows of chunk n, or the last one's again; rows behind the end are read
-    // as the last row
-    const auto load_rows = [&](Load& x, int n, auto state) {
-        n = min(n, chunks - 1);
-        const int t0 = begin + n * kChunk + 16 * tile;
-        const uint16_t* const row = rows + min(t0 + r, end - 1) * rows_tok;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) x.x[ks] = *reinterpret_cast<const uint4*>(row + 32 * ks);
-        const float* const vec = reinterpret_cast<const float*>(units + int64_t(n) * p.Hv * kUnitElems + kUnitVec);
-        x.e = *reinterpret_cast<const f32x4_t*>(vec + (state.value ? kVecC : kVecE) + 16 * tile + 4 * g4);
-        if constexpr (state.value) {
-            x.bad = vec[kVecBad];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x.v[i] = v[min(t0 + 4 * g4 + i, end - 1) * p.v.tok];
-        }
-    };
-    const auto load_tri = [&](Load& x, int n, auto state) {
-        const uint16_t* const u = units + int64_t(min(n, chunks - 1)) * p.Hv * kUnitElems;
-        if constexpr (state.value) x.d = *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(u + kUnitVec) + kVecD + 16 * tile + 4 * g4);
-#pragma unroll
-        for (int q = 0; q < (state.value ? 3 : 2); ++q) {
-            const uint16_t* const part = u + (state.value ? kUnitT : kUnitP) + q * kTPart;
-            x.tri[0][q] = *reinterpret_cast<const uint4*>(part + tri0);
-            x.tri[1][q] = *reinterpret_cast<const uint4*>(part + tri1);
-        }
-    };
-    const auto load_kt = [&](Load& x, int n) {
-        n = min(n, chunks - 1);
-        x.last = reinterpret_cast<const float*>(units + int64_t(n) * p.Hv * kUnitElems + kUnitVec)[kVecLast];
-        const uint16_t* const k = kts + int64_t(n) * p.Hk * (DK * kChunk);
-#pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) x.kt[i] = *reinterpret_cast<const uint4*>(k + i * kFrag);
-    };
-    const auto s_part = [&](int ks, int q) { return *reinterpret_cast<const uint4*>(s_s + q * NS + r * LS + 32 * ks + 8 * g4); };
-    const auto u_part = [&](const uint16_t* m, int ks, int q) {
-        return *reinterpret_cast<const uint4*>(m + q * NU + r * LU + 32 * ks + 8 * g4);
-    };
-    const auto put3 = [&](uint16_t* to, int step, float x0, float x1, float x2, float x3) {
-        uint32_t a[2], d[2], e[2];
-        split3(x0, x1, a[0], d[0], e[0]);
-        split3(x2, x3, a[1], d[1], e[1]);
-        *reinterpret_cast<uint2*>(to) = make_uint2(a[0], a[1]);
-        *reinterpret_cast<uint2*>(to + step) = make_uint2(d[0], d[1]);
-        *reinterpret_cast<uint2*>(to + 2 * step) = make_uint2(e[0], e[1]);
-    };
-    Load x;
+    const int64_t unit_step = int64_t(p.Hv) * kUnitElems;
+    const uint16_t* const units = c.units + (int64_t(b) * c.count * p.Hv + h) * kUnitElems + 8 * lane;
 
-    if (!keeps) {  // rows of out
-        uint16_t* const out = p.out + b * p.o_batch + h * p.o_head + col0 + r;
-        constexpr std::false_type outs;
-        load_rows(x, 0, outs);
-        load_tri(x, 0, outs);
-        lds_barrier();
+    if (w >= 8) {  // the loads: a quarter of each chunk's
+        const int64_t kt_step = int64_t(p.Hk) * (DK * kChunk);
+        const int krow = tile_row(tile, r), vrow = 32 * (tile & 1) + (lane >> 1);
+        const uint16_t* unit = units;
+        const uint16_t* kt = c.kt + (int64_t(b) * c.count * p.Hk + hk) * (DK * kChunk) + 8 * lane;
+        const uint16_t* k = p.k.p + b * p.k.batch + hk * p.k.head + begin * p.k.tok + 8 * g4;
+        const uint16_t* v = p.v.p + b * p.v.batch + h * p.v.head + begin * p.v.tok + col0 + 8 * (lane & 1);
+        int64_t k_at = krow * p.k.tok, v_at = vrow * p.v.tok;
+        const auto stage = [&](int n) {
+            if (n >= chunks) return;
+            Stage& to = s_in[n & 1];
+            const int last = end - 1 - begin - n * kChunk;
+            if (last < kChunk - 1) k_at = min(krow, last) * p.k.tok, v_at = min(vrow, last) * p.v.tok;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) load_lds(k + k_at + 32 * ks, to.k + (tile * KS + ks) * 64);
+#pragma unroll
+            for (int i = 0; i < 5; ++i)
+                if (4 * i + tile < 3 * kTriFrags) load_lds(unit + kUnitT + (4 * i + tile) * kFrag, to.t + (4 * i + tile) * 64);
+#pragma unroll
+            for (int i = 0; i < DK / 32; ++i) load_lds(kt + (4 * i + tile) * kFrag, to.kt + (4 * i + tile) * 64);
+            if (tile < 2)
+                load_lds(v + v_at, to.v + tile * 32 * kScanCols);
+            else if (tile == 2)
+                load_lds(unit + kUnitVec, to.vec);
+            k += kChunk * p.k.tok, v += kChunk * p.v.tok, unit += unit_step, kt += kt_step;
+        };
+        stage(0);
+        __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+        lds_barrier();  // chunk 0 is there
+        stage(1);
         for (int n = 0; n < chunks; ++n) {
-            lds_barrier();
-            if (__builtin_amdgcn_readfirstlane(s_bad[n & 1]) != 0) {
-                load_rows(x, n + 1, outs);
-                load_tri(x, n + 1, outs);
+            lds_barrier();  // (1)
+            lds_barrier();  // (2)
+            __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);  // chunk n + 1 is there, for all after (3)
+            const bool slow = __builtin_amdgcn_readfirstlane(s_bad[n & 1]) != 0;
+            lds_barrier();  // (3)
+            if (slow) {
                 lds_barrier();
                 lds_barrier();
                 lds_barrier();
-                continue;
             }
-            f32x4_t a0 = zero, a1 = zero;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const uint4 s0 = s_part(ks, 0), s1 = s_part(ks, 1);
-                uint4 x0 = x.x[ks], x1;
-                if constexpr (F16) split_f16(x.x[ks], x0, x1);
-                a0 = mma(x0, s0, a0);
-                a1 = mma(x0, s1, a1);
-                if constexpr (F16) a1 = mma(x1, s0, a1);
-            }
-            a0 = (a0 + a1) * x.e;
-            a1 = zero;
-            load_rows(x, n + 1, outs);
-            lds_barrier();
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                if (ks > tile >> 1) continue;
-                const uint4 u0 = u_part(s_u, ks, 0), u1 = u_part(s_u, ks, 1);
-                a0 = mma(x.tri[ks][0], u0, a0);
-                a1 = mma(x.tri[ks][0], u1, a1);
-                a1 = mma(x.tri[ks][1], u0, a1);
-            }
-            a0 += a1;
-            load_tri(x, n + 1, outs);
-            const int t = begin + n * kChunk + 16 * tile + 4 * g4;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (t + i < end) out[(t + i) * p.o_tok] = uint16_t(Elem<F16>::pack_p(a0[i], 0.0f));
-            lds_barrier();
+            stage(n + 2);  // in chunk n's place: its last reads came before (3)
         }
         return;
     }
 
-    float* const st = p.state + ((int64_t(slot) * p.Hv + h) * DK + tile * (DK / 4)) * p.Dv + col0 + r;
-    f32x4_t s[MT];
-    const auto put_state = [&]() {
+    if (w >= 4) {  // rows of out
+        const int qrow = tile_row(tile, r);
+        const uint16_t* q = p.q.p + b * p.q.batch + hk * p.q.head + begin * p.q.tok + 8 * g4;
+        uint16_t* out = p.out + b * p.o_batch + h * p.o_head + (begin + tok0) * p.o_tok + col0 + r;
+        const uint16_t* unit = units + kUnitP;
+        const int tri0 = tri_frag(tile, 0) * kFrag, tri1 = tri_frag(tile, tile >> 1) * kFrag;
+        int64_t q_at = qrow * p.q.tok;
+        uint4 fq[KS], tri[2][2];
+        f32x4_t e;
+        const auto load_rows = [&](int n) {
+            const int last = end - 1 - begin - n * kChunk;
+            if (last < 0) return;
+            if (last < kChunk - 1) q_at = min(qrow, last) * p.q.tok;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-            put3(s_s + r * LS + tile * (DK / 4) + 16 * m + 4 * g4, NS, s[m][0], s[m][1], s[m][2], s[m][3]);
+            for (int ks = 0; ks < KS; ++ks) fq[ks] = *reinterpret_cast<const uint4*>(q + q_at + 32 * ks);
+            q += kChunk * p.q.tok;
+        };
+        const auto load_tri = [&](int n) {
+            if (n >= chunks) return;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                tri[0][i] = *reinterpret_cast<const uint4*>(unit + i * kTPart + tri0);
+                tri[1][i] = *reinterpret_cast<const uint4*>(unit + i * kTPart + tri1);
+            }
+            unit += unit_step;
+        };
+        load_rows(0);
+        load_tri(0);
+        lds_barrier();  // chunk 0 is there
+        for (int n = 0; n < chunks; ++n) {
+            lds_barrier();  // (1)
+            e = *reinterpret_cast<const f32x4_t*>(s_in[n & 1].vec + kVecE + tok0);
+            f32x4_t a0 = zero, a1 = zero;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const uint4 s0 = s_s[ks * 64 + lane], s1 = s_s[(KS + ks) * 64 + lane];
+                uint4 x0 = fq[ks], x1;
+                if constexpr (F16) split_f16(fq[ks], x0, x1);
+                a0 = mma(x0, s0, a0);
+                a1 = mma(x0, s1, a1);
+                if constexpr (F16) a1 = mma(x1, s0, a1);
+            }
+            a0 = (a0 + a1) * e;
+            a1 = zero;
+            lds_barrier();  // (2)
+            const int slow_word = s_bad[n & 1];
+            load_rows(n + 1);
+            const bool slow = __builtin_amdgcn_readfirstlane(slow_word) != 0;
+            lds_barrier();  // (3)
+            if (slow) {
+                lds_barrier();
+                lds_barrier();
+                lds_barrier();
+            } else {
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    if (ks > tile >> 1) continue;
+                    const uint4 u0 = s_u[ks * 64 + lane], u1 = s_u[(2 + ks) * 64 + lane];
+                    a0 = mma(tri[ks][0], u0, a0);
+                    a1 = mma(tri[ks][0], u1, a1);
+                    a1 = mma(tri[ks][1], u0, a1);
+                }
+                a0 += a1;
+                const int left = end - begin - n * kChunk - tok0;
+                uint16_t* to = out;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (i < left) *to = uint16_t(Elem<F16>::pack_p(a0[i], 0.0f));
+                    to += p.o_tok;
+                }
+            }
+            load_tri(n + 1);
+            out += kChunk * p.o_tok;
+        }
+        return;
+    }
+
+    const int row0 = tile_row(MT * w, 4 * g4);  // the lane's first row of the state; tile m: + 4 m
+    float* const st = p.state + ((int64_t(slot) * p.Hv + h) * DK + row0) * p.Dv + col0 + r;
+    f32x4_t s[MT];
+    Op fk[4];  // K: the tokens of tile j, the lane's rows of the state
+    const auto put3 = [&](uint2* to, float x0, float x1, float x2, float x3) {
+        uint32_t a[2], d[2], e[2];
+        split3(x0, x1, a[0], d[0], e[0]);
+        split3(x2, x3, a[1], d[1], e[1]);
+        to[0] = make_uint2(a[0], a[1]);
+        to[kPart] = make_uint2(d[0], d[1]);
+        to[2 * kPart] = make_uint2(e[0], e[1]);
     };
-    constexpr std::true_type keep;
+    const auto load_k = [&](const Stage& in) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (MT == 2) {
+                const uint4 x = in.k[(j * KS + w) * 64 + lane];
+                fk[j].w[0] = x.x, fk[j].w[1] = x.y, fk[j].w[2] = x.z, fk[j].w[3] = x.w;
+            } else {
+                const uint2 x = reinterpret_cast<const uint2*>(in.k)[2 * ((j * KS + (w >> 1)) * 64 + lane) + (w & 1)];
+                fk[j].w[0] = x.x, fk[j].w[1] = x.y;
+            }
+        }
+    };
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[m][i] = st[int64_t(16 * m + 4 * g4 + i) * p.Dv];
-    put_state();
+        for (int i = 0; i < 4; ++i) s[m][i] = st[int64_t(4 * m + i) * p.Dv];
     if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
-    load_rows(x, 0, keep);
-    load_tri(x, 0, keep);
-    load_kt(x, 0);
     lds_barrier();
+    load_k(s_in[0]);
     for (int n = 0; n < chunks; ++n) {
-        {  // (1) rows of Y
+        const Stage& in = s_in[n & 1];
+        uint4 ft[2][3];
+        float v[4];
+        f32x4_t e;
+        {  // (1)
+            Op s0, s1, s2;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                split3(s[m][0], s[m][1], s0.w[2 * m], s1.w[2 * m], s2.w[2 * m]);
+                split3(s[m][2], s[m][3], s0.w[2 * m + 1], s1.w[2 * m + 1], s2.w[2 * m + 1]);
+            }
+            f32x4_t x[4];
+            Op k0[4], k1[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                k0[j] = fk[j];
+                if constexpr (F16) split_f16(fk[j], k0[j], k1[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = mma_step(k0[j], s2, zero);
+            if constexpr (F16)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = mma_step(k1[j], s1, x[j]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = mma_step(k0[j], s1, x[j]);
+            if constexpr (F16)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = mma_step(k1[j], s0, x[j]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = mma_step(k0[j], s0, x[j]);
+            if constexpr (MT == 2) {
+                s_s[w * 64 + lane] = make_uint4(s0.w[0], s0.w[1], s0.w[2], s0.w[3]);
+                s_s[(KS + w) * 64 + lane] = make_uint4(s1.w[0], s1.w[1], s1.w[2], s1.w[3]);
+            } else {
+                uint2* const to = reinterpret_cast<uint2*>(s_s) + 2 * ((w >> 1) * 64 + lane) + (w & 1);
+                to[0] = make_uint2(s0.w[0], s0.w[1]);
+                to[2 * KS * 64] = make_uint2(s1.w[0], s1.w[1]);
+            }
+            e = *reinterpret_cast<const f32x4_t*>(in.vec + kVecC + tok0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = Elem<F16>::lo(in.v[(tok0 + i) * kScanCols + r]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s_x[(w * 4 + j) * 64 + lane] = x[j];
+        }
+        lds_barrier();  // (1)
+        uint4 fkt[2 * MT];
+        f32x4_t d;
+        float last;
+        {  // (2)
+            const f32x4_t x0 = s_x[tile * 64 + lane], x1 = s_x[(4 + tile) * 64 + lane], x2 = s_x[(8 + tile) * 64 + lane],
+                          x3 = s_x[(12 + tile) * 64 + lane];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                ft[0][i] = in.t[(i * kTriFrags + tri_frag(tile, 0)) * 64 + lane];
+                ft[1][i] = in.t[(i * kTriFrags + tri_frag(tile, tile >> 1)) * 64 + lane];
+            }
+            const float bad = in.vec[kVecBad];
+            const f32x4_t z = (x0 + x1) + (x2 + x3);
+            float y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = v[i] - e[i] * z[i];
+            put3(reinterpret_cast<uint2*>(s_y) + half, y[0], y[1], y[2], y[3]);
+            // an overflow of this sum only means more care
+            if (!((fabsf(y[0]) + fabsf(y[1])) + (fabsf(y[2]) + fabsf(y[3])) < INFINITY) || bad != 0.0f) s_bad[n & 1] = 1;
+        }
+        lds_barrier();  // (2)
+        const int slow_word = s_bad[n & 1];
+        {  // (3)
             f32x4_t a0 = zero, a1 = zero, a2 = zero;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const uint4 s0 = s_part(ks, 0), s1 = s_part(ks, 1), s2 = s_part(ks, 2);
-                uint4 x0 = x.x[ks], x1;
-                if constexpr (F16) split_f16(x.x[ks], x0, x1);
-                a0 = mma(x0, s0, a0);
-                a1 = mma(x0, s1, a1);
-                a2 = mma(x0, s2, a2);
-                if constexpr (F16) a1 = mma(x1, s0, a1), a2 = mma(x1, s1, a2);
+            for (int ks = 0; ks < 2; ++ks) {
+                if (ks > tile >> 1) continue;
+                const uint4 y0 = s_y[ks * 64 + lane], y1 = s_y[(2 + ks) * 64 + lane], y2 = s_y[(4 + ks) * 64 + lane];
+                a2 = mma(ft[ks][0], y2, a2);
+                a1 = mma(ft[ks][0], y1, a1);
+                a0 = mma(ft[ks][0], y0, a0);
+                a2 = mma(ft[ks][1], y1, a2);
+                a1 = mma(ft[ks][1], y0, a1);
+                a2 = mma(ft[ks][2], y0, a2);
             }
-            const f32x4_t z = a0 + (a1 + a2);
-            const int t = begin + n * kChunk + 16 * tile + 4 * g4;
-            float y[4];
-            bool odd = x.bad != 0.0f;
+            d = *reinterpret_cast<const f32x4_t*>(in.vec + kVecD + tok0);
+            last = in.vec[kVecLast];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                y[i] = t + i < end ? Elem<F16>::lo(x.v[i]) - x.e[i] * z[i] : 0.0f;
-                odd |= !(fabsf(y[i]) < INFINITY);
-            }
-            put3(s_y + r * LU + 16 * tile + 4 * g4, NU, y[0], y[1], y[2], y[3]);
-            if (odd) s_bad[n & 1] = 1;
-            load_rows(x, n + 1, keep);
+            for (int i = 0; i < 2 * MT; ++i) fkt[i] = in.kt[(2 * MT * w + i) * 64 + lane];
+            const f32x4_t u = a0 + (a1 + a2);
+            put3(reinterpret_cast<uint2*>(s_d) + half, d[0] * u[0], d[1] * u[1], d[2] * u[2], d[3] * u[3]);
+            uint32_t a[2], g[2];
+            split2(u[0], u[1], a[0], g[0]);
+            split2(u[2], u[3], a[1], g[1]);
+            uint2* const to = reinterpret_cast<uint2*>(s_u) + half;
+            to[0] = make_uint2(a[0], a[1]);
+            to[kPart] = make_uint2(g[0], g[1]);
         }
-        lds_barrier();
-        const bool slow = __builtin_amdgcn_readfirstlane(s_bad[n & 1]) != 0;
-        if (threadIdx.x == 0) s_bad[(n + 1) & 1] = 0;  // read last a chunk ago, set next after more barriers
+        const bool slow = __builtin_amdgcn_readfirstlane(slow_word) != 0;
+        lds_barrier();  // (3)
+        if (threadIdx.x == 0) s_bad[(n + 1) & 1] = 0;  // read last a chunk ago, set next after (1)
         if (slow) {
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s_w[(tile * (DK / 4) + 16 * m + 4 * g4 + i) * LW + r] = s[m][i];
+                for (int i = 0; i < 4; ++i) s_w[(row0 + 4 * m + i) * LW + r] = s[m][i];
             lds_barrier();
             if (w == 0) {
                 constexpr int NR = DK / 16;
@@ -677,61 +819,37 @@ __global__ __launch_bounds__(512) void delta_chunk_scan_kernel(DeltaParams p, Ch
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[m][i] = s_w[(tile * (DK / 4) + 16 * m + 4 * g4 + i) * LW + r];
-            put_state();
-            load_tri(x, n + 1, keep);
-            load_kt(x, n + 1);
-            lds_barrier();
+                for (int i = 0; i < 4; ++i) s[m][i] = s_w[(row0 + 4 * m + i) * LW + r];
+            lds_barrier();  // before (1) writes over it
+            if (n + 1 < chunks) load_k(s_in[(n + 1) & 1]);
             continue;
         }
-        {  // (2) rows of U
-            f32x4_t a0 = zero, a1 = zero, a2 = zero;
+        // (4)
+        uint4 dp[2][3];
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                if (ks > tile >> 1) continue;
-                const uint4 y0 = u_part(s_y, ks, 0), y1 = u_part(s_y, ks, 1), y2 = u_part(s_y, ks, 2);
-                a0 = mma(x.tri[ks][0], y0, a0);
-                a1 = mma(x.tri[ks][0], y1, a1);
-                a2 = mma(x.tri[ks][0], y2, a2);
-                a1 = mma(x.tri[ks][1], y0, a1);
-                a2 = mma(x.tri[ks][1], y1, a2);
-                a2 = mma(x.tri[ks][2], y0, a2);
-            }
-            const f32x4_t u = a0 + (a1 + a2);
-            put3(s_d + r * LU + 16 * tile + 4 * g4, NU, x.d[0] * u[0], x.d[1] * u[1], x.d[2] * u[2], x.d[3] * u[3]);
-            uint32_t a[2], d[2];
-            split2(u[0], u[1], a[0], d[0]);
-            split2(u[2], u[3], a[1], d[1]);
-            uint16_t* const to = s_u + r * LU + 16 * tile + 4 * g4;
-            *reinterpret_cast<uint2*>(to) = make_uint2(a[0], a[1]);
-            *reinterpret_cast<uint2*>(to + NU) = make_uint2(d[0], d[1]);
-            load_tri(x, n + 1, keep);
-        }
-        lds_barrier();
-        // (3) rows of the new state
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < 3; ++i) dp[ks][i] = s_d[(2 * i + ks) * 64 + lane];
+        if (n + 1 < chunks) load_k(s_in[(n + 1) & 1]);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            f32x4_t a0 = s[m] * x.last, a1 = zero, a2 = zero;
+            f32x4_t a0 = s[m] * last, a1 = zero, a2 = zero;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-                const uint4 d0 = u_part(s_d, ks, 0), d1 = u_part(s_d, ks, 1), d2 = u_part(s_d, ks, 2);
-                uint4 k0 = x.kt[2 * m + ks], k1;
-                if constexpr (F16) split_f16(x.kt[2 * m + ks], k0, k1);
-                a0 = mma(k0, d0, a0);
-                a1 = mma(k0, d1, a1);
-                a2 = mma(k0, d2, a2);
-                if constexpr (F16) a1 = mma(k1, d0, a1), a2 = mma(k1, d1, a2);
+                uint4 k0 = fkt[2 * m + ks], k1;
+                if constexpr (F16) split_f16(fkt[2 * m + ks], k0, k1);
+                a2 = mma(k0, dp[ks][2], a2);
+                a1 = mma(k0, dp[ks][1], a1);
+                a0 = mma(k0, dp[ks][0], a0);
+                if constexpr (F16) a2 = mma(k1, dp[ks][1], a2), a1 = mma(k1, dp[ks][0], a1);
             }
             s[m] = a0 + (a1 + a2);
         }
-        load_kt(x, n + 1);
-        put_state();
-        lds_barrier();
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) st[int64_t(16 * m + 4 * g4 + i) * p.Dv] = s[m][i];
+        for (int i = 0; i < 4; ++i) st[int64_t(4 * m + i) * p.Dv] = s[m][i];
 }
 
 // Chunks of one pair of launches: their units stay near 128 MB, within the
@@ -759,7 +877,7 @@ int launch_chunks(const DeltaParams& p, void* ws, hipStream_t stream) {
         c.first = int32_t(first), c.count = int32_t(std::min(per, all - first));
         hipLaunchKernelGGL(prepare, dim3(unsigned(int64_t(p.B) * c.count * p.Hv)), dim3(256), 0, stream, p, c);
         GENLLM_LAUNCH_CHECK("delta_chunk_prepare_kernel");
-        hipLaunchKernelGGL(scan, dim3(unsigned(p.B * p.Hv * (p.Dv / kScanCols))), dim3(512), 0, stream, p, c);
+        hipLaunchKernelGGL(scan, dim3(unsigned(p.B * p.Hv * (p.Dv / kScanCols))), dim3(kScanThreads), 0, stream, p, c);
         GENLLM_LAUNCH_CHECK("delta_chunk_scan_kernel");
     }
     return GENLLM_OK;
