@@ -494,6 +494,17 @@ __device__ __forceinline__ void split_f16(const Operand<MT>& x, Operand<MT>& a, 
     for (int i = 0; i < 2 * MT; ++i) split2(Elem<true>::lo(x.w[i]), Elem<true>::hi(x.w[i]), a.w[i], b.w[i]);
 }
 
+// The kernel's first argument, read again where it is used: a rare path then
+// keeps none of it in registers through the loop around it.
+__device__ __forceinline__ DeltaParams kernel_params() {
+    typedef const __attribute__((address_space(4))) void kernarg;
+    kernarg* a = (kernarg*)__builtin_amdgcn_kernarg_segment_ptr();
+    __asm__ volatile("" : "+s"(a));
+    DeltaParams p;
+    __builtin_memcpy(&p, (const void*)a, sizeof(p));
+    return p;
+}
+
 // 16 columns of one head's state from chunk to chunk, in twelve waves.  Waves 0
 // to 3 keep the state: wave w its rows of the tiles MT w .. in fp32, as the
 // products leave them, which is also how the next product takes them.  Per chunk:
@@ -523,7 +534,7 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
     __shared__ uint4 s_y[3 * 2 * 64];       // Y in three parts [part][step][lane], a tile's half of each
     __shared__ uint4 s_d[3 * 2 * 64];       // diag(e^(G_last - G)) U in three parts
     __shared__ uint4 s_u[2 * 2 * 64];       // U in two
-    __shared__ int s_bad[2];
+    __shared__ int s_bad;                   // the last chunk that has to run token by token, from 1
     float* const s_w = reinterpret_cast<float*>(s_x);  // the state of a chunk that runs token by token
     static_assert(DK * LW * sizeof(float) <= sizeof(s_x), "s_w lies in s_x");
     const int heads = p.B * p.Hv;
@@ -582,7 +593,8 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
             lds_barrier();  // (1)
             lds_barrier();  // (2)
             __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);  // chunk n + 1 is there, for all after (3)
-            const bool slow = __builtin_amdgcn_readfirstlane(s_bad[n & 1]) != 0;
+            const int slow_word = s_bad;
+            const bool slow = __builtin_amdgcn_readfirstlane(slow_word) == n + 1;
             lds_barrier();  // (3)
             if (slow) {
                 lds_barrier();
@@ -639,9 +651,9 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
             a0 = (a0 + a1) * e;
             a1 = zero;
             lds_barrier();  // (2)
-            const int slow_word = s_bad[n & 1];
+            const int slow_word = s_bad;
             load_rows(n + 1);
-            const bool slow = __builtin_amdgcn_readfirstlane(slow_word) != 0;
+            const bool slow = __builtin_amdgcn_readfirstlane(slow_word) == n + 1;
             lds_barrier();  // (3)
             if (slow) {
                 lds_barrier();
@@ -674,7 +686,6 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
     const int row0 = tile_row(MT * w, 4 * g4);  // the lane's first row of the state; tile m: + 4 m
     float* const st = p.state + ((int64_t(slot) * p.Hv + h) * DK + row0) * p.Dv + col0 + r;
     f32x4_t s[MT];
-    Op fk[4];  // K: the tokens of tile j, the lane's rows of the state
     const auto put3 = [&](uint2* to, float x0, float x1, float x2, float x3) {
         uint32_t a[2], d[2], e[2];
         split3(x0, x1, a[0], d[0], e[0]);
@@ -683,7 +694,8 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
         to[kPart] = make_uint2(d[0], d[1]);
         to[2 * kPart] = make_uint2(e[0], e[1]);
     };
-    const auto load_k = [&](const Stage& in) {
+    // K: the tokens of tile j, the lane's rows of the state
+    const auto load_k = [&](const Stage& in, Op (&fk)[4]) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if constexpr (MT == 2) {
@@ -699,15 +711,24 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[m][i] = st[int64_t(4 * m + i) * p.Dv];
-    if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
+    if (threadIdx.x == 0) s_bad = 0;
     lds_barrier();
-    load_k(s_in[0]);
     for (int n = 0; n < chunks; ++n) {
         const Stage& in = s_in[n & 1];
         uint4 ft[2][3];
-        float v[4];
+        uint16_t v[4];
         f32x4_t e;
         {  // (1)
+            Op fk[4];
+            load_k(in, fk);
+            e = *reinterpret_cast<const f32x4_t*>(in.vec + kVecC + tok0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = in.v[(tok0 + i) * kScanCols + r];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                ft[0][i] = in.t[(i * kTriFrags + tri_frag(tile, 0)) * 64 + lane];
+                ft[1][i] = in.t[(i * kTriFrags + tri_frag(tile, tile >> 1)) * 64 + lane];
+            }
             Op s0, s1, s2;
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
@@ -741,36 +762,30 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
                 to[0] = make_uint2(s0.w[0], s0.w[1]);
                 to[2 * KS * 64] = make_uint2(s1.w[0], s1.w[1]);
             }
-            e = *reinterpret_cast<const f32x4_t*>(in.vec + kVecC + tok0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = Elem<F16>::lo(in.v[(tok0 + i) * kScanCols + r]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) s_x[(w * 4 + j) * 64 + lane] = x[j];
         }
         lds_barrier();  // (1)
         uint4 fkt[2 * MT];
-        f32x4_t d;
-        float last;
+        const f32x4_t d = *reinterpret_cast<const f32x4_t*>(in.vec + kVecD + tok0);
+        const float last = in.vec[kVecLast];
         {  // (2)
             const f32x4_t x0 = s_x[tile * 64 + lane], x1 = s_x[(4 + tile) * 64 + lane], x2 = s_x[(8 + tile) * 64 + lane],
                           x3 = s_x[(12 + tile) * 64 + lane];
-#pragma unroll
-            for (int i = 0; i < 3; ++i) {
-                ft[0][i] = in.t[(i * kTriFrags + tri_frag(tile, 0)) * 64 + lane];
-                ft[1][i] = in.t[(i * kTriFrags + tri_frag(tile, tile >> 1)) * 64 + lane];
-            }
             const float bad = in.vec[kVecBad];
             const f32x4_t z = (x0 + x1) + (x2 + x3);
             float y[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = v[i] - e[i] * z[i];
+            for (int i = 0; i < 4; ++i) y[i] = Elem<F16>::lo(v[i]) - e[i] * z[i];
             put3(reinterpret_cast<uint2*>(s_y) + half, y[0], y[1], y[2], y[3]);
             // an overflow of this sum only means more care
-            if (!((fabsf(y[0]) + fabsf(y[1])) + (fabsf(y[2]) + fabsf(y[3])) < INFINITY) || bad != 0.0f) s_bad[n & 1] = 1;
+            if (!((fabsf(y[0]) + fabsf(y[1])) + (fabsf(y[2]) + fabsf(y[3])) < INFINITY) || bad != 0.0f) s_bad = n + 1;
         }
         lds_barrier();  // (2)
-        const int slow_word = s_bad[n & 1];
+        const int slow_word = s_bad;
         {  // (3)
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i) fkt[i] = in.kt[(2 * MT * w + i) * 64 + lane];
             f32x4_t a0 = zero, a1 = zero, a2 = zero;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
@@ -783,10 +798,6 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
                 a1 = mma(ft[ks][1], y0, a1);
                 a2 = mma(ft[ks][2], y0, a2);
             }
-            d = *reinterpret_cast<const f32x4_t*>(in.vec + kVecD + tok0);
-            last = in.vec[kVecLast];
-#pragma unroll
-            for (int i = 0; i < 2 * MT; ++i) fkt[i] = in.kt[(2 * MT * w + i) * 64 + lane];
             const f32x4_t u = a0 + (a1 + a2);
             put3(reinterpret_cast<uint2*>(s_d) + half, d[0] * u[0], d[1] * u[1], d[2] * u[2], d[3] * u[3]);
             uint32_t a[2], g[2];
@@ -796,9 +807,8 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
             to[0] = make_uint2(a[0], a[1]);
             to[kPart] = make_uint2(g[0], g[1]);
         }
-        const bool slow = __builtin_amdgcn_readfirstlane(slow_word) != 0;
+        const bool slow = __builtin_amdgcn_readfirstlane(slow_word) == n + 1;
         lds_barrier();  // (3)
-        if (threadIdx.x == 0) s_bad[(n + 1) & 1] = 0;  // read last a chunk ago, set next after (1)
         if (slow) {
 #pragma unroll
             for (int m = 0; m < MT; ++m)
@@ -811,7 +821,7 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
                 f32x4_t sr[NR];
 #pragma unroll
                 for (int i = 0; i < NR; ++i) sr[i] = *reinterpret_cast<const f32x4_t*>(s_w + (lane / 4 * NR + i) * LW + 4 * (lane & 3));
-                recur<DK, 4, F16>(p, sr, b, h, col0 + 4 * (lane & 3), t0, min(end, t0 + kChunk));
+                recur<DK, 4, F16>(kernel_params(), sr, b, h, col0 + 4 * (lane & 3), t0, min(end, t0 + kChunk));
 #pragma unroll
                 for (int i = 0; i < NR; ++i) *reinterpret_cast<f32x4_t*>(s_w + (lane / 4 * NR + i) * LW + 4 * (lane & 3)) = sr[i];
             }
@@ -821,7 +831,6 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[m][i] = s_w[(row0 + 4 * m + i) * LW + r];
             lds_barrier();  // before (1) writes over it
-            if (n + 1 < chunks) load_k(s_in[(n + 1) & 1]);
             continue;
         }
         // (4)
@@ -830,7 +839,6 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int i = 0; i < 3; ++i) dp[ks][i] = s_d[(2 * i + ks) * 64 + lane];
-        if (n + 1 < chunks) load_k(s_in[(n + 1) & 1]);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             f32x4_t a0 = s[m] * last, a1 = zero, a2 = zero;
