@@ -224,7 +224,6 @@ __device__ __forceinline__ constexpr int tile_row(int t, int rho) {
 
 struct ChunkPlan {
     uint16_t* units = nullptr;  // [batch][chunk][Hv][kUnitElems]
-    uint16_t* kt = nullptr;     // [batch][chunk][Hk][Dk / 16][2] fragments of K^T
     int32_t first = 0, count = 0;  // chunks of this launch
 };
 
@@ -281,6 +280,15 @@ __device__ __forceinline__ void load_lds(const void* from, void* to) {
                                      (__attribute__((address_space(3))) uint32_t*)to, 16, 0, 0);
 }
 
+__device__ __forceinline__ uint2 read_transposed(const uint2* p) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)p));
+}
+// Place of row r, elements 8 g .. + 7 of a 16 x 32 block: rows of four units, so that
+// four lanes of a load cover 64 bytes (16 rows at once took four times the cache
+// accesses), rotated so that neither 16 rows of one g nor 4 rows of all g meet in
+// an LDS bank.
+__device__ __forceinline__ constexpr int row_unit(int r, int g) { return 4 * r + (g ^ (r >> 2)); }
+
 // Four waves per chunk and value head; wave w has row tile w of the 64 x 64
 // matrices.  (1 + L)^-1 by halves: the four diagonal 16 x 16 blocks by
 // substitution, a lane per column; then T10 = -T11 (L10 T00) for 16- and for
@@ -291,6 +299,8 @@ __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p,
     __shared__ __attribute__((aligned(16))) float s_l[64 * LD];   // L, then the products M in its upper blocks
     __shared__ __attribute__((aligned(16))) float s_t[64 * LD];   // P, then the inverse
     __shared__ __attribute__((aligned(16))) uint16_t s_k[64 * LK];
+    uint16_t* const s_q = reinterpret_cast<uint16_t*>(s_t);  // until P
+    static_assert(sizeof(uint16_t) * 64 * LK <= sizeof(s_t), "s_q lies in s_t");
     __shared__ double s_g[64];
     __shared__ float s_beta[64], s_rk[64], s_rq[64];
     const int h = int(blockIdx.x % uint32_t(p.Hv)), rest = int(blockIdx.x / uint32_t(p.Hv));
@@ -301,20 +311,32 @@ __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p,
     const int left = len - t0;  // tokens of this chunk and behind it
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g4 = lane >> 4;
     const int hk = h / p.G;
-    const bool writes_kt = h % p.G == 0;
     uint16_t* const unit = c.units + ((int64_t(b) * c.count + n) * p.Hv + h) * kUnitElems;
     float* const vec = reinterpret_cast<float*>(unit + kUnitVec);
 
-    // rows of K and Q of tile w; rows behind the end are zeros
+    // rows of K and Q of tile w through LDS, four lanes to 64 bytes of a row; rows
+    // behind the end are zeros
     uint4 own[KS], qf[KS];
-    const uint16_t* const kp = p.k.p + b * p.k.batch + hk * p.k.head + 8 * g4;
-    const uint16_t* const qp = p.q.p + b * p.q.batch + hk * p.q.head + 8 * g4;
+    {
+        const int row = 16 * w + (lane >> 2), at = 8 * (lane & 3);
+        const bool there = row < left;
+        const uint16_t* const kp = p.k.p + b * p.k.batch + hk * p.k.head + (t0 + row) * p.k.tok + at;
+        const uint16_t* const qp = p.q.p + b * p.q.batch + hk * p.q.head + (t0 + row) * p.q.tok + at;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-        own[ks] = qf[ks] = make_uint4(0, 0, 0, 0);
-        if (16 * w + r < left) {
-            own[ks] = *reinterpret_cast<const uint4*>(kp + (t0 + 16 * w + r) * p.k.tok + 32 * ks);
-            qf[ks] = *reinterpret_cast<const uint4*>(qp + (t0 + 16 * w + r) * p.q.tok + 32 * ks);
+        for (int ks = 0; ks < KS; ++ks) {
+            own[ks] = qf[ks] = make_uint4(0, 0, 0, 0);
+            if (there) own[ks] = *reinterpret_cast<const uint4*>(kp + 32 * ks), qf[ks] = *reinterpret_cast<const uint4*>(qp + 32 * ks);
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            *reinterpret_cast<uint4*>(s_k + row * LK + 32 * ks + at) = own[ks];
+            *reinterpret_cast<uint4*>(s_q + row * LK + 32 * ks + at) = qf[ks];
+        }
+        // a wave reads back its own rows
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            own[ks] = *reinterpret_cast<const uint4*>(s_k + (16 * w + r) * LK + 32 * ks + 8 * g4);
+            qf[ks] = *reinterpret_cast<const uint4*>(s_q + (16 * w + r) * LK + 32 * ks + 8 * g4);
         }
     }
     // gates of token `lane`, the running sum in 64 bits (differences of far sums
@@ -340,7 +362,6 @@ __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p,
             qq = __builtin_fmaf(Elem<F16>::lo(d[i]), Elem<F16>::lo(d[i]), qq);
             qq = __builtin_fmaf(Elem<F16>::hi(d[i]), Elem<F16>::hi(d[i]), qq);
         }
-        *reinterpret_cast<uint4*>(s_k + (16 * w + r) * LK + 32 * ks + 8 * g4) = own[ks];
     }
     kk += __shfl_xor(kk, 16);
     qq += __shfl_xor(qq, 16);
@@ -380,7 +401,7 @@ __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p,
     }
     __syncthreads();
 
-    // P's fragments of row tile w, the vectors, K^T
+    // P's fragments of row tile w and the vectors
     for (int ks = 0; ks <= w >> 1; ++ks) {
         const int row = tile_row(w, r), col = 32 * ks + 8 * g4;
         const float* const src = s_t + row * LD + col;
@@ -398,19 +419,6 @@ __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p,
         vec[kVecD + lane] = s_rk[lane] * expf(float(last - s_g[lane]));
         vec[kVecE + lane] = s_rq[lane] * expf(float(s_g[lane]));
         if (lane == 0) vec[kVecLast] = expf(float(last)), vec[kVecBad] = bad ? 1.0f : 0.0f;
-    }
-    if (writes_kt) {
-        uint16_t* const kt = c.kt + ((int64_t(b) * c.count + n) * p.Hk + hk) * (DK * kChunk);
-#pragma unroll
-        for (int m = w; m < DK / 16; m += 4)
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                const uint16_t* const src = s_k + (32 * ks + 8 * g4) * LK + tile_row(m, r);
-                uint32_t a[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = pack2(src[2 * i * LK], src[(2 * i + 1) * LK]);
-                *reinterpret_cast<uint4*>(kt + (2 * m + ks) * kFrag + 8 * lane) = make_uint4(a[0], a[1], a[2], a[3]);
-            }
     }
     // the inverse of diagonal block w: column r in every lane group, by substitution
     float x[16];
@@ -522,9 +530,9 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
     constexpr int LW = 20;
     using Op = Operand<MT>;
     struct Stage {
-        uint4 k[4 * KS * 64];                      // [token tile][step][lane]
+        uint4 k[4 * KS * 64];                      // [token tile][step][row_unit]
+        uint4 q[4 * KS * 64];
         uint4 t[3 * kTriFrags * 64];               // [part][fragment][lane]
-        uint4 kt[DK / 16 * 2 * 64];                // [state tile][step][lane]
         uint16_t v[kChunk * kScanCols];
         float vec[kVecFloats];
     };
@@ -556,34 +564,36 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
     const int half = 2 * ((tile >> 1) * 64 + lane) + (tile & 1);  // the lane's half of an operand, in uint2
     constexpr int kPart = 2 * 2 * 64;                             // uint2 per part of s_y, s_d, s_u
 
+    const int unit_at = row_unit(r, g4);  // the lane's operand in K and Q
     const int64_t unit_step = int64_t(p.Hv) * kUnitElems;
     const uint16_t* const units = c.units + (int64_t(b) * c.count * p.Hv + h) * kUnitElems + 8 * lane;
 
     if (w >= 8) {  // the loads: a quarter of each chunk's
-        const int64_t kt_step = int64_t(p.Hk) * (DK * kChunk);
-        const int krow = tile_row(tile, r), vrow = 32 * (tile & 1) + (lane >> 1);
+        // lane l of a load takes unit l of its fragment: four lanes cover 64 bytes of a row
+        const int krow = tile_row(tile, lane >> 2), vrow = 32 * (tile & 1) + (lane >> 1), chunk = (lane & 3) ^ (lane >> 4);
         const uint16_t* unit = units;
-        const uint16_t* kt = c.kt + (int64_t(b) * c.count * p.Hk + hk) * (DK * kChunk) + 8 * lane;
-        const uint16_t* k = p.k.p + b * p.k.batch + hk * p.k.head + begin * p.k.tok + 8 * g4;
+        const uint16_t* k = p.k.p + b * p.k.batch + hk * p.k.head + begin * p.k.tok + 8 * chunk;
+        const uint16_t* q = p.q.p + b * p.q.batch + hk * p.q.head + begin * p.q.tok + 8 * chunk;
         const uint16_t* v = p.v.p + b * p.v.batch + h * p.v.head + begin * p.v.tok + col0 + 8 * (lane & 1);
-        int64_t k_at = krow * p.k.tok, v_at = vrow * p.v.tok;
+        int64_t k_at = krow * p.k.tok, q_at = krow * p.q.tok, v_at = vrow * p.v.tok;
         const auto stage = [&](int n) {
             if (n >= chunks) return;
             Stage& to = s_in[n & 1];
             const int last = end - 1 - begin - n * kChunk;
-            if (last < kChunk - 1) k_at = min(krow, last) * p.k.tok, v_at = min(vrow, last) * p.v.tok;
+            if (last < kChunk - 1)
+                k_at = min(krow, last) * p.k.tok, q_at = min(krow, last) * p.q.tok, v_at = min(vrow, last) * p.v.tok;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) load_lds(k + k_at + 32 * ks, to.k + (tile * KS + ks) * 64);
 #pragma unroll
             for (int i = 0; i < 5; ++i)
                 if (4 * i + tile < 3 * kTriFrags) load_lds(unit + kUnitT + (4 * i + tile) * kFrag, to.t + (4 * i + tile) * 64);
-#pragma unroll
-            for (int i = 0; i < DK / 32; ++i) load_lds(kt + (4 * i + tile) * kFrag, to.kt + (4 * i + tile) * 64);
             if (tile < 2)
                 load_lds(v + v_at, to.v + tile * 32 * kScanCols);
             else if (tile == 2)
                 load_lds(unit + kUnitVec, to.vec);
-            k += kChunk * p.k.tok, v += kChunk * p.v.tok, unit += unit_step, kt += kt_step;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) load_lds(q + q_at + 32 * ks, to.q + (tile * KS + ks) * 64);
+            k += kChunk * p.k.tok, q += kChunk * p.q.tok, v += kChunk * p.v.tok, unit += unit_step;
         };
         stage(0);
         __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
@@ -607,22 +617,11 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
     }
 
     if (w >= 4) {  // rows of out
-        const int qrow = tile_row(tile, r);
-        const uint16_t* q = p.q.p + b * p.q.batch + hk * p.q.head + begin * p.q.tok + 8 * g4;
         uint16_t* out = p.out + b * p.o_batch + h * p.o_head + (begin + tok0) * p.o_tok + col0 + r;
         const uint16_t* unit = units + kUnitP;
         const int tri0 = tri_frag(tile, 0) * kFrag, tri1 = tri_frag(tile, tile >> 1) * kFrag;
-        int64_t q_at = qrow * p.q.tok;
-        uint4 fq[KS], tri[2][2];
+        uint4 tri[2][2];
         f32x4_t e;
-        const auto load_rows = [&](int n) {
-            const int last = end - 1 - begin - n * kChunk;
-            if (last < 0) return;
-            if (last < kChunk - 1) q_at = min(qrow, last) * p.q.tok;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) fq[ks] = *reinterpret_cast<const uint4*>(q + q_at + 32 * ks);
-            q += kChunk * p.q.tok;
-        };
         const auto load_tri = [&](int n) {
             if (n >= chunks) return;
 #pragma unroll
@@ -632,7 +631,6 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
             }
             unit += unit_step;
         };
-        load_rows(0);
         load_tri(0);
         lds_barrier();  // chunk 0 is there
         for (int n = 0; n < chunks; ++n) {
@@ -642,8 +640,8 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const uint4 s0 = s_s[ks * 64 + lane], s1 = s_s[(KS + ks) * 64 + lane];
-                uint4 x0 = fq[ks], x1;
-                if constexpr (F16) split_f16(fq[ks], x0, x1);
+                uint4 x0 = s_in[n & 1].q[(tile * KS + ks) * 64 + unit_at], x1;
+                if constexpr (F16) split_f16(x0, x0, x1);
                 a0 = mma(x0, s0, a0);
                 a1 = mma(x0, s1, a1);
                 if constexpr (F16) a1 = mma(x1, s0, a1);
@@ -652,7 +650,6 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
             a1 = zero;
             lds_barrier();  // (2)
             const int slow_word = s_bad;
-            load_rows(n + 1);
             const bool slow = __builtin_amdgcn_readfirstlane(slow_word) == n + 1;
             lds_barrier();  // (3)
             if (slow) {
@@ -699,13 +696,22 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if constexpr (MT == 2) {
-                const uint4 x = in.k[(j * KS + w) * 64 + lane];
+                const uint4 x = in.k[(j * KS + w) * 64 + unit_at];
                 fk[j].w[0] = x.x, fk[j].w[1] = x.y, fk[j].w[2] = x.z, fk[j].w[3] = x.w;
             } else {
-                const uint2 x = reinterpret_cast<const uint2*>(in.k)[2 * ((j * KS + (w >> 1)) * 64 + lane) + (w & 1)];
+                const uint2 x = reinterpret_cast<const uint2*>(in.k)[2 * ((j * KS + (w >> 1)) * 64 + unit_at) + (w & 1)];
                 fk[j].w[0] = x.x, fk[j].w[1] = x.y;
             }
         }
+    };
+    // K^T: the lane's row of state tile m, eight tokens, from two transposing
+    // reads: 16 lanes give 4 rows of 16 elements, lane i takes column i of them
+    const auto k_t = [&](const Stage& in, int m, int ks) {
+        const int state_tile = MT * w + m;
+        const uint2* const at = reinterpret_cast<const uint2*>(in.k) +
+                                2 * ((2 * ks * KS + (state_tile >> 1)) * 64 + row_unit(4 * g4 + (r >> 2), r & 3)) + (state_tile & 1);
+        const uint2 lo = read_transposed(at), hi = read_transposed(at + 2 * KS * 64);
+        return make_uint4(lo.x, lo.y, hi.x, hi.y);
     };
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -785,7 +791,9 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
         const int slow_word = s_bad;
         {  // (3)
 #pragma unroll
-            for (int i = 0; i < 2 * MT; ++i) fkt[i] = in.kt[(2 * MT * w + i) * 64 + lane];
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) fkt[2 * m + ks] = k_t(in, m, ks);
             f32x4_t a0 = zero, a1 = zero, a2 = zero;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
@@ -878,7 +886,6 @@ int launch_chunks(const DeltaParams& p, void* ws, hipStream_t stream) {
     const int64_t per = chunks_per_launch(p.B, p.seq.S, p.Hv), all = (int64_t(p.seq.S) + kChunk - 1) / kChunk;
     ChunkPlan c;
     c.units = static_cast<uint16_t*>(ws);
-    c.kt = c.units + size_t(p.B) * per * p.Hv * kUnitElems;
     auto* prepare = p.Dk == 128 ? delta_chunk_prepare_kernel<128, F16> : delta_chunk_prepare_kernel<64, F16>;
     auto* scan = p.Dk == 128 ? delta_chunk_scan_kernel<128, F16> : delta_chunk_scan_kernel<64, F16>;
     for (int64_t first = 0; first < all; first += per) {
@@ -914,7 +921,7 @@ extern "C" size_t genllm_gated_delta_workspace_bytes(int32_t batch, int32_t seq_
     if (batch <= 0 || seq_len <= 0 || n_k_heads <= 0 || n_v_heads <= 0 || k_dim <= 0 || v_dim <= 0 || !in_chunks(seq_len))
         return 0;
     const size_t n = size_t(batch) * size_t(chunks_per_launch(batch, seq_len, n_v_heads));
-    return n * (size_t(n_v_heads) * kUnitBytes + size_t(n_k_heads) * k_dim * kChunk * 2);
+    return n * size_t(n_v_heads) * kUnitBytes;
 }
 
 extern "C" int genllm_gated_delta_rule(const void* q, int64_t q_batch_stride, int64_t q_tok_stride, int64_t q_head_stride,
