@@ -289,20 +289,41 @@ __device__ __forceinline__ uint2 read_transposed(const uint2* p) {
 // an LDS bank.
 __device__ __forceinline__ constexpr int row_unit(int r, int g) { return 4 * r + (g ^ (r >> 2)); }
 
-// Four waves per chunk and value head; wave w has row tile w of the 64 x 64
-// matrices.  (1 + L)^-1 by halves: the four diagonal 16 x 16 blocks by
-// substitution, a lane per column; then T10 = -T11 (L10 T00) for 16- and for
-// 32-wide blocks, as fp32 matrix products.
+// Inclusive sum over the lanes of a wave in 64 bits: within rows of 16 lanes by
+// DPP shifts, then the last lane of a row to the next row, and of lane 31 to the
+// upper half.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, int(uint32_t(u)), CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, int(uint32_t(u >> 32)), CTRL, ROWS, 0xF, false);
+    return x + __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+__device__ __forceinline__ double wave_running_sum(double x) {
+    x = dpp_add<0x111, 0xF>(x);  // row_shr:1
+    x = dpp_add<0x112, 0xF>(x);
+    x = dpp_add<0x114, 0xF>(x);
+    x = dpp_add<0x118, 0xF>(x);
+    x = dpp_add<0x142, 0xA>(x);  // row_bcast:15 into rows 1 and 3
+    return dpp_add<0x143, 0xC>(x);  // row_bcast:31 into rows 2 and 3
+}
+
+// Four waves per chunk and value head.  Products of rows with rows are formed
+// with the roles that leave four neighbours of a row in a lane (rows of the other
+// factor in the order tile_row for P), so that P leaves the registers as
+// fragments and L enters LDS in 16-byte writes.  (1 + L)^-1 by halves: the four
+// diagonal 16 x 16 blocks by substitution, a lane per column; then T10 = -T11
+// (L10 T00) for 16- and for 32-wide blocks, as fp32 matrix products.
 template <int DK, bool F16>
 __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p, ChunkPlan c) {
     constexpr int KS = DK / 32, LD = 68, LK = DK + 8;
-    __shared__ __attribute__((aligned(16))) float s_l[64 * LD];   // L, then the products M in its upper blocks
-    __shared__ __attribute__((aligned(16))) float s_t[64 * LD];   // P, then the inverse
-    __shared__ __attribute__((aligned(16))) uint16_t s_k[64 * LK];
-    uint16_t* const s_q = reinterpret_cast<uint16_t*>(s_t);  // until P
-    static_assert(sizeof(uint16_t) * 64 * LK <= sizeof(s_t), "s_q lies in s_t");
-    __shared__ double s_g[64];
-    __shared__ float s_beta[64], s_rk[64], s_rq[64];
+    __shared__ __attribute__((aligned(16))) float s_l[64 * LD];  // L, then the products M in its upper blocks
+    __shared__ __attribute__((aligned(16))) float s_t[64 * LD];  // the inverse
+    uint16_t* const s_k = reinterpret_cast<uint16_t*>(s_t);      // K until then
+    static_assert(sizeof(uint16_t) * 64 * LK <= sizeof(s_t), "s_k lies in s_t");
+    __shared__ __attribute__((aligned(16))) double s_g[64];  // running sums of log2 of the decays
+    __shared__ __attribute__((aligned(16))) float s_beta[64], s_rk[64], s_rq[64];
+    __shared__ int s_bad;
     const int h = int(blockIdx.x % uint32_t(p.Hv)), rest = int(blockIdx.x / uint32_t(p.Hv));
     const int n = rest % c.count, b = rest / c.count;
     const int t0 = (c.first + n) * kChunk;
@@ -314,112 +335,118 @@ __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p,
     uint16_t* const unit = c.units + ((int64_t(b) * c.count + n) * p.Hv + h) * kUnitElems;
     float* const vec = reinterpret_cast<float*>(unit + kUnitVec);
 
-    // rows of K and Q of tile w through LDS, four lanes to 64 bytes of a row; rows
-    // behind the end are zeros
-    uint4 own[KS], qf[KS];
+    // K's rows of tile w, four lanes to 64 bytes of a row, into LDS; Q's rows in
+    // the order of P's fragments, as operands; rows behind the end are zeros
+    uint4 kin[KS], qf[KS];
     {
-        const int row = 16 * w + (lane >> 2), at = 8 * (lane & 3);
-        const bool there = row < left;
-        const uint16_t* const kp = p.k.p + b * p.k.batch + hk * p.k.head + (t0 + row) * p.k.tok + at;
-        const uint16_t* const qp = p.q.p + b * p.q.batch + hk * p.q.head + (t0 + row) * p.q.tok + at;
+        const int row = 16 * w + (lane >> 2), q_row = tile_row(w, r);
+        const uint16_t* const kp = p.k.p + b * p.k.batch + hk * p.k.head + (t0 + row) * p.k.tok + 8 * (lane & 3);
+        const uint16_t* const qp = p.q.p + b * p.q.batch + hk * p.q.head + (t0 + q_row) * p.q.tok + 8 * g4;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            own[ks] = qf[ks] = make_uint4(0, 0, 0, 0);
-            if (there) own[ks] = *reinterpret_cast<const uint4*>(kp + 32 * ks), qf[ks] = *reinterpret_cast<const uint4*>(qp + 32 * ks);
-        }
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            *reinterpret_cast<uint4*>(s_k + row * LK + 32 * ks + at) = own[ks];
-            *reinterpret_cast<uint4*>(s_q + row * LK + 32 * ks + at) = qf[ks];
-        }
-        // a wave reads back its own rows
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            own[ks] = *reinterpret_cast<const uint4*>(s_k + (16 * w + r) * LK + 32 * ks + 8 * g4);
-            qf[ks] = *reinterpret_cast<const uint4*>(s_q + (16 * w + r) * LK + 32 * ks + 8 * g4);
+            kin[ks] = qf[ks] = make_uint4(0, 0, 0, 0);
+            if (row < left) kin[ks] = *reinterpret_cast<const uint4*>(kp + 32 * ks);
+            if (q_row < left) qf[ks] = *reinterpret_cast<const uint4*>(qp + 32 * ks);
         }
     }
-    // gates of token `lane`, the running sum in 64 bits (differences of far sums
-    // enter the exponents); exp(-2000) is 0 in either precision
+    if (threadIdx.x == 0) s_bad = 0;
     float g = 0.0f, beta = 0.0f;
-    if (lane < left) gates<F16>(p, b, t0 + lane, h, g, beta);
-    g = g < -2000.0f ? -2000.0f : g;
-    double sum = g;
+    if (w == 0 && lane < left) gates<F16>(p, b, t0 + lane, h, g, beta);
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const double up = __shfl_up(sum, m);
-        if (lane >= m) sum += up;
-    }
-    float kk = 0.0f, qq = 0.0f;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-        const uint32_t a[4] = {own[ks].x, own[ks].y, own[ks].z, own[ks].w};
-        const uint32_t d[4] = {qf[ks].x, qf[ks].y, qf[ks].z, qf[ks].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            kk = __builtin_fmaf(Elem<F16>::lo(a[i]), Elem<F16>::lo(a[i]), kk);
-            kk = __builtin_fmaf(Elem<F16>::hi(a[i]), Elem<F16>::hi(a[i]), kk);
-            qq = __builtin_fmaf(Elem<F16>::lo(d[i]), Elem<F16>::lo(d[i]), qq);
-            qq = __builtin_fmaf(Elem<F16>::hi(d[i]), Elem<F16>::hi(d[i]), qq);
-        }
-    }
-    kk += __shfl_xor(kk, 16);
-    qq += __shfl_xor(qq, 16);
-    kk += __shfl_xor(kk, 32);
-    qq += __shfl_xor(qq, 32);
-    const bool there = 16 * w + r < left;
-    const float rk = there ? l2_factor(kk, p.l2_eps) : 0.0f;
-    const float rq = there ? p.scale * l2_factor(qq, p.l2_eps) : 0.0f;
-    if (g4 == 0) s_rk[16 * w + r] = rk, s_rq[16 * w + r] = rq;
-    if (w == 0) s_g[lane] = sum, s_beta[lane] = beta;
+    for (int ks = 0; ks < KS; ++ks) *reinterpret_cast<uint4*>(s_k + (16 * w + (lane >> 2)) * LK + 32 * ks + 8 * (lane & 3)) = kin[ks];
+    __syncthreads();
     // what is not finite (or an infinite factor) would reach earlier tokens
     // through the zeros of T: the scan runs such a chunk token by token
-    const bool odd = !(fabsf(rk) < INFINITY) || !(fabsf(kk) < INFINITY) || !(fabsf(g) < INFINITY) || !(fabsf(beta) < INFINITY);
-    const int bad = __syncthreads_or(odd);
-
-    // L below and P on and below the diagonal, tile (w, j)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (j > w) continue;
-        f32x4_t ak = {0.0f, 0.0f, 0.0f, 0.0f}, aq = ak;
+    bool odd = false;
+    if (w == 0) {
+        // the running sum in 64 bits: differences of far sums enter the exponents;
+        // exp(-2000) is 0 in either precision
+        odd = !(fabsf(g < -2000.0f ? -2000.0f : g) < INFINITY) || !(fabsf(beta) < INFINITY);
+        s_g[lane] = wave_running_sum(double(g < -2000.0f ? -2000.0f : g) * 1.4426950408889634);
+        s_beta[lane] = beta;
+    }
+    const auto k_rows = [&](int row, int ks) { return *reinterpret_cast<const uint4*>(s_k + row * LK + 32 * ks + 8 * g4); };
+    const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    {  // the rows' norms: diagonals of K K^T and Q Q^T
+        f32x4_t kk = zero, qq = zero;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            const uint4 kj = *reinterpret_cast<const uint4*>(s_k + (16 * j + r) * LK + 32 * ks + 8 * g4);
-            ak = Elem<F16>::mma32(own[ks], kj, ak);
-            aq = Elem<F16>::mma32(qf[ks], kj, aq);
+            const uint4 x = k_rows(16 * w + r, ks);
+            kk = Elem<F16>::mma32(x, x, kk);
+            qq = Elem<F16>::mma32(qf[ks], qf[ks], qq);
         }
-        const int col = 16 * j + r;
-        const double gc = s_g[col];
-        const float rc = s_rk[col];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = 16 * w + 4 * g4 + i;
-            const float e = row >= col ? expf(float(s_g[row] - gc)) * rc : 0.0f;
-            s_l[row * LD + col] = row > col ? s_beta[row] * s_rk[row] * e * ak[i] : 0.0f;
-            s_t[row * LD + col] = row >= col ? s_rq[row] * e * aq[i] : 0.0f;
+        if (r >> 2 == g4) {
+            const int i = r & 3, k_row = 16 * w + r, q_row = tile_row(w, r);
+            const float k2 = i == 0 ? kk[0] : i == 1 ? kk[1] : i == 2 ? kk[2] : kk[3];
+            const float q2 = i == 0 ? qq[0] : i == 1 ? qq[1] : i == 2 ? qq[2] : qq[3];
+            const float rk = k_row < left ? l2_factor(k2, p.l2_eps) : 0.0f;
+            s_rk[k_row] = rk;
+            s_rq[q_row] = q_row < left ? p.scale * l2_factor(q2, p.l2_eps) : 0.0f;
+            odd |= !(fabsf(rk) < INFINITY) || !(fabsf(k2) < INFINITY);
         }
     }
+    if (odd) s_bad = 1;
     __syncthreads();
 
-    // P's fragments of row tile w and the vectors
-    for (int ks = 0; ks <= w >> 1; ++ks) {
-        const int row = tile_row(w, r), col = 32 * ks + 8 * g4;
-        const float* const src = s_t + row * LD + col;
-        uint32_t a[4], d[4];
+    // e^(G_row - G_col) with the columns' norms, four columns
+    const auto fade = [&](double g_row, int row, int col, float (&f)[4]) {
+        const double2 g01 = *reinterpret_cast<const double2*>(s_g + col), g23 = *reinterpret_cast<const double2*>(s_g + col + 2);
+        const f32x4_t rk = *reinterpret_cast<const f32x4_t*>(s_rk + col);
+        const double gc[4] = {g01.x, g01.y, g23.x, g23.y};
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            split2(col + 2 * i > row ? 0.0f : src[2 * i], col + 2 * i + 1 > row ? 0.0f : src[2 * i + 1], a[i], d[i]);
-        uint16_t* const to = unit + kUnitP + tri_frag(w, ks) * kFrag + 8 * lane;
-        *reinterpret_cast<uint4*>(to) = make_uint4(a[0], a[1], a[2], a[3]);
-        *reinterpret_cast<uint4*>(to + kTPart) = make_uint4(d[0], d[1], d[2], d[3]);
+        for (int i = 0; i < 4; ++i) f[i] = row >= col + i ? exp2_fast(float(g_row - gc[i])) * rk[i] : 0.0f;
+    };
+    {  // P: rows tile_row(w, r), the fragments of tile w
+        const int row = tile_row(w, r);
+        const double g_row = s_g[row];
+        const float rq = s_rq[row];
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            if (ks > w >> 1) continue;
+            uint32_t a[4], d[4];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                f32x4_t x = zero;
+#pragma unroll
+                for (int q = 0; q < KS; ++q) x = Elem<F16>::mma32(k_rows(tile_row(2 * ks + half, r), q), qf[q], x);
+                float f[4];
+                fade(g_row, row, 32 * ks + 8 * g4 + 4 * half, f);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    split2(rq * f[2 * i] * x[2 * i], rq * f[2 * i + 1] * x[2 * i + 1], a[2 * half + i], d[2 * half + i]);
+            }
+            uint16_t* const to = unit + kUnitP + tri_frag(w, ks) * kFrag + 8 * lane;
+            *reinterpret_cast<uint4*>(to) = make_uint4(a[0], a[1], a[2], a[3]);
+            *reinterpret_cast<uint4*>(to + kTPart) = make_uint4(d[0], d[1], d[2], d[3]);
+        }
+    }
+    {  // L: rows of tile 3 - w, the longest for the wave with the fewest of P
+        const int ti = 3 - w, row = 16 * ti + r;
+        const double g_row = s_g[row];
+        const float f_row = s_beta[row] * s_rk[row];
+        uint4 kf[KS];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) kf[ks] = k_rows(row, ks);
+        for (int tj = 0; tj <= ti; ++tj) {
+            f32x4_t x = zero;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) x = Elem<F16>::mma32(k_rows(16 * tj + r, ks), kf[ks], x);
+            const int col = 16 * tj + 4 * g4;
+            float f[4];
+            fade(g_row, row, col, f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = row > col + i ? f_row * f[i] * x[i] : 0.0f;
+            *reinterpret_cast<f32x4_t*>(s_l + row * LD + col) = x;
+        }
     }
     if (w == 3) {
-        const double last = s_g[63];
-        vec[kVecC + lane] = s_rk[lane] * expf(float(s_g[lane]));
-        vec[kVecD + lane] = s_rk[lane] * expf(float(last - s_g[lane]));
-        vec[kVecE + lane] = s_rq[lane] * expf(float(s_g[lane]));
-        if (lane == 0) vec[kVecLast] = expf(float(last)), vec[kVecBad] = bad ? 1.0f : 0.0f;
+        const double last = s_g[63], at = s_g[lane];
+        vec[kVecC + lane] = s_rk[lane] * exp2_fast(float(at));
+        vec[kVecD + lane] = s_rk[lane] * exp2_fast(float(last - at));
+        vec[kVecE + lane] = s_rq[lane] * exp2_fast(float(at));
+        if (lane == 0) vec[kVecLast] = exp2_fast(float(last)), vec[kVecBad] = s_bad ? 1.0f : 0.0f;
     }
+    __syncthreads();  // K has been read, L is there
     // the inverse of diagonal block w: column r in every lane group, by substitution
     float x[16];
 #pragma unroll
@@ -430,7 +457,6 @@ __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p,
         for (int m = 0; m < i; ++m) a = __builtin_fmaf(-row[m], x[m], a);
         x[i] = a;
     }
-    __syncthreads();  // P has been read
 #pragma unroll
     for (int i = 0; i < 16; ++i)
         if (i / 4 == g4) s_t[(16 * w + i) * LD + 16 * w + r] = x[i];
@@ -448,7 +474,6 @@ __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p,
 #pragma unroll
         for (int e = 0; e < 4; ++e) m[(16 * i + 4 * g4 + e) * LD + 16 * j + r] = sign * v[e];
     };
-    const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
     if ((w & 1) == 0) {  // blocks (1, 0) and (3, 2)
         const f32x4_t m = mm16(row_of(s_l, w + 1, w), col_of(s_t, w, w), zero);
         put(s_t, w + 1, w, mm16(row_of(s_t, w + 1, w + 1), m, zero), -1.0f);
@@ -467,14 +492,18 @@ __global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p,
         put(s_t, bi, bj, m, -1.0f);
     }
     __syncthreads();
-    for (int ks = 0; ks <= w >> 1; ++ks) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+        if (ks > w >> 1) continue;
         const int row = tile_row(w, r), col = 32 * ks + 8 * g4;
-        const float* const src = s_t + row * LD + col;
+        const f32x4_t* const src = reinterpret_cast<const f32x4_t*>(s_t + row * LD + col);
+        const f32x4_t* const bt = reinterpret_cast<const f32x4_t*>(s_beta + col);
+        const f32x4_t t[2] = {src[0] * bt[0], src[1] * bt[1]};
         uint32_t a[4], d[4], e[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            split3(col + 2 * i > row ? 0.0f : src[2 * i] * s_beta[col + 2 * i],
-                   col + 2 * i + 1 > row ? 0.0f : src[2 * i + 1] * s_beta[col + 2 * i + 1], a[i], d[i], e[i]);
+        for (int i = 0; i < 4; ++i)  // right of the diagonal lies what was never written
+            split3(col + 2 * i > row ? 0.0f : t[i >> 1][2 * (i & 1)], col + 2 * i + 1 > row ? 0.0f : t[i >> 1][2 * (i & 1) + 1],
+                   a[i], d[i], e[i]);
         uint16_t* const to = unit + kUnitT + tri_frag(w, ks) * kFrag + 8 * lane;
         *reinterpret_cast<uint4*>(to) = make_uint4(a[0], a[1], a[2], a[3]);
         *reinterpret_cast<uint4*>(to + kTPart) = make_uint4(d[0], d[1], d[2], d[3]);
@@ -680,6 +709,7 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
         return;
     }
 
+    __builtin_amdgcn_s_setprio(3);  // the chain goes first where waves meet on a SIMD
     const int row0 = tile_row(MT * w, 4 * g4);  // the lane's first row of the state; tile m: + 4 m
     float* const st = p.state + ((int64_t(slot) * p.Hv + h) * DK + row0) * p.Dv + col0 + r;
     f32x4_t s[MT];
