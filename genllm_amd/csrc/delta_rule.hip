@@ -315,7 +315,7 @@ __device__ __forceinline__ double wave_running_sum(double x) {
 // diagonal 16 x 16 blocks by substitution, a lane per column; then T10 = -T11
 // (L10 T00) for 16- and for 32-wide blocks, as fp32 matrix products.
 template <int DK, bool F16>
-__global__ __launch_bounds__(256) void delta_chunk_prepare_kernel(DeltaParams p, ChunkPlan c) {
+__global__ __launch_bounds__(256, 4) void delta_chunk_prepare_kernel(DeltaParams p, ChunkPlan c) {
     constexpr int KS = DK / 32, LD = 68, LK = DK + 8;
     __shared__ __attribute__((aligned(16))) float s_l[64 * LD];  // L, then the products M in its upper blocks
     __shared__ __attribute__((aligned(16))) float s_t[64 * LD];  // the inverse
