@@ -231,20 +231,32 @@ struct ChunkPlan {
 __device__ __forceinline__ uint32_t top2(float lo, float hi) {
     return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
-__device__ __forceinline__ float top(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); }
+// what a part leaves of (lo, hi), exactly: x - 1 part.lo - 0 part.hi.  (A part that
+// is infinite makes both NaN: nothing finite is lost, as such a chunk runs token
+// by token.)
+__device__ __forceinline__ void residual2(uint32_t part, float& lo, float& hi) {
+    const bf16x2_t_ x = __builtin_bit_cast(bf16x2_t_, part);
+    // (-1, 0) and (0, -1) from registers: as an inline constant the instruction
+    // takes -1.0 for the fp32 pattern, the other pair
+    uint32_t first = 0x0000BF80u, second = 0xBF800000u;
+    __asm__("" : "+s"(first), "+s"(second));
+    lo = __builtin_amdgcn_fdot2_f32_bf16(x, __builtin_bit_cast(bf16x2_t_, first), lo, false);
+    hi = __builtin_amdgcn_fdot2_f32_bf16(x, __builtin_bit_cast(bf16x2_t_, second), hi, false);
+}
 
 // (lo, hi) in three bf16 parts each, exactly: 8 + 8 + 8 bits
 __device__ __forceinline__ void split3(float lo, float hi, uint32_t& a, uint32_t& b, uint32_t& c) {
     a = top2(lo, hi);
-    lo -= top(lo), hi -= top(hi);
+    residual2(a, lo, hi);
     b = top2(lo, hi);
-    lo -= top(lo), hi -= top(hi);
+    residual2(b, lo, hi);
     c = top2(lo, hi);
 }
 // in two parts, the second rounded: 2^-17
 __device__ __forceinline__ void split2(float lo, float hi, uint32_t& a, uint32_t& b) {
     a = top2(lo, hi);
-    b = Elem<false>::pack_p(lo - top(lo), hi - top(hi));
+    residual2(a, lo, hi);
+    b = Elem<false>::pack_p(lo, hi);
 }
 // eight fp16 elements in two bf16 parts each, exactly (11 bits)
 __device__ __forceinline__ void split_f16(const uint4& x, uint4& a, uint4& b) {
