@@ -39,7 +39,7 @@ struct AxesParams {
     const float* sin_tab = nullptr;
     const int32_t* pos = nullptr;  // [n_axes][pos_stride]
     int64_t pos_stride = 0;
-    uint16_t axis_bits[16] = {};  // two bits per pair, eight pairs per entry
+    uint32_t axis_bits[8] = {};  // two bits per pair, sixteen pairs per word
 };
 
 template <bool F16>
@@ -97,7 +97,10 @@ __global__ __launch_bounds__(256) void norm_rope_axes_kernel(AxesParams p) {
     }
     for (int i = int(threadIdx.x); i < tokens * half; i += 256) {
         const int t = i / half, pair = i - t * half;
-        const int axis = int(p.axis_bits[pair >> 3] >> (2 * (pair & 7))) & 3;
+        uint32_t word = p.axis_bits[0];  // selected, not indexed: no load from the argument block in front of the position's
+#pragma unroll
+        for (int j = 1; j < 8; ++j) word = pair >> 4 == j ? p.axis_bits[j] : word;
+        const int axis = int(word >> (2 * (pair & 15))) & 3;
         const int32_t at = p.pos[axis * p.pos_stride + t0 + t];
         float c = __builtin_nanf(""), s = c;  // a position outside the tables
         if (uint32_t(at) < uint32_t(p.max_seq)) {
@@ -107,14 +110,6 @@ __global__ __launch_bounds__(256) void norm_rope_axes_kernel(AxesParams p) {
         s_tab[2 * t * half + pair] = c;
         s_tab[(2 * t + 1) * half + pair] = s;
     }
-    float gq[16], gk[16];
-    const bool norm_q = p.q.gamma != nullptr, norm_k = p.k.gamma != nullptr;
-    const auto load_gamma = [&](const float* g, float (&f)[16]) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = g[e0 + i], f[8 + i] = g[e1 + i];
-    };
-    if (norm_q) load_gamma(p.q.gamma, gq);
-    if (norm_k) load_gamma(p.k.gamma, gk);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
@@ -122,7 +117,10 @@ __global__ __launch_bounds__(256) void norm_rope_axes_kernel(AxesParams p) {
         float y[16];
         unpack8<F16>(lo[i], y);
         unpack8<F16>(hi[i], y + 8);
-        if (is_k[i] ? norm_k : norm_q) {
+        const float* const gamma = is_k[i] ? p.k.gamma : p.q.gamma;
+        if (gamma) {
+            const f32x4_t g[4] = {*reinterpret_cast<const f32x4_t*>(gamma + e0), *reinterpret_cast<const f32x4_t*>(gamma + e0 + 4),
+                                  *reinterpret_cast<const f32x4_t*>(gamma + e1), *reinterpret_cast<const f32x4_t*>(gamma + e1 + 4)};
             float ss = 0.0f;
 #pragma unroll
             for (int j = 0; j < 16; ++j) ss = __builtin_fmaf(y[j], y[j], ss);
@@ -132,7 +130,7 @@ __global__ __launch_bounds__(256) void norm_rope_axes_kernel(AxesParams p) {
             if constexpr (L >= 16) ss += dpp<kDppRowMirror>(ss);
             const float f = 1.0f / __builtin_sqrtf(ss * (1.0f / D) + p.eps);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) y[j] = y[j] * f * (is_k[i] ? gk[j] : gq[j]);
+            for (int j = 0; j < 16; ++j) y[j] = y[j] * f * g[j >> 2][j & 3];
         }
         if (turns) {
             const f32x4_t* const tab = reinterpret_cast<const f32x4_t*>(s_tab + 2 * tok[i] * half + e0);
@@ -179,7 +177,7 @@ int launch_axes(AxesParams& p, int D, hipStream_t stream) {
 }
 
 bool rows_ok(const AxesRows& r) {
-    return aligned_to(r.x, 16) && aligned_to(r.out, 16) && aligned_to(r.gamma, 4) &&
+    return aligned_to(r.x, 16) && aligned_to(r.out, 16) && aligned_to(r.gamma, 16) &&
            ((r.x_tok | r.x_head | r.o_tok | r.o_head) & 7) == 0;
 }
 
@@ -224,7 +222,7 @@ extern "C" int genllm_qk_norm_rope_axes(const void* q, int64_t q_tok_stride, int
             while (i >= first + sections[axis]) first += sections[axis++];
         }
         ++count[axis];
-        p.axis_bits[i / 8] = uint16_t(p.axis_bits[i / 8] | axis << (2 * (i % 8)));
+        p.axis_bits[i / 16] |= uint32_t(axis) << (2 * (i % 16));
     }
     for (int i = 0; i < n_axes; ++i)
         if (count[i] != sections[i])
@@ -244,7 +242,7 @@ extern "C" int genllm_qk_norm_rope_axes(const void* q, int64_t q_tok_stride, int
     p.k = {static_cast<const uint16_t*>(k), k_tok_stride, k_head_stride, static_cast<uint16_t*>(k_out), ko_tok_stride,
            ko_head_stride, gamma_k};
     if ((n_q_heads && !rows_ok(p.q)) || (n_k_heads && !rows_ok(p.k)))
-        return fail(GENLLM_ERR_INVALID, "qk_norm_rope_axes: q, k and their outputs must be rows of 16-byte alignment");
+        return fail(GENLLM_ERR_INVALID, "qk_norm_rope_axes: q, k, their outputs and gammas must be 16-byte aligned");
     if (!aligned_to(cos_tab, 4) || !aligned_to(sin_tab, 4) || !aligned_to(positions, 4))
         return fail(GENLLM_ERR_INVALID, "qk_norm_rope_axes: a pointer is not aligned to its type");
     p.Hq = n_q_heads, p.Hk = n_k_heads, p.S = seq_len, p.rope_dim = rope_dim, p.max_seq = max_seq;

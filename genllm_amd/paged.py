@@ -19,7 +19,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import DTYPE_BF16, DTYPE_F16, PAGE, GenllmError, LayerInfo, call, lib
+from ._lib import DTYPE_BF16, DTYPE_F16, PAGE, GenllmError, LayerInfo, call, check, lib
 
 
 # The current stream's handle without the Stream object around it: 0.1 against
@@ -427,12 +427,13 @@ def _need(op, name, t, shape, dtype, device):
                          f"{t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
 
 
-def _call_on(dev: int, stream, name, *args):
-    """call() with device `dev` current, on `stream` or that device's current stream."""
-    if _current_device is None or dev != _current_device():
-        with torch.cuda.device(dev):
-            return call(name, *args, _stream(stream))
-    return call(name, *args, _raw_stream(dev) if stream is None and _raw_stream is not None else _stream(stream))
+def _elsewhere(dev: int) -> bool:
+    """Whether `dev` is not the current device: the call is then made again with it current."""
+    return _current_device is None or dev != _current_device()
+
+
+def _stream_on(dev: int, stream):
+    return _raw_stream(dev) if stream is None and _raw_stream is not None else _stream(stream)
 
 
 def _element_code(op, t):
@@ -470,6 +471,10 @@ def gated_delta_rule(q, k, v, a, b, state, out, scale: float, a_log=None, dt_bia
     op = "gated_delta_rule"
     code = _element_code(op, q)
     qshape, vshape, dt, dev = q.shape, v.shape, q.dtype, q.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return gated_delta_rule(q, k, v, a, b, state, out, scale, a_log, dt_bias, l2_eps, seq_lens, state_ids, workspace,
+                                    stream)
     B, S, Hk, Dk = qshape
     Hv, Dv = vshape[-2:]
     gate = torch.float32 if a_log is None else dt
@@ -506,12 +511,15 @@ def gated_delta_rule(q, k, v, a, b, state, out, scale: float, a_log=None, dt_bia
         if stream is not None:  # it goes back to the current stream's pool while `stream` still uses it
             workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream)
                                     else torch.cuda.ExternalStream(int(getattr(stream, "cuda_stream", stream)), device=q.device))
-    _call_on(dev, stream, "genllm_gated_delta_rule", q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2],
-             v.data_ptr(), vs[0], vs[1], vs[2], a.data_ptr(), as_[0], as_[1], b.data_ptr(), bs[0], bs[1],
-             None if a_log is None else a_log.data_ptr(), None if dt_bias is None else dt_bias.data_ptr(), state.data_ptr(),
-             state.shape[0], None if state_ids is None else state_ids.data_ptr(),
-             None if seq_lens is None else seq_lens.data_ptr(), out.data_ptr(), os_[0], os_[1], os_[2], B, S, Hk, Hv, Dk, Dv,
-             code, scale, -1.0 if l2_eps is None else l2_eps, ws, ws_bytes)
+    rc = (_lib._lib or lib()).genllm_gated_delta_rule(
+        q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
+        a.data_ptr(), as_[0], as_[1], b.data_ptr(), bs[0], bs[1], None if a_log is None else a_log.data_ptr(),
+        None if dt_bias is None else dt_bias.data_ptr(), state.data_ptr(), state.shape[0],
+        None if state_ids is None else state_ids.data_ptr(), None if seq_lens is None else seq_lens.data_ptr(),
+        out.data_ptr(), os_[0], os_[1], os_[2], B, S, Hk, Hv, Dk, Dv, code, scale, -1.0 if l2_eps is None else l2_eps, ws,
+        ws_bytes, _stream_on(dev, stream))
+    if rc:
+        check(rc)
 
 
 def causal_conv(x, weight, out, state=None, bias=None, silu: bool = True, seq_lens=None, state_ids=None, stream=None):
@@ -524,6 +532,9 @@ def causal_conv(x, weight, out, state=None, bias=None, silu: bool = True, seq_le
     op = "causal_conv"
     code = _element_code(op, x)
     shape, dt, dev = x.shape, x.dtype, x.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return causal_conv(x, weight, out, state, bias, silu, seq_lens, state_ids, stream)
     B, S, Ch = shape
     W = weight.shape[-1]
     xs, os_ = x.stride(), out.stride()
@@ -541,10 +552,12 @@ def causal_conv(x, weight, out, state=None, bias=None, silu: bool = True, seq_le
             raise ValueError(f"{op}: state must be contiguous {dt} [n, {W - 1}, {Ch}] on {x.device}")
     if seq_lens is not None or state_ids is not None:
         _check_entries(op, B, x.device, seq_lens, state_ids)
-    _call_on(dev, stream, "genllm_causal_conv", x.data_ptr(), xs[0], xs[1], weight.data_ptr(),
-             None if bias is None else bias.data_ptr(), out.data_ptr(), os_[0], os_[1], sp, n,
-             None if state_ids is None else state_ids.data_ptr(), None if seq_lens is None else seq_lens.data_ptr(), B, S,
-             Ch, W, code, int(silu))
+    rc = (_lib._lib or lib()).genllm_causal_conv(
+        x.data_ptr(), xs[0], xs[1], weight.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), os_[0],
+        os_[1], sp, n, None if state_ids is None else state_ids.data_ptr(),
+        None if seq_lens is None else seq_lens.data_ptr(), B, S, Ch, W, code, int(silu), _stream_on(dev, stream))
+    if rc:
+        check(rc)
 
 
 def qk_norm_rope_axes(q, k, q_out, k_out, gamma_q, gamma_k, eps: float, cos, sin, positions, sections,
@@ -559,6 +572,10 @@ def qk_norm_rope_axes(q, k, q_out, k_out, gamma_q, gamma_k, eps: float, cos, sin
     op = "qk_norm_rope_axes"
     code = _element_code(op, q)
     shape, dt, dev = q.shape, q.dtype, q.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return qk_norm_rope_axes(q, k, q_out, k_out, gamma_q, gamma_k, eps, cos, sin, positions, sections, interleaved,
+                                     stream)
     S, Hq, D = shape
     n_axes = len(sections)
     qs, qos = q.stride(), q_out.stride()
@@ -575,7 +592,8 @@ def qk_norm_rope_axes(q, k, q_out, k_out, gamma_q, gamma_k, eps: float, cos, sin
             _need(op, "k_out", k_out, (S, Hk, D), dt, q.device)
         kp, kop = k.data_ptr(), k_out.data_ptr()
     for gamma in (gamma_q, gamma_k):
-        if gamma is not None:
+        if gamma is not None and not (gamma.shape == (D,) and gamma.dtype == torch.float32 and gamma.get_device() == dev
+                                      and gamma.is_contiguous()):
             _need(op, "gamma", gamma, (D,), torch.float32, q.device)
     table = cos.shape
     max_seq, rope_dim = table
@@ -585,10 +603,13 @@ def qk_norm_rope_axes(q, k, q_out, k_out, gamma_q, gamma_k, eps: float, cos, sin
     ps = positions.stride()
     if positions.shape != (n_axes, S) or positions.dtype != torch.int32 or positions.get_device() != dev or (ps[1] != 1 and S > 1):
         raise ValueError(f"{op}: positions must be int32 [{n_axes}, {S}] on {q.device}, the tokens dense")
-    _call_on(dev, stream, "genllm_qk_norm_rope_axes", q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), qos[0], qos[1],
-             None if gamma_q is None else gamma_q.data_ptr(), Hq, kp, ks[0], ks[1], kop, kos[0], kos[1],
-             None if gamma_k is None else gamma_k.data_ptr(), Hk, eps, cos.data_ptr(), sin.data_ptr(), max_seq, rope_dim,
-             positions.data_ptr(), ps[0], n_axes, _section_array(tuple(sections)), int(interleaved), S, D, code)
+    rc = (_lib._lib or lib()).genllm_qk_norm_rope_axes(
+        q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), qos[0], qos[1], None if gamma_q is None else gamma_q.data_ptr(), Hq,
+        kp, ks[0], ks[1], kop, kos[0], kos[1], None if gamma_k is None else gamma_k.data_ptr(), Hk, eps, cos.data_ptr(),
+        sin.data_ptr(), max_seq, rope_dim, positions.data_ptr(), ps[0], n_axes, _section_array(tuple(sections)),
+        int(interleaved), S, D, code, _stream_on(dev, stream))
+    if rc:
+        check(rc)
 
 
 @functools.lru_cache(maxsize=64)
