@@ -110,9 +110,10 @@ __device__ __forceinline__ void unpack(const uint32_t (&w)[N / 2], float (&f)[N]
     for (int i = 0; i < N / 2; ++i) f[2 * i] = Elem<F16>::lo(w[i]), f[2 * i + 1] = Elem<F16>::hi(w[i]);
 }
 
-// 1 / sqrt(sum + eps), or 1 without a normalisation
+// 1 / sqrt(sum + eps), or 1 without a normalisation; the hardware's reciprocal
+// root is off by one step of fp32 at most
 __device__ __forceinline__ float l2_factor(float sum, float eps) {
-    return eps < 0.0f ? 1.0f : 1.0f / __builtin_sqrtf(sum + eps);
+    return eps < 0.0f ? 1.0f : __builtin_amdgcn_rsqf(sum + eps);
 }
 
 // The sum over the lanes with the same lane % CQ, CQ = 4 or 8: within rows of 16
@@ -132,8 +133,8 @@ __device__ __forceinline__ float sum_of_groups(float x) {
 // of columns col .. + 3.  S^T k and S^T q of the state before the token are summed
 // in one pass over the registers and one reduction over the row groups; then
 //   u = beta (v - alpha S^T k),  o = scale (alpha S^T q + (k.q) u),
-// and the state is updated.  A token's rows are loaded while the one before it
-// runs (four tokens of 8 sequences 9.2 -> 6.9 us, with the sums by lane exchanges).
+// and the state is updated.  At most 64 tokens: lane l forms the gates of token t0 +
+// l for all.  A token's rows are loaded while the one before it runs.
 template <int DK, int CQ, bool F16>
 __device__ __forceinline__ void recur(const DeltaParams& p, f32x4_t (&s)[DK * CQ / 64], int b, int h, int col, int t0, int t1) {
     constexpr int NR = DK * CQ / 64;
@@ -144,26 +145,31 @@ __device__ __forceinline__ void recur(const DeltaParams& p, f32x4_t (&s)[DK * CQ
     uint16_t* const out = p.out + b * p.o_batch + h * p.o_head + col;
     struct Token {
         uint32_t k[NR / 2], q[NR / 2], v[2];
-        GateLoad gate;
     };
     const auto load = [&](Token& x, int t) {
         load_words<NR>(k + t * p.k.tok, x.k);
         load_words<NR>(q + t * p.q.tok, x.q);
         load_words<4>(v + t * p.v.tok, x.v);
-        x.gate = load_gates(p, b, t, h);
     };
     Token next;
     load(next, t0);
-    float rate, bias;
-    gate_rates(p, h, rate, bias);
+    float alphas, betas;
+    {
+        const int t = min(t0 + int(threadIdx.x & 63), t1 - 1);
+        const GateLoad gate = load_gates(p, b, t, h);
+        float rate, bias, g;
+        gate_rates(p, h, rate, bias);
+        gates<F16>(p, gate, rate, bias, g, betas);
+        alphas = exp2_fast(kLog2e * g);
+    }
     for (int t = t0; t < t1; ++t) {
-        float kf[NR], qf[NR], vf[4], g, beta;
+        float kf[NR], qf[NR], vf[4];
         unpack<F16, NR>(next.k, kf);
         unpack<F16, NR>(next.q, qf);
         unpack<F16, 4>(next.v, vf);
-        const GateLoad gate = next.gate;
         if (t + 1 < t1) load(next, t + 1);
-        gates<F16>(p, gate, rate, bias, g, beta);
+        const float alpha = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(alphas), t - t0));
+        const float beta = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(betas), t - t0));
         float r[11] = {};  // k.k, q.q, k.q, S^T k, S^T q
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
@@ -179,7 +185,7 @@ __device__ __forceinline__ void recur(const DeltaParams& p, f32x4_t (&s)[DK * CQ
 #pragma unroll
         for (int j = 0; j < 11; ++j) r[j] = sum_of_groups<CQ>(r[j]);
         const float rk = l2_factor(r[0], p.l2_eps), rq = p.scale * l2_factor(r[1], p.l2_eps);
-        const float alpha = expf(g), kq = r[2] * rk;
+        const float kq = r[2] * rk;
         float u[4], o[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -961,9 +967,16 @@ int64_t chunks_per_launch(int64_t B, int64_t S, int64_t Hv) {
     return std::min(all, std::max<int64_t>(fit, 1));
 }
 
-// Up to this many tokens per entry the rule runs token by token.
-constexpr int kRecurrentTokens = 16;
-bool in_chunks(int64_t S) { return S > kRecurrentTokens; }
+// Whether the rule runs in chunks.  Token by token a call takes about 0.7 us a
+// token while its waves (16 columns each) find SIMDs of their own, the two chunk
+// kernels 12.5 us for any prompt of up to 64 tokens: 16 / 32 heads of 128, 12 tokens
+// 12.2 against 12.5 us, 16 tokens 15.1 against 12.5.  More waves share the chunk
+// kernels' CUs and fill the SIMDs better: 8 sequences, 24 tokens 34.7 against 40.3,
+// 32 tokens 43.2 against 40.7; 64 sequences, 24 tokens 196 against 303, 48 tokens 349
+// against 331.
+constexpr int64_t kManyWaves = 1024;  // one per SIMD
+int64_t column_waves(int64_t B, int64_t Hv, int64_t Dv) { return B * Hv * (Dv / 16); }
+bool in_chunks(int64_t B, int64_t S, int64_t Hv, int64_t Dv) { return S > (column_waves(B, Hv, Dv) >= kManyWaves ? 28 : 12); }
 
 template <bool F16>
 int launch_chunks(const DeltaParams& p, void* ws, hipStream_t stream) {
@@ -982,9 +995,12 @@ int launch_chunks(const DeltaParams& p, void* ws, hipStream_t stream) {
     return GENLLM_OK;
 }
 
-template <bool F16>
+// 32 columns per wave where that leaves every SIMD one, else 16: the wider wave
+// reads and sums a token's q and k once for twice the columns (16 / 32 heads of
+// 128, 8 tokens: 8 sequences 16.6 against 18.5 us, 64 sequences 91 against 97; one
+// sequence 12.2 against 9.5).
+template <int CQ, bool F16>
 int launch_recurrent(const DeltaParams& p, hipStream_t stream) {
-    constexpr int CQ = 4;
     const int64_t units = int64_t(p.B) * p.Hv * (p.Dv / (4 * CQ));
     auto* kern = p.Dk == 128 ? delta_recurrent_kernel<128, CQ, F16> : delta_recurrent_kernel<64, CQ, F16>;
     hipLaunchKernelGGL(kern, dim3(unsigned((units + 3) / 4)), dim3(256), 0, stream, p, units);
@@ -1002,7 +1018,8 @@ using namespace genllm;
 
 extern "C" size_t genllm_gated_delta_workspace_bytes(int32_t batch, int32_t seq_len, int32_t n_k_heads, int32_t n_v_heads,
                                                      int32_t k_dim, int32_t v_dim) {
-    if (batch <= 0 || seq_len <= 0 || n_k_heads <= 0 || n_v_heads <= 0 || k_dim <= 0 || v_dim <= 0 || !in_chunks(seq_len))
+    if (batch <= 0 || seq_len <= 0 || n_k_heads <= 0 || n_v_heads <= 0 || k_dim <= 0 || v_dim <= 0 ||
+        !in_chunks(batch, seq_len, n_v_heads, v_dim))
         return 0;
     const size_t n = size_t(batch) * size_t(chunks_per_launch(batch, seq_len, n_v_heads));
     return n * size_t(n_v_heads) * kUnitBytes;
@@ -1062,7 +1079,7 @@ extern "C" int genllm_gated_delta_rule(const void* q, int64_t q_batch_stride, in
     p.seq.ids = state_ids, p.seq.lens = seq_lens, p.seq.n_states = n_states, p.seq.S = seq_len;
     p.B = batch, p.Hk = n_k_heads, p.Hv = n_v_heads, p.G = n_v_heads / n_k_heads, p.Dk = k_dim, p.Dv = v_dim;
     p.scale = scale, p.l2_eps = l2_eps < 0.0f ? -1.0f : l2_eps;
-    if (in_chunks(seq_len)) {
+    if (in_chunks(batch, seq_len, n_v_heads, v_dim)) {
         const size_t need = genllm_gated_delta_workspace_bytes(batch, seq_len, n_k_heads, n_v_heads, k_dim, v_dim);
         if (!workspace || workspace_bytes < need || !aligned_to(workspace, 16))
             return fail(GENLLM_ERR_INVALID, "gated_delta_rule: a workspace of " + std::to_string(need) +
@@ -1070,5 +1087,8 @@ extern "C" int genllm_gated_delta_rule(const void* q, int64_t q_batch_stride, in
                                                 std::to_string(workspace_bytes) + ")");
         return f16 ? launch_chunks<true>(p, workspace, as_stream(stream)) : launch_chunks<false>(p, workspace, as_stream(stream));
     }
-    return f16 ? launch_recurrent<true>(p, as_stream(stream)) : launch_recurrent<false>(p, as_stream(stream));
+    const hipStream_t s = as_stream(stream);
+    if (column_waves(batch, n_v_heads, v_dim) >= 2 * kManyWaves)
+        return f16 ? launch_recurrent<8, true>(p, s) : launch_recurrent<8, false>(p, s);
+    return f16 ? launch_recurrent<4, true>(p, s) : launch_recurrent<4, false>(p, s);
 }
