@@ -266,7 +266,8 @@ __device__ __forceinline__ constexpr int tile_row(int t, int rho) {
 
 struct ChunkPlan {
     uint16_t* units = nullptr;  // [batch][chunk][Hv][kUnitElems]
-    int32_t first = 0, count = 0;  // chunks of this launch
+    int32_t first = 0, count = 0;      // chunks of this launch
+    int32_t b_first = 0, b_count = 0;  // batch entries of this launch
 };
 
 // the top 16 bits of an fp32 value are a bf16 value; two of them in one word
@@ -380,14 +381,14 @@ __global__ __launch_bounds__(256, 4) void delta_chunk_prepare_kernel(DeltaParams
     __shared__ __attribute__((aligned(16))) float s_beta[64], s_rk[64], s_rq[64];
     __shared__ int s_bad;
     const int h = int(blockIdx.x % uint32_t(p.Hv)), rest = int(blockIdx.x / uint32_t(p.Hv));
-    const int n = rest % c.count, b = rest / c.count;
+    const int n = rest % c.count, b_at = rest / c.count, b = c.b_first + b_at;
     const int t0 = (c.first + n) * kChunk;
     const int slot = entry_state(p.seq, b), len = entry_len(p.seq, b);
     if (slot < 0 || t0 >= len) return;
     const int left = len - t0;  // tokens of this chunk and behind it
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g4 = lane >> 4;
     const int hk = h / p.G;
-    uint16_t* const unit = c.units + ((int64_t(b) * c.count + n) * p.Hv + h) * kUnitElems;
+    uint16_t* const unit = c.units + ((int64_t(b_at) * c.count + n) * p.Hv + h) * kUnitElems;
     float* const vec = reinterpret_cast<float*>(unit + kUnitVec);
 
     // K's rows of tile w, four lanes to 64 bytes of a row, into LDS; Q's rows in
@@ -634,9 +635,9 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
     float* const s_w = reinterpret_cast<float*>(s_x);  // the state of a chunk that runs token by token
     static_assert(DK * LW * sizeof(float) <= sizeof(s_x), "s_w lies in s_x");
     prefetch_kernargs<sizeof(DeltaParams) + sizeof(ChunkPlan)>();
-    const int heads = p.B * p.Hv;
+    const int heads = c.b_count * p.Hv;
     const int bh = int(blockIdx.x) % heads, col0 = int(blockIdx.x) / heads * kScanCols;
-    const int b = bh / p.Hv, h = bh - b * p.Hv, hk = h / p.G;
+    const int b_at = bh / p.Hv, b = c.b_first + b_at, h = bh - b_at * p.Hv, hk = h / p.G;
     const int slot = entry_state(p.seq, b), len = entry_len(p.seq, b);
     const int begin = c.first * kChunk;
     if (slot == kEntryEmpty || begin >= len) return;
@@ -655,7 +656,7 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
 
     const int unit_at = row_unit(r, g4);  // the lane's operand in K and Q
     const int64_t unit_step = int64_t(p.Hv) * kUnitElems;
-    const uint16_t* const units = c.units + (int64_t(b) * c.count * p.Hv + h) * kUnitElems + 8 * lane;
+    const uint16_t* const units = c.units + (int64_t(b_at) * c.count * p.Hv + h) * kUnitElems + 8 * lane;
 
     if (w >= 8) {  // the loads: a quarter of each chunk's
         // lane l of a load takes unit l of its fragment: four lanes cover 64 bytes of a row
@@ -967,13 +968,25 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
         for (int i = 0; i < 4; ++i) st[int64_t(4 * m + i) * p.Dv] = s[m][i];
 }
 
-// Chunks of one pair of launches: their units stay near 128 MB, within the
-// 256 MB cache between the two kernels, however long the sequence is.
+// What one pair of launches takes: entries of the batch and chunks of each, with
+// units of about 96 MB, which the caches hold between the two kernels (8192 tokens:
+// 48 MB 308, 64 to 96 MB 288, 128 MB 311 us; 32768 tokens: 64 MB 1153, 96 MB 1133,
+// 256 MB 1288 us).  Whole entries where they fit, as many as fill the GPU where not: a
+// launch's start costs a workgroup about two chunks' time.
 constexpr size_t kUnitBytes = kUnitElems * 2;
-int64_t chunks_per_launch(int64_t B, int64_t S, int64_t Hv) {
+struct LaunchPlan {
+    int64_t entries, chunks;
+};
+LaunchPlan launch_plan(int64_t B, int64_t S, int64_t Hv, int64_t Dv) {
     const int64_t all = (S + kChunk - 1) / kChunk;
-    const int64_t fit = int64_t((size_t(128) << 20) / kUnitBytes) / (B * Hv);
-    return std::min(all, std::max<int64_t>(fit, 1));
+    const int64_t units = std::max<int64_t>(int64_t((size_t(96) << 20) / kUnitBytes) / Hv, 1);  // chunks of all heads
+    const int64_t fill = (256 + Hv * (Dv / kScanCols) - 1) / (Hv * (Dv / kScanCols));
+    const auto even = [](int64_t n, int64_t most) {  // n in equal parts of at most `most`
+        const int64_t parts = (n + most - 1) / most;
+        return (n + parts - 1) / parts;
+    };
+    const int64_t entries = even(B, std::max(units / all, fill));
+    return {entries, even(all, std::max<int64_t>(units / entries, 1))};
 }
 
 // Whether the rule runs in chunks.  Token by token a call takes about 0.7 us a
@@ -989,18 +1002,22 @@ bool in_chunks(int64_t B, int64_t S, int64_t Hv, int64_t Dv) { return S > (colum
 
 template <bool F16>
 int launch_chunks(const DeltaParams& p, void* ws, hipStream_t stream) {
-    const int64_t per = chunks_per_launch(p.B, p.seq.S, p.Hv), all = (int64_t(p.seq.S) + kChunk - 1) / kChunk;
+    const LaunchPlan plan = launch_plan(p.B, p.seq.S, p.Hv, p.Dv);
+    const int64_t all = (int64_t(p.seq.S) + kChunk - 1) / kChunk;
     ChunkPlan c;
     c.units = static_cast<uint16_t*>(ws);
     auto* prepare = p.Dk == 128 ? delta_chunk_prepare_kernel<128, F16> : delta_chunk_prepare_kernel<64, F16>;
     auto* scan = p.Dk == 128 ? delta_chunk_scan_kernel<128, F16> : delta_chunk_scan_kernel<64, F16>;
-    for (int64_t first = 0; first < all; first += per) {
-        c.first = int32_t(first), c.count = int32_t(std::min(per, all - first));
-        hipLaunchKernelGGL(prepare, dim3(unsigned(int64_t(p.B) * c.count * p.Hv)), dim3(256), 0, stream, p, c);
-        GENLLM_LAUNCH_CHECK("delta_chunk_prepare_kernel");
-        hipLaunchKernelGGL(scan, dim3(unsigned(p.B * p.Hv * (p.Dv / kScanCols))), dim3(kScanThreads), 0, stream, p, c);
-        GENLLM_LAUNCH_CHECK("delta_chunk_scan_kernel");
-    }
+    for (int64_t b_first = 0; b_first < p.B; b_first += plan.entries)
+        for (int64_t first = 0; first < all; first += plan.chunks) {
+            c.b_first = int32_t(b_first), c.b_count = int32_t(std::min(plan.entries, p.B - b_first));
+            c.first = int32_t(first), c.count = int32_t(std::min(plan.chunks, all - first));
+            const int64_t heads = int64_t(c.b_count) * p.Hv;
+            hipLaunchKernelGGL(prepare, dim3(unsigned(heads * c.count)), dim3(256), 0, stream, p, c);
+            GENLLM_LAUNCH_CHECK("delta_chunk_prepare_kernel");
+            hipLaunchKernelGGL(scan, dim3(unsigned(heads * (p.Dv / kScanCols))), dim3(kScanThreads), 0, stream, p, c);
+            GENLLM_LAUNCH_CHECK("delta_chunk_scan_kernel");
+        }
     return GENLLM_OK;
 }
 
@@ -1030,8 +1047,8 @@ extern "C" size_t genllm_gated_delta_workspace_bytes(int32_t batch, int32_t seq_
     if (batch <= 0 || seq_len <= 0 || n_k_heads <= 0 || n_v_heads <= 0 || k_dim <= 0 || v_dim <= 0 ||
         !in_chunks(batch, seq_len, n_v_heads, v_dim))
         return 0;
-    const size_t n = size_t(batch) * size_t(chunks_per_launch(batch, seq_len, n_v_heads));
-    return n * size_t(n_v_heads) * kUnitBytes;
+    const LaunchPlan plan = launch_plan(batch, seq_len, n_v_heads, v_dim);
+    return size_t(plan.entries) * size_t(plan.chunks) * size_t(n_v_heads) * kUnitBytes;
 }
 
 extern "C" int genllm_gated_delta_rule(const void* q, int64_t q_batch_stride, int64_t q_tok_stride, int64_t q_head_stride,
@@ -1081,6 +1098,7 @@ extern "C" int genllm_gated_delta_rule(const void* q, int64_t q_batch_stride, in
     if (!aligned_to(a, gate_align) || !aligned_to(b, gate_align) || !aligned_to(a_log, 4) || !aligned_to(dt_bias, 4) ||
         !aligned_to(state_ids, 4) || !aligned_to(seq_lens, 4))
         return fail(GENLLM_ERR_INVALID, "gated_delta_rule: a pointer is not aligned to its type");
+    if (seq_len > (1 << 30)) return fail(GENLLM_ERR_INVALID, "gated_delta_rule: seq_len must be at most 2^30");
     if (int64_t(batch) * n_v_heads > (int64_t(1) << 19))  // a grid has at most 2^32 threads
         return fail(GENLLM_ERR_INVALID, "gated_delta_rule: batch * n_v_heads must be at most 2^19");
     p.a = a, p.b = b, p.a_batch = a_batch_stride, p.a_tok = a_tok_stride, p.b_batch = b_batch_stride, p.b_tok = b_tok_stride;

@@ -429,7 +429,7 @@ def _need(op, name, t, shape, dtype, device):
 
 def _elsewhere(dev: int) -> bool:
     """Whether `dev` is not the current device: the call is then made again with it current."""
-    return _current_device is None or dev != _current_device()
+    return dev != (_current_device or torch.cuda.current_device)()
 
 
 def _stream_on(dev: int, stream):

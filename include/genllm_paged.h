@@ -367,11 +367,14 @@ int genllm_linear(const void *x, const void *w, const void *bias, void *out, int
  * beta, fp32.  g must be <= 0 (-inf clears the state).  q, k [batch][seq_len]
  * [n_k_heads][k_dim]; v, out [batch][seq_len][n_v_heads][v_dim]; a, b [batch]
  * [seq_len][n_v_heads]; state [n_states][n_v_heads][k_dim][v_dim], read and
- * replaced.  k_dim and v_dim 64 or 128, rows 16-byte aligned.  A token or a few
- * run token by token; longer calls run in chunks and need a workspace of
- * genllm_gated_delta_workspace_bytes (0 where none is needed), whose contents
- * do not matter before or after the call; calls that share one must be
- * ordered. */
+ * replaced.  k_dim and v_dim 64 or 128, rows and the state 16-byte aligned.  out
+ * may be v (the same address and strides) and must not overlap the other
+ * inputs.  A NaN or infinite input shows from its token on, as in the rule.  A few
+ * tokens (up to 12, or 28 for many heads) run token by token; longer calls run
+ * in chunks and need a workspace of genllm_gated_delta_workspace_bytes (0 where
+ * none is needed, about 100 MB at most below 3000 value heads), 16-byte
+ * aligned, whose contents do not matter before or after the call; calls that
+ * share one must be ordered. */
 size_t genllm_gated_delta_workspace_bytes(int32_t batch, int32_t seq_len, int32_t n_k_heads, int32_t n_v_heads,
                                           int32_t k_dim, int32_t v_dim);
 int genllm_gated_delta_rule(const void *q, int64_t q_batch_stride, int64_t q_tok_stride, int64_t q_head_stride,

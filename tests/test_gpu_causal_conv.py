@@ -145,6 +145,30 @@ def test_turns_add_up_and_graph():
         assert torch.equal(whole, parts) and torch.equal(end, x["state"])
 
 
+def test_other_stream_and_channels_beside_each_other():
+    """On a stream of the caller's, from one half of a tensor's channels into the other."""
+    x = inputs(12, 2, 30, 64, 4)
+    both = torch.cat([x["x"], torch.zeros_like(x["x"])], -1)
+    want, new = causal_conv(x["x"], x["w"], x["state"], x["bias"])
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    paged.causal_conv(both[..., :64], x["w"], both[..., 64:], x["state"], bias=x["bias"], stream=stream)
+    stream.synchronize()
+    assert_rounded(both[..., 64:], want, "beside", slack(x))
+    assert torch.equal(both[..., :64], x["x"]) and torch.equal(x["state"].cpu().double(), new)
+
+
+def test_nothing_to_do():
+    x = inputs(13, 2, 4, 16, 4)
+    before = x["state"].clone()
+    out = torch.full((2, 4, 16), 3.0, dtype=BF16, device="cuda")
+    paged.causal_conv(x["x"][:, :0], x["w"], out[:, :0], x["state"])
+    paged.causal_conv(x["x"][:0], x["w"], out[:0], x["state"])
+    paged.causal_conv(x["x"], x["w"], out, x["state"], seq_lens=torch.zeros(2, dtype=torch.int32, device="cuda"))
+    torch.cuda.synchronize()
+    assert torch.equal(before, x["state"]) and bool((out == 3.0).all())
+
+
 def test_python_refusals():
     x = inputs(11, 1, 8, 16, 4)
     out = torch.zeros(1, 8, 16, dtype=BF16, device="cuda")

@@ -287,6 +287,121 @@ def test_other_stream_and_repeats(S):
     assert_state(outs[0][1], new, S, "stream")
 
 
+@pytest.mark.parametrize("S", [1, 2, 28, 29])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_many_heads(S, dtype):
+    """Enough heads for the wider waves, on both sides of the line between tokens and chunks."""
+    check(inputs(160 + S, 64, S, 2, 4, 64 if S > 2 else 128, 128, dtype), f"many heads, S={S}")
+
+
+@pytest.mark.parametrize("S", [4, 90, 150])
+def test_padding_holds_nan(S):
+    """What lies behind an entry's end never counts."""
+    x = inputs(170 + S, 3, S, 2, 4, 64, 64)
+    lens = torch.tensor([S, S // 2, 3], dtype=torch.int32)
+    want, new = reference(x, None, lens)
+    for c in ("q", "k", "v", "a", "b"):
+        x[c] = x[c].clone()
+        for i in range(3):
+            x[c][i, int(lens[i]) :] = math.nan
+    out = out_like(x, fill=-1.0)
+    call(x, out, seq_lens=lens.cuda())
+    torch.cuda.synchronize()
+    for i in range(3):
+        n = int(lens[i])
+        assert_rounded(out[i, :n], want[i, :n], f"entry {i}")
+        assert_state(x["state"][i], new[i], n, f"entry {i}")
+        assert bool((out[i, n:] == -1.0).all())
+
+
+@pytest.mark.parametrize("B,S,Hv,lens", [(1, 6400, 64, None), (3, 1600, 96, None), (2, 3300, 96, [3300, 1000])])
+def test_more_than_one_launch_holds(B, S, Hv, lens):
+    """Calls whose chunks or entries go through several launches: the bits of shorter calls, cut at whole chunks (the
+    state passes between calls as it passes between launches)."""
+    x = inputs(180 + B, B, S, Hv // 2, Hv, 64, 64)
+    first = x["state"].clone()
+    ln = torch.tensor(lens, dtype=torch.int32) if lens else None
+    whole = out_like(x, fill=2.0)
+    call(x, whole, **(dict(seq_lens=ln.cuda()) if lens else {}))
+    end = x["state"].clone()
+    x["state"].copy_(first)
+    parts, at = out_like(x, fill=2.0), 0
+    for n in (64, 640, 320, S - 1024):
+        y = dict(x, **{c: x[c][:, at : at + n] for c in ("q", "k", "v", "a", "b")})
+        call(y, parts[:, at : at + n], **(dict(seq_lens=(ln - at).cuda()) if lens else {}))
+        at += n
+    torch.cuda.synchronize()
+    assert torch.equal(whole, parts) and torch.equal(end, x["state"])
+    assert bool(torch.isfinite(end).all())
+
+
+@pytest.mark.parametrize("S", [1, 5, 70, 200])
+def test_out_is_v(S):
+    x = inputs(190 + S, 2, S, 2, 4, 64, 128)
+    want, new = reference(x)
+    call(x, x["v"])
+    torch.cuda.synchronize()
+    assert_rounded(x["v"], want, "out is v")
+    assert_state(x["state"], new, S, "out is v")
+
+
+def test_out_is_v_where_tokens_run_alone():
+    """A chunk that runs token by token, written over its own v."""
+    x = inputs(195, 1, 150, 1, 2, 64, 64, raw=False)
+    x["v"][0, 80, 0, 3] = math.nan
+    want, _ = reference(x)
+    call(x, x["v"])
+    torch.cuda.synchronize()
+    keep = [c for c in range(64) if c != 3]
+    assert_rounded(x["v"][..., keep], want[..., keep], "other columns")
+    assert_rounded(x["v"][:, :80], want[:, :80], "before")
+    assert bool(torch.isnan(x["v"][0, 80:, 0, 3]).all())
+
+
+def test_two_streams_and_a_shared_workspace_in_order():
+    """Two calls at once, each with its own workspace; then two graphs that share one, replayed in turn."""
+    xs = [inputs(200 + i, 1, 300, 2, 4, 128, 128) for i in range(2)]
+    refs = [reference(x) for x in xs]
+    firsts = [x["state"].clone() for x in xs]
+    outs = [out_like(x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    for x, out, s in zip(xs, outs, streams):
+        call(x, out, stream=s)
+    torch.cuda.synchronize()
+    for x, out, (want, new) in zip(xs, outs, refs):
+        assert_rounded(out, want, "at once")
+        assert_state(x["state"], new, 300, "at once")
+    eager = [(o.clone(), x["state"].clone()) for o, x in zip(outs, xs)]
+    ws = torch.empty(paged.gated_delta_workspace_bytes(1, 300, 2, 4, 128, 128), dtype=torch.uint8, device="cuda")
+    graphs = []
+    for x, out in zip(xs, outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(x, out, workspace=ws)
+        graphs.append(g)
+    for _ in range(3):
+        for x, f, out in zip(xs, firsts, outs):
+            x["state"].copy_(f)
+            out.zero_()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for x, out, (o, s) in zip(xs, outs, eager):
+            assert torch.equal(out, o) and torch.equal(x["state"], s)
+
+
+def test_large_and_small_values():
+    """Keys, values and states far from 1: the normalised keys' scale does not matter, the values' goes through."""
+    for scale in (1e-18, 1e18):
+        x = inputs(210, 1, 100, 1, 2, 64, 64)
+        x["v"].mul_(scale)
+        x["state"].mul_(scale)
+        x["k"].mul_(2.0 ** 20 if scale > 1 else 2.0 ** -5)
+        x["q"].mul_(2.0 ** -5)
+        check(x, f"values of {scale}")
+
+
 def test_nothing_to_do():
     x = inputs(140, 2, 4, 1, 2, 64, 64)
     before = x["state"].clone()

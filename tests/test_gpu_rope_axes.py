@@ -117,6 +117,25 @@ def test_graph_replays():
         assert all(torch.equal(a, b) for a, b in zip(got, outs))
 
 
+@pytest.mark.parametrize("S,Hq,Hk,D", [(700, 40, 8, 256), (3000, 12, 4, 128), (1, 70, 9, 256), (5, 200, 60, 64)])
+def test_many_rows(S, Hq, Hk, D):
+    """Several rows per lane, and tokens with more heads than a workgroup has rows."""
+    check(inputs(20, S, Hq, Hk, D, 64, 3, rows=64), (11, 11, 10), True, f"{S} x {Hq}+{Hk} of {D}")
+
+
+def test_other_stream():
+    x = inputs(21, 40, 8, 2, 256, 64, 3)
+    outs = [torch.zeros_like(x["q"]), torch.zeros_like(x["k"])]
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    paged.qk_norm_rope_axes(x["q"], x["k"], *outs, x["gamma_q"], x["gamma_k"], EPS, x["cos"], x["sin"], x["pos"],
+                            (11, 11, 10), True, stream=stream)
+    stream.synchronize()
+    for c, o in zip("qk", outs):
+        want = norm_rope_axes(x[c], x["gamma_" + c], EPS, x["cos"], x["sin"], x["pos"], (11, 11, 10), True)
+        assert_rounded(o, want, c, SLACK)
+
+
 def test_python_refusals():
     x = inputs(8, 4, 2, 1, 64, 64, 3)
     o, p = torch.zeros_like(x["q"]), torch.zeros_like(x["k"])

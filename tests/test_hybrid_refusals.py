@@ -46,7 +46,7 @@ def axes(sections=(11, 11, 10), **kw):
     (dict(state=0x80004), INV, b"16-byte aligned"), (dict(a=0x40001), INV, b"aligned to its type"),
     (dict(a=0x40002, a_log=None, dt=None), INV, b"aligned to its type"), (dict(ids=0x1002), INV, b"aligned to its type"),
     (dict(ot=0), INV, b"share memory"), (dict(oh=0), INV, b"share memory"),
-    (dict(B=1 << 16, Hv=16, n=1 << 16), INV, b"2^19"), (dict(S=100), INV, b"workspace"),
+    (dict(B=1 << 16, Hv=16, n=1 << 16), INV, b"2^19"), (dict(S=100), INV, b"workspace"), (dict(S=(1 << 30) + 1), INV, b"2^30"),
     (dict(S=100, ws=0xA00000, wsb=100), INV, b"workspace"), (dict(S=100, ws=0xA00004, wsb=1 << 40), INV, b"workspace"),
 ])
 def test_gated_delta_rule(kw, code, msg):
