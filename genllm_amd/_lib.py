@@ -136,6 +136,26 @@ def lib() -> C.CDLL:
     return _lib
 
 
+_calls = None
+
+
+def calls():
+    """The module of calls on tensors (csrc/calls.cpp), bound to the loaded library; raises if it has not been built."""
+    global _calls
+    if _calls is None:
+        L = lib()
+        try:
+            from . import _calls as module
+        except ImportError as e:
+            raise RuntimeError(f"{HERE}/_calls.so does not load ({e}): run __graft_entry__.build() "
+                               "(make -C genllm_amd/csrc)") from e
+        module.bind(*(C.cast(getattr(L, name), _P).value
+                      for name in ("genllm_gated_delta_workspace_bytes", "genllm_gated_delta_rule", "genllm_causal_conv",
+                                   "genllm_qk_norm_rope_axes")))
+        _calls = module
+    return _calls
+
+
 def check(rc: int):
     if rc != OK:
         raise GenllmError(rc, lib().genllm_last_error().decode())

@@ -417,43 +417,12 @@ def linear(x, w, out, bias=None, workspace=None, stream=None):
 
 
 # ----------------------------------------------------------- hybrid layers
-_ELEMENT_CODES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
-
-
-def _need(op, name, t, shape, dtype, device):
-    """t is a tensor of that shape, type and device whose last dim is dense."""
-    if t.shape != shape or t.dtype != dtype or t.device != device or (t.stride(-1) != 1 and t.shape[-1] > 1):
-        raise ValueError(f"{op}: {name} must be {dtype} {tuple(shape)} on {device}, the last dim dense; got "
-                         f"{t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
-
-
-def _elsewhere(dev: int) -> bool:
-    """Whether `dev` is not the current device: the call is then made again with it current."""
-    return dev != (_current_device or torch.cuda.current_device)()
-
-
-def _stream_on(dev: int, stream):
-    return _raw_stream(dev) if stream is None and _raw_stream is not None else _stream(stream)
-
-
-def _element_code(op, t):
-    code = _ELEMENT_CODES.get(t.dtype)
-    if code is None:
-        raise ValueError(f"{op}: bf16 or float16 elements, got {t.dtype}")
-    if not t.is_cuda:
-        raise ValueError("expected a GPU tensor")
-    return code
+# Their arguments are checked and passed on in csrc/calls.cpp.
 
 
 @functools.lru_cache(maxsize=1024)
 def gated_delta_workspace_bytes(batch: int, seq_len: int, n_k_heads: int, n_v_heads: int, k_dim: int, v_dim: int) -> int:
     return lib().genllm_gated_delta_workspace_bytes(batch, seq_len, n_k_heads, n_v_heads, k_dim, v_dim)
-
-
-def _check_entries(op, B, device, seq_lens, state_ids):
-    for name, t in (("seq_lens", seq_lens), ("state_ids", state_ids)):
-        if t is not None:
-            _need(op, name, t, (B,), torch.int32, device)
 
 
 def gated_delta_rule(q, k, v, a, b, state, out, scale: float, a_log=None, dt_bias=None, l2_eps=None, seq_lens=None,
@@ -468,56 +437,16 @@ def gated_delta_rule(q, k, v, a, b, state, out, scale: float, a_log=None, dt_bia
     (None: take them as they are).  seq_lens, state_ids [B] int32 on the
     GPU.  workspace: a device buffer of at least gated_delta_workspace_bytes(...)
     bytes when that is non-zero; None allocates one for this call."""
-    op = "gated_delta_rule"
-    code = _element_code(op, q)
-    qshape, vshape, dt, dev = q.shape, v.shape, q.dtype, q.get_device()
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
-            return gated_delta_rule(q, k, v, a, b, state, out, scale, a_log, dt_bias, l2_eps, seq_lens, state_ids, workspace,
-                                    stream)
-    B, S, Hk, Dk = qshape
-    Hv, Dv = vshape[-2:]
-    gate = torch.float32 if a_log is None else dt
-    qs, ks, vs, os_, as_, bs = q.stride(), k.stride(), v.stride(), out.stride(), a.stride(), b.stride()
-    # one pass over what has to agree; what does not is named below
-    if not (k.shape == qshape and vshape == (B, S, Hv, Dv) and out.shape == vshape and a.shape == b.shape == (B, S, Hv)
-            and k.dtype == v.dtype == out.dtype == dt and a.dtype == b.dtype == gate
-            and k.get_device() == v.get_device() == out.get_device() == a.get_device() == b.get_device() == dev
-            and qs[3] == ks[3] == vs[3] == os_[3] == 1 and (as_[2] == bs[2] == 1 or Hv == 1)):
-        device = q.device
-        for name, t, shape, dtype in (("q", q, qshape, dt), ("k", k, qshape, dt), ("v", v, (B, S, Hv, Dv), dt),
-                                      ("out", out, (B, S, Hv, Dv), dt), ("a", a, (B, S, Hv), gate),
-                                      ("b", b, (B, S, Hv), gate)):
-            _need(op, name, t, shape, dtype, device)
-    if state.shape[1:] != (Hv, Dk, Dv) or state.dtype != torch.float32 or state.get_device() != dev or not state.is_contiguous():
-        raise ValueError(f"{op}: state must be contiguous float32 [n, {Hv}, {Dk}, {Dv}] on {q.device}")
-    if (a_log is None) != (dt_bias is None):
-        raise ValueError(f"{op}: a_log and dt_bias go together")
-    if a_log is not None and not (a_log.shape == dt_bias.shape == (Hv,) and a_log.dtype == dt_bias.dtype == torch.float32
-                                  and a_log.get_device() == dt_bias.get_device() == dev
-                                  and a_log.is_contiguous() and dt_bias.is_contiguous()):
-        raise ValueError(f"{op}: a_log and dt_bias must be contiguous float32 [{Hv}] on {q.device}")
-    if seq_lens is not None or state_ids is not None:
-        _check_entries(op, B, q.device, seq_lens, state_ids)
-    need = gated_delta_workspace_bytes(B, S, Hk, Hv, Dk, Dv)
-    ws, ws_bytes = None, 0
-    if workspace is not None:
-        if workspace.get_device() != dev:
-            raise ValueError(f"{op}: the workspace must be on {q.device}")
-        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    elif need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        ws, ws_bytes = workspace.data_ptr(), need
-        if stream is not None:  # it goes back to the current stream's pool while `stream` still uses it
-            workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream)
-                                    else torch.cuda.ExternalStream(int(getattr(stream, "cuda_stream", stream)), device=q.device))
-    rc = (_lib._lib or lib()).genllm_gated_delta_rule(
-        q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
-        a.data_ptr(), as_[0], as_[1], b.data_ptr(), bs[0], bs[1], None if a_log is None else a_log.data_ptr(),
-        None if dt_bias is None else dt_bias.data_ptr(), state.data_ptr(), state.shape[0],
-        None if state_ids is None else state_ids.data_ptr(), None if seq_lens is None else seq_lens.data_ptr(),
-        out.data_ptr(), os_[0], os_[1], os_[2], B, S, Hk, Hv, Dk, Dv, code, scale, -1.0 if l2_eps is None else l2_eps, ws,
-        ws_bytes, _stream_on(dev, stream))
+    if stream is not None:
+        if workspace is None:
+            need = gated_delta_workspace_bytes(*q.shape[:3], v.shape[2], q.shape[3], v.shape[3])
+            if need:  # it goes back to the current stream's pool while `stream` still uses it
+                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+                workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream)
+                                        else torch.cuda.ExternalStream(_stream(stream), device=q.device))
+        stream = _stream(stream)
+    rc = (_lib._calls or _lib.calls()).gated_delta_rule(q, k, v, a, b, state, out, scale, a_log, dt_bias, l2_eps, seq_lens,
+                                                        state_ids, workspace, stream)
     if rc:
         check(rc)
 
@@ -529,33 +458,8 @@ def causal_conv(x, weight, out, state=None, bias=None, silu: bool = True, seq_le
     [C, W] with W 2 to 4, bias [C] or None, state [n, W - 1, C] or None (zeros
     before each sequence, none kept), all bf16 or all float16.  seq_lens,
     state_ids [B] int32 on the GPU."""
-    op = "causal_conv"
-    code = _element_code(op, x)
-    shape, dt, dev = x.shape, x.dtype, x.get_device()
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
-            return causal_conv(x, weight, out, state, bias, silu, seq_lens, state_ids, stream)
-    B, S, Ch = shape
-    W = weight.shape[-1]
-    xs, os_ = x.stride(), out.stride()
-    if not (out.shape == shape and out.dtype == dt and out.get_device() == dev and (xs[2] == os_[2] == 1 or Ch == 1)):
-        _need(op, "x", x, shape, dt, x.device)
-        _need(op, "out", out, shape, dt, x.device)
-    if weight.shape != (Ch, W) or weight.dtype != dt or weight.get_device() != dev or not weight.is_contiguous():
-        raise ValueError(f"{op}: weight must be contiguous {dt} [{Ch}, W] on {x.device}")
-    if bias is not None:
-        _need(op, "bias", bias, (Ch,), dt, x.device)
-    n, sp = 0, None
-    if state is not None:
-        n, sp = state.shape[0], state.data_ptr()
-        if state.shape != (n, W - 1, Ch) or state.dtype != dt or state.get_device() != dev or not state.is_contiguous():
-            raise ValueError(f"{op}: state must be contiguous {dt} [n, {W - 1}, {Ch}] on {x.device}")
-    if seq_lens is not None or state_ids is not None:
-        _check_entries(op, B, x.device, seq_lens, state_ids)
-    rc = (_lib._lib or lib()).genllm_causal_conv(
-        x.data_ptr(), xs[0], xs[1], weight.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), os_[0],
-        os_[1], sp, n, None if state_ids is None else state_ids.data_ptr(),
-        None if seq_lens is None else seq_lens.data_ptr(), B, S, Ch, W, code, int(silu), _stream_on(dev, stream))
+    rc = (_lib._calls or _lib.calls()).causal_conv(x, weight, out, state, bias, silu, seq_lens, state_ids,
+                                                   None if stream is None else _stream(stream))
     if rc:
         check(rc)
 
@@ -569,52 +473,10 @@ def qk_norm_rope_axes(q, k, q_out, k_out, gamma_q, gamma_k, eps: float, cos, sin
     gamma_q, gamma_k [D] float32 or None (no norm).  cos, sin [max_seq, rope_dim]
     float32, contiguous, as rope_cache makes them; positions [n_axes, S] int32 on
     the GPU; sections: the pairs of each axis, on the host."""
-    op = "qk_norm_rope_axes"
-    code = _element_code(op, q)
-    shape, dt, dev = q.shape, q.dtype, q.get_device()
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
-            return qk_norm_rope_axes(q, k, q_out, k_out, gamma_q, gamma_k, eps, cos, sin, positions, sections, interleaved,
-                                     stream)
-    S, Hq, D = shape
-    n_axes = len(sections)
-    qs, qos = q.stride(), q_out.stride()
-    if not (q_out.shape == shape and q_out.dtype == dt and q_out.get_device() == dev and qs[2] == qos[2] == 1):
-        _need(op, "q", q, shape, dt, q.device)
-        _need(op, "q_out", q_out, shape, dt, q.device)
-    Hk, kp, ks, kop, kos = 0, None, (0, 0), None, (0, 0)
-    if k is not None:
-        kshape, ks, kos = k.shape, k.stride(), k_out.stride()
-        Hk = kshape[1]
-        if not (kshape == k_out.shape == (S, Hk, D) and k.dtype == k_out.dtype == dt
-                and k.get_device() == k_out.get_device() == dev and ks[2] == kos[2] == 1):
-            _need(op, "k", k, (S, Hk, D), dt, q.device)
-            _need(op, "k_out", k_out, (S, Hk, D), dt, q.device)
-        kp, kop = k.data_ptr(), k_out.data_ptr()
-    for gamma in (gamma_q, gamma_k):
-        if gamma is not None and not (gamma.shape == (D,) and gamma.dtype == torch.float32 and gamma.get_device() == dev
-                                      and gamma.is_contiguous()):
-            _need(op, "gamma", gamma, (D,), torch.float32, q.device)
-    table = cos.shape
-    max_seq, rope_dim = table
-    if not (sin.shape == table and cos.dtype == sin.dtype == torch.float32 and cos.get_device() == sin.get_device() == dev
-            and cos.is_contiguous() and sin.is_contiguous()):
-        raise ValueError(f"{op}: cos and sin must be contiguous float32 [max_seq, rope_dim] on {q.device}")
-    ps = positions.stride()
-    if positions.shape != (n_axes, S) or positions.dtype != torch.int32 or positions.get_device() != dev or (ps[1] != 1 and S > 1):
-        raise ValueError(f"{op}: positions must be int32 [{n_axes}, {S}] on {q.device}, the tokens dense")
-    rc = (_lib._lib or lib()).genllm_qk_norm_rope_axes(
-        q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), qos[0], qos[1], None if gamma_q is None else gamma_q.data_ptr(), Hq,
-        kp, ks[0], ks[1], kop, kos[0], kos[1], None if gamma_k is None else gamma_k.data_ptr(), Hk, eps, cos.data_ptr(),
-        sin.data_ptr(), max_seq, rope_dim, positions.data_ptr(), ps[0], n_axes, _section_array(tuple(sections)),
-        int(interleaved), S, D, code, _stream_on(dev, stream))
+    rc = (_lib._calls or _lib.calls()).qk_norm_rope_axes(q, k, q_out, k_out, gamma_q, gamma_k, eps, cos, sin, positions, sections,
+                                                         interleaved, None if stream is None else _stream(stream))
     if rc:
         check(rc)
-
-
-@functools.lru_cache(maxsize=64)
-def _section_array(sections):
-    return (C.c_int32 * len(sections))(*sections)
 
 
 def fill_normal_bf16(t: torch.Tensor, seed: int, offset: int = 0, stream=None):

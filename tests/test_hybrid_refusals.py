@@ -3,8 +3,9 @@ addresses below are aligned placeholders that no check lets through to a launch.
 import ctypes as C
 
 import pytest
+import torch
 
-from genllm_amd import _lib
+from genllm_amd import _lib, paged
 
 INV, UNS = _lib.ERR_INVALID, _lib.ERR_UNSUPPORTED
 NAN, INF = float("nan"), float("inf")
@@ -96,3 +97,31 @@ def test_qk_norm_rope_axes(kw, code, msg):
 def test_qk_norm_rope_axes_nothing_to_do():
     for kw in (dict(S=0), dict(Hq=0, Hk=0, q=None, k=None)):
         assert axes(**kw) == _lib.OK
+
+
+def _bf16(*shape):
+    return torch.zeros(shape, dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("call", [
+    lambda t: paged.gated_delta_rule(t, t, t, t, t, t, t, 1.0),
+    lambda t: paged.causal_conv(t, t, t),
+    lambda t: paged.qk_norm_rope_axes(t, None, t, None, None, None, 1e-6, t, t, t, (1,)),
+])
+def test_calls_on_tensors(call):
+    """What is no tensor, has another type or is not on a GPU is refused before anything else is looked at."""
+    for bad, msg in ((3, "must be a tensor"), (None, "must be a tensor"), (torch.zeros(2, 2, 2), "bf16 or float16"),
+                     (_bf16(2, 2, 2), "GPU tensor"), (_bf16(2, 2, 2).to_sparse(), "strided")):
+        with pytest.raises(ValueError, match=msg):
+            call(bad)
+
+
+def test_calls_argument_count():
+    m = _lib.calls()
+    for f in (m.gated_delta_rule, m.causal_conv, m.qk_norm_rope_axes):
+        with pytest.raises(TypeError):
+            f(1)
+    with pytest.raises(TypeError):
+        m.bind(0)
+    with pytest.raises(ValueError):
+        m.bind(0, 0, 0, 0)
