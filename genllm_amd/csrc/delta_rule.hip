@@ -252,7 +252,8 @@ constexpr int kTriFrags = 6;
 constexpr int kTPart = kTriFrags * kFrag;        // elements of one part of T or P
 constexpr int kUnitT = 0, kUnitP = 3 * kTPart;   // T in three parts, P in two
 constexpr int kUnitVec = 5 * kTPart;             // floats: see kVec*
-constexpr int kVecC = 0, kVecD = 64, kVecE = 128, kVecLast = 192, kVecBad = 193, kVecFloats = 256;
+constexpr int kVecC = 0, kVecD = 64, kVecE = 128, kVecLast = 192, kVecBad = 196, kVecFloats = 256;
+// kVecBad: a flag per wave of the preparation, read by the wave of the scan with that number
 constexpr int kUnitElems = kUnitVec + 2 * kVecFloats;
 __device__ __forceinline__ constexpr int tri_frag(int tile, int ks) { return tile < 2 ? tile : 2 * tile - 2 + ks; }
 
@@ -415,13 +416,14 @@ __global__ __launch_bounds__(256, 4) void delta_chunk_prepare_kernel(DeltaParams
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) *reinterpret_cast<uint4*>(s_k + (16 * w + (lane >> 2)) * LK + 32 * ks + 8 * (lane & 3)) = kin[ks];
     __syncthreads();
-    // what is not finite (or an infinite factor) would reach earlier tokens
-    // through the zeros of T: the scan runs such a chunk token by token
+    // What is not finite, or a factor that may overflow, would reach earlier tokens
+    // through the zeros of T: the scan runs such a chunk token by token.  64 log
+    // decays of at most 1 leave e^G below 2^93.
     bool odd = false;
     if (w == 0) {
         // the running sum in 64 bits: differences of far sums enter the exponents;
         // exp(-2000) is 0 in either precision
-        odd = !(fabsf(g < -2000.0f ? -2000.0f : g) < INFINITY) || !(fabsf(beta) < INFINITY);
+        odd = !(g <= 1.0f) || !(fabsf(beta) < INFINITY);
         s_g[lane] = wave_running_sum(double(g < -2000.0f ? -2000.0f : g) * 1.4426950408889634);
         s_beta[lane] = beta;
     }
@@ -504,7 +506,7 @@ __global__ __launch_bounds__(256, 4) void delta_chunk_prepare_kernel(DeltaParams
         vec[kVecC + lane] = s_rk[lane] * exp2_fast(float(at));
         vec[kVecD + lane] = s_rk[lane] * exp2_fast(float(last - at));
         vec[kVecE + lane] = s_rq[lane] * exp2_fast(float(at));
-        if (lane == 0) vec[kVecLast] = exp2_fast(float(last)), vec[kVecBad] = s_bad ? 1.0f : 0.0f;
+        if (lane == 0) vec[kVecLast] = exp2_fast(float(last));
     }
     __syncthreads();  // K has been read, L is there
     // the inverse of diagonal block w: column r in every lane group, by substitution
@@ -552,23 +554,30 @@ __global__ __launch_bounds__(256, 4) void delta_chunk_prepare_kernel(DeltaParams
         put(s_t, bi, bj, m, -1.0f);
     }
     __syncthreads();
+    float sum = 0.0f;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
         if (ks > w >> 1) continue;
         const int row = tile_row(w, r), col = 32 * ks + 8 * g4;
         const f32x4_t* const src = reinterpret_cast<const f32x4_t*>(s_t + row * LD + col);
         const f32x4_t* const bt = reinterpret_cast<const f32x4_t*>(s_beta + col);
-        const f32x4_t t[2] = {src[0] * bt[0], src[1] * bt[1]};
+        f32x4_t t[2] = {src[0] * bt[0], src[1] * bt[1]};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (col + i > row) t[i >> 2][i & 3] = 0.0f;  // what was never written
+            sum += fabsf(t[i >> 2][i & 3]);
+        }
         uint32_t a[4], d[4], e[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)  // right of the diagonal lies what was never written
-            split3(col + 2 * i > row ? 0.0f : t[i >> 1][2 * (i & 1)], col + 2 * i + 1 > row ? 0.0f : t[i >> 1][2 * (i & 1) + 1],
-                   a[i], d[i], e[i]);
+        for (int i = 0; i < 4; ++i) split3(t[i >> 1][2 * (i & 1)], t[i >> 1][2 * (i & 1) + 1], a[i], d[i], e[i]);
         uint16_t* const to = unit + kUnitT + tri_frag(w, ks) * kFrag + 8 * lane;
         *reinterpret_cast<uint4*>(to) = make_uint4(a[0], a[1], a[2], a[3]);
         *reinterpret_cast<uint4*>(to + kTPart) = make_uint4(d[0], d[1], d[2], d[3]);
         *reinterpret_cast<uint4*>(to + 2 * kTPart) = make_uint4(e[0], e[1], e[2], e[3]);
     }
+    // keys far above 1 without a normalisation: T may overflow where the rule itself does not
+    const bool over = __ballot(!(sum < INFINITY)) != 0;
+    if (lane == 0) vec[kVecBad + w] = over || s_bad ? 1.0f : 0.0f;
 }
 
 // A right operand of MT tiles' rows in lane order: 8 (MT = 2, a step of 32) or 4
@@ -683,7 +692,7 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
             k += kChunk * p.k.tok, v += kChunk * p.v.tok, unit += unit_step;
         };
         // Q, which the waves of out take after (1): half a chunk later, so that the
-        // loads spread over it (2048 tokens 59 -> 56 us)
+        // loads spread over it (2048 tokens 59 -> 57.6 us)
         const auto stage_q = [&](int n) {
             if (n >= chunks) return;
             const int last = end - 1 - begin - n * kChunk;
@@ -878,7 +887,7 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
         {  // (2)
             const f32x4_t x0 = s_x[tile * 64 + lane], x1 = s_x[(4 + tile) * 64 + lane], x2 = s_x[(8 + tile) * 64 + lane],
                           x3 = s_x[(12 + tile) * 64 + lane];
-            const float bad = in.vec[kVecBad];
+            const float bad = in.vec[kVecBad + tile];
             const f32x4_t z = (x0 + x1) + (x2 + x3);
             float y[4];
 #pragma unroll

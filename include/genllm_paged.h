@@ -361,10 +361,10 @@ int genllm_linear(const void *x, const void *w, const void *bias, void *out, int
  * n_k_heads)) the state S [k_dim][v_dim], fp32, takes token after token:
  *     S <- exp(g) S;  u = beta (v - S^T k);  S <- S + k u^T;  out = scale S^T q
  * with q, k the given rows or, where l2_eps >= 0, x / sqrt(sum x^2 + l2_eps)
- * (l2_eps < 0: as given; |k| should then be about 1 or less, as the rule itself
- * asks for).  a_log, dt_bias [n_v_heads] fp32: g = -exp(a_log) softplus(a +
+ * (l2_eps < 0: as given; with beta |k|^2 above 2 the rule itself diverges).  a_log, dt_bias [n_v_heads] fp32: g = -exp(a_log) softplus(a +
  * dt_bias) and beta = sigmoid(b), a and b elements; both null: a is g and b is
- * beta, fp32.  g must be <= 0 (-inf clears the state).  q, k [batch][seq_len]
+ * beta, fp32.  g is meant to be <= 0 (-inf clears the state); 64 tokens of which
+ * one has g > 1 run token by token, as those with what is not finite do.  q, k [batch][seq_len]
  * [n_k_heads][k_dim]; v, out [batch][seq_len][n_v_heads][v_dim]; a, b [batch]
  * [seq_len][n_v_heads]; state [n_states][n_v_heads][k_dim][v_dim], read and
  * replaced.  k_dim and v_dim 64 or 128, rows and the state 16-byte aligned.  out

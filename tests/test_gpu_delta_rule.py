@@ -402,6 +402,42 @@ def test_large_and_small_values():
         check(x, f"values of {scale}")
 
 
+@pytest.mark.parametrize("S", [5, 100, 200])
+@pytest.mark.parametrize("factor", [4, 16, 256])
+def test_keys_far_above_one(S, factor):
+    """Keys that are not normalised: a token's part grows by 1 - |k|^2 with every later one, as in the rule, and the
+    inverse of a whole chunk would overflow.  Only the last tokens have a value, so that the rule itself stays finite."""
+    x = inputs(160 + S, 1, S, 1, 2, 64, 64, raw=False, l2=False)
+    x["k"][:] = x["k"][:, :1] * factor
+    x["b"][:] = 1.0
+    x["a"][:] = 0.0
+    x["v"][:, : S - 3] = 0
+    x["state"][:] = 0
+    check(x, f"keys of {factor}, S={S}")
+
+
+@pytest.mark.parametrize("S", [6, 64, 150])
+@pytest.mark.parametrize("grow", [0.5, 5.0])
+def test_growing_states(S, grow):
+    """Positive log decays: the state grows, and by more than fp32 holds where nothing has been written yet."""
+    x = inputs(165 + S, 1, S, 1, 2, 64, 64, raw=False)
+    n = min(30, S // 2)
+    x["a"][:, :n] = grow
+    x["v"][:, :n] = 0
+    x["state"][:] = 0
+    check(x, f"growing by {grow}, S={S}")
+
+
+def test_large_betas():
+    for beta in (-3.0, 100.0, 1e30):
+        x = inputs(170, 1, 80, 1, 2, 64, 64, raw=False)
+        x["b"][0, 70, 0] = beta
+        x["v"][0, 71:] = 0
+        x["b"][0, 71:] = 0
+        x["a"][0, 71:] = 0
+        check(x, f"beta {beta}")
+
+
 def test_nothing_to_do():
     x = inputs(140, 2, 4, 1, 2, 64, 64)
     before = x["state"].clone()
