@@ -5,7 +5,10 @@
 //   (y[i], y[i + R/2]) rotated by row pos[axis(i)][token] of the cos/sin tables,
 //   i < R/2; the dims from R on pass through
 //
-// in fp32, rounded once.  Pair i belongs to the axis of its section: one section
+// in fp32, rounded once.  Every element is read and written once, which bounds long
+// calls (32 / 8 heads of 128, with cold caches: 2048 tokens 13.8 us, 3.0 TB/s; 32768
+// tokens 134 us, 5.0 TB/s); a short one is the launch and two loads after each other,
+// position then table (64 tokens 3.1 us).  Pair i belongs to the axis of its section: one section
 // after another, or interleaved (pair i to axis i mod n while that axis has
 // pairs left, else to axis 0).
 #include <algorithm>
@@ -60,7 +63,7 @@ __device__ __forceinline__ uint4 pack8(const float* f) {
 // pass through.  A workgroup has 256 NI / (D/16) rows of neighbouring tokens, or a
 // part of one token's heads: it gathers those tokens' cos and sin once, into LDS,
 // while its rows are on their way (a gather of 16 values per thread and row
-// instead: 11.4 against 5.9 us for 2048 tokens of 10 heads of 256).
+// instead: 11.4 against 7.5 us for 2048 tokens of 10 heads of 256).
 template <int D, int NI, bool F16>
 __global__ __launch_bounds__(256) void norm_rope_axes_kernel(AxesParams p) {
     constexpr int L = D / 16;
@@ -162,7 +165,11 @@ int launch_axes_rows(AxesParams& p, hipStream_t stream) {
     return GENLLM_OK;
 }
 
-// Four rows per lane where that still gives every CU four workgroups, else one
+// Four rows per lane where that still gives every CU four workgroups: a table row
+// serves four times the heads and more loads are in flight per lane.  Else one (one
+// against four, us: 32 / 8 heads of 128, 64 tokens 3.1 / 5.2, 1024 8.3 / 10.6, 4096
+// 24.2 / 24.2, 8192 43.2 / 40.4, 32768 154 / 134; 8 / 2 of 256, 2048 8.7 / 10.8, 8192 24.7 /
+// 25.5, 32768 79.0 / 77.8).
 template <int D, bool F16>
 int launch_axes_dim(AxesParams& p, hipStream_t stream) {
     const int64_t lanes = int64_t(p.S) * (int64_t(p.Hq) + p.Hk) * (D / 16);
@@ -241,6 +248,11 @@ extern "C" int genllm_qk_norm_rope_axes(const void* q, int64_t q_tok_stride, int
            qo_head_stride, gamma_q};
     p.k = {static_cast<const uint16_t*>(k), k_tok_stride, k_head_stride, static_cast<uint16_t*>(k_out), ko_tok_stride,
            ko_head_stride, gamma_k};
+    const auto moved = [](const AxesRows& r) { return r.x == r.out && (r.x_tok != r.o_tok || r.x_head != r.o_head); };
+    if ((n_q_heads && moved(p.q)) || (n_k_heads && moved(p.k)))
+        return fail(GENLLM_ERR_INVALID, "qk_norm_rope_axes: an output over its input needs the same strides");
+    if (n_q_heads && n_k_heads && (p.q.x == p.k.out || p.k.x == p.q.out || p.q.out == p.k.out))
+        return fail(GENLLM_ERR_INVALID, "qk_norm_rope_axes: an output overlaps the other input or output");
     if ((n_q_heads && !rows_ok(p.q)) || (n_k_heads && !rows_ok(p.k)))
         return fail(GENLLM_ERR_INVALID, "qk_norm_rope_axes: q, k, their outputs and gammas must be 16-byte aligned");
     if (!aligned_to(cos_tab, 4) || !aligned_to(sin_tab, 4) || !aligned_to(positions, 4))

@@ -403,7 +403,8 @@ int genllm_causal_conv(const void *x, int64_t x_batch_stride, int64_t x_tok_stri
  * gamma), then the rotation by positions on n_axes axes (1 to 4), in one pass,
  * fp32, rounded once.  q, k and their outputs are rows of head_dim (64, 128 or
  * 256) at tok and head strides of their own, 16-byte aligned as the gammas are
- * (an output may be its input, with the same strides); a head count of 0 leaves that part out.
+ * (an output may be its input, with the same strides, and must not overlap the
+ * inputs otherwise); a head count of 0 leaves that part out.
  * The first rope_dim dims (a multiple of 16) rotate in pairs (i, i + rope_dim/2)
  * by row positions[axis * pos_stride + token] (device) of the tables
  * [max_seq][rope_dim] that genllm_rope_cache makes, the others pass through.

@@ -47,6 +47,8 @@ def axes(sections=(11, 11, 10), **kw):
     (dict(state=0x80004), INV, b"16-byte aligned"), (dict(a=0x40001), INV, b"aligned to its type"),
     (dict(a=0x40002, a_log=None, dt=None), INV, b"aligned to its type"), (dict(ids=0x1002), INV, b"aligned to its type"),
     (dict(ot=0), INV, b"share memory"), (dict(oh=0), INV, b"share memory"),
+    (dict(out=0x10000), INV, b"overlaps"), (dict(out=0x20000), INV, b"overlaps"), (dict(out=0x80000), INV, b"overlaps"),
+    (dict(out=0x30000, ot=4096), INV, b"overlaps"),
     (dict(B=1 << 16, Hv=16, n=1 << 16), INV, b"2^19"), (dict(S=100), INV, b"workspace"), (dict(S=(1 << 30) + 1), INV, b"2^30"),
     (dict(S=100, ws=0xA00000, wsb=100), INV, b"workspace"), (dict(S=100, ws=0xA00004, wsb=1 << 40), INV, b"workspace"),
 ])
@@ -64,6 +66,7 @@ def test_gated_delta_rule_nothing_to_do():
     *[({p: None}, INV, b"null pointer") for p in ("x", "w", "out")],
     (dict(W=1), UNS, b"widths"), (dict(W=5), UNS, b"widths"), (dict(dtype=7), UNS, b"bf16 or fp16"),
     (dict(C=-1), INV, b"negative"), (dict(n=1), INV, b"fewer states"), (dict(state=None, ids=0x1000), INV, b"without a state"),
+    (dict(state=0x100000), INV, b"state overlaps"), (dict(state=0x900000), INV, b"state overlaps"),
     (dict(x=0x100001), INV, b"aligned"), (dict(ot=0), INV, b"share memory"), (dict(out=0x100000), INV, b"overlaps"),
     (dict(out=0x100000 + 2 * 64 * 3), INV, b"overlaps"), (dict(out=0x100000 - 64), INV, b"overlaps"),
     (dict(out=0x100000 + 2 * 64, xt=96, ot=96, xb=96 * 64, ob=96 * 64), INV, b"overlaps"),
@@ -87,6 +90,8 @@ def test_causal_conv_nothing_to_do():
     (dict(sections=(20, 20, -8)), INV, b"negative section"), (dict(sections=(2, 15, 15)), INV, b"interleaved"),
     (dict(eps=-1.0), INV, b"eps"), (dict(eps=NAN), INV, b"eps"), (dict(S=-1), INV, b"negative"), (dict(Hk=-1), INV, b"negative"),
     (dict(q=0x10008), INV, b"16-byte"), (dict(kot=4), INV, b"16-byte"), (dict(gk=0x60002), INV, b"16-byte"),
+    (dict(qo=0x10000), INV, b"same strides"), (dict(ko=0x40000), INV, b"same strides"), (dict(qo=0x40000), INV, b"overlaps"),
+    (dict(ko=0x10000), INV, b"overlaps"), (dict(ko=0x20000), INV, b"overlaps"),
     (dict(cos=0x70001), INV, b"aligned to its type"), (dict(qot=0), INV, b"share memory"), (dict(koh=0), INV, b"share memory"),
 ])
 def test_qk_norm_rope_axes(kw, code, msg):
