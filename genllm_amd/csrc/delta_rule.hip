@@ -625,7 +625,7 @@ __device__ __forceinline__ DeltaParams kernel_params() {
 //   shares and Y = V - diag(e^G) K S0 for token tile w; (3) wave w: tile w of U = T Y;
 //   (4) wave w: its rows of the new state, S <- e^(G_last) S + K^T diag(e^(G_last - G)) U.
 // Waves 4 to 7 have the state and U from LDS and form out, tile w - 4: Q S0
-// during (2), P U during (4).  Waves 8 to 11 load what waves 0 to 3 need straight
+// during (2), P U and the reads of the next Q during (4).  Waves 8 to 11 load what waves 0 to 3 need straight
 // into LDS, two chunks ahead: the chain (1) to (4) is bound by the instructions
 // that one wave can issue, and 53 KB a chunk keep the memory pipe busy.  Rows
 // behind the end come as copies of the last row; T has zeros in their place.
@@ -640,12 +640,12 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
     using Op = Operand<MT>;
     struct Stage {
         uint4 k[4 * KS * 64];                      // [token tile][step][row_unit]
-        uint4 q[4 * KS * 64];
         uint4 t[3 * kTriFrags * 64];               // [part][fragment][lane]
         uint16_t v[kChunk * kScanCols];
         float vec[kVecFloats];
     };
     __shared__ __attribute__((aligned(16))) Stage s_in[2];
+    __shared__ uint4 s_q[4 * KS * 64];
     __shared__ f32x4_t s_x[4 * 4 * 64];     // shares of K S0 [wave][token tile][lane]
     __shared__ uint4 s_s[2 * KS * 64];      // the state in two parts [part][step][lane]
     __shared__ uint4 s_y[3 * 2 * 64];       // Y in three parts [part][step][lane], a tile's half of each
@@ -702,14 +702,14 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
                 load_lds(unit + kUnitVec, to.vec);
             k += kChunk * p.k.tok, v += kChunk * p.v.tok, unit += unit_step;
         };
-        // Q, which the waves of out take after (1): half a chunk later, so that the
+        // Q, which the waves of out have taken by (1): half a chunk later, so that the
         // loads spread over it (2048 tokens 59 -> 57.6 us)
         const auto stage_q = [&](int n) {
             if (n >= chunks) return;
             const int last = end - 1 - begin - n * kChunk;
             if (last < kChunk - 1) q_at = min(krow, last) * p.q.tok;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) load_lds(q + q_at + 32 * ks, s_in[n & 1].q + (tile * KS + ks) * 64);
+            for (int ks = 0; ks < KS; ++ks) load_lds(q + q_at + 32 * ks, s_q + (tile * KS + ks) * 64);
             q += kChunk * p.q.tok;
         };
         stage(0);
@@ -719,7 +719,7 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
         stage(1);
         for (int n = 0; n < chunks; ++n) {
             lds_barrier();  // (1)
-            stage_q(n + 1);  // where chunk n - 1's was
+            stage_q(n + 1);  // in chunk n's place
             lds_barrier();   // (2)
             __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);  // chunk n + 1 is there, for all after (3)
             const int slow_word = s_bad;
@@ -750,8 +750,17 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
             }
             unit += unit_step;
         };
+        uint4 q0[KS], q1[KS];
+        const auto load_q = [&]() {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                q0[ks] = s_q[(tile * KS + ks) * 64 + unit_at];
+                if constexpr (F16) split_f16(q0[ks], q0[ks], q1[ks]);
+            }
+        };
         load_tri(0);
         lds_barrier();  // chunk 0 is there
+        load_q();
         for (int n = 0; n < chunks; ++n) {
             lds_barrier();  // (1)
             e = *reinterpret_cast<const f32x4_t*>(s_in[n & 1].vec + kVecE + tok0);
@@ -759,11 +768,9 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const uint4 s0 = s_s[ks * 64 + lane], s1 = s_s[(KS + ks) * 64 + lane];
-                uint4 x0 = s_in[n & 1].q[(tile * KS + ks) * 64 + unit_at], x1;
-                if constexpr (F16) split_f16(x0, x0, x1);
-                a0 = mma(x0, s0, a0);
-                a1 = mma(x0, s1, a1);
-                if constexpr (F16) a1 = mma(x1, s0, a1);
+                a0 = mma(q0[ks], s0, a0);
+                a1 = mma(q0[ks], s1, a1);
+                if constexpr (F16) a1 = mma(q1[ks], s0, a1);
             }
             a0 = (a0 + a1) * e;
             a1 = zero;
@@ -794,6 +801,7 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
                 }
             }
             load_tri(n + 1);
+            load_q();  // of chunk n + 1
             out += kChunk * p.o_tok;
         }
         return;
@@ -841,25 +849,37 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
     lds_barrier();
     for (int n = 0; n < chunks; ++n) {
         const Stage& in = s_in[n & 1];
+        // all of the chunk that (1) to (3) take is on its way before the first use: left to
+        // itself the compiler puts most of these reads in front of the barrier (4 x 700
+        // tokens of 8 heads of 64 x 128, both kernels: 29.3 -> 28.6 us, with Q's reads in (4))
+        Op fk[4];
+        load_k(in, fk);
+        __builtin_amdgcn_sched_barrier(0);
         uint4 ft[2][3];
-        uint16_t v[4];
-        f32x4_t e;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            ft[0][i] = in.t[(i * kTriFrags + tri_frag(tile, 0)) * 64 + lane];
+            ft[1][i] = in.t[(i * kTriFrags + tri_frag(tile, tile >> 1)) * 64 + lane];
+        }
+        const f32x4_t e = *reinterpret_cast<const f32x4_t*>(in.vec + kVecC + tok0);
+        const f32x4_t d = *reinterpret_cast<const f32x4_t*>(in.vec + kVecD + tok0);
+        const float last = in.vec[kVecLast], bad = in.vec[kVecBad + tile];
+        const uint2 v = read_transposed(reinterpret_cast<const uint2*>(in.v) + 4 * (tok0 + (r >> 2)) + (r & 3));
+        __builtin_amdgcn_sched_barrier(0);
         {  // (1)
-            Op fk[4];
-            load_k(in, fk);
-            e = *reinterpret_cast<const f32x4_t*>(in.vec + kVecC + tok0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = in.v[(tok0 + i) * kScanCols + r];
-#pragma unroll
-            for (int i = 0; i < 3; ++i) {
-                ft[0][i] = in.t[(i * kTriFrags + tri_frag(tile, 0)) * 64 + lane];
-                ft[1][i] = in.t[(i * kTriFrags + tri_frag(tile, tile >> 1)) * 64 + lane];
-            }
             Op s0, s1, s2;
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
                 split3(s[m][0], s[m][1], s0.w[2 * m], s1.w[2 * m], s2.w[2 * m]);
                 split3(s[m][2], s[m][3], s0.w[2 * m + 1], s1.w[2 * m + 1], s2.w[2 * m + 1]);
+            }
+            if constexpr (MT == 2) {
+                s_s[w * 64 + lane] = make_uint4(s0.w[0], s0.w[1], s0.w[2], s0.w[3]);
+                s_s[(KS + w) * 64 + lane] = make_uint4(s1.w[0], s1.w[1], s1.w[2], s1.w[3]);
+            } else {
+                uint2* const to = reinterpret_cast<uint2*>(s_s) + 2 * ((w >> 1) * 64 + lane) + (w & 1);
+                to[0] = make_uint2(s0.w[0], s0.w[1]);
+                to[2 * KS * 64] = make_uint2(s1.w[0], s1.w[1]);
             }
             f32x4_t x[4];
             Op k0[4], k1[4];
@@ -880,29 +900,19 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
                 for (int j = 0; j < 4; ++j) x[j] = mma_step(k1[j], s0, x[j]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = mma_step(k0[j], s0, x[j]);
-            if constexpr (MT == 2) {
-                s_s[w * 64 + lane] = make_uint4(s0.w[0], s0.w[1], s0.w[2], s0.w[3]);
-                s_s[(KS + w) * 64 + lane] = make_uint4(s1.w[0], s1.w[1], s1.w[2], s1.w[3]);
-            } else {
-                uint2* const to = reinterpret_cast<uint2*>(s_s) + 2 * ((w >> 1) * 64 + lane) + (w & 1);
-                to[0] = make_uint2(s0.w[0], s0.w[1]);
-                to[2 * KS * 64] = make_uint2(s1.w[0], s1.w[1]);
-            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) s_x[(w * 4 + j) * 64 + lane] = x[j];
         }
         lds_barrier();  // (1)
         uint4 fkt[2 * MT];
-        const f32x4_t d = *reinterpret_cast<const f32x4_t*>(in.vec + kVecD + tok0);
-        const float last = in.vec[kVecLast];
         {  // (2)
             const f32x4_t x0 = s_x[tile * 64 + lane], x1 = s_x[(4 + tile) * 64 + lane], x2 = s_x[(8 + tile) * 64 + lane],
                           x3 = s_x[(12 + tile) * 64 + lane];
-            const float bad = in.vec[kVecBad + tile];
             const f32x4_t z = (x0 + x1) + (x2 + x3);
+            const float vf[4] = {Elem<F16>::lo(v.x), Elem<F16>::hi(v.x), Elem<F16>::lo(v.y), Elem<F16>::hi(v.y)};
             float y[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = Elem<F16>::lo(v[i]) - e[i] * z[i];
+            for (int i = 0; i < 4; ++i) y[i] = vf[i] - e[i] * z[i];
             put3(reinterpret_cast<uint2*>(s_y) + half, y[0], y[1], y[2], y[3]);
             // an overflow of this sum only means more care
             if (!((fabsf(y[0]) + fabsf(y[1])) + (fabsf(y[2]) + fabsf(y[3])) < INFINITY) || bad != 0.0f) s_bad = n + 1;
@@ -910,21 +920,27 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
         lds_barrier();  // (2)
         const int slow_word = s_bad;
         {  // (3)
+            uint4 y[2][3];
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int i = 0; i < 3; ++i) y[ks][i] = s_y[(2 * i + ks) * 64 + lane];
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) fkt[2 * m + ks] = k_t(in, m, ks);
+            __builtin_amdgcn_sched_barrier(0);
             f32x4_t a0 = zero, a1 = zero, a2 = zero;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
                 if (ks > tile >> 1) continue;
-                const uint4 y0 = s_y[ks * 64 + lane], y1 = s_y[(2 + ks) * 64 + lane], y2 = s_y[(4 + ks) * 64 + lane];
-                a2 = mma(ft[ks][0], y2, a2);
-                a1 = mma(ft[ks][0], y1, a1);
-                a0 = mma(ft[ks][0], y0, a0);
-                a2 = mma(ft[ks][1], y1, a2);
-                a1 = mma(ft[ks][1], y0, a1);
-                a2 = mma(ft[ks][2], y0, a2);
+                a2 = mma(ft[ks][0], y[ks][2], a2);
+                a1 = mma(ft[ks][0], y[ks][1], a1);
+                a0 = mma(ft[ks][0], y[ks][0], a0);
+                a2 = mma(ft[ks][1], y[ks][1], a2);
+                a1 = mma(ft[ks][1], y[ks][0], a1);
+                a2 = mma(ft[ks][2], y[ks][0], a2);
             }
             const f32x4_t u = a0 + (a1 + a2);
             put3(reinterpret_cast<uint2*>(s_d) + half, d[0] * u[0], d[1] * u[1], d[2] * u[2], d[3] * u[3]);
