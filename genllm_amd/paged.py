@@ -438,7 +438,7 @@ def gated_delta_rule(q, k, v, a, b, state, out, scale: float, a_log=None, dt_bia
     GPU.  workspace: a device buffer of at least gated_delta_workspace_bytes(...)
     bytes when that is non-zero; None allocates one for this call."""
     if stream is not None:
-        if workspace is None:
+        if workspace is None and all(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 4 for t in (q, v)):
             need = gated_delta_workspace_bytes(*q.shape[:3], v.shape[2], q.shape[3], v.shape[3])
             if need:  # it goes back to the current stream's pool while `stream` still uses it
                 workspace = torch.empty(need, dtype=torch.uint8, device=q.device)

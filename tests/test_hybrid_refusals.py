@@ -110,6 +110,7 @@ def _bf16(*shape):
 
 @pytest.mark.parametrize("call", [
     lambda t: paged.gated_delta_rule(t, t, t, t, t, t, t, 1.0),
+    lambda t: paged.gated_delta_rule(t, t, t, t, t, t, t, 1.0, stream=0),
     lambda t: paged.causal_conv(t, t, t),
     lambda t: paged.qk_norm_rope_axes(t, None, t, None, None, None, 1e-6, t, t, t, (1,)),
 ])
