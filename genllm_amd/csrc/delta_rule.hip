@@ -625,7 +625,7 @@ __device__ __forceinline__ DeltaParams kernel_params() {
 //   shares and Y = V - diag(e^G) K S0 for token tile w; (3) wave w: tile w of U = T Y;
 //   (4) wave w: its rows of the new state, S <- e^(G_last) S + K^T diag(e^(G_last - G)) U.
 // Waves 4 to 7 have the state and U from LDS and form out, tile w - 4: Q S0
-// during (2), P U and the reads of the next Q during (4).  Waves 8 to 11 load what waves 0 to 3 need straight
+// during (2), P U during (4).  Waves 8 to 11 load what waves 0 to 3 need straight
 // into LDS, two chunks ahead: the chain (1) to (4) is bound by the instructions
 // that one wave can issue, and 53 KB a chunk keep the memory pipe busy.  Rows
 // behind the end come as copies of the last row; T has zeros in their place.
@@ -640,12 +640,12 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
     using Op = Operand<MT>;
     struct Stage {
         uint4 k[4 * KS * 64];                      // [token tile][step][row_unit]
+        uint4 q[4 * KS * 64];
         uint4 t[3 * kTriFrags * 64];               // [part][fragment][lane]
         uint16_t v[kChunk * kScanCols];
         float vec[kVecFloats];
     };
     __shared__ __attribute__((aligned(16))) Stage s_in[2];
-    __shared__ uint4 s_q[4 * KS * 64];
     __shared__ f32x4_t s_x[4 * 4 * 64];     // shares of K S0 [wave][token tile][lane]
     __shared__ uint4 s_s[2 * KS * 64];      // the state in two parts [part][step][lane]
     __shared__ uint4 s_y[3 * 2 * 64];       // Y in three parts [part][step][lane], a tile's half of each
@@ -702,14 +702,14 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
                 load_lds(unit + kUnitVec, to.vec);
             k += kChunk * p.k.tok, v += kChunk * p.v.tok, unit += unit_step;
         };
-        // Q, which the waves of out have taken by (1): half a chunk later, so that the
+        // Q, which the waves of out take after (1), or have taken before it: half a chunk later, so that the
         // loads spread over it (2048 tokens 59 -> 57.6 us)
         const auto stage_q = [&](int n) {
             if (n >= chunks) return;
             const int last = end - 1 - begin - n * kChunk;
             if (last < kChunk - 1) q_at = min(krow, last) * p.q.tok;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) load_lds(q + q_at + 32 * ks, s_q + (tile * KS + ks) * 64);
+            for (int ks = 0; ks < KS; ++ks) load_lds(q + q_at + 32 * ks, s_in[n & 1].q + (tile * KS + ks) * 64);
             q += kChunk * p.q.tok;
         };
         stage(0);
@@ -719,7 +719,7 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
         stage(1);
         for (int n = 0; n < chunks; ++n) {
             lds_barrier();  // (1)
-            stage_q(n + 1);  // in chunk n's place
+            stage_q(n + 1);  // where chunk n - 1's was
             lds_barrier();   // (2)
             __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);  // chunk n + 1 is there, for all after (3)
             const int slow_word = s_bad;
@@ -750,21 +750,24 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
             }
             unit += unit_step;
         };
+        // fp16: Q is read and split during (4) of the chunk before (2048 tokens of 32 heads of
+        // 128 86.8 -> 83.2 us); bf16, with nothing to split, after (1) (68.3 against 69.4)
         uint4 q0[KS], q1[KS];
-        const auto load_q = [&]() {
+        const auto load_q = [&](int at) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                q0[ks] = s_q[(tile * KS + ks) * 64 + unit_at];
+                q0[ks] = s_in[at & 1].q[(tile * KS + ks) * 64 + unit_at];
                 if constexpr (F16) split_f16(q0[ks], q0[ks], q1[ks]);
             }
         };
         load_tri(0);
         lds_barrier();  // chunk 0 is there
-        load_q();
+        if constexpr (F16) load_q(0);
         for (int n = 0; n < chunks; ++n) {
             lds_barrier();  // (1)
             e = *reinterpret_cast<const f32x4_t*>(s_in[n & 1].vec + kVecE + tok0);
             f32x4_t a0 = zero, a1 = zero;
+            if constexpr (!F16) load_q(n);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const uint4 s0 = s_s[ks * 64 + lane], s1 = s_s[(KS + ks) * 64 + lane];
@@ -801,12 +804,15 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
                 }
             }
             load_tri(n + 1);
-            load_q();  // of chunk n + 1
+            if constexpr (F16) load_q(n + 1);
             out += kChunk * p.o_tok;
         }
         return;
     }
 
+    const auto in_order = [] {
+        if constexpr (!F16) __builtin_amdgcn_sched_barrier(0);
+    };
     __builtin_amdgcn_s_setprio(3);  // the chain goes first where waves meet on a SIMD
     const int row0 = tile_row(MT * w, 4 * g4);  // the lane's first row of the state; tile m: + 4 m
     float* const st = p.state + ((int64_t(slot) * p.Hv + h) * DK + row0) * p.Dv + col0 + r;
@@ -849,12 +855,13 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
     lds_barrier();
     for (int n = 0; n < chunks; ++n) {
         const Stage& in = s_in[n & 1];
-        // all of the chunk that (1) to (3) take is on its way before the first use: left to
-        // itself the compiler puts most of these reads in front of the barrier (4 x 700
-        // tokens of 8 heads of 64 x 128, both kernels: 29.3 -> 28.6 us, with Q's reads in (4))
+        // bf16: all of the chunk that (1) to (3) take is on its way before the first use (left
+        // to itself the compiler puts most of these reads in front of the barrier; 2048 tokens
+        // of 32 heads of 128, both kernels, 68.6 -> 68.3 us; fp16, with more registers in use,
+        // 83.2 without this order, 84.0 with it)
         Op fk[4];
         load_k(in, fk);
-        __builtin_amdgcn_sched_barrier(0);
+        in_order();
         uint4 ft[2][3];
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
@@ -865,7 +872,7 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
         const f32x4_t d = *reinterpret_cast<const f32x4_t*>(in.vec + kVecD + tok0);
         const float last = in.vec[kVecLast], bad = in.vec[kVecBad + tile];
         const uint2 v = read_transposed(reinterpret_cast<const uint2*>(in.v) + 4 * (tok0 + (r >> 2)) + (r & 3));
-        __builtin_amdgcn_sched_barrier(0);
+        in_order();
         {  // (1)
             Op s0, s1, s2;
 #pragma unroll
@@ -924,13 +931,14 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-                for (int i = 0; i < 3; ++i) y[ks][i] = s_y[(2 * i + ks) * 64 + lane];
-            __builtin_amdgcn_sched_barrier(0);
+                for (int i = 0; i < 3; ++i)
+                    if (ks <= tile >> 1) y[ks][i] = s_y[(2 * i + ks) * 64 + lane];
+            in_order();
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) fkt[2 * m + ks] = k_t(in, m, ks);
-            __builtin_amdgcn_sched_barrier(0);
+            in_order();
             f32x4_t a0 = zero, a1 = zero, a2 = zero;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
