@@ -325,6 +325,14 @@ __device__ __forceinline__ f32x4_t mm16(const f32x4_t& a, const f32x4_t& b, f32x
     return acc;
 }
 
+// The value head of workgroup i of Hv.  Workgroups go round the eight XCDs, and i, i +
+// 8, .. share an L2: an XCD takes Hv / 8 heads in a row, where the key heads allow it,
+// so that K and Q of a key head are read from memory once for its value heads (16 / 32
+// heads of 128, 2048 tokens: the preparation 18.4 -> 16.7 us, its reads 36 -> 19 MB).
+__device__ __forceinline__ int head_of(const DeltaParams& p, int i) {
+    return p.Hk & 7 ? i : (i & 7) * (p.Hv >> 3) + (i >> 3);
+}
+
 // LDS written before it is seen after it; loads from memory stay in flight (a
 // __syncthreads would wait for them too)
 __device__ __forceinline__ void lds_barrier() {
@@ -373,10 +381,10 @@ __device__ __forceinline__ double wave_running_sum(double x) {
 // fragments and L enters LDS in 16-byte writes.  (1 + L)^-1 by halves: the four
 // diagonal 16 x 16 blocks by substitution, a lane per column; then T10 = -T11
 // (L10 T00) for 16- and for 32-wide blocks, as fp32 matrix products.
-// 18.4 us for 2048 tokens of 16 / 32 heads of 128 (32 MB of units written, 17 MB read, 2.7
+// 16.7 us for 2048 tokens of 16 / 32 heads of 128 (32 MB of units written, 19 MB read, 3.1
 // TB/s): 1024 workgroups, all on the GPU at once, four to a CU, each bound by its own
 // chain (loads, norms, L, the substitution's 120 dependent steps, four products after
-// each other).  One workgroup's chain alone is most of it: 2048 workgroups take 33.3 us.
+// each other): 64 workgroups alone take 8 us, 2048 take 32.
 template <int DK, bool F16>
 __global__ __launch_bounds__(256, 4) void delta_chunk_prepare_kernel(DeltaParams p, ChunkPlan c) {
     constexpr int KS = DK / 32, LD = 68, LK = DK + 8;
@@ -388,7 +396,7 @@ __global__ __launch_bounds__(256, 4) void delta_chunk_prepare_kernel(DeltaParams
     __shared__ __attribute__((aligned(16))) double s_g[64];  // running sums of log2 of the decays
     __shared__ __attribute__((aligned(16))) float s_beta[64], s_rk[64], s_rq[64];
     __shared__ int s_bad;
-    const int h = int(blockIdx.x % uint32_t(p.Hv)), rest = int(blockIdx.x / uint32_t(p.Hv));
+    const int h = head_of(p, int(blockIdx.x % uint32_t(p.Hv))), rest = int(blockIdx.x / uint32_t(p.Hv));
     const int n = rest % c.count, b_at = rest / c.count, b = c.b_first + b_at;
     const int t0 = (c.first + n) * kChunk;
     const int slot = entry_state(p.seq, b), len = entry_len(p.seq, b);
@@ -657,7 +665,7 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
     prefetch_kernargs<sizeof(DeltaParams) + sizeof(ChunkPlan)>();
     const int heads = c.b_count * p.Hv;
     const int bh = int(blockIdx.x) % heads, col0 = int(blockIdx.x) / heads * kScanCols;
-    const int b_at = bh / p.Hv, b = c.b_first + b_at, h = bh - b_at * p.Hv, hk = h / p.G;
+    const int b_at = bh / p.Hv, b = c.b_first + b_at, h = head_of(p, bh - b_at * p.Hv), hk = h / p.G;
     const int slot = entry_state(p.seq, b), len = entry_len(p.seq, b);
     const int begin = c.first * kChunk;
     if (slot == kEntryEmpty || begin >= len) return;
