@@ -243,8 +243,7 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(DeltaParams p, int
 
 // ------------------------------------------------------------------ chunks
 constexpr int kChunk = 64;
-constexpr int kScanThreads = 768;
-constexpr int kScanCols = 16;  // columns of the state per workgroup of the scan
+constexpr int kScanCols = 16;  // columns of the state per chain of the scan
 
 // What the scan needs of one chunk and value head, in the order its lanes read
 // it: operand fragments of 64 lanes x 16 bytes.  Of the 64 x 64 triangles only
@@ -626,7 +625,7 @@ __device__ __forceinline__ DeltaParams kernel_params() {
     return p;
 }
 
-// 16 columns of one head's state from chunk to chunk, in twelve waves.  Waves 0
+// 16 columns of one head's state from chunk to chunk (a chain), in twelve waves.  Waves 0
 // to 3 keep the state: wave w its rows of the tiles MT w .. in fp32, as the
 // products leave them, which is also how the next product takes them.  Per chunk:
 //   (1) wave w: its rows' share of K S0 for all tokens; (2) wave w: the sum of the
@@ -639,32 +638,40 @@ __device__ __forceinline__ DeltaParams kernel_params() {
 // behind the end come as copies of the last row; T has zeros in their place.
 // 2048 tokens of 16 / 32 heads of 128: 57 us for 32 chunks, a workgroup per CU.  The
 // chain alone, with nothing loaded or stored, takes 51: three exchanges through LDS and
-// a product's latency between each two, 1.6 us a chunk.  More columns per workgroup
-// would leave CUs idle; fewer would read K, Q and T more often.
-template <int DK, bool F16>
-__global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaParams p, ChunkPlan c) {
+// a product's latency between each two, 1.6 us a chunk.
+// NC = 2: two chains of neighbouring columns beside each other, waves 0 to 3 and 4 to 7,
+// with K, Q and T in common.  They hide each other's latency where there are more
+// chains than CUs; the waves of out and of the loads, 8 to 11 and 12 to 15, serve both.
+// T and Q have one buffer then, and are taken into registers before (1).
+template <int NC>
+constexpr int kScanThreads = 256 * NC + 512;
+template <int DK, int NC, bool F16>
+__global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(DeltaParams p, ChunkPlan c) {
     constexpr int KS = DK / 32, MT = DK / 64;  // MT: 16-row tiles of the state per wave
     constexpr int LW = 20;
+    constexpr int TQ = NC == 1 ? 2 : 1;        // buffers of T and Q
+    constexpr bool kAhead = F16 || NC == 2;    // Q is in registers before (1)
     using Op = Operand<MT>;
     struct Stage {
         uint4 k[4 * KS * 64];                      // [token tile][step][row_unit]
-        uint4 q[4 * KS * 64];
-        uint4 t[3 * kTriFrags * 64];               // [part][fragment][lane]
-        uint16_t v[kChunk * kScanCols];
+        uint16_t v[kChunk * kScanCols * NC];
         float vec[kVecFloats];
     };
+    struct Exchange {                              // of one chain
+        f32x4_t x[4 * 4 * 64];                     // shares of K S0 [wave][token tile][lane]
+        uint4 s[2 * KS * 64];                      // the state in two parts [part][step][lane]
+        uint4 y[3 * 2 * 64];                       // Y in three parts [part][step][lane], a tile's half of each
+        uint4 d[3 * 2 * 64];                       // diag(e^(G_last - G)) U in three parts
+        uint4 u[2 * 2 * 64];                       // U in two
+    };
     __shared__ __attribute__((aligned(16))) Stage s_in[2];
-    __shared__ f32x4_t s_x[4 * 4 * 64];     // shares of K S0 [wave][token tile][lane]
-    __shared__ uint4 s_s[2 * KS * 64];      // the state in two parts [part][step][lane]
-    __shared__ uint4 s_y[3 * 2 * 64];       // Y in three parts [part][step][lane], a tile's half of each
-    __shared__ uint4 s_d[3 * 2 * 64];       // diag(e^(G_last - G)) U in three parts
-    __shared__ uint4 s_u[2 * 2 * 64];       // U in two
-    __shared__ int s_bad;                   // the last chunk that has to run token by token, from 1
-    float* const s_w = reinterpret_cast<float*>(s_x);  // the state of a chunk that runs token by token
-    static_assert(DK * LW * sizeof(float) <= sizeof(s_x), "s_w lies in s_x");
+    __shared__ uint4 s_q[TQ][4 * KS * 64];
+    __shared__ uint4 s_t[TQ][3 * kTriFrags * 64];  // [part][fragment][lane]
+    __shared__ __attribute__((aligned(16))) Exchange s_ex[NC];
+    __shared__ int s_bad;  // the last chunk that has to run token by token, from 1
     prefetch_kernargs<sizeof(DeltaParams) + sizeof(ChunkPlan)>();
     const int heads = c.b_count * p.Hv;
-    const int bh = int(blockIdx.x) % heads, col0 = int(blockIdx.x) / heads * kScanCols;
+    const int bh = int(blockIdx.x) % heads, col0 = int(blockIdx.x) / heads * (kScanCols * NC);
     const int b_at = bh / p.Hv, b = c.b_first + b_at, h = head_of(p, bh - b_at * p.Hv), hk = h / p.G;
     const int slot = entry_state(p.seq, b), len = entry_len(p.seq, b);
     const int begin = c.first * kChunk;
@@ -672,7 +679,7 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
     const int end = min(len, begin + c.count * kChunk);
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g4 = lane >> 4;
     if (slot == kEntryBad) {
-        if (w == 0) nan_rows<4, F16>(p, b, h, col0 + 4 * (lane & 3), begin, end);
+        if (w < NC) nan_rows<4, F16>(p, b, h, col0 + kScanCols * w + 4 * (lane & 3), begin, end);
         return;
     }
     const int tile = w & 3;
@@ -686,14 +693,22 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
     const int64_t unit_step = int64_t(p.Hv) * kUnitElems;
     const uint16_t* const units = c.units + (int64_t(b_at) * c.count * p.Hv + h) * kUnitElems + 8 * lane;
 
-    if (w >= 8) {  // the loads: a quarter of each chunk's
+    if (w >= 4 * NC + 4) {  // the loads: a quarter of each chunk's
         // lane l of a load takes unit l of its fragment: four lanes cover 64 bytes of a row
-        const int krow = tile_row(tile, lane >> 2), vrow = 32 * (tile & 1) + (lane >> 1), chunk = (lane & 3) ^ (lane >> 4);
+        const int krow = tile_row(tile, lane >> 2), chunk = (lane & 3) ^ (lane >> 4);
+        const int vrow = NC == 1 ? 32 * (tile & 1) + (lane >> 1) : 16 * tile + (lane >> 2), vcol = 8 * (lane & (2 * NC - 1));
         const uint16_t* unit = units;
         const uint16_t* k = p.k.p + b * p.k.batch + hk * p.k.head + begin * p.k.tok + 8 * chunk;
         const uint16_t* q = p.q.p + b * p.q.batch + hk * p.q.head + begin * p.q.tok + 8 * chunk;
-        const uint16_t* v = p.v.p + b * p.v.batch + h * p.v.head + begin * p.v.tok + col0 + 8 * (lane & 1);
+        const uint16_t* v = p.v.p + b * p.v.batch + h * p.v.head + begin * p.v.tok + col0 + vcol;
         int64_t k_at = krow * p.k.tok, q_at = krow * p.q.tok, v_at = vrow * p.v.tok;
+        const auto stage_t = [&](int n) {
+            if (n >= chunks) return;
+#pragma unroll
+            for (int i = 0; i < 5; ++i)
+                if (4 * i + tile < 3 * kTriFrags) load_lds(unit + kUnitT + (4 * i + tile) * kFrag, s_t[n & (TQ - 1)] + (4 * i + tile) * 64);
+            unit += unit_step;
+        };
         const auto stage = [&](int n) {
             if (n >= chunks) return;
             Stage& to = s_in[n & 1];
@@ -701,14 +716,10 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
             if (last < kChunk - 1) k_at = min(krow, last) * p.k.tok, v_at = min(vrow, last) * p.v.tok;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) load_lds(k + k_at + 32 * ks, to.k + (tile * KS + ks) * 64);
-#pragma unroll
-            for (int i = 0; i < 5; ++i)
-                if (4 * i + tile < 3 * kTriFrags) load_lds(unit + kUnitT + (4 * i + tile) * kFrag, to.t + (4 * i + tile) * 64);
-            if (tile < 2)
-                load_lds(v + v_at, to.v + tile * 32 * kScanCols);
-            else if (tile == 2)
-                load_lds(unit + kUnitVec, to.vec);
-            k += kChunk * p.k.tok, v += kChunk * p.v.tok, unit += unit_step;
+            if constexpr (NC == 1) stage_t(n);
+            if (tile < 2 * NC) load_lds(v + v_at, to.v + tile * 32 * kScanCols);
+            if (tile == 2) load_lds(units + n * unit_step + kUnitVec, to.vec);
+            k += kChunk * p.k.tok, v += kChunk * p.v.tok;
         };
         // Q, which the waves of out take after (1), or have taken before it: half a chunk later, so that the
         // loads spread over it (2048 tokens 59 -> 57.6 us)
@@ -717,17 +728,19 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
             const int last = end - 1 - begin - n * kChunk;
             if (last < kChunk - 1) q_at = min(krow, last) * p.q.tok;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) load_lds(q + q_at + 32 * ks, s_in[n & 1].q + (tile * KS + ks) * 64);
+            for (int ks = 0; ks < KS; ++ks) load_lds(q + q_at + 32 * ks, s_q[n & (TQ - 1)] + (tile * KS + ks) * 64);
             q += kChunk * p.q.tok;
         };
         stage(0);
+        if constexpr (NC == 2) stage_t(0);
         stage_q(0);
         __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
         lds_barrier();  // chunk 0 is there
         stage(1);
         for (int n = 0; n < chunks; ++n) {
             lds_barrier();  // (1)
-            stage_q(n + 1);  // where chunk n - 1's was
+            stage_q(n + 1);  // where chunk n - 1's was, or n's, which has been read
+            if constexpr (NC == 2) stage_t(n + 1);  // chunk n's has been read
             lds_barrier();   // (2)
             __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);  // chunk n + 1 is there, for all after (3)
             const int slow_word = s_bad;
@@ -743,7 +756,7 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
         return;
     }
 
-    if (w >= 4) {  // rows of out
+    if (w >= 4 * NC) {  // rows of out
         uint16_t* out = p.out + b * p.o_batch + h * p.o_head + (begin + tok0) * p.o_tok + col0 + r;
         const uint16_t* unit = units + kUnitP;
         const int tri0 = tri_frag(tile, 0) * kFrag, tri1 = tri_frag(tile, tile >> 1) * kFrag;
@@ -764,27 +777,32 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
         const auto load_q = [&](int at) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                q0[ks] = s_in[at & 1].q[(tile * KS + ks) * 64 + unit_at];
+                q0[ks] = s_q[at & (TQ - 1)][(tile * KS + ks) * 64 + unit_at];
                 if constexpr (F16) split_f16(q0[ks], q0[ks], q1[ks]);
             }
         };
         load_tri(0);
         lds_barrier();  // chunk 0 is there
-        if constexpr (F16) load_q(0);
+        if constexpr (kAhead) load_q(0);
         for (int n = 0; n < chunks; ++n) {
             lds_barrier();  // (1)
             e = *reinterpret_cast<const f32x4_t*>(s_in[n & 1].vec + kVecE + tok0);
-            f32x4_t a0 = zero, a1 = zero;
-            if constexpr (!F16) load_q(n);
+            f32x4_t a0[NC], a1[NC];
+            if constexpr (!kAhead) load_q(n);
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const uint4 s0 = s_s[ks * 64 + lane], s1 = s_s[(KS + ks) * 64 + lane];
-                a0 = mma(q0[ks], s0, a0);
-                a1 = mma(q0[ks], s1, a1);
-                if constexpr (F16) a1 = mma(q1[ks], s0, a1);
+            for (int g = 0; g < NC; ++g) {
+                const Exchange& ex = s_ex[g];
+                a0[g] = a1[g] = zero;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const uint4 s0 = ex.s[ks * 64 + lane], s1 = ex.s[(KS + ks) * 64 + lane];
+                    a0[g] = mma(q0[ks], s0, a0[g]);
+                    a1[g] = mma(q0[ks], s1, a1[g]);
+                    if constexpr (F16) a1[g] = mma(q1[ks], s0, a1[g]);
+                }
+                a0[g] = (a0[g] + a1[g]) * e;
+                a1[g] = zero;
             }
-            a0 = (a0 + a1) * e;
-            a1 = zero;
             lds_barrier();  // (2)
             const int slow_word = s_bad;
             const bool slow = __builtin_amdgcn_readfirstlane(slow_word) == n + 1;
@@ -794,25 +812,29 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
                 lds_barrier();
                 lds_barrier();
             } else {
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    if (ks > tile >> 1) continue;
-                    const uint4 u0 = s_u[ks * 64 + lane], u1 = s_u[(2 + ks) * 64 + lane];
-                    a0 = mma(tri[ks][0], u0, a0);
-                    a1 = mma(tri[ks][0], u1, a1);
-                    a1 = mma(tri[ks][1], u0, a1);
-                }
-                a0 += a1;
                 const int left = end - begin - n * kChunk - tok0;
-                uint16_t* to = out;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (i < left) *to = uint16_t(Elem<F16>::pack_p(a0[i], 0.0f));
-                    to += p.o_tok;
+                for (int g = 0; g < NC; ++g) {
+                    const Exchange& ex = s_ex[g];
+#pragma unroll
+                    for (int ks = 0; ks < 2; ++ks) {
+                        if (ks > tile >> 1) continue;
+                        const uint4 u0 = ex.u[ks * 64 + lane], u1 = ex.u[(2 + ks) * 64 + lane];
+                        a0[g] = mma(tri[ks][0], u0, a0[g]);
+                        a1[g] = mma(tri[ks][0], u1, a1[g]);
+                        a1[g] = mma(tri[ks][1], u0, a1[g]);
+                    }
+                    a0[g] += a1[g];
+                    uint16_t* to = out + kScanCols * g;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (i < left) *to = uint16_t(Elem<F16>::pack_p(a0[g][i], 0.0f));
+                        to += p.o_tok;
+                    }
                 }
             }
             load_tri(n + 1);
-            if constexpr (F16) load_q(n + 1);
+            if constexpr (kAhead) load_q(n + 1);
             out += kChunk * p.o_tok;
         }
         return;
@@ -821,9 +843,14 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
     const auto in_order = [] {
         if constexpr (!F16) __builtin_amdgcn_sched_barrier(0);
     };
+    const int chain = NC == 1 ? 0 : w >> 2, cw = NC == 1 ? w : w & 3;  // the wave's chain, and its number there
+    Exchange& ex = s_ex[chain];
+    const int col = col0 + kScanCols * chain;
+    float* const s_w = reinterpret_cast<float*>(ex.x);  // the state of a chunk that runs token by token
+    static_assert(DK * LW * sizeof(float) <= sizeof(ex.x), "s_w lies in x");
     __builtin_amdgcn_s_setprio(3);  // the chain goes first where waves meet on a SIMD
-    const int row0 = tile_row(MT * w, 4 * g4);  // the lane's first row of the state; tile m: + 4 m
-    float* const st = p.state + ((int64_t(slot) * p.Hv + h) * DK + row0) * p.Dv + col0 + r;
+    const int row0 = tile_row(MT * cw, 4 * g4);  // the lane's first row of the state; tile m: + 4 m
+    float* const st = p.state + ((int64_t(slot) * p.Hv + h) * DK + row0) * p.Dv + col + r;
     f32x4_t s[MT];
     const auto put3 = [&](uint2* to, float x0, float x1, float x2, float x3) {
         uint32_t a[2], d[2], e[2];
@@ -838,10 +865,10 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if constexpr (MT == 2) {
-                const uint4 x = in.k[(j * KS + w) * 64 + unit_at];
+                const uint4 x = in.k[(j * KS + cw) * 64 + unit_at];
                 fk[j].w[0] = x.x, fk[j].w[1] = x.y, fk[j].w[2] = x.z, fk[j].w[3] = x.w;
             } else {
-                const uint2 x = reinterpret_cast<const uint2*>(in.k)[2 * ((j * KS + (w >> 1)) * 64 + unit_at) + (w & 1)];
+                const uint2 x = reinterpret_cast<const uint2*>(in.k)[2 * ((j * KS + (cw >> 1)) * 64 + unit_at) + (cw & 1)];
                 fk[j].w[0] = x.x, fk[j].w[1] = x.y;
             }
         }
@@ -849,7 +876,7 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
     // K^T: the lane's row of state tile m, eight tokens, from two transposing
     // reads: 16 lanes give 4 rows of 16 elements, lane i takes column i of them
     const auto k_t = [&](const Stage& in, int m, int ks) {
-        const int state_tile = MT * w + m;
+        const int state_tile = MT * cw + m;
         const uint2* const at = reinterpret_cast<const uint2*>(in.k) +
                                 2 * ((2 * ks * KS + (state_tile >> 1)) * 64 + row_unit(4 * g4 + (r >> 2), r & 3)) + (state_tile & 1);
         const uint2 lo = read_transposed(at), hi = read_transposed(at + 2 * KS * 64);
@@ -870,16 +897,17 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
         Op fk[4];
         load_k(in, fk);
         in_order();
+        const uint4* const t = s_t[n & (TQ - 1)];
         uint4 ft[2][3];
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
-            ft[0][i] = in.t[(i * kTriFrags + tri_frag(tile, 0)) * 64 + lane];
-            ft[1][i] = in.t[(i * kTriFrags + tri_frag(tile, tile >> 1)) * 64 + lane];
+            ft[0][i] = t[(i * kTriFrags + tri_frag(tile, 0)) * 64 + lane];
+            ft[1][i] = t[(i * kTriFrags + tri_frag(tile, tile >> 1)) * 64 + lane];
         }
         const f32x4_t e = *reinterpret_cast<const f32x4_t*>(in.vec + kVecC + tok0);
         const f32x4_t d = *reinterpret_cast<const f32x4_t*>(in.vec + kVecD + tok0);
         const float last = in.vec[kVecLast], bad = in.vec[kVecBad + tile];
-        const uint2 v = read_transposed(reinterpret_cast<const uint2*>(in.v) + 4 * (tok0 + (r >> 2)) + (r & 3));
+        const uint2 v = read_transposed(reinterpret_cast<const uint2*>(in.v) + 4 * (NC * (tok0 + (r >> 2)) + chain) + (r & 3));
         in_order();
         {  // (1)
             Op s0, s1, s2;
@@ -889,10 +917,10 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
                 split3(s[m][2], s[m][3], s0.w[2 * m + 1], s1.w[2 * m + 1], s2.w[2 * m + 1]);
             }
             if constexpr (MT == 2) {
-                s_s[w * 64 + lane] = make_uint4(s0.w[0], s0.w[1], s0.w[2], s0.w[3]);
-                s_s[(KS + w) * 64 + lane] = make_uint4(s1.w[0], s1.w[1], s1.w[2], s1.w[3]);
+                ex.s[cw * 64 + lane] = make_uint4(s0.w[0], s0.w[1], s0.w[2], s0.w[3]);
+                ex.s[(KS + cw) * 64 + lane] = make_uint4(s1.w[0], s1.w[1], s1.w[2], s1.w[3]);
             } else {
-                uint2* const to = reinterpret_cast<uint2*>(s_s) + 2 * ((w >> 1) * 64 + lane) + (w & 1);
+                uint2* const to = reinterpret_cast<uint2*>(ex.s) + 2 * ((cw >> 1) * 64 + lane) + (cw & 1);
                 to[0] = make_uint2(s0.w[0], s0.w[1]);
                 to[2 * KS * 64] = make_uint2(s1.w[0], s1.w[1]);
             }
@@ -916,19 +944,19 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = mma_step(k0[j], s0, x[j]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s_x[(w * 4 + j) * 64 + lane] = x[j];
+            for (int j = 0; j < 4; ++j) ex.x[(cw * 4 + j) * 64 + lane] = x[j];
         }
         lds_barrier();  // (1)
         uint4 fkt[2 * MT];
         {  // (2)
-            const f32x4_t x0 = s_x[tile * 64 + lane], x1 = s_x[(4 + tile) * 64 + lane], x2 = s_x[(8 + tile) * 64 + lane],
-                          x3 = s_x[(12 + tile) * 64 + lane];
+            const f32x4_t x0 = ex.x[tile * 64 + lane], x1 = ex.x[(4 + tile) * 64 + lane], x2 = ex.x[(8 + tile) * 64 + lane],
+                          x3 = ex.x[(12 + tile) * 64 + lane];
             const f32x4_t z = (x0 + x1) + (x2 + x3);
             const float vf[4] = {Elem<F16>::lo(v.x), Elem<F16>::hi(v.x), Elem<F16>::lo(v.y), Elem<F16>::hi(v.y)};
             float y[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[i] = vf[i] - e[i] * z[i];
-            put3(reinterpret_cast<uint2*>(s_y) + half, y[0], y[1], y[2], y[3]);
+            put3(reinterpret_cast<uint2*>(ex.y) + half, y[0], y[1], y[2], y[3]);
             // an overflow of this sum only means more care
             if (!((fabsf(y[0]) + fabsf(y[1])) + (fabsf(y[2]) + fabsf(y[3])) < INFINITY) || bad != 0.0f) s_bad = n + 1;
         }
@@ -940,7 +968,7 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                 for (int i = 0; i < 3; ++i)
-                    if (ks <= tile >> 1) y[ks][i] = s_y[(2 * i + ks) * 64 + lane];
+                    if (ks <= tile >> 1) y[ks][i] = ex.y[(2 * i + ks) * 64 + lane];
             in_order();
 #pragma unroll
             for (int m = 0; m < MT; ++m)
@@ -959,11 +987,11 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
                 a2 = mma(ft[ks][2], y[ks][0], a2);
             }
             const f32x4_t u = a0 + (a1 + a2);
-            put3(reinterpret_cast<uint2*>(s_d) + half, d[0] * u[0], d[1] * u[1], d[2] * u[2], d[3] * u[3]);
+            put3(reinterpret_cast<uint2*>(ex.d) + half, d[0] * u[0], d[1] * u[1], d[2] * u[2], d[3] * u[3]);
             uint32_t a[2], g[2];
             split2(u[0], u[1], a[0], g[0]);
             split2(u[2], u[3], a[1], g[1]);
-            uint2* const to = reinterpret_cast<uint2*>(s_u) + half;
+            uint2* const to = reinterpret_cast<uint2*>(ex.u) + half;
             to[0] = make_uint2(a[0], a[1]);
             to[kPart] = make_uint2(g[0], g[1]);
         }
@@ -975,13 +1003,13 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s_w[(row0 + 4 * m + i) * LW + r] = s[m][i];
             lds_barrier();
-            if (w == 0) {
+            if (cw == 0) {
                 constexpr int NR = DK / 16;
                 const int t0 = begin + n * kChunk;
                 f32x4_t sr[NR];
 #pragma unroll
                 for (int i = 0; i < NR; ++i) sr[i] = *reinterpret_cast<const f32x4_t*>(s_w + (lane / 4 * NR + i) * LW + 4 * (lane & 3));
-                recur<DK, 4, F16>(kernel_params(), sr, b, h, col0 + 4 * (lane & 3), t0, min(end, t0 + kChunk));
+                recur<DK, 4, F16>(kernel_params(), sr, b, h, col + 4 * (lane & 3), t0, min(end, t0 + kChunk));
 #pragma unroll
                 for (int i = 0; i < NR; ++i) *reinterpret_cast<f32x4_t*>(s_w + (lane / 4 * NR + i) * LW + 4 * (lane & 3)) = sr[i];
             }
@@ -998,7 +1026,7 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-            for (int i = 0; i < 3; ++i) dp[ks][i] = s_d[(2 * i + ks) * 64 + lane];
+            for (int i = 0; i < 3; ++i) dp[ks][i] = ex.d[(2 * i + ks) * 64 + lane];
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             f32x4_t a0 = s[m] * last, a1 = zero, a2 = zero;
@@ -1023,34 +1051,43 @@ __global__ __launch_bounds__(kScanThreads) void delta_chunk_scan_kernel(DeltaPar
 // What one pair of launches takes: entries of the batch and chunks of each, with
 // units of about 96 MB, which the caches hold between the two kernels (8192 tokens:
 // 48 MB 308, 64 to 96 MB 288, 128 MB 311 us; 32768 tokens: 64 MB 1153, 96 MB 1133,
-// 256 MB 1288 us).  Whole entries where they fit, as many as fill the GPU where not: a
-// launch's start costs a workgroup about two chunks' time.
+// 256 MB 1288 us).  Whole entries where they fit, a multiple of what fills the GPU: a
+// launch's start costs a workgroup about two chunks' time.  More chains than CUs go
+// two to a workgroup (both kernels, us, one chain per workgroup against this: 2048
+// tokens of 32 heads of 128, 3 sequences 234 / 186, 8 sequences 635 / 445, fp16 684 / 536;
+// 40 heads 127 / 94, 64 heads 153 / 115; as many chains as CUs, 32 heads, 66 / 89).
 constexpr size_t kUnitBytes = kUnitElems * 2;
+constexpr int64_t kCus = 256;
 struct LaunchPlan {
     int64_t entries, chunks;
 };
 LaunchPlan launch_plan(int64_t B, int64_t S, int64_t Hv, int64_t Dv) {
     const int64_t all = (S + kChunk - 1) / kChunk;
     const int64_t units = std::max<int64_t>(int64_t((size_t(96) << 20) / kUnitBytes) / Hv, 1);  // chunks of all heads
-    const int64_t fill = (256 + Hv * (Dv / kScanCols) - 1) / (Hv * (Dv / kScanCols));
+    const int64_t chains = Hv * (Dv / kScanCols), round = B * chains > kCus ? 2 * kCus : kCus;
+    const int64_t fill = (round + chains - 1) / chains;  // entries
     const auto even = [](int64_t n, int64_t most) {  // n in equal parts of at most `most`
         const int64_t parts = (n + most - 1) / most;
         return (n + parts - 1) / parts;
     };
-    const int64_t entries = even(B, std::max(units / all, fill));
+    const int64_t entries = even(B, std::max(units / all / fill, int64_t(1)) * fill);
     return {entries, even(all, std::max<int64_t>(units / entries, 1))};
 }
 
 // Whether the rule runs in chunks.  Token by token a call takes about 0.7 us a
 // token while its waves (16 columns each) find SIMDs of their own, the two chunk
-// kernels 12.5 us for any prompt of up to 64 tokens: 16 / 32 heads of 128, 12 tokens
-// 12.2 against 12.5 us, 16 tokens 15.1 against 12.5.  More waves share the chunk
-// kernels' CUs and fill the SIMDs better: 8 sequences, 24 tokens 34.7 against 40.3,
-// 32 tokens 43.2 against 40.7; 64 sequences, 24 tokens 196 against 303, 48 tokens 349
-// against 331.
+// kernels 12.7 us for any prompt of up to 64 tokens: 16 / 32 heads of 128, 12 tokens
+// 12.1 against 12.7 us, 16 tokens 15.0 against 12.6.  More waves share the chunk
+// kernels' CUs and fill the SIMDs better: 2 sequences, 16 tokens 15.6 against 16.7, 20
+// tokens 18.2 against 16.8; 4 sequences, 24 tokens 22.1 against 24.5, 28 tokens 24.8
+// against 24.4; 8 sequences, 28 tokens 39.3 against 39.0; 64 sequences, 32 tokens 245
+// against 268, 40 tokens 298 against 278.
 constexpr int64_t kManyWaves = 1024;  // one per SIMD
 int64_t column_waves(int64_t B, int64_t Hv, int64_t Dv) { return B * Hv * (Dv / 16); }
-bool in_chunks(int64_t B, int64_t S, int64_t Hv, int64_t Dv) { return S > (column_waves(B, Hv, Dv) >= kManyWaves ? 28 : 12); }
+bool in_chunks(int64_t B, int64_t S, int64_t Hv, int64_t Dv) {
+    const int64_t waves = column_waves(B, Hv, Dv);
+    return S > (waves >= kManyWaves ? 28 : 2 * waves >= kManyWaves ? 16 : 12);
+}
 
 template <bool F16>
 int launch_chunks(const DeltaParams& p, void* ws, hipStream_t stream) {
@@ -1059,7 +1096,8 @@ int launch_chunks(const DeltaParams& p, void* ws, hipStream_t stream) {
     ChunkPlan c;
     c.units = static_cast<uint16_t*>(ws);
     auto* prepare = p.Dk == 128 ? delta_chunk_prepare_kernel<128, F16> : delta_chunk_prepare_kernel<64, F16>;
-    auto* scan = p.Dk == 128 ? delta_chunk_scan_kernel<128, F16> : delta_chunk_scan_kernel<64, F16>;
+    auto* one = p.Dk == 128 ? delta_chunk_scan_kernel<128, 1, F16> : delta_chunk_scan_kernel<64, 1, F16>;
+    auto* two = p.Dk == 128 ? delta_chunk_scan_kernel<128, 2, F16> : delta_chunk_scan_kernel<64, 2, F16>;
     for (int64_t b_first = 0; b_first < p.B; b_first += plan.entries)
         for (int64_t first = 0; first < all; first += plan.chunks) {
             c.b_first = int32_t(b_first), c.b_count = int32_t(std::min(plan.entries, p.B - b_first));
@@ -1067,7 +1105,11 @@ int launch_chunks(const DeltaParams& p, void* ws, hipStream_t stream) {
             const int64_t heads = int64_t(c.b_count) * p.Hv;
             hipLaunchKernelGGL(prepare, dim3(unsigned(heads * c.count)), dim3(256), 0, stream, p, c);
             GENLLM_LAUNCH_CHECK("delta_chunk_prepare_kernel");
-            hipLaunchKernelGGL(scan, dim3(unsigned(heads * (p.Dv / kScanCols))), dim3(kScanThreads), 0, stream, p, c);
+            const int64_t chains = heads * (p.Dv / kScanCols);
+            if (chains > kCus)
+                hipLaunchKernelGGL(two, dim3(unsigned(chains / 2)), dim3(kScanThreads<2>), 0, stream, p, c);
+            else
+                hipLaunchKernelGGL(one, dim3(unsigned(chains)), dim3(kScanThreads<1>), 0, stream, p, c);
             GENLLM_LAUNCH_CHECK("delta_chunk_scan_kernel");
         }
     return GENLLM_OK;

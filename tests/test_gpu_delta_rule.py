@@ -402,6 +402,73 @@ def test_large_and_small_values():
         check(x, f"values of {scale}")
 
 
+# more chains of 16 columns than CUs: two per workgroup
+@pytest.mark.parametrize("Dk,Dv", [(64, 64), (64, 128), (128, 64), (128, 128)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("layout", ["token", "wide"])
+def test_paired_chains(Dk, Dv, dtype, layout):
+    """A padded batch over a pool: a whole entry, a short one, one behind its first chunk, an empty one, one without a
+    sequence, a repeated state."""
+    Hv = 16 * 64 // Dv
+    S, B = 140, 6
+    x = inputs(230 + Dk + Dv, B, S, Hv // 2, Hv, Dk, Dv, dtype, n=8, layout=layout)
+    ids = torch.tensor([5, 0, 7, 2, -1, 0], dtype=torch.int32)
+    lens = torch.tensor([S, 30, 65, 0, S, 100], dtype=torch.int32)
+    before = x["state"].clone()
+    want, new = reference(x, ids.long().clamp(min=0), lens)
+    out = out_like(x, fill=3.25)
+    call(x, out, seq_lens=lens.cuda(), state_ids=ids.cuda())
+    torch.cuda.synchronize()
+    for i in range(3):
+        n = int(lens[i])
+        assert bool((out[i, n:] == 3.25).all())
+        assert_rounded(out[i, :n], want[i, :n], f"entry {i}")
+        assert_state(x["state"][ids[i]], new[i], n, f"entry {i}")
+    assert bool((out[3:5] == 3.25).all())
+    assert bool(torch.isnan(out[5, :100]).all()) and bool((out[5, 100:] == 3.25).all())
+    for j in (1, 2, 3, 4, 6):
+        assert torch.equal(x["state"][j], before[j])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("column", [5, 20])
+def test_paired_chains_where_tokens_run_alone(dtype, column):
+    """A NaN in one chain of a pair sends the chunk of both token by token, written over v; then whole chunks again."""
+    x = inputs(260 + column, 2, 200, 20, 40, 64, 64, dtype, raw=False)
+    x["v"][1, 70, 3, column] = math.nan
+    x["k"][0, 150, 7] = math.inf
+    want, _ = reference(x)
+    call(x, x["v"])
+    torch.cuda.synchronize()
+    got = x["v"]
+    assert bool(torch.isnan(got[1, 70:, 3, column]).all())
+    keep = [c for c in range(64) if c != column]
+    assert_rounded(got[1, :, 3][:, keep], want[1, :, 3][:, keep], "other columns")
+    assert_rounded(got[1, :70, 3], want[1, :70, 3], "before")
+    others = [h for h in range(40) if h != 3]
+    assert_rounded(got[1][:, others], want[1][:, others], "other heads")
+    assert_rounded(got[0, :150], want[0, :150], "before the key")
+    others = [h for h in range(40) if h not in (14, 15)]
+    assert_rounded(got[0][:, others], want[0][:, others], "heads of other keys")
+    assert not bool(torch.isfinite(got[0, 150, 14:16]).any())
+
+
+def test_paired_chains_replayed():
+    x = inputs(270, 3, 100, 24, 24, 64, 64)
+    first, out = x["state"].clone(), out_like(x)
+    call(x, out)
+    want, new = out.clone(), x["state"].clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(x, out)
+    for _ in range(4):
+        x["state"].copy_(first)
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(x["state"], new)
+
+
 @pytest.mark.parametrize("S", [5, 100, 200])
 @pytest.mark.parametrize("factor", [4, 16, 256])
 def test_keys_far_above_one(S, factor):
