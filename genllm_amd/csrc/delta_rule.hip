@@ -25,10 +25,9 @@
 // of every chunk and head at once; delta_chunk_scan_kernel takes 16 columns of
 // a head's state from chunk to chunk through the matrix cores.  The state and
 // everything that enters it keep 24 bits there: an fp32 value is the exact sum
-// of three bf16 parts (24 = 3 x 8 bits), k is one part (fp16: two, 11 bits), and
-// the products of parts below 2^-24 are left out.  What enters out only (Q, P,
-// and S and U beside them) takes two parts, 2^-17 of a term, against out's own
-// rounding of 2^-8 (fp16: 2^-11).  One part would be 2^-9 of every term.
+// of three bf16 parts (24 = 3 x 8 bits), q and k are one part (fp16: two, 11 bits),
+// and the products of parts below 2^-24 are left out.  out is formed the same way
+// and rounded once, so that it has the bits of the rule token by token.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -252,9 +251,9 @@ constexpr int kScanCols = 16;  // columns of the state per chain of the scan
 constexpr int kFrag = 64 * 8;                    // elements of a fragment
 constexpr int kTriFrags = 6;
 constexpr int kTPart = kTriFrags * kFrag;        // elements of one part of T or P
-constexpr int kUnitT = 0, kUnitP = 3 * kTPart;   // T in three parts, P in two
-constexpr int kUnitVec = 5 * kTPart;             // floats: see kVec*
-constexpr int kVecC = 0, kVecD = 64, kVecE = 128, kVecLast = 192, kVecBad = 196, kVecFloats = 256;
+constexpr int kUnitT = 0, kUnitP = 3 * kTPart;   // T and P in three parts
+constexpr int kUnitVec = 6 * kTPart;             // floats: see kVec*
+constexpr int kVecC = 0, kVecD = 64, kVecE = 128, kVecLast = 192, kVecBad = 196, kVecFloats = 208;
 // kVecBad: a flag per wave of the preparation, read by the wave of the scan with that number
 constexpr int kUnitElems = kUnitVec + 2 * kVecFloats;
 __device__ __forceinline__ constexpr int tri_frag(int tile, int ks) { return tile < 2 ? tile : 2 * tile - 2 + ks; }
@@ -479,7 +478,7 @@ __global__ __launch_bounds__(256, 4) void delta_chunk_prepare_kernel(DeltaParams
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             if (ks > w >> 1) continue;
-            uint32_t a[4], d[4];
+            uint32_t a[4], d[4], e[4];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 f32x4_t x = zero;
@@ -489,11 +488,13 @@ __global__ __launch_bounds__(256, 4) void delta_chunk_prepare_kernel(DeltaParams
                 fade(g_row, row, 32 * ks + 8 * g4 + 4 * half, f);
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    split2(rq * f[2 * i] * x[2 * i], rq * f[2 * i + 1] * x[2 * i + 1], a[2 * half + i], d[2 * half + i]);
+                    split3(rq * f[2 * i] * x[2 * i], rq * f[2 * i + 1] * x[2 * i + 1], a[2 * half + i], d[2 * half + i],
+                           e[2 * half + i]);
             }
             uint16_t* const to = unit + kUnitP + tri_frag(w, ks) * kFrag + 8 * lane;
             *reinterpret_cast<uint4*>(to) = make_uint4(a[0], a[1], a[2], a[3]);
             *reinterpret_cast<uint4*>(to + kTPart) = make_uint4(d[0], d[1], d[2], d[3]);
+            *reinterpret_cast<uint4*>(to + 2 * kTPart) = make_uint4(e[0], e[1], e[2], e[3]);
         }
     }
     {  // L: rows of tile 3 - w, the longest for the wave with the fewest of P
@@ -632,7 +633,7 @@ __device__ __forceinline__ DeltaParams kernel_params() {
 //   shares and Y = V - diag(e^G) K S0 for token tile w; (3) wave w: tile w of U = T Y;
 //   (4) wave w: its rows of the new state, S <- e^(G_last) S + K^T diag(e^(G_last - G)) U.
 // Waves 4 to 7 have the state and U from LDS and form out, tile w - 4: Q S0
-// during (2), P U during (4).  Waves 8 to 11 load what waves 0 to 3 need straight
+// during (2) and (3) (the third part of S0 there), P U during (4).  Waves 8 to 11 load what waves 0 to 3 need straight
 // into LDS, two chunks ahead: the chain (1) to (4) is bound by the instructions
 // that one wave can issue, and 53 KB a chunk keep the memory pipe busy.  Rows
 // behind the end come as copies of the last row; T has zeros in their place.
@@ -658,11 +659,11 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
         float vec[kVecFloats];
     };
     struct Exchange {                              // of one chain
-        f32x4_t x[4 * 4 * 64];                     // shares of K S0 [wave][token tile][lane]
-        uint4 s[2 * KS * 64];                      // the state in two parts [part][step][lane]
+        f32x4_t x[4 * 3 * 64];                     // shares of K S0 for other waves [token tile][wave][lane]
+        uint4 s[3 * KS * 64];                      // the state in three parts [part][step][lane]
         uint4 y[3 * 2 * 64];                       // Y in three parts [part][step][lane], a tile's half of each
         uint4 d[3 * 2 * 64];                       // diag(e^(G_last - G)) U in three parts
-        uint4 u[2 * 2 * 64];                       // U in two
+        uint4 u[3 * 2 * 64];                       // U
     };
     __shared__ __attribute__((aligned(16))) Stage s_in[2];
     __shared__ uint4 s_q[TQ][4 * KS * 64];
@@ -687,7 +688,7 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
     const int tok0 = tile_row(tile, 4 * g4);  // the lane's four tokens of tile `tile`
     const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
     const int half = 2 * ((tile >> 1) * 64 + lane) + (tile & 1);  // the lane's half of an operand, in uint2
-    constexpr int kPart = 2 * 2 * 64;                             // uint2 per part of s_y, s_d, s_u
+    constexpr int kPart = 2 * 2 * 64;                             // uint2 per part of y, d and u
 
     const int unit_at = row_unit(r, g4);  // the lane's operand in K and Q
     const int64_t unit_step = int64_t(p.Hv) * kUnitElems;
@@ -718,7 +719,7 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
             for (int ks = 0; ks < KS; ++ks) load_lds(k + k_at + 32 * ks, to.k + (tile * KS + ks) * 64);
             if constexpr (NC == 1) stage_t(n);
             if (tile < 2 * NC) load_lds(v + v_at, to.v + tile * 32 * kScanCols);
-            if (tile == 2) load_lds(units + n * unit_step + kUnitVec, to.vec);
+            if (tile == 2 && lane < kVecFloats / 4) load_lds(units + n * unit_step + kUnitVec, to.vec);
             k += kChunk * p.k.tok, v += kChunk * p.v.tok;
         };
         // Q, which the waves of out take after (1), or have taken before it: half a chunk later, so that the
@@ -760,12 +761,12 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
         uint16_t* out = p.out + b * p.o_batch + h * p.o_head + (begin + tok0) * p.o_tok + col0 + r;
         const uint16_t* unit = units + kUnitP;
         const int tri0 = tri_frag(tile, 0) * kFrag, tri1 = tri_frag(tile, tile >> 1) * kFrag;
-        uint4 tri[2][2];
+        uint4 tri[2][3];
         f32x4_t e;
         const auto load_tri = [&](int n) {
             if (n >= chunks) return;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < 3; ++i) {
                 tri[0][i] = *reinterpret_cast<const uint4*>(unit + i * kTPart + tri0);
                 tri[1][i] = *reinterpret_cast<const uint4*>(unit + i * kTPart + tri1);
             }
@@ -798,14 +799,19 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
                     const uint4 s0 = ex.s[ks * 64 + lane], s1 = ex.s[(KS + ks) * 64 + lane];
                     a0[g] = mma(q0[ks], s0, a0[g]);
                     a1[g] = mma(q0[ks], s1, a1[g]);
-                    if constexpr (F16) a1[g] = mma(q1[ks], s0, a1[g]);
+                    if constexpr (F16) a1[g] = mma(q1[ks], s0, a1[g]), a1[g] = mma(q1[ks], s1, a1[g]);
                 }
-                a0[g] = (a0[g] + a1[g]) * e;
-                a1[g] = zero;
             }
             lds_barrier();  // (2)
             const int slow_word = s_bad;
             const bool slow = __builtin_amdgcn_readfirstlane(slow_word) == n + 1;
+#pragma unroll
+            for (int g = 0; g < NC; ++g) {  // the third part: these waves have nothing else to do here
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) a1[g] = mma(q0[ks], s_ex[g].s[(2 * KS + ks) * 64 + lane], a1[g]);
+                a0[g] = (a0[g] + a1[g]) * e;
+                a1[g] = zero;
+            }
             lds_barrier();  // (3)
             if (slow) {
                 lds_barrier();
@@ -816,15 +822,19 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
 #pragma unroll
                 for (int g = 0; g < NC; ++g) {
                     const Exchange& ex = s_ex[g];
+                    f32x4_t a2 = zero;
 #pragma unroll
                     for (int ks = 0; ks < 2; ++ks) {
                         if (ks > tile >> 1) continue;
-                        const uint4 u0 = ex.u[ks * 64 + lane], u1 = ex.u[(2 + ks) * 64 + lane];
+                        const uint4 u0 = ex.u[ks * 64 + lane], u1 = ex.u[(2 + ks) * 64 + lane], u2 = ex.u[(4 + ks) * 64 + lane];
                         a0[g] = mma(tri[ks][0], u0, a0[g]);
                         a1[g] = mma(tri[ks][0], u1, a1[g]);
+                        a2 = mma(tri[ks][0], u2, a2);
                         a1[g] = mma(tri[ks][1], u0, a1[g]);
+                        a2 = mma(tri[ks][1], u1, a2);
+                        a2 = mma(tri[ks][2], u0, a2);
                     }
-                    a0[g] += a1[g];
+                    a0[g] += a1[g] + a2;
                     uint16_t* to = out + kScanCols * g;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -860,16 +870,17 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
         to[kPart] = make_uint2(d[0], d[1]);
         to[2 * kPart] = make_uint2(e[0], e[1]);
     };
-    // K: the tokens of tile j, the lane's rows of the state
+    // K: the tokens of all tiles, the wave's own first, and the lane's rows of the state
     const auto load_k = [&](const Stage& in, Op (&fk)[4]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int i = 0; i < 4; ++i) {
+            const int j = (cw + i) & 3;
             if constexpr (MT == 2) {
                 const uint4 x = in.k[(j * KS + cw) * 64 + unit_at];
-                fk[j].w[0] = x.x, fk[j].w[1] = x.y, fk[j].w[2] = x.z, fk[j].w[3] = x.w;
+                fk[i].w[0] = x.x, fk[i].w[1] = x.y, fk[i].w[2] = x.z, fk[i].w[3] = x.w;
             } else {
                 const uint2 x = reinterpret_cast<const uint2*>(in.k)[2 * ((j * KS + (cw >> 1)) * 64 + unit_at) + (cw & 1)];
-                fk[j].w[0] = x.x, fk[j].w[1] = x.y;
+                fk[i].w[0] = x.x, fk[i].w[1] = x.y;
             }
         }
     };
@@ -909,6 +920,7 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
         const float last = in.vec[kVecLast], bad = in.vec[kVecBad + tile];
         const uint2 v = read_transposed(reinterpret_cast<const uint2*>(in.v) + 4 * (NC * (tok0 + (r >> 2)) + chain) + (r & 3));
         in_order();
+        f32x4_t x[4];
         {  // (1)
             Op s0, s1, s2;
 #pragma unroll
@@ -919,12 +931,13 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
             if constexpr (MT == 2) {
                 ex.s[cw * 64 + lane] = make_uint4(s0.w[0], s0.w[1], s0.w[2], s0.w[3]);
                 ex.s[(KS + cw) * 64 + lane] = make_uint4(s1.w[0], s1.w[1], s1.w[2], s1.w[3]);
+                ex.s[(2 * KS + cw) * 64 + lane] = make_uint4(s2.w[0], s2.w[1], s2.w[2], s2.w[3]);
             } else {
                 uint2* const to = reinterpret_cast<uint2*>(ex.s) + 2 * ((cw >> 1) * 64 + lane) + (cw & 1);
                 to[0] = make_uint2(s0.w[0], s0.w[1]);
                 to[2 * KS * 64] = make_uint2(s1.w[0], s1.w[1]);
+                to[4 * KS * 64] = make_uint2(s2.w[0], s2.w[1]);
             }
-            f32x4_t x[4];
             Op k0[4], k1[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -944,14 +957,13 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = mma_step(k0[j], s0, x[j]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) ex.x[(cw * 4 + j) * 64 + lane] = x[j];
+            for (int j = 1; j < 4; ++j) ex.x[(((cw + j) & 3) * 3 + j - 1) * 64 + lane] = x[j];
         }
         lds_barrier();  // (1)
         uint4 fkt[2 * MT];
         {  // (2)
-            const f32x4_t x0 = ex.x[tile * 64 + lane], x1 = ex.x[(4 + tile) * 64 + lane], x2 = ex.x[(8 + tile) * 64 + lane],
-                          x3 = ex.x[(12 + tile) * 64 + lane];
-            const f32x4_t z = (x0 + x1) + (x2 + x3);
+            const f32x4_t x1 = ex.x[3 * tile * 64 + lane], x2 = ex.x[(3 * tile + 1) * 64 + lane], x3 = ex.x[(3 * tile + 2) * 64 + lane];
+            const f32x4_t z = (x[0] + x1) + (x2 + x3);
             const float vf[4] = {Elem<F16>::lo(v.x), Elem<F16>::hi(v.x), Elem<F16>::lo(v.y), Elem<F16>::hi(v.y)};
             float y[4];
 #pragma unroll
@@ -963,12 +975,12 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
         lds_barrier();  // (2)
         const int slow_word = s_bad;
         {  // (3)
-            uint4 y[2][3];
+            uint4 y[2][3];  // NC = 2: the second step for all tiles, as a branch here leaves one of its parts in scratch memory
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                 for (int i = 0; i < 3; ++i)
-                    if (ks <= tile >> 1) y[ks][i] = ex.y[(2 * i + ks) * 64 + lane];
+                    if (NC == 2 || ks <= tile >> 1) y[ks][i] = ex.y[(2 * i + ks) * 64 + lane];
             in_order();
 #pragma unroll
             for (int m = 0; m < MT; ++m)
@@ -988,12 +1000,7 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
             }
             const f32x4_t u = a0 + (a1 + a2);
             put3(reinterpret_cast<uint2*>(ex.d) + half, d[0] * u[0], d[1] * u[1], d[2] * u[2], d[3] * u[3]);
-            uint32_t a[2], g[2];
-            split2(u[0], u[1], a[0], g[0]);
-            split2(u[2], u[3], a[1], g[1]);
-            uint2* const to = reinterpret_cast<uint2*>(ex.u) + half;
-            to[0] = make_uint2(a[0], a[1]);
-            to[kPart] = make_uint2(g[0], g[1]);
+            put3(reinterpret_cast<uint2*>(ex.u) + half, u[0], u[1], u[2], u[3]);
         }
         const bool slow = __builtin_amdgcn_readfirstlane(slow_word) == n + 1;
         lds_barrier();  // (3)

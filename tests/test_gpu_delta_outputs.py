@@ -1,0 +1,102 @@
+"""Outputs of the delta rule's chunked form hold the bits of 32-bit arithmetic before their one rounding.
+
+All terms of the sums below are positive, so that a sum is as large as its terms' absolute values and the error of each part
+shows relative to the result.  Half steps of fp32 (2^-24, relative) between the inputs and an output, at most:
+
+  q's norm: sum of squares 5, root and reciprocal 2, scale and product 2                                 9
+  the same for k's, where it is normalised                                                               9
+  decay: its rate and softplus 5 and the running difference's rounding 1, of |G| <= 1; 2^x 2; product 1  9
+  u: beta 4, its product 1, the sums of parts (six products, three accumulators) 8                      13
+  S or P: parts' sums (six products of two steps, or three of four) 12, products and their sum 2        14
+
+which is 54: 2^-18 is 64 of them.  Two bf16 parts leave up to 2^-16 of each term."""
+import math
+
+import pytest
+import torch
+
+from genllm_amd import paged
+from hybrid import delta_rule
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16 = torch.bfloat16, torch.float16
+SLACK = 2.0 ** -18
+
+
+def assert_one_rounding(got, want, label, scale=None):
+    """|got - want| within half a step of want's own binade and SLACK of the terms' size (want's own where all are positive).
+    Below the smallest normal value the steps get no smaller: tiny eps / 2 is half of one (fp16 2^-14 2^-10 / 2 = 2^-25)."""
+    g, w = got.detach().cpu().double(), want
+    bits = {BF16: 8, F16: 11}[got.dtype]
+    half = torch.ldexp(torch.ones_like(w), torch.frexp(w)[1] - 1 - bits)
+    half = half.clamp(min=torch.finfo(got.dtype).tiny * torch.finfo(got.dtype).eps / 2)
+    bound = half + SLACK * (w.abs() if scale is None else scale)
+    worst = ((g - w).abs() / bound).max().item()
+    over = ((g - w).abs() > bound).double().mean().item()
+    print(f"[{label}] worst {worst:.4f} of its bound, {over:.2e} of the elements above", flush=True)
+    assert worst <= 1.0, f"{label}: {worst} times the bound"
+
+
+def call(x, out, l2_eps=1e-6):
+    paged.gated_delta_rule(x["q"], x["k"], x["v"], x["a"], x["b"], x["state"], out, x["scale"], l2_eps=l2_eps)
+    torch.cuda.synchronize()
+
+
+def positive(g, *shape):
+    return torch.rand(shape, generator=g) + 0.25
+
+
+SHAPES = [(1, 70, 1, 2, 128, 128), (2, 200, 2, 4, 64, 64), (1, 130, 3, 3, 64, 128), (1, 100, 2, 2, 128, 64),
+          (2, 140, 12, 24, 128, 128), (3, 90, 24, 24, 64, 64)]  # the last two: two chains per workgroup
+
+
+@pytest.mark.parametrize("B,S,Hk,Hv,Dk,Dv", SHAPES)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_state_read(B, S, Hk, Hv, Dk, Dv, dtype):
+    """beta 0: out is the decayed state beside q."""
+    g = torch.Generator().manual_seed(S + Dk)
+    x = {"q": positive(g, B, S, Hk, Dk).to(dtype).cuda(), "k": positive(g, B, S, Hk, Dk).to(dtype).cuda(),
+         "v": positive(g, B, S, Hv, Dv).to(dtype).cuda(), "a": (-torch.rand(B, S, Hv, generator=g) / S).cuda(),
+         "b": torch.zeros(B, S, Hv).cuda(), "state": positive(g, B, Hv, Dk, Dv).cuda(), "scale": 0.37}
+    want, new = delta_rule(x["q"], x["k"], x["v"], x["a"], x["b"], x["state"], x["scale"], l2_eps=1e-6)
+    out = torch.zeros(B, S, Hv, Dv, dtype=dtype, device="cuda")
+    call(x, out)
+    assert_one_rounding(out, want, f"state read {dtype} {Dk}x{Dv}")
+
+
+@pytest.mark.parametrize("B,S,Hk,Hv,Dk,Dv", SHAPES)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_writes_read(B, S, Hk, Hv, Dk, Dv, dtype):
+    """Keys along the axes, no two alike in a chunk, and nothing left from one chunk to the next: u = beta v, and out is
+    the chunk's own writes beside q."""
+    g = torch.Generator().manual_seed(S + Dk)
+    k = torch.zeros(B, S, Hk, Dk)
+    k[:, torch.arange(S), :, torch.arange(S) % 64] = 1.0
+    a = -torch.rand(B, S, Hv, generator=g) / 64
+    a[:, ::64] = -math.inf
+    x = {"q": positive(g, B, S, Hk, Dk).to(dtype).cuda(), "k": k.to(dtype).cuda(),
+         "v": positive(g, B, S, Hv, Dv).to(dtype).cuda(), "a": a.cuda(),
+         "b": positive(g, B, S, Hv).cuda(), "state": positive(g, B, Hv, Dk, Dv).cuda(), "scale": 0.37}
+    want, new = delta_rule(x["q"], x["k"], x["v"], x["a"], x["b"], x["state"], x["scale"], l2_eps=1e-6)
+    out = torch.zeros(B, S, Hv, Dv, dtype=dtype, device="cuda")
+    call(x, out)
+    assert_one_rounding(out, want, f"writes read {dtype} {Dk}x{Dv}")
+
+
+@pytest.mark.parametrize("S", [33, 70, 500])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_prompt(S, dtype):
+    """Usual values: errors against the sums of the terms' absolute values, of which the row's largest output is a
+    part at least."""
+    g = torch.Generator().manual_seed(S)
+    B, Hk, Hv, D = 1, 2, 4, 128
+    x = {c: torch.nn.functional.silu(torch.randn(B, S, H, D, generator=g) * 1.5).to(dtype).cuda()
+         for c, H in (("q", Hk), ("k", Hk), ("v", Hv))}
+    x["a"] = (-torch.rand(B, S, Hv, generator=g)).cuda()
+    x["b"] = torch.rand(B, S, Hv, generator=g).cuda()
+    x["state"], x["scale"] = (torch.randn(B, Hv, D, D, generator=g) * 0.3).cuda(), D ** -0.5
+    want, new = delta_rule(x["q"], x["k"], x["v"], x["a"], x["b"], x["state"], x["scale"], l2_eps=1e-6)
+    out = torch.zeros(B, S, Hv, D, dtype=dtype, device="cuda")
+    call(x, out)
+    assert_one_rounding(out, want, f"prompt of {S} {dtype}", want.abs().amax(-1, keepdim=True))
