@@ -266,6 +266,14 @@ __device__ __forceinline__ constexpr int tile_row(int t, int rho) {
     return 32 * (t >> 1) + 8 * (rho >> 2) + 4 * (t & 1) + (rho & 3);
 }
 
+// Below these sizes no step of a chunk leaves fp32: 8 lanes hold a row of T, so that |U| < 8
+// kMaxT kMaxY = 2^93 and |e^(G_last - G) U| < 2^123 with the keys' factors in it.  A chunk with
+// more runs token by token: an infinite u of one token, times the zeros of P, would make
+// the outputs of earlier ones NaN.
+constexpr float kMaxT = 0x1p20f;  // the sum of |T| over 8 columns
+constexpr float kMaxY = 0x1p70f;  // the sum of |Y| over 4 rows
+constexpr float kMaxD = 0x1p30f;  // e^(G_last - G) with the key's factor
+
 struct ChunkPlan {
     uint16_t* units = nullptr;  // [batch][chunk][Hv][kUnitElems]
     int32_t first = 0, count = 0;      // chunks of this launch
@@ -430,7 +438,7 @@ __global__ __launch_bounds__(256, 4) void delta_chunk_prepare_kernel(DeltaParams
     for (int ks = 0; ks < KS; ++ks) *reinterpret_cast<uint4*>(s_k + (16 * w + (lane >> 2)) * LK + 32 * ks + 8 * (lane & 3)) = kin[ks];
     __syncthreads();
     // What is not finite, or a factor that may overflow, would reach earlier tokens
-    // through the zeros of T: the scan runs such a chunk token by token.  64 log
+    // through the zeros of T and P: the scan runs such a chunk token by token.  64 log
     // decays of at most 1 leave e^G below 2^93.
     bool odd = false;
     if (w == 0) {
@@ -516,10 +524,13 @@ __global__ __launch_bounds__(256, 4) void delta_chunk_prepare_kernel(DeltaParams
             *reinterpret_cast<f32x4_t*>(s_l + row * LD + col) = x;
         }
     }
+    bool over = false;
     if (w == 3) {
         const double last = s_g[63], at = s_g[lane];
+        const float d = s_rk[lane] * exp2_fast(float(last - at));
+        over = !(d < kMaxD);
         vec[kVecC + lane] = s_rk[lane] * exp2_fast(float(at));
-        vec[kVecD + lane] = s_rk[lane] * exp2_fast(float(last - at));
+        vec[kVecD + lane] = d;
         vec[kVecE + lane] = s_rq[lane] * exp2_fast(float(at));
         if (lane == 0) vec[kVecLast] = exp2_fast(float(last));
     }
@@ -590,8 +601,8 @@ __global__ __launch_bounds__(256, 4) void delta_chunk_prepare_kernel(DeltaParams
         *reinterpret_cast<uint4*>(to + kTPart) = make_uint4(d[0], d[1], d[2], d[3]);
         *reinterpret_cast<uint4*>(to + 2 * kTPart) = make_uint4(e[0], e[1], e[2], e[3]);
     }
-    // keys far above 1 without a normalisation: T may overflow where the rule itself does not
-    const bool over = __ballot(!(sum < INFINITY)) != 0;
+    // keys far above 1 without a normalisation: T grows with every token, and may overflow where the rule itself does not
+    over = __ballot(over || !(sum < kMaxT)) != 0;
     if (lane == 0) vec[kVecBad + w] = over || s_bad ? 1.0f : 0.0f;
 }
 
@@ -969,8 +980,7 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[i] = vf[i] - e[i] * z[i];
             put3(reinterpret_cast<uint2*>(ex.y) + half, y[0], y[1], y[2], y[3]);
-            // an overflow of this sum only means more care
-            if (!((fabsf(y[0]) + fabsf(y[1])) + (fabsf(y[2]) + fabsf(y[3])) < INFINITY) || bad != 0.0f) s_bad = n + 1;
+            if (!((fabsf(y[0]) + fabsf(y[1])) + (fabsf(y[2]) + fabsf(y[3])) < kMaxY) || bad != 0.0f) s_bad = n + 1;
         }
         lds_barrier();  // (2)
         const int slow_word = s_bad;

@@ -369,7 +369,8 @@ int genllm_linear(const void *x, const void *w, const void *bias, void *out, int
  * [seq_len][n_v_heads]; state [n_states][n_v_heads][k_dim][v_dim], read and
  * replaced.  k_dim and v_dim 64 or 128, rows and the state 16-byte aligned.  out
  * may be v (the same address and strides) and must not overlap the other
- * inputs.  A NaN or infinite input shows from its token on, as in the rule.  A few
+ * inputs.  A NaN or infinite input, or a state that outgrows fp32, shows from its token on,
+ * as in the rule.  The sums k.k, q.q, k.q, S^T k and S^T q over a row as given are in fp32.  A few
  * tokens (up to 12, or 28 for many sequences) run token by token; longer calls run
  * in chunks and need a workspace of genllm_gated_delta_workspace_bytes (0 where
  * none is needed, about 100 MB at most below 3000 value heads), 16-byte

@@ -16,7 +16,7 @@ import pytest
 import torch
 
 from genllm_amd import paged
-from hybrid import delta_rule
+from hybrid import assert_rounded, delta_rule
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +100,27 @@ def test_prompt(S, dtype):
     out = torch.zeros(B, S, Hv, D, dtype=dtype, device="cuda")
     call(x, out)
     assert_one_rounding(out, want, f"prompt of {S} {dtype}", want.abs().amax(-1, keepdim=True))
+
+
+@pytest.mark.parametrize("squared,v,S", [(5, 8.0, 64), (4, 1.0, 128), (4, 1.0, 79), (17, 2.0, 90)])
+@pytest.mark.parametrize("heads", [1, 40])  # 40: two chains per workgroup
+def test_tokens_before_an_overflow(squared, v, S, heads):
+    """Equal keys with beta |k|^2 above 2: every token's u is 1 - |k|^2 times the last one's, until it leaves fp32.
+    Outputs up to there are the rule's.  Each token adds at most eight half steps of fp32 to what it multiplies,
+    relative, and 2^-14 is 1024 of them."""
+    k = torch.zeros(1, S, heads, 64)
+    k[..., 0], k[..., 1] = {4: (2, 0), 5: (2, 1), 17: (4, 1)}[squared]
+    x = {"q": torch.zeros(1, S, heads, 64), "k": k, "v": torch.full((1, S, heads, 128), v)}
+    x["q"][..., :2] = torch.tensor([0.5, 1.0])
+    x = {c: t.to(BF16).cuda() for c, t in x.items()}
+    x["a"], x["b"] = torch.zeros(1, S, heads).cuda(), torch.ones(1, S, heads).cuda()
+    x["state"], x["scale"] = torch.zeros(1, heads, 64, 128).cuda(), 0.125
+    want, _ = delta_rule(x["q"], x["k"], x["v"], x["a"], x["b"], x["state"], x["scale"])
+    # u and the products that form it are at most 64 times out here
+    n = int((want.abs().amax((0, 2, 3)) < 2.0 ** 121).sum())
+    assert 0 < n <= S
+    out = torch.zeros(1, S, heads, 128, dtype=BF16, device="cuda")
+    call(x, out, l2_eps=None)
+    assert_rounded(out[:, :n], want[:, :n], f"|k|^2 {squared}, {n} tokens of {S}")
+    if n < S:
+        assert not bool(torch.isfinite(out[:, -1]).any()) or bool((out[:, -1].abs() > 2.0 ** 100).any())
