@@ -36,6 +36,19 @@ def _stream(stream) -> int | None:
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
+def _workspace(nbytes: int, device, stream, make=None):
+    """A workspace for one call on `stream` (None: the current one).  It comes from that stream's own pool: a block of
+    the current stream's may still be in use by what that stream has queued, which `stream` does not wait for; and what
+    make (torch.empty, torch.zeros) launches is in order with the call."""
+    make = make or torch.empty
+    if stream is None:
+        return make(nbytes, dtype=torch.uint8, device=device)
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(_stream(stream), device=device)
+    with torch.cuda.stream(stream):
+        return make(nbytes, dtype=torch.uint8, device=device)
+
+
 def _ptr(t) -> int | None:
     if t is None:
         return None
@@ -436,14 +449,12 @@ def gated_delta_rule(q, k, v, a, b, state, out, scale: float, a_log=None, dt_bia
     the log decay and b beta, float32.  l2_eps: normalise q and k rows with it
     (None: take them as they are).  seq_lens, state_ids [B] int32 on the
     GPU.  workspace: a device buffer of at least gated_delta_workspace_bytes(...)
-    bytes when that is non-zero; None allocates one for this call."""
+    bytes when that is non-zero; None takes one for this call from the pool of the stream that it runs on."""
     if stream is not None:
         if workspace is None and all(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 4 for t in (q, v)):
             need = gated_delta_workspace_bytes(*q.shape[:3], v.shape[2], q.shape[3], v.shape[3])
-            if need:  # it goes back to the current stream's pool while `stream` still uses it
-                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-                workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream)
-                                        else torch.cuda.ExternalStream(_stream(stream), device=q.device))
+            if need:
+                workspace = _workspace(need, q.device, stream)
         stream = _stream(stream)
     rc = (_lib._calls or _lib.calls()).gated_delta_rule(q, k, v, a, b, state, out, scale, a_log, dt_bias, l2_eps, seq_lens,
                                                         state_ids, workspace, stream)
