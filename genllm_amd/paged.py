@@ -350,8 +350,7 @@ def paged_decode(q, out, k_pool, v_pool, k_ids, v_ids, n_pages: int, n_cached: i
     None allocates a zero-filled one for this call."""
     Hq, S, D, qs, os_ = _attn_args(q, out, q_layout)
     if workspace is None:
-        workspace = torch.zeros(decode_workspace_bytes(Hq, n_kv_heads, S, D, n_pages), dtype=torch.uint8,
-                                device=q.device)
+        workspace = _workspace(decode_workspace_bytes(Hq, n_kv_heads, S, D, n_pages), q.device, stream, torch.zeros)
     ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
     call("genllm_paged_decode", _ptr(q), qs[0], qs[1], _ptr(out), os_[0], os_[1], _ptr(k_pool), _ptr(v_pool),
          _ptr(k_ids), _ptr(v_ids), n_pages, n_cached, S, Hq, n_kv_heads, D, float(scale), int(causal),

@@ -78,3 +78,54 @@ def test_delta_rule_beside_pending_work(handle):
     torch.cuda.synchronize()
     assert pool_bytes(s) >= need
     assert bool((kept == 3).all()) and torch.equal(out, want) and torch.equal(state, left)
+
+
+def test_decode_takes_its_workspace_on_the_stream(pools, monkeypatch):
+    """Allocated and cleared under the call's stream: the clearing has to come before the kernels."""
+
+    class Row:
+        shape, device = (8, 1, 128), "cuda"
+
+        def stride(self, i):
+            return 128
+
+    class Block:
+        def numel(self):
+            return 64
+
+        def element_size(self):
+            return 1
+
+    calls = []
+    monkeypatch.setattr(paged, "call", lambda *a: calls.append(a))
+    monkeypatch.setattr(paged, "_ptr", lambda t: t)
+    monkeypatch.setattr(torch, "zeros", lambda n, dtype, device, was=torch.zeros: (was(n, dtype, device), Block())[1])
+    s = torch.cuda.Stream(77)
+    paged.paged_decode(Row(), Row(), 0, 0, 0, 0, 4, 60, 2, 0.1, stream=s)
+    assert [(f, u) for f, _, u in pools] == [("zeros", s)] and calls[0][-1] == 77
+    paged.paged_decode(Row(), Row(), 0, 0, 0, 0, 4, 60, 2, 0.1, stream=88)
+    assert pools[1][2].cuda_stream == 88 and calls[1][-1] == 88
+
+
+@pytest.mark.gpu
+def test_decode_beside_pending_work():
+    g = torch.Generator().manual_seed(5)
+    pages, H, D, n = 64, 2, 128, 1000
+    k, v = (torch.randn(pages, 16, H, D, generator=g).bfloat16().cuda() for _ in "kv")
+    ids = torch.randperm(pages, generator=g).int().cuda()
+    q = torch.randn(8, 1, D, generator=g).bfloat16().cuda()
+    want, out = torch.zeros_like(q), torch.zeros_like(q)
+    args = (k, v, ids, ids, -(-n // 16), n, H, D ** -0.5)
+    paged.paged_decode(q, want, *args)
+    need = paged.decode_workspace_bytes(8, H, 1, D, -(-n // 16))
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    block = torch.empty(need, dtype=torch.uint8, device="cuda")
+    torch.cuda._sleep(20_000_000)
+    block.fill_(3)
+    kept = block.clone()
+    del block
+    paged.paged_decode(q, out, *args, stream=s)
+    torch.cuda.synchronize()
+    assert pool_bytes(s) >= need
+    assert bool((kept == 3).all()) and torch.equal(out, want)
