@@ -1145,6 +1145,10 @@ int launch_recurrent(const DeltaParams& p, hipStream_t stream) {
     return GENLLM_OK;
 }
 
+bool dim_served(int32_t d) { return d == 64 || d == 128; }
+bool heads_served(int64_t B, int64_t Hv) { return B * Hv <= (int64_t(1) << 19); }  // a grid has at most 2^32 threads
+bool tokens_served(int64_t S) { return S <= (int64_t(1) << 30); }
+
 bool strides_ok(const Rows3& r) { return aligned_to(r.p, 16) && ((r.batch | r.tok | r.head) & 7) == 0; }
 
 }  // namespace
@@ -1155,8 +1159,8 @@ using namespace genllm;
 
 extern "C" size_t genllm_gated_delta_workspace_bytes(int32_t batch, int32_t seq_len, int32_t n_k_heads, int32_t n_v_heads,
                                                      int32_t k_dim, int32_t v_dim) {
-    if (batch <= 0 || seq_len <= 0 || n_k_heads <= 0 || n_v_heads <= 0 || k_dim <= 0 || v_dim <= 0 ||
-        !in_chunks(batch, seq_len, n_v_heads, v_dim))
+    if (batch <= 0 || seq_len <= 0 || n_k_heads <= 0 || n_v_heads <= 0 || !dim_served(k_dim) || !dim_served(v_dim) ||
+        !heads_served(batch, n_v_heads) || !tokens_served(seq_len) || !in_chunks(batch, seq_len, n_v_heads, v_dim))
         return 0;
     const LaunchPlan plan = launch_plan(batch, seq_len, n_v_heads, v_dim);
     return size_t(plan.entries) * size_t(plan.chunks) * size_t(n_v_heads) * kUnitBytes;
@@ -1176,7 +1180,7 @@ extern "C" int genllm_gated_delta_rule(const void* q, int64_t q_batch_stride, in
         return fail(GENLLM_ERR_INVALID, "gated_delta_rule: negative or zero size");
     if (n_v_heads % n_k_heads)
         return fail(GENLLM_ERR_INVALID, "gated_delta_rule: n_v_heads must be a multiple of n_k_heads");
-    if ((k_dim != 64 && k_dim != 128) || (v_dim != 64 && v_dim != 128))
+    if (!dim_served(k_dim) || !dim_served(v_dim))
         return fail(GENLLM_ERR_UNSUPPORTED, "gated_delta_rule: k_dim and v_dim of 64 or 128 are served");
     if (dtype != GENLLM_DTYPE_BF16 && dtype != GENLLM_DTYPE_F16)
         return fail(GENLLM_ERR_UNSUPPORTED, "gated_delta_rule: bf16 or fp16 elements");
@@ -1212,8 +1216,8 @@ extern "C" int genllm_gated_delta_rule(const void* q, int64_t q_batch_stride, in
     if (!aligned_to(a, gate_align) || !aligned_to(b, gate_align) || !aligned_to(a_log, 4) || !aligned_to(dt_bias, 4) ||
         !aligned_to(state_ids, 4) || !aligned_to(seq_lens, 4))
         return fail(GENLLM_ERR_INVALID, "gated_delta_rule: a pointer is not aligned to its type");
-    if (seq_len > (1 << 30)) return fail(GENLLM_ERR_INVALID, "gated_delta_rule: seq_len must be at most 2^30");
-    if (int64_t(batch) * n_v_heads > (int64_t(1) << 19))  // a grid has at most 2^32 threads
+    if (!tokens_served(seq_len)) return fail(GENLLM_ERR_INVALID, "gated_delta_rule: seq_len must be at most 2^30");
+    if (!heads_served(batch, n_v_heads))
         return fail(GENLLM_ERR_INVALID, "gated_delta_rule: batch * n_v_heads must be at most 2^19");
     p.a = a, p.b = b, p.a_batch = a_batch_stride, p.a_tok = a_tok_stride, p.b_batch = b_batch_stride, p.b_tok = b_tok_stride;
     p.a_log = a_log, p.dt_bias = dt_bias, p.state = state;

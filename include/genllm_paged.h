@@ -373,7 +373,7 @@ int genllm_linear(const void *x, const void *w, const void *bias, void *out, int
  * as in the rule.  The sums k.k, q.q, k.q, S^T k and S^T q over a row as given are in fp32.  A few
  * tokens (up to 12, or 28 for many sequences) run token by token; longer calls run
  * in chunks and need a workspace of genllm_gated_delta_workspace_bytes (0 where
- * none is needed, about 100 MB at most below 3000 value heads), 16-byte
+ * none is needed or the sizes are refused, about 100 MB at most below 3000 value heads), 16-byte
  * aligned, whose contents do not matter before or after the call; calls that
  * share one must be ordered. */
 size_t genllm_gated_delta_workspace_bytes(int32_t batch, int32_t seq_len, int32_t n_k_heads, int32_t n_v_heads,
