@@ -35,6 +35,7 @@
 
 #include "common.hpp"
 #include "kernels.hpp"
+#include "rows.hpp"
 #include "sequences.hpp"
 
 namespace genllm {
@@ -1151,6 +1152,35 @@ bool tokens_served(int64_t S) { return S <= (int64_t(1) << 30); }
 
 bool strides_ok(const Rows3& r) { return aligned_to(r.p, 16) && ((r.batch | r.tok | r.head) & 7) == 0; }
 
+// "NAME overlaps NAME" where a call would write what it or another workgroup reads.
+// out may be v itself: a workgroup has read an element before it writes over it.
+std::string overlap_of(const DeltaParams& p, const void* ws, size_t ws_bytes) {
+    const auto rows = [&](const void* at, int64_t batch, int64_t tok, int64_t head, int64_t heads, int64_t bytes, int64_t elem) {
+        Rows r = Rows::whole(at, bytes * elem);
+        const int64_t n[3] = {p.B, p.seq.S, heads}, stride[3] = {batch * elem, tok * elem, head * elem};
+        std::copy(n, n + 3, r.n), std::copy(stride, stride + 3, r.stride);
+        return r;
+    };
+    const Rows v = rows(p.v.p, p.v.batch, p.v.tok, p.v.head, p.Hv, p.Dv, 2);
+    const int64_t gate = p.a_log ? 2 : 4, states = p.seq.ids ? p.seq.n_states : p.B;
+    const NamedRows written[] = {{"out", rows(p.out, p.o_batch, p.o_tok, p.o_head, p.Hv, p.Dv, 2)},
+                               {"the state", Rows::whole(p.state, states * p.Hv * p.Dk * p.Dv * 4)},
+                               {"the workspace", Rows::whole(ws, int64_t(ws_bytes))}};
+    const NamedRows read[] = {{"q", rows(p.q.p, p.q.batch, p.q.tok, p.q.head, p.Hk, p.Dk, 2)},
+                            {"k", rows(p.k.p, p.k.batch, p.k.tok, p.k.head, p.Hk, p.Dk, 2)},
+                            {"v", v},
+                            {"a", rows(p.a, p.a_batch, p.a_tok, 0, 1, p.Hv, gate)},
+                            {"b", rows(p.b, p.b_batch, p.b_tok, 0, 1, p.Hv, gate)},
+                            {"a_log", Rows::whole(p.a_log, p.Hv * 4)},
+                            {"dt_bias", Rows::whole(p.dt_bias, p.Hv * 4)},
+                            {"state_ids", Rows::whole(p.seq.ids, p.B * 4)},
+                            {"seq_lens", Rows::whole(p.seq.lens, p.B * 4)}};
+    const char *a, *b;
+    const auto out_is_v = [&](const Rows& w, const Rows& r) { return w.same_as(v) && r.same_as(v); };
+    if (find_overlap(written, read, out_is_v, a, b)) return std::string(a) + " overlaps " + b;
+    return rows_shared_within(written[0].rows) ? "rows of out share memory" : std::string();
+}
+
 }  // namespace
 
 }  // namespace genllm
@@ -1208,9 +1238,6 @@ extern "C" int genllm_gated_delta_rule(const void* q, int64_t q_batch_stride, in
     if (!strides_ok(p.q) || !strides_ok(p.k) || !strides_ok(p.v) ||
         !strides_ok({p.out, o_batch_stride, o_tok_stride, o_head_stride}) || !aligned_to(state, 16))
         return fail(GENLLM_ERR_INVALID, "gated_delta_rule: q, k, v, out rows and the state must be 16-byte aligned");
-    if (out == q || out == k || out == state ||
-        (out == v && (v_batch_stride != o_batch_stride || v_tok_stride != o_tok_stride || v_head_stride != o_head_stride)))
-        return fail(GENLLM_ERR_INVALID, "gated_delta_rule: out overlaps an input");
     const bool f16 = dtype == GENLLM_DTYPE_F16;
     const uintptr_t gate_align = a_log ? 2 : 4;
     if (!aligned_to(a, gate_align) || !aligned_to(b, gate_align) || !aligned_to(a_log, 4) || !aligned_to(dt_bias, 4) ||
@@ -1224,14 +1251,19 @@ extern "C" int genllm_gated_delta_rule(const void* q, int64_t q_batch_stride, in
     p.seq.ids = state_ids, p.seq.lens = seq_lens, p.seq.n_states = n_states, p.seq.S = seq_len;
     p.B = batch, p.Hk = n_k_heads, p.Hv = n_v_heads, p.G = n_v_heads / n_k_heads, p.Dk = k_dim, p.Dv = v_dim;
     p.scale = scale, p.l2_eps = l2_eps < 0.0f ? -1.0f : l2_eps;
-    if (in_chunks(batch, seq_len, n_v_heads, v_dim)) {
-        const size_t need = genllm_gated_delta_workspace_bytes(batch, seq_len, n_k_heads, n_v_heads, k_dim, v_dim);
+    const bool chunks = in_chunks(batch, seq_len, n_v_heads, v_dim);
+    size_t need = 0;
+    if (chunks) {
+        need = genllm_gated_delta_workspace_bytes(batch, seq_len, n_k_heads, n_v_heads, k_dim, v_dim);
         if (!workspace || workspace_bytes < need || !aligned_to(workspace, 16))
             return fail(GENLLM_ERR_INVALID, "gated_delta_rule: a workspace of " + std::to_string(need) +
                                                 " bytes, 16-byte aligned, is needed (have " +
                                                 std::to_string(workspace_bytes) + ")");
-        return f16 ? launch_chunks<true>(p, workspace, as_stream(stream)) : launch_chunks<false>(p, workspace, as_stream(stream));
     }
+    if (const std::string why = overlap_of(p, chunks ? workspace : nullptr, need); !why.empty())
+        return fail(GENLLM_ERR_INVALID, "gated_delta_rule: " + why);
+    if (chunks)
+        return f16 ? launch_chunks<true>(p, workspace, as_stream(stream)) : launch_chunks<false>(p, workspace, as_stream(stream));
     const hipStream_t s = as_stream(stream);
     if (column_waves(batch, n_v_heads, v_dim) >= 2 * kManyWaves)
         return f16 ? launch_recurrent<8, true>(p, s) : launch_recurrent<8, false>(p, s);

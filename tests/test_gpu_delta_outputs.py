@@ -124,3 +124,26 @@ def test_tokens_before_an_overflow(squared, v, S, heads):
     assert_rounded(out[:, :n], want[:, :n], f"|k|^2 {squared}, {n} tokens of {S}")
     if n < S:
         assert not bool(torch.isfinite(out[:, -1]).any()) or bool((out[:, -1].abs() > 2.0 ** 100).any())
+
+
+@pytest.mark.parametrize("S", [3, 80])
+@pytest.mark.parametrize("order", ["token", "head"])
+def test_one_buffer_for_all(S, order):
+    """q, k, v and out in one buffer, beside each other in every row or head by head: nothing is shared, and nothing else
+    in the buffer is written."""
+    g = torch.Generator().manual_seed(S)
+    B, Hk, Hv, D = 2, 2, 4, 64
+    H = 2 * Hk + 2 * Hv + 1  # the last head is nobody's
+    if order == "token":
+        buf = torch.randn(B, S, H, D, generator=g).bfloat16().cuda()
+    else:
+        buf = torch.randn(B, H, S, D, generator=g).bfloat16().cuda().transpose(1, 2)
+    first = buf.clone()
+    q, k, v, out, _ = torch.split(buf, [Hk, Hk, Hv, Hv, 1], 2)
+    x = {"q": q, "k": k, "v": v, "a": (-torch.rand(B, S, Hv, generator=g)).cuda(), "b": torch.rand(B, S, Hv, generator=g).cuda(),
+         "state": torch.randn(B, Hv, D, D, generator=g).cuda(), "scale": 0.125}
+    want, _ = delta_rule(q, k, v, x["a"], x["b"], x["state"], x["scale"], l2_eps=1e-6)
+    call(x, out)
+    assert_rounded(out, want, f"one buffer, {order}")
+    keep = [h for h in range(H) if not 2 * Hk + Hv <= h < 2 * Hk + 2 * Hv]
+    assert torch.equal(buf[:, :, keep], first[:, :, keep])

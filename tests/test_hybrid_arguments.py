@@ -19,3 +19,34 @@ def test_workspace_at_the_limits():
     f = _lib.lib().genllm_gated_delta_workspace_bytes
     assert f(1, 12, 16, 32, 128, 128) == 0 and f(1, 1 << 30, 16, 32, 128, 128) > 0
     assert 0 < f(1 << 15, 64, 16, 16, 64, 64) < 1 << 30 and f(1, 64, 1, 1 << 19, 64, 64) > 0
+
+
+def delta(**kw):
+    """A call on placeholder addresses far apart from each other; only ones that are refused are made."""
+    a = dict(q=0x1000000, qb=4096, qt=1024, qh=128, k=0x2000000, kb=4096, kt=1024, kh=128, v=0x3000000, vb=8192, vt=2048, vh=128,
+             a=0x4000000, ab=64, at=16, b=0x5000000, bb=64, bt=16, a_log=0x6000000, dt=0x7000000, state=0x10000000, n=4,
+             ids=None, lens=None, out=0x9000000, ob=8192, ot=2048, oh=128, B=2, S=4, Hk=8, Hv=16, Dk=128, Dv=128, dtype=30,
+             scale=0.1, l2=1e-6, ws=None, wsb=0, stream=None)
+    assert not set(kw) - set(a)
+    return _lib.lib().genllm_gated_delta_rule(*dict(a, **kw).values())
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(out=0x1000000 + 2 * 1024), b"out overlaps q"),  # a token further on
+    (dict(out=0x1000000 - 0x8000 + 16), b"out overlaps q"),  # the last row's last elements
+    (dict(out=0x2000000 + 16), b"out overlaps k"), (dict(out=0x3000000 + 2 * 128), b"out overlaps v"),
+    (dict(out=0x3000000 - 2 * 2048), b"out overlaps v"), (dict(out=0x3000000, ob=8192 * 2), b"out overlaps v"),
+    (dict(out=0x4000000), b"out overlaps a"), (dict(out=0x5000000), b"out overlaps b"),
+    (dict(out=0x5000000 - 0x8000 + 16), b"out overlaps b"), (dict(out=0x6000020), b"out overlaps a_log"),
+    (dict(out=0x10000000 + 0x100000), b"the state overlaps out"), (dict(state=0x3000000), b"the state overlaps v"),
+    (dict(state=0x4000000 - 0x100000), b"the state overlaps a"),
+    # states that only ids reach
+    (dict(ids=0x8000000, out=0x10000000 + 3 * 0x100000), b"the state overlaps out"), (dict(ids=0x9000100), b"out overlaps state_ids"),
+    (dict(lens=0x10000010), b"the state overlaps seq_lens"), (dict(ot=1024), b"rows of out share memory"),
+    (dict(oh=64), b"rows of out share memory"),
+    (dict(S=100, qb=1 << 17, kb=1 << 17, vb=1 << 18, ob=1 << 18, ws=0x3000000, wsb=1 << 30), b"the workspace overlaps v"),
+    (dict(S=100, qb=1 << 17, kb=1 << 17, vb=1 << 18, ob=1 << 18, ws=0xFFFF000, wsb=1 << 30), b"the workspace overlaps the state"),
+    (dict(S=100, qb=1 << 17, kb=1 << 17, vb=1 << 18, ob=1 << 18, ws=0x9000000, wsb=1 << 30), b"the workspace overlaps out")])
+def test_delta_rule_refuses_what_it_would_write_over(kw, msg):
+    assert delta(**kw) == _lib.ERR_INVALID
+    assert msg in _lib.lib().genllm_last_error(), _lib.lib().genllm_last_error()
