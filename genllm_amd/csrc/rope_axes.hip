@@ -14,9 +14,11 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <string>
 
 #include "common.hpp"
 #include "kernels.hpp"
+#include "rows.hpp"
 #include "sequences.hpp"
 
 namespace genllm {
@@ -188,6 +190,36 @@ bool rows_ok(const AxesRows& r) {
            ((r.x_tok | r.x_head | r.o_tok | r.o_head) & 7) == 0;
 }
 
+// "NAME overlaps NAME" where a row would be written that another workgroup reads.  An
+// output may be its own input: a row is in registers before it is written.
+std::string overlap_of(const AxesParams& p, int D, int n_axes) {
+    const auto rows = [&](const uint16_t* at, int64_t tok, int64_t head, int32_t heads) {
+        Rows r = Rows::whole(heads ? at : nullptr, 2 * D);
+        r.n[0] = p.S, r.n[1] = heads, r.stride[0] = 2 * tok, r.stride[1] = 2 * head;
+        return r;
+    };
+    const Rows q = rows(p.q.x, p.q.x_tok, p.q.x_head, p.Hq), k = rows(p.k.x, p.k.x_tok, p.k.x_head, p.Hk);
+    const int64_t table = int64_t(p.max_seq) * p.rope_dim * 4;
+    Rows pos = Rows::whole(p.pos, int64_t(p.S) * 4);
+    pos.n[0] = n_axes, pos.stride[0] = p.pos_stride * 4;
+    const NamedRows written[] = {{"q_out", rows(p.q.out, p.q.o_tok, p.q.o_head, p.Hq)}, {"k_out", rows(p.k.out, p.k.o_tok, p.k.o_head, p.Hk)}};
+    const NamedRows read[] = {{"q", q},
+                              {"k", k},
+                              {"gamma_q", Rows::whole(p.Hq ? p.q.gamma : nullptr, D * 4)},
+                              {"gamma_k", Rows::whole(p.Hk ? p.k.gamma : nullptr, D * 4)},
+                              {"cos", Rows::whole(p.cos_tab, table)},
+                              {"sin", Rows::whole(p.sin_tab, table)},
+                              {"positions", pos}};
+    const char *a, *b;
+    const auto in_place = [&](const Rows& w, const Rows& r) {
+        return w.same_as(r) && (&r == &read[0].rows ? &w == &written[0].rows : &r == &read[1].rows && &w == &written[1].rows);
+    };
+    if (find_overlap(written, read, in_place, a, b)) return std::string(a) + " overlaps " + b;
+    for (const NamedRows& w : written)
+        if (rows_shared_within(w.rows)) return std::string("rows of ") + w.name + " share memory";
+    return {};
+}
+
 }  // namespace
 
 }  // namespace genllm
@@ -251,14 +283,14 @@ extern "C" int genllm_qk_norm_rope_axes(const void* q, int64_t q_tok_stride, int
     const auto moved = [](const AxesRows& r) { return r.x == r.out && (r.x_tok != r.o_tok || r.x_head != r.o_head); };
     if ((n_q_heads && moved(p.q)) || (n_k_heads && moved(p.k)))
         return fail(GENLLM_ERR_INVALID, "qk_norm_rope_axes: an output over its input needs the same strides");
-    if (n_q_heads && n_k_heads && (p.q.x == p.k.out || p.k.x == p.q.out || p.q.out == p.k.out))
-        return fail(GENLLM_ERR_INVALID, "qk_norm_rope_axes: an output overlaps the other input or output");
     if ((n_q_heads && !rows_ok(p.q)) || (n_k_heads && !rows_ok(p.k)))
         return fail(GENLLM_ERR_INVALID, "qk_norm_rope_axes: q, k, their outputs and gammas must be 16-byte aligned");
     if (!aligned_to(cos_tab, 4) || !aligned_to(sin_tab, 4) || !aligned_to(positions, 4))
         return fail(GENLLM_ERR_INVALID, "qk_norm_rope_axes: a pointer is not aligned to its type");
     p.Hq = n_q_heads, p.Hk = n_k_heads, p.S = seq_len, p.rope_dim = rope_dim, p.max_seq = max_seq;
     p.eps = eps, p.cos_tab = cos_tab, p.sin_tab = sin_tab, p.pos = positions, p.pos_stride = pos_stride;
+    if (const std::string why = overlap_of(p, head_dim, n_axes); !why.empty())
+        return fail(GENLLM_ERR_INVALID, "qk_norm_rope_axes: " + why);
     return dtype == GENLLM_DTYPE_F16 ? launch_axes<true>(p, head_dim, as_stream(stream))
                                      : launch_axes<false>(p, head_dim, as_stream(stream));
 }

@@ -1,4 +1,6 @@
 """Sizes and addresses that the hybrid layers' entry points have to refuse or answer without any device work."""
+import ctypes as C
+
 import pytest
 
 from genllm_amd import _lib
@@ -49,4 +51,28 @@ def delta(**kw):
     (dict(S=100, qb=1 << 17, kb=1 << 17, vb=1 << 18, ob=1 << 18, ws=0x9000000, wsb=1 << 30), b"the workspace overlaps out")])
 def test_delta_rule_refuses_what_it_would_write_over(kw, msg):
     assert delta(**kw) == _lib.ERR_INVALID
+    assert msg in _lib.lib().genllm_last_error(), _lib.lib().genllm_last_error()
+
+
+def axes(sections=(11, 11, 10), **kw):
+    """Eight heads of q and two of k beside each other in rows of 2560; outputs head by head."""
+    a = dict(q=0x1000000, qt=2560, qh=256, qo=0x2000000, qot=256, qoh=1024, gq=0x3000000, Hq=8, k=0x1000000 + 2 * 2048, kt=2560,
+             kh=256, ko=0x5000000, kot=256, koh=1024, gk=0x6000000, Hk=2, eps=1e-6, cos=0x7000000, sin=0x8000000, rows=100,
+             rope=64, pos=0x9000000, ps=4, n=3, sec=(C.c_int32 * 8)(*sections), inter=1, S=4, D=256, dtype=30, stream=None)
+    assert not set(kw) - set(a)
+    return _lib.lib().genllm_qk_norm_rope_axes(*dict(a, **kw).values())
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(qo=0x1000000 + 2 * 2560, qot=2560, qoh=256), b"q_out overlaps q"),  # a token further on
+    (dict(qo=0x1000000 + 2 * 256, qot=2560, qoh=256), b"q_out overlaps q"),  # a head further on
+    (dict(qo=0x1000000 + 2 * 512, qot=2560, qoh=256), b"q_out overlaps q"),
+    (dict(ko=0x1000000 + 2 * 2048 + 16, kot=2560, koh=256), b"k_out overlaps"), (dict(ko=0x1000000, kot=2560, koh=256), b"k_out overlaps q"),
+    (dict(ko=0x2000000 + 2 * 7 * 1024), b"k_out overlaps q_out"), (dict(ko=0x2000000 - 2 * 2048 + 16), b"k_out overlaps q_out"),
+    (dict(qo=0x3000000), b"q_out overlaps gamma_q"), (dict(ko=0x3000000), b"k_out overlaps gamma_q"),
+    (dict(qo=0x6000000 - 512), b"q_out overlaps gamma_k"), (dict(qo=0x7000000 + 99 * 256), b"q_out overlaps cos"),
+    (dict(ko=0x8000000 - 16), b"k_out overlaps sin"), (dict(ko=0x9000000), b"k_out overlaps positions"),
+    (dict(qot=128), b"rows of q_out share memory"), (dict(koh=256), b"rows of k_out share memory")])
+def test_rotation_refuses_what_it_would_write_over(kw, msg):
+    assert axes(**kw) == _lib.ERR_INVALID
     assert msg in _lib.lib().genllm_last_error(), _lib.lib().genllm_last_error()
