@@ -12,9 +12,11 @@
 // another, id then state (3.3 us).
 #include <algorithm>
 #include <climits>
+#include <string>
 
 #include "common.hpp"
 #include "kernels.hpp"
+#include "rows.hpp"
 #include "sequences.hpp"
 
 namespace genllm {
@@ -179,24 +181,24 @@ int launch_conv_w(ConvParams& p, int width, hipStream_t stream) {
                       : width == 3 ? launch_conv<3, V, F16>(p, stream) : launch_conv<4, V, F16>(p, stream);
 }
 
-// Whether rows of out may lie over rows of x: their address ranges meet, and they
-// are not channels beside each other of rows with the same strides.
-bool rows_overlap(const void* x, int64_t xb, int64_t xt, const void* o, int64_t ob, int64_t ot, int64_t B, int64_t S,
-                  int64_t C) {
-    const auto range = [&](const void* p, int64_t b, int64_t t, uintptr_t& lo, uintptr_t& hi) {
-        const int64_t eb = (B - 1) * b, et = (S - 1) * t;
-        lo = reinterpret_cast<uintptr_t>(p) + 2 * ((eb < 0 ? eb : 0) + (et < 0 ? et : 0));
-        hi = reinterpret_cast<uintptr_t>(p) + 2 * ((eb > 0 ? eb : 0) + (et > 0 ? et : 0) + C);
+// "NAME overlaps NAME" where rows would be written that another workgroup reads.
+std::string overlap_of(const ConvParams& p, int width) {
+    const auto rows = [&](const uint16_t* at, int64_t batch, int64_t tok) {
+        Rows r = Rows::whole(at, int64_t(p.C) * 2);
+        r.n[0] = p.B, r.n[1] = p.seq.S, r.stride[0] = 2 * batch, r.stride[1] = 2 * tok;
+        return r;
     };
-    uintptr_t xl, xh, ol, oh;
-    range(x, xb, xt, xl, xh);
-    range(o, ob, ot, ol, oh);
-    if (xh <= ol || oh <= xl) return false;
-    // multiples of one row pitch apart from each other, the offset between them leaves both rows room in it
-    const int64_t pitch = S > 1 ? xt : xb;
-    if (pitch <= 0 || (S > 1 && xt != ot) || (B > 1 && xb != ob) || (S > 1 && B > 1 && xb % pitch)) return true;
-    const int64_t d = (int64_t(reinterpret_cast<uintptr_t>(o) - reinterpret_cast<uintptr_t>(x)) / 2 % pitch + pitch) % pitch;
-    return d < C || pitch - d < C;
+    const int64_t states = p.seq.ids ? p.seq.n_states : p.B;
+    const NamedRows written[] = {{"out", rows(p.out, p.o_batch, p.o_tok)},
+                                 {"the state", Rows::whole(p.state, states * (width - 1) * p.C * 2)}};
+    const NamedRows read[] = {{"x", rows(p.x, p.x_batch, p.x_tok)},
+                              {"the weight", Rows::whole(p.w, int64_t(p.C) * width * 2)},
+                              {"the bias", Rows::whole(p.bias, int64_t(p.C) * 2)},
+                              {"state_ids", Rows::whole(p.seq.ids, int64_t(p.B) * 4)},
+                              {"seq_lens", Rows::whole(p.seq.lens, int64_t(p.B) * 4)}};
+    const char *a, *b;
+    if (find_overlap(written, read, [](const Rows&, const Rows&) { return false; }, a, b)) return std::string(a) + " overlaps " + b;
+    return rows_shared_within(written[0].rows) ? "rows of out share memory" : std::string();
 }
 
 }  // namespace
@@ -228,9 +230,6 @@ extern "C" int genllm_causal_conv(const void* x, int64_t x_batch_stride, int64_t
     if (seq_len == 1) x_tok_stride = o_tok_stride = 0;
     if ((batch > 1 && !o_batch_stride) || (seq_len > 1 && !o_tok_stride))
         return fail(GENLLM_ERR_INVALID, "causal_conv: rows of out share memory");
-    if (rows_overlap(x, x_batch_stride, x_tok_stride, out, o_batch_stride, o_tok_stride, batch, seq_len, channels))
-        return fail(GENLLM_ERR_INVALID, "causal_conv: out overlaps x");
-    if (state == x || state == out) return fail(GENLLM_ERR_INVALID, "causal_conv: the state overlaps x or out");
     ConvParams p;
     p.x = static_cast<const uint16_t*>(x), p.x_batch = x_batch_stride, p.x_tok = x_tok_stride;
     p.out = static_cast<uint16_t*>(out), p.o_batch = o_batch_stride, p.o_tok = o_tok_stride;
@@ -238,6 +237,7 @@ extern "C" int genllm_causal_conv(const void* x, int64_t x_batch_stride, int64_t
     p.state = static_cast<uint16_t*>(state);
     p.seq.ids = state_ids, p.seq.lens = seq_lens, p.seq.n_states = n_states, p.seq.S = seq_len;
     p.B = batch, p.C = channels, p.silu = silu != 0;
+    if (const std::string why = overlap_of(p, width); !why.empty()) return fail(GENLLM_ERR_INVALID, "causal_conv: " + why);
     // 16 bytes per access, or one element where rows do not allow it (2048 tokens of 8192 channels 17.6 against 27.7 us)
     const bool wide = channels % 8 == 0 && ((x_batch_stride | x_tok_stride | o_batch_stride | o_tok_stride) & 7) == 0 &&
                       aligned_to(x, 16) && aligned_to(out, 16) && aligned_to(state, 16) && aligned_to(weight, 16) &&

@@ -76,3 +76,23 @@ def axes(sections=(11, 11, 10), **kw):
 def test_rotation_refuses_what_it_would_write_over(kw, msg):
     assert axes(**kw) == _lib.ERR_INVALID
     assert msg in _lib.lib().genllm_last_error(), _lib.lib().genllm_last_error()
+
+
+def conv(**kw):
+    a = dict(x=0x1000000, xb=4096, xt=64, w=0x2000000, bias=0x3000000, out=0x9000000, ob=4096, ot=64, state=0x8000000, n=4, ids=None,
+             lens=None, B=2, S=64, C=64, W=4, dtype=30, silu=1, stream=None)
+    assert not set(kw) - set(a)
+    return _lib.lib().genllm_causal_conv(*dict(a, **kw).values())
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(state=0x1000000 + 64), b"the state overlaps x"), (dict(state=0x1000000 - 2 * 3 * 64 * 2 + 2), b"the state overlaps x"),
+    (dict(state=0x9000000 + 2 * 4096 * 2 - 2), b"the state overlaps out"), (dict(state=0x2000000), b"the state overlaps the weight"),
+    (dict(state=0x3000000 - 2), b"the state overlaps the bias"), (dict(out=0x2000000 + 510), b"out overlaps the weight"),
+    # a state that only ids reach
+    (dict(ids=0x7000000, out=0x8000000 + 3 * 3 * 64 * 2), b"the state overlaps out"), (dict(lens=0x9000000), b"out overlaps seq_lens"),
+    (dict(out=0x1000000 + 2 * 64, xt=128, ot=128, ob=8192 + 64, xb=8192), b"out overlaps x"),  # beside x in the first entry only
+    (dict(ot=32, ob=4096), b"rows of out share memory"), (dict(ob=128, ot=128), b"rows of out share memory")])
+def test_convolution_refuses_what_it_would_write_over(kw, msg):
+    assert conv(**kw) == _lib.ERR_INVALID
+    assert msg in _lib.lib().genllm_last_error(), _lib.lib().genllm_last_error()
