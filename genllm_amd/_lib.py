@@ -148,7 +148,7 @@ def calls():
             from . import _calls as module
         except ImportError as e:
             raise RuntimeError(f"{HERE}/_calls.so does not load ({e}): run __graft_entry__.build() "
-                               "(make -C genllm_amd/csrc)") from e
+                               "(make -C genllm_amd/csrc calls)") from e
         module.bind(*(C.cast(getattr(L, name), _P).value
                       for name in ("genllm_gated_delta_workspace_bytes", "genllm_gated_delta_rule", "genllm_causal_conv",
                                    "genllm_qk_norm_rope_axes")))

@@ -15,7 +15,7 @@ def build_library(clean: bool = True, jobs: int = 8) -> str:
     """Compile every HIP source for gfx950 and link libgenllm_hip.so; the Python calls on tensors into _calls.so."""
     if clean:
         subprocess.run(["make", "-s", "-C", CSRC, "clean"], check=True)
-    subprocess.run(["make", "-s", "-C", CSRC, f"-j{jobs}", f"PYTHON={sys.executable}"], check=True)
+    subprocess.run(["make", "-s", "-C", CSRC, f"-j{jobs}", f"PYTHON={sys.executable}", "all", "calls"], check=True)
     for path in (LIB, CALLS):
         if not os.path.exists(path):
             raise RuntimeError("build did not produce " + path)
