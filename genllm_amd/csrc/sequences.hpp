@@ -16,17 +16,19 @@ struct Sequences {
 };
 
 constexpr int kEntryEmpty = -1;  // no sequence here: nothing is read or written
-constexpr int kEntryBad = -2;    // no such state, or an earlier entry's: NaN results, no state is touched
+constexpr int kEntryBad = -2;    // no such state, or that of an earlier entry with tokens: NaN results, no state is touched
 
 // The state of entry b.  Every lane of the wave calls it with the same b; the
 // result is uniform.  Two entries with one state would race on it, so that the
-// later one is bad.
+// later one is bad.  An entry without tokens leaves its state alone, and so does not
+// count: a server's idle rows may keep the ids they had.
 __device__ __forceinline__ int entry_state(const Sequences& s, int b) {
     if (!s.ids) return b;
     const int id = s.ids[b];
     if (id < 0) return kEntryEmpty;
     bool bad = id >= s.n_states;
-    for (int i = int(threadIdx.x & 63); i < b; i += 64) bad |= s.ids[i] == id;
+    for (int i = int(threadIdx.x & 63); i < b; i += 64)
+        if (s.ids[i] == id && (!s.lens || s.lens[i] > 0)) bad = true;
     return __ballot(bad) != 0 ? kEntryBad : __builtin_amdgcn_readfirstlane(id);
 }
 

@@ -353,9 +353,9 @@ int genllm_linear(const void *x, const void *w, const void *bias, void *out, int
  * tokens (device; null: all have seq_len; values are clamped to 0..seq_len) and
  * the state state_ids[b] (device; null: state b).  Rows of out behind an
  * entry's last token are left as they were.  An entry with a negative id or no
- * tokens reads and writes nothing.  An id past the states, or one that an
- * earlier entry of the batch has, gives NaN in the entry's rows of out and
- * leaves the states alone.
+ * tokens changes nothing, and what its rows hold does not matter.  An id past the
+ * states, or one that an earlier entry with tokens has, gives NaN in the entry's
+ * rows of out and leaves the states alone.
  *
  * genllm_gated_delta_rule: per entry and value head h (key head h / (n_v_heads /
  * n_k_heads)) the state S [k_dim][v_dim], fp32, takes token after token:
