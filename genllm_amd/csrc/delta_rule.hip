@@ -862,9 +862,6 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
         return;
     }
 
-    const auto in_order = [] {
-        if constexpr (!F16) __builtin_amdgcn_sched_barrier(0);
-    };
     const int chain = NC == 1 ? 0 : w >> 2, cw = NC == 1 ? w : w & 3;  // the wave's chain, and its number there
     Exchange& ex = s_ex[chain];
     const int col = col0 + kScanCols * chain;
@@ -913,13 +910,8 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
     lds_barrier();
     for (int n = 0; n < chunks; ++n) {
         const Stage& in = s_in[n & 1];
-        // bf16: all of the chunk that (1) to (3) take is on its way before the first use (left
-        // to itself the compiler puts most of these reads in front of the barrier; 2048 tokens
-        // of 32 heads of 128, both kernels, 68.6 -> 68.3 us; fp16, with more registers in use,
-        // 83.2 without this order, 84.0 with it)
         Op fk[4];
         load_k(in, fk);
-        in_order();
         const uint4* const t = s_t[n & (TQ - 1)];
         uint4 ft[2][3];
 #pragma unroll
@@ -931,7 +923,6 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
         const f32x4_t d = *reinterpret_cast<const f32x4_t*>(in.vec + kVecD + tok0);
         const float last = in.vec[kVecLast], bad = in.vec[kVecBad + tile];
         const uint2 v = read_transposed(reinterpret_cast<const uint2*>(in.v) + 4 * (NC * (tok0 + (r >> 2)) + chain) + (r & 3));
-        in_order();
         f32x4_t x[4];
         {  // (1)
             Op s0, s1, s2;
@@ -992,12 +983,10 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
 #pragma unroll
                 for (int i = 0; i < 3; ++i)
                     if (NC == 2 || ks <= tile >> 1) y[ks][i] = ex.y[(2 * i + ks) * 64 + lane];
-            in_order();
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) fkt[2 * m + ks] = k_t(in, m, ks);
-            in_order();
             f32x4_t a0 = zero, a1 = zero, a2 = zero;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
