@@ -335,7 +335,7 @@ __device__ __forceinline__ f32x4_t mm16(const f32x4_t& a, const f32x4_t& b, f32x
 // The value head of workgroup i of Hv.  Workgroups go round the eight XCDs, and i, i +
 // 8, .. share an L2: an XCD takes Hv / 8 heads in a row, where the key heads allow it,
 // so that K and Q of a key head are read from memory once for its value heads (16 / 32
-// heads of 128, 2048 tokens: the preparation 18.4 -> 16.7 us, its reads 36 -> 19 MB).
+// heads of 128, 2048 tokens, both kernels 70.2 -> 69.0 us; the preparation's reads 36 -> 19 MB).
 __device__ __forceinline__ int head_of(const DeltaParams& p, int i) {
     return p.Hk & 7 ? i : (i & 7) * (p.Hv >> 3) + (i >> 3);
 }
@@ -388,10 +388,10 @@ __device__ __forceinline__ double wave_running_sum(double x) {
 // fragments and L enters LDS in 16-byte writes.  (1 + L)^-1 by halves: the four
 // diagonal 16 x 16 blocks by substitution, a lane per column; then T10 = -T11
 // (L10 T00) for 16- and for 32-wide blocks, as fp32 matrix products.
-// 16.7 us for 2048 tokens of 16 / 32 heads of 128 (32 MB of units written, 19 MB read, 3.1
+// 17.8 us for 2048 tokens of 16 / 32 heads of 128 (39 MB of units written, 19 MB read, 3.2
 // TB/s): 1024 workgroups, all on the GPU at once, four to a CU, each bound by its own
 // chain (loads, norms, L, the substitution's 120 dependent steps, four products after
-// each other): 64 workgroups alone take 8 us, 2048 take 32.
+// each other): 64 workgroups alone take 8.4 us, 2048 take 34.
 template <int DK, bool F16>
 __global__ __launch_bounds__(256, 4) void delta_chunk_prepare_kernel(DeltaParams p, ChunkPlan c) {
     constexpr int KS = DK / 32, LD = 68, LK = DK + 8;
@@ -645,13 +645,15 @@ __device__ __forceinline__ DeltaParams kernel_params() {
 //   shares and Y = V - diag(e^G) K S0 for token tile w; (3) wave w: tile w of U = T Y;
 //   (4) wave w: its rows of the new state, S <- e^(G_last) S + K^T diag(e^(G_last - G)) U.
 // Waves 4 to 7 have the state and U from LDS and form out, tile w - 4: Q S0
-// during (2) and (3) (the third part of S0 there), P U during (4).  Waves 8 to 11 load what waves 0 to 3 need straight
-// into LDS, two chunks ahead: the chain (1) to (4) is bound by the instructions
-// that one wave can issue, and 53 KB a chunk keep the memory pipe busy.  Rows
-// behind the end come as copies of the last row; T has zeros in their place.
-// 2048 tokens of 16 / 32 heads of 128: 57 us for 32 chunks, a workgroup per CU.  The
-// chain alone, with nothing loaded or stored, takes 51: three exchanges through LDS and
-// a product's latency between each two, 1.6 us a chunk.
+// during (2) and (3) (the third part of S0 there: in (2) it takes 1 % longer), P U during
+// (4).  Waves 8 to 11 load what waves 0 to 3 need straight into LDS, two chunks ahead: the
+// chain (1) to (4) is bound by the instructions that one wave can issue, and 53 KB a
+// chunk keep the memory pipe busy.  Rows behind the end come as copies of the last row;
+// T has zeros in their place.
+// 2048 tokens of 16 / 32 heads of 128, a workgroup per CU, 32 chunks: 53 us in calls after
+// each other, 58 to 61 in a few with idle time before.  The chain alone, with nothing loaded
+// or stored, takes 47 of the 53: three exchanges through LDS and a product's latency
+// between each two, 1.5 us a chunk.
 // NC = 2: two chains of neighbouring columns beside each other, waves 0 to 3 and 4 to 7,
 // with K, Q and T in common.  They hide each other's latency where there are more
 // chains than CUs; the waves of out and of the loads, 8 to 11 and 12 to 15, serve both.
@@ -735,7 +737,7 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
             k += kChunk * p.k.tok, v += kChunk * p.v.tok;
         };
         // Q, which the waves of out take after (1), or have taken before it: half a chunk later, so that the
-        // loads spread over it (2048 tokens 59 -> 57.6 us)
+        // loads spread over it (2048 tokens, both kernels, 72.0 -> 69.0 us)
         const auto stage_q = [&](int n) {
             if (n >= chunks) return;
             const int last = end - 1 - begin - n * kChunk;
@@ -785,7 +787,7 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
             unit += unit_step;
         };
         // fp16: Q is read and split during (4) of the chunk before (2048 tokens of 32 heads of
-        // 128 86.8 -> 83.2 us); bf16, with nothing to split, after (1) (68.3 against 69.4)
+        // 128, both kernels, 92.1 -> 86.9 us); bf16, with nothing to split, after (1) (69.0 against 70.6)
         uint4 q0[KS], q1[KS];
         const auto load_q = [&](int at) {
 #pragma unroll
@@ -1057,13 +1059,15 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
 
 // What one pair of launches takes: entries of the batch and chunks of each, with
 // units of about 96 MB, which the caches hold between the two kernels (8192 tokens:
-// 48 MB 308, 64 to 96 MB 288, 128 MB 311 us; 32768 tokens: 64 MB 1153, 96 MB 1133,
-// 256 MB 1288 us).  Whole entries where they fit, a multiple of what fills the GPU: a
+// 48 and 64 MB 314, 80 to 128 MB 297, 256 MB 327 us; 32768 tokens: 64 MB 1215, 96 MB 1173,
+// 115 MB 1163, 128 MB 1196, 256 MB 1355 us).  Whole entries where they fit, a multiple of what fills the GPU: a
 // launch's start costs a workgroup about two chunks' time.  More chains than CUs go
 // two to a workgroup (both kernels, us, one chain per workgroup against this: 2048
-// tokens of 32 heads of 128, 3 sequences 234 / 186, 8 sequences 635 / 445, fp16 684 / 536;
-// 40 heads 127 / 94, 64 heads 153 / 115; as many chains as CUs, 32 heads, 66 / 89).
+// tokens of 32 heads of 128, 3 sequences 229 / 199, 8 sequences 602 / 483, fp16 714 / 581;
+// 40 heads 127 / 107, 64 heads 149 / 119; as many chains as CUs, 32 heads, 69 / 100).
 constexpr size_t kUnitBytes = kUnitElems * 2;
+// CUs of the whole card, not of the current device: a call's plan has to be the one that
+// its workspace was sized for, wherever that was asked.  A partition with fewer CUs gets larger launches.
 constexpr int64_t kCus = 256;
 struct LaunchPlan {
     int64_t entries, chunks;
@@ -1084,11 +1088,13 @@ LaunchPlan launch_plan(int64_t B, int64_t S, int64_t Hv, int64_t Dv) {
 // Whether the rule runs in chunks.  Token by token a call takes about 0.7 us a
 // token while its waves (16 columns each) find SIMDs of their own, the two chunk
 // kernels 12.7 us for any prompt of up to 64 tokens: 16 / 32 heads of 128, 12 tokens
-// 12.1 against 12.7 us, 16 tokens 15.0 against 12.6.  More waves share the chunk
-// kernels' CUs and fill the SIMDs better: 2 sequences, 16 tokens 15.6 against 16.7, 20
-// tokens 18.2 against 16.8; 4 sequences, 24 tokens 22.1 against 24.5, 28 tokens 24.8
-// against 24.4; 8 sequences, 28 tokens 39.3 against 39.0; 64 sequences, 32 tokens 245
-// against 268, 40 tokens 298 against 278.
+// 11.6 against 12.7 us, 16 tokens 14.5 against 13.3.  More waves share the chunk
+// kernels' CUs and fill the SIMDs better: 2 sequences, 16 tokens 14.9 against 16.1, 20
+// tokens 17.6 against 16.0; 8 sequences, 24 tokens 33.9 against 35.7, 28 tokens 36.8
+// against 36.1; 64 sequences, 28 tokens 223 against 250, 32 tokens 249 against 250, 40
+// tokens 300 against 265.  (Between the lines: 4 sequences, 24 tokens 24.4 against 22.6, 28
+// tokens 27.7 against 22.7.)  64-wide heads, 4 / 8, are faster token by token up to 12 to 16
+// tokens, and up to 28 to 32 for 64 sequences: 9.6 / 12.5 and 11.8 / 12.2; 28.4 / 29.9 and 31.9 / 30.4.
 constexpr int64_t kManyWaves = 1024;  // one per SIMD
 int64_t column_waves(int64_t B, int64_t Hv, int64_t Dv) { return B * Hv * (Dv / 16); }
 bool in_chunks(int64_t B, int64_t S, int64_t Hv, int64_t Dv) {

@@ -361,19 +361,22 @@ int genllm_linear(const void *x, const void *w, const void *bias, void *out, int
  * n_k_heads)) the state S [k_dim][v_dim], fp32, takes token after token:
  *     S <- exp(g) S;  u = beta (v - S^T k);  S <- S + k u^T;  out = scale S^T q
  * with q, k the given rows or, where l2_eps >= 0, x / sqrt(sum x^2 + l2_eps)
- * (l2_eps < 0: as given; with beta |k|^2 above 2 the rule itself diverges).  a_log, dt_bias [n_v_heads] fp32: g = -exp(a_log) softplus(a +
- * dt_bias) and beta = sigmoid(b), a and b elements; both null: a is g and b is
- * beta, fp32.  g is meant to be <= 0 (-inf clears the state); 64 tokens of which
- * one has g > 1 run token by token, as those with what is not finite do.  q, k [batch][seq_len]
- * [n_k_heads][k_dim]; v, out [batch][seq_len][n_v_heads][v_dim]; a, b [batch]
- * [seq_len][n_v_heads]; state [n_states][n_v_heads][k_dim][v_dim], read and
- * replaced.  k_dim and v_dim 64 or 128, rows and the state 16-byte aligned.  out
- * may be v (the same address and strides) and must not overlap the other
- * inputs.  A NaN or infinite input, or a state that outgrows fp32, shows from its token on,
- * as in the rule.  The sums k.k, q.q, k.q, S^T k and S^T q over a row as given are in fp32.  A few
- * tokens (up to 12, or 28 for many sequences) run token by token; longer calls run
- * in chunks and need a workspace of genllm_gated_delta_workspace_bytes (0 where
- * none is needed or the sizes are refused, about 100 MB at most below 3000 value heads), 16-byte
+ * (l2_eps < 0: as given; with beta |k|^2 above 2 the rule itself diverges).
+ * a_log, dt_bias [n_v_heads] fp32: g = -exp(a_log) softplus(a + dt_bias) and
+ * beta = sigmoid(b), a and b elements; both null: a is g and b is beta, fp32.
+ * g is meant to be <= 0 (-inf clears the state); 64 tokens of which one has g > 1
+ * run token by token, as those with what is not finite or too large do.
+ * q, k [batch][seq_len][n_k_heads][k_dim]; v, out [batch][seq_len][n_v_heads]
+ * [v_dim]; a, b [batch][seq_len][n_v_heads]; state [n_states][n_v_heads][k_dim]
+ * [v_dim], read and replaced.  k_dim and v_dim 64 or 128, rows and the state
+ * 16-byte aligned.  out may be v (the same address and strides); a call whose
+ * out, state or workspace lies over any other operand is refused.  A NaN or
+ * infinite input, or a state that outgrows fp32, shows from its token on, as in
+ * the rule.  The sums k.k, q.q, k.q, S^T k and S^T q over a row as given, and all
+ * others, are in fp32; out is rounded once.  A few tokens (up to 12; 16 or 28 for
+ * more heads and sequences) run token by token; longer calls run in chunks and
+ * need a workspace of genllm_gated_delta_workspace_bytes (0 where none is needed
+ * or the sizes are refused, about 100 MB at most up to 2600 value heads), 16-byte
  * aligned, whose contents do not matter before or after the call; calls that
  * share one must be ordered. */
 size_t genllm_gated_delta_workspace_bytes(int32_t batch, int32_t seq_len, int32_t n_k_heads, int32_t n_v_heads,
@@ -391,8 +394,8 @@ int genllm_gated_delta_rule(const void *q, int64_t q_batch_stride, int64_t q_tok
 
 /* Causal depthwise convolution of width 2, 3 or 4 over the tokens, per channel:
  *     y[t] = bias + sum_j weight[j] x[t - (width-1) + j],  out = y or silu(y)
- * (silu != 0), fp32, rounded once.  x, out [batch][seq_len][channels]; out
- * must not overlap x; weight [channels][width]; bias [channels] or null; state
+ * (silu != 0), fp32, rounded once.  x, out [batch][seq_len][channels]; out and
+ * the state must not overlap each other or an input; weight [channels][width]; bias [channels] or null; state
  * [n_states][width-1][channels]: the sequence's inputs before x[0], replaced by
  * its last width-1 inputs; null: zeros, and none are kept. */
 int genllm_causal_conv(const void *x, int64_t x_batch_stride, int64_t x_tok_stride, const void *weight,
