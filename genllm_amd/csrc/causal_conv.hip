@@ -7,9 +7,9 @@
 //
 // in fp32, rounded once.  The new state is the line's last W - 1 rows.  Bound by
 // memory: a thread keeps its window in registers, so that 8 tokens cost 11 loads, three
-// of them from the cache (8192 channels, cold caches: 2048 tokens 17.6 us, 3.8 TB/s;
-// 8192 tokens 53 us, 5.0 TB/s).  A single token is the launch and one load after
-// another, id then state (3.3 us).
+// of them from the cache (8192 channels: 2048 tokens 14.75 us in calls after each other, 4.6
+// TB/s; behind a 1 GiB fill of other memory 22.6 us, 8192 tokens 73).  A single token is the
+// launch and one load after another, id then state (4.4 us).
 #include <algorithm>
 #include <climits>
 #include <string>
@@ -91,8 +91,8 @@ __device__ __forceinline__ void load_weights(const ConvParams& p, int c, float (
 // write the new ones.  x / (1 + exp(-x)) by the hardware's exp2 and reciprocal,
 // each off by about one step of fp32, with both sides of the fraction divided by 2^8: the
 // reciprocal gives 0 for what is above 2^126, and 1 + exp(-x) is from x = -87.3 on, where
-// the result is still 2^-120 (with the library's exp and division 2048 tokens
-// of 8192 channels take 24.4 us instead of 17.6).
+// the result is still 2^-120 (one more product: 2048 tokens of 8192 channels 14.5 -> 14.75
+// us; with the library's exp and division, behind a fill, 29.0 instead of 22.6).
 template <int W, int V, int TT, bool F16>
 __global__ __launch_bounds__(256) void causal_conv_kernel(ConvParams p) {
     static_assert(TT >= W - 1, "only a first tile may see the state");
@@ -240,7 +240,7 @@ extern "C" int genllm_causal_conv(const void* x, int64_t x_batch_stride, int64_t
     p.seq.ids = state_ids, p.seq.lens = seq_lens, p.seq.n_states = n_states, p.seq.S = seq_len;
     p.B = batch, p.C = channels, p.silu = silu != 0;
     if (const std::string why = overlap_of(p, width); !why.empty()) return fail(GENLLM_ERR_INVALID, "causal_conv: " + why);
-    // 16 bytes per access, or one element where rows do not allow it (2048 tokens of 8192 channels 17.6 against 27.7 us)
+    // 16 bytes per access, or one element where rows do not allow it (2048 tokens of 8192 channels, behind a 1 GiB fill, 22.6 against 34.3 us)
     const bool wide = channels % 8 == 0 && ((x_batch_stride | x_tok_stride | o_batch_stride | o_tok_stride) & 7) == 0 &&
                       aligned_to(x, 16) && aligned_to(out, 16) && aligned_to(state, 16) && aligned_to(weight, 16) &&
                       aligned_to(bias, 16);

@@ -267,10 +267,10 @@ __device__ __forceinline__ constexpr int tile_row(int t, int rho) {
     return 32 * (t >> 1) + 8 * (rho >> 2) + 4 * (t & 1) + (rho & 3);
 }
 
-// Below these sizes no step of a chunk leaves fp32: 8 lanes hold a row of T, so that |U| < 8
-// kMaxT kMaxY = 2^93 and |e^(G_last - G) U| < 2^123 with the keys' factors in it.  A chunk with
-// more runs token by token: an infinite u of one token, times the zeros of P, would make
-// the outputs of earlier ones NaN.
+// Below these sizes U stays in fp32: 8 lanes hold a row of T, so that |U| < 8 kMaxT kMaxY =
+// 2^93, and |e^(G_last - G) U| < 2^123 with the keys' factors in it.  A chunk with more runs
+// token by token: an infinite u of one token, times the zeros of P, would make the outputs
+// of earlier ones NaN.
 constexpr float kMaxT = 0x1p20f;  // the sum of |T| over 8 columns
 constexpr float kMaxY = 0x1p70f;  // the sum of |Y| over 4 rows
 constexpr float kMaxD = 0x1p30f;  // e^(G_last - G) with the key's factor
@@ -1060,14 +1060,14 @@ __global__ __launch_bounds__(kScanThreads<NC>) void delta_chunk_scan_kernel(Delt
 // What one pair of launches takes: entries of the batch and chunks of each, with
 // units of about 96 MB, which the caches hold between the two kernels (8192 tokens:
 // 48 and 64 MB 314, 80 to 128 MB 297, 256 MB 327 us; 32768 tokens: 64 MB 1215, 96 MB 1173,
-// 115 MB 1163, 128 MB 1196, 256 MB 1355 us).  Whole entries where they fit, a multiple of what fills the GPU: a
-// launch's start costs a workgroup about two chunks' time.  More chains than CUs go
-// two to a workgroup (both kernels, us, one chain per workgroup against this: 2048
+// 115 MB 1163, 128 MB 1196, 256 MB 1355 us).  Whole entries where they fit, a multiple of
+// what fills the GPU: a launch's start costs a workgroup about two chunks' time.  More
+// chains than CUs go two to a workgroup (both kernels, us, one chain per workgroup against this: 2048
 // tokens of 32 heads of 128, 3 sequences 229 / 199, 8 sequences 602 / 483, fp16 714 / 581;
 // 40 heads 127 / 107, 64 heads 149 / 119; as many chains as CUs, 32 heads, 69 / 100).
 constexpr size_t kUnitBytes = kUnitElems * 2;
 // CUs of the whole card, not of the current device: a call's plan has to be the one that
-// its workspace was sized for, wherever that was asked.  A partition with fewer CUs gets larger launches.
+// its workspace was sized for, wherever that was asked.
 constexpr int64_t kCus = 256;
 struct LaunchPlan {
     int64_t entries, chunks;
