@@ -113,6 +113,12 @@ SIGNATURES = {
     "genllm_causal_conv": (_int, [_P, _i64, _i64, _P, _P, _P, _i64, _i64, _P, _i32, _P, _P] + [_i32] * 6 + [_P]),
     "genllm_qk_norm_rope_axes": (_int, [_P, _i64, _i64, _P, _i64, _i64, _P, _i32] * 2
                                  + [_f, _P, _P, _i32, _i32, _P, _i64, _i32, _P, _i32, _i32, _i32, _i32, _P]),
+    "genllm_kv_scatter_f8": (_int, [_P, _i64, _i64, _i64] * 4 + [_P, _P, _i32] + [_P, _i64] * 2 + [_i32, _P, _P] + [_i32] * 5 + [_P]),
+    "genllm_kv_gather_f8": (_int, [_P, _i64, _i64, _i64] * 2 + [_P, _P, _i32] + [_P, _i64] * 2 + [_i32, _P, _P]
+                            + [_P, _i64, _i64, _i64] * 2 + [_i32] * 5 + [_P]),
+    "genllm_paged_attention_batch_workspace_bytes": (_sz, [_i32] * 6),
+    "genllm_paged_attention_batch": (_int, [_P, _i64, _i64, _i64] * 4 + [_P, _P, _i32] + [_P, _i64] * 2 + [_i32, _P, _P] + [_i32] * 6
+                                     + [_f, _i32, _i32, _i32, _P, _sz, _P]),
     "genllm_fill_normal_bf16": (_int, [_P, _sz, _u64, _u64, _P]),
     "genllm_fill_normal_f16": (_int, [_P, _sz, _u64, _u64, _P]),
     "genllm_selftest_mfma": (_int, [_i32, _P, _P, _P, _P]),
@@ -149,9 +155,11 @@ def calls():
         except ImportError as e:
             raise RuntimeError(f"{HERE}/_calls.so does not load ({e}): run __graft_entry__.build() "
                                "(make -C genllm_amd/csrc calls)") from e
-        module.bind(*(C.cast(getattr(L, name), _P).value
-                      for name in ("genllm_gated_delta_workspace_bytes", "genllm_gated_delta_rule", "genllm_causal_conv",
-                                   "genllm_qk_norm_rope_axes")))
+        for bind, names in ((module.bind, ("genllm_gated_delta_workspace_bytes", "genllm_gated_delta_rule", "genllm_causal_conv",
+                                           "genllm_qk_norm_rope_axes")),
+                            (module.bind_batch, ("genllm_kv_scatter_f8", "genllm_kv_gather_f8",
+                                                 "genllm_paged_attention_batch_workspace_bytes", "genllm_paged_attention_batch"))):
+            bind(*(C.cast(getattr(L, name), _P).value for name in names))
         _calls = module
     return _calls
 

@@ -1,8 +1,8 @@
-// calls.cpp -- the Python calls of the hybrid layers' operators: argument checks on
-// torch tensors, the device and its current stream, and the call into the C ABI of
-// include/genllm_paged.h.  These calls have up to 45 arguments: read and checked in
-// Python and passed through ctypes, a single token's calls took 7.5 to 10 us of host
-// time; from here they take 4.0 to 4.3, most of it the launch.  The entry points'
+// calls.cpp -- the Python calls of the hybrid layers' and the batch operators: argument
+// checks on torch tensors, the device and its current stream, and the call into the C ABI
+// of include/genllm_paged.h.  These calls have up to 45 arguments: read and checked in
+// Python and passed through ctypes, a single token's calls of the hybrid layers took 7.5
+// to 10 us of host time; from here they take 4.0 to 4.3, most of it the launch.  The entry points'
 // addresses come from the ctypes binding, so that a process has one copy of the
 // library.  Every function returns the status code; the interpreter's lock is released
 // while the C call runs, as ctypes does.
@@ -25,6 +25,10 @@ decltype(&genllm_gated_delta_workspace_bytes) g_delta_workspace = nullptr;
 decltype(&genllm_gated_delta_rule) g_delta = nullptr;
 decltype(&genllm_causal_conv) g_conv = nullptr;
 decltype(&genllm_qk_norm_rope_axes) g_axes = nullptr;
+decltype(&genllm_kv_scatter_f8) g_scatter = nullptr;
+decltype(&genllm_kv_gather_f8) g_gather = nullptr;
+decltype(&genllm_paged_attention_batch_workspace_bytes) g_batch_workspace = nullptr;
+decltype(&genllm_paged_attention_batch) g_batch = nullptr;
 
 struct Refused {
     std::string why;
@@ -238,6 +242,116 @@ int qk_norm_rope_axes(PyObject* const* arg) {
                   int32_t(axes), sections, inter, c.size(S), c.size(D), c.code(), stream);
 }
 
+// A pool [blocks, 16, heads, D] of `type`'s elements or of 8-bit codes, the last dim dense.
+const at::Tensor& pool_of(const Checks& c, PyObject* o, const char* name, int64_t heads, int64_t d, bool f8, int64_t blocks) {
+    const at::Tensor& t = c.tensor(o, name);
+    const at::ScalarType type = f8 ? (t.scalar_type() == at::kByte ? at::kByte : at::kFloat8_e4m3fn) : c.dtype;
+    const int64_t n = blocks >= 0 ? blocks : t.dim() ? t.size(0) : 0, sizes[4] = {n, GENLLM_PAGE_BLOCK_SIZE, heads, d};
+    return c.rows(t, name, sizes, type);
+}
+// E8M0 bytes [blocks, heads]
+uint8_t* scales_of(const Checks& c, PyObject* o, const char* name, int64_t blocks, int64_t heads) {
+    const at::Tensor& t = c.tensor(o, name);
+    const int64_t sizes[2] = {blocks, heads};
+    return data<uint8_t>(c.whole(t, name, sizes, t.scalar_type() == at::kByte ? at::kByte : at::kFloat8_e8m0fnu));
+}
+const at::Tensor& table_of(const Checks& c, PyObject* o, const char* name, int64_t batch, int64_t pages) {
+    const at::Tensor& t = c.tensor(o, name);
+    const int64_t sizes[2] = {batch, pages >= 0 ? pages : t.dim() == 2 ? t.size(1) : 0};
+    return c.rows(t, name, sizes, at::kInt);
+}
+const int32_t* counts_of(const Checks& c, PyObject* o, const char* name, int64_t batch) {
+    const int64_t sizes[1] = {batch};
+    return data<int32_t>(c.whole(c.tensor(o, name), name, sizes, at::kInt));
+}
+
+// Rows (k, v or k_out, v_out), k_pool, v_pool, k_scales, v_scales, k_ids, v_ids, start_pos, seq_lens, stream
+template <bool kScatter>
+int pages_f8(PyObject* const* arg) {
+    Checks c{kScatter ? "kv_scatter_f8" : "kv_gather_f8"};
+    const at::Tensor& k = c.elements(arg[0], kScatter ? "k" : "k_out", 4);
+    const at::Tensor& v = c.rows(c.tensor(arg[1], kScatter ? "v" : "v_out"), kScatter ? "v" : "v_out", k.sizes(), c.dtype);
+    const int64_t B = k.size(0), S = k.size(1), H = k.size(2), D = k.size(3), es[1] = {B};
+    const at::Tensor& kp = pool_of(c, arg[2], "k_pool", H, D, true, -1);
+    const int64_t blocks = kp.size(0);
+    const at::Tensor& vp = pool_of(c, arg[3], "v_pool", H, D, true, blocks);
+    uint8_t* const ks = scales_of(c, arg[4], "k_scales", blocks, H);
+    uint8_t* const vs = scales_of(c, arg[5], "v_scales", blocks, H);
+    const at::Tensor& ki = table_of(c, arg[6], "k_ids", B, -1);
+    const at::Tensor& vi = table_of(c, arg[7], "v_ids", B, ki.size(1));
+    const int32_t* start = counts_of(c, arg[8], "start_pos", B);
+    const int32_t* lens = c.optional<int32_t>(arg[9], "seq_lens", es, at::kInt);
+    const c10::DeviceGuard guard(c.device);
+    void* const stream = stream_of(arg[10], c.device);
+    const Unlocked unlocked;
+    if constexpr (kScatter)
+        return g_scatter(data(k), k.stride(0), k.stride(1), k.stride(2), data(v), v.stride(0), v.stride(1), v.stride(2), data(kp),
+                         kp.stride(0), kp.stride(1), kp.stride(2), data(vp), vp.stride(0), vp.stride(1), vp.stride(2), ks, vs,
+                         c.size(blocks), data<int32_t>(ki), ki.stride(0), data<int32_t>(vi), vi.stride(0), c.size(ki.size(1)), start,
+                         lens, c.size(B), c.size(S), c.size(H), c.size(D), c.code(), stream);
+    else
+        return g_gather(data(kp), kp.stride(0), kp.stride(1), kp.stride(2), data(vp), vp.stride(0), vp.stride(1), vp.stride(2), ks, vs,
+                        c.size(blocks), data<int32_t>(ki), ki.stride(0), data<int32_t>(vi), vi.stride(0), c.size(ki.size(1)), start, lens,
+                        data(k), k.stride(0), k.stride(1), k.stride(2), data(v), v.stride(0), v.stride(1), v.stride(2), c.size(B),
+                        c.size(S), c.size(H), c.size(D), c.code(), stream);
+}
+
+// q, out, k_pool, v_pool, k_ids, v_ids, n_cached, scale, q_lens, k_scales, v_scales, causal, window, sinks, workspace, stream
+int paged_attention_batch(PyObject* const* arg) {
+    Checks c{"paged_attention_batch"};
+    const at::Tensor& q = c.elements(arg[0], "q", 4);
+    const at::Tensor& out = c.rows(c.tensor(arg[1], "out"), "out", q.sizes(), c.dtype);
+    const int64_t B = q.size(0), S = q.size(1), Hq = q.size(2), D = q.size(3), es[1] = {B};
+    const bool f8 = arg[9] != Py_None;
+    if (f8 != (arg[10] != Py_None)) c.refuse("k_scales and v_scales go together");
+    const at::Tensor& first = c.tensor(arg[2], "k_pool");
+    if (first.dim() != 4) c.refuse("k_pool must have 4 dims");
+    const int64_t blocks = first.size(0), Hk = first.size(2);
+    const at::Tensor& kp = pool_of(c, arg[2], "k_pool", Hk, D, f8, blocks);
+    const at::Tensor& vp = pool_of(c, arg[3], "v_pool", Hk, D, f8, blocks);
+    uint8_t *ks = nullptr, *vs = nullptr;
+    if (f8) {
+        ks = scales_of(c, arg[9], "k_scales", blocks, Hk);
+        vs = scales_of(c, arg[10], "v_scales", blocks, Hk);
+    }
+    const at::Tensor& ki = table_of(c, arg[4], "k_ids", B, -1);
+    const at::Tensor& vi = table_of(c, arg[5], "v_ids", B, ki.size(1));
+    const int32_t* n = counts_of(c, arg[6], "n_cached", B);
+    const int32_t* lens = c.optional<int32_t>(arg[8], "q_lens", es, at::kInt);
+    const float scale = float(number(arg[7]));
+    const int causal = PyObject_IsTrue(arg[11]);
+    if (causal < 0) throw python_error();
+    const auto count = [&](PyObject* o, const char* name) -> int32_t {
+        const long x = PyLong_AsLong(o);
+        if (x == -1 && PyErr_Occurred()) throw python_error();
+        if (x < 0) c.refuse(std::string(name) + " must not be negative");
+        return x > INT32_MAX ? INT32_MAX : int32_t(x);
+    };
+    int32_t window = 0;
+    if (arg[12] != Py_None && (window = count(arg[12], "window")) == 0) c.refuse("window must be at least 1, or None");
+    const int32_t sinks = count(arg[13], "sinks");
+    const int32_t z[6] = {c.size(B), c.size(S), c.size(Hq), c.size(Hk), c.size(D), c.size(ki.size(1))};
+    const c10::DeviceGuard guard(c.device);
+    at::Tensor own;
+    void* ws = nullptr;
+    size_t ws_bytes = 0;
+    if (arg[14] != Py_None) {
+        const at::Tensor& w = c.tensor(arg[14], "workspace");
+        if (w.device() != c.device || !w.is_contiguous()) c.refuse("the workspace must be contiguous on the tensors' device");
+        ws = data(w), ws_bytes = w.nbytes();
+    } else if (const size_t need = g_batch_workspace(z[0], z[1], z[2], z[3], z[4], z[5])) {
+        // from the current stream's pool, as above
+        own = at::empty({int64_t(need)}, at::TensorOptions().dtype(at::kByte).device(c.device));
+        ws = data(own), ws_bytes = need;
+    }
+    void* const stream = stream_of(arg[15], c.device);
+    const Unlocked unlocked;
+    return g_batch(data(q), q.stride(0), q.stride(1), q.stride(2), data(out), out.stride(0), out.stride(1), out.stride(2), data(kp),
+                   kp.stride(0), kp.stride(1), kp.stride(2), data(vp), vp.stride(0), vp.stride(1), vp.stride(2), ks, vs, c.size(blocks),
+                   data<int32_t>(ki), ki.stride(0), data<int32_t>(vi), vi.stride(0), z[5], n, lens, z[0], z[1], z[2], z[3], z[4],
+                   c.code(), scale, causal, window, sinks, ws, ws_bytes, stream);
+}
+
 template <int (*F)(PyObject* const*), Py_ssize_t N>
 PyObject* entry(PyObject*, PyObject* const* arg, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -245,8 +359,8 @@ PyObject* entry(PyObject*, PyObject* const* arg, Py_ssize_t n) {
         PyErr_Format(PyExc_TypeError, "%zd arguments expected, got %zd", N, n);
         return nullptr;
     }
-    if (!g_delta) {
-        PyErr_SetString(PyExc_RuntimeError, "bind() comes first");
+    if (!g_delta || !g_batch) {
+        PyErr_SetString(PyExc_RuntimeError, "bind() and bind_batch() come first");
         return nullptr;
     }
     try {
@@ -258,18 +372,23 @@ PyObject* entry(PyObject*, PyObject* const* arg, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// the addresses of the four C functions
-PyObject* bind(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+bool addresses(PyObject* const* arg, Py_ssize_t n, void* (&p)[4]) {
     if (n != 4) {
         PyErr_SetString(PyExc_TypeError, "bind() takes four addresses");
-        return nullptr;
+        return false;
     }
-    void* p[4];
     for (int i = 0; i < 4; ++i)
         if (!(p[i] = PyLong_AsVoidPtr(arg[i]))) {
             if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind(): a null address");
-            return nullptr;
+            return false;
         }
+    return true;
+}
+
+// the addresses of the hybrid layers' C functions
+PyObject* bind(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+    void* p[4];
+    if (!addresses(arg, n, p)) return nullptr;
     g_delta_workspace = reinterpret_cast<decltype(g_delta_workspace)>(p[0]);
     g_delta = reinterpret_cast<decltype(g_delta)>(p[1]);
     g_conv = reinterpret_cast<decltype(g_conv)>(p[2]);
@@ -277,16 +396,31 @@ PyObject* bind(PyObject*, PyObject* const* arg, Py_ssize_t n) {
     Py_RETURN_NONE;
 }
 
+// and of the batch operators'
+PyObject* bind_batch(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+    void* p[4];
+    if (!addresses(arg, n, p)) return nullptr;
+    g_scatter = reinterpret_cast<decltype(g_scatter)>(p[0]);
+    g_gather = reinterpret_cast<decltype(g_gather)>(p[1]);
+    g_batch_workspace = reinterpret_cast<decltype(g_batch_workspace)>(p[2]);
+    g_batch = reinterpret_cast<decltype(g_batch)>(p[3]);
+    Py_RETURN_NONE;
+}
+
 PyCFunction fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) { return reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f)); }
 
 PyMethodDef methods[] = {
-    {"bind", fast(bind), METH_FASTCALL, "The addresses of the C functions"},
+    {"bind", fast(bind), METH_FASTCALL, "The addresses of the hybrid layers' C functions"},
+    {"bind_batch", fast(bind_batch), METH_FASTCALL, "The addresses of the batch operators' C functions"},
     {"gated_delta_rule", fast(entry<gated_delta_rule, 15>), METH_FASTCALL, "genllm_gated_delta_rule on tensors"},
     {"causal_conv", fast(entry<causal_conv, 9>), METH_FASTCALL, "genllm_causal_conv on tensors"},
     {"qk_norm_rope_axes", fast(entry<qk_norm_rope_axes, 13>), METH_FASTCALL, "genllm_qk_norm_rope_axes on tensors"},
+    {"kv_scatter_f8", fast(entry<pages_f8<true>, 11>), METH_FASTCALL, "genllm_kv_scatter_f8 on tensors"},
+    {"kv_gather_f8", fast(entry<pages_f8<false>, 11>), METH_FASTCALL, "genllm_kv_gather_f8 on tensors"},
+    {"paged_attention_batch", fast(entry<paged_attention_batch, 16>), METH_FASTCALL, "genllm_paged_attention_batch on tensors"},
     {nullptr, nullptr, 0, nullptr}};
 
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", "Calls of the hybrid layers' operators", -1, methods,
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", "Calls of the hybrid layers' and the batch operators", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,0 +1,315 @@
+// paged_batch.hpp -- what the kernels of paged_attention_batch share: the launch's
+// parameters, how a padded batch of unlike lengths is divided among workgroups, the
+// pages that a row tile visits, and the form that takes one key after another.
+#pragma once
+
+#include <climits>
+
+#include "common.hpp"
+
+namespace genllm {
+
+struct BatchAttn {
+    const int32_t* n_cached = nullptr;  // [B]
+    const int32_t* q_lens = nullptr;    // [B], or null: S each
+    const uint16_t* q = nullptr;
+    int64_t q_batch = 0, q_tok = 0, q_head = 0;  // elements
+    const char* k_pool = nullptr;
+    const char* v_pool = nullptr;
+    int64_t k_block = 0, v_block = 0;                    // bytes
+    int32_t k_tok = 0, k_head = 0, v_tok = 0, v_head = 0;  // bytes within a block
+    const uint8_t* k_scales = nullptr;  // [blocks][Hkv], 2^(byte - 127); null with 16-bit pools
+    const uint8_t* v_scales = nullptr;
+    const int32_t* k_ids = nullptr;
+    const int32_t* v_ids = nullptr;
+    int64_t k_ids_row = 0, v_ids_row = 0;
+    uint16_t* out = nullptr;
+    int64_t o_batch = 0, o_tok = 0, o_head = 0;
+    int32_t B = 0, S = 0, Hq = 0, Hkv = 0, G = 0;
+    int32_t blocks = 0;    // ids outside [0, blocks) are no pages: NaN for the rows that see them
+    int32_t capacity = 0;  // tokens that a row of the tables holds
+    int32_t window = 0;    // keys a query sees up to itself; kNoWindow: all
+    int32_t sinks = 0;     // first tokens that stay visible behind a window
+    int32_t causal = 1;
+    float c = 0.0f;        // scale * log2(e), at least FLT_MIN
+    // division of the work
+    int32_t target = 1;    // workgroups to fill the GPU with
+    int32_t least = 1;     // steps that a split takes at least
+    int32_t can_split = 0; // else every row tile has one workgroup
+    float* partial = nullptr;  // o [workgroup][tile row][D], then {m, l} [workgroup][tile row]
+    int32_t slots = 0;         // workgroups that the partials have room for
+};
+
+constexpr int32_t kNoWindow = 1 << 30;
+
+// Keys in pages: the first `sink_pages` of a sequence, then from sink_pages + skip on.
+struct Span {
+    int sink_pages, skip, pages;
+    __device__ __forceinline__ int page(int j) const { return j + (j >= sink_pages ? skip : 0); }
+};
+
+// The pages that hold a key for some query of positions first_pos.. (negative: before
+// the sequence) with keys before `end`.
+__device__ __forceinline__ Span span_of(const BatchAttn& p, int first_pos, int end) {
+    const int total = (end + kPage - 1) / kPage;
+    const int w0 = max(0, first_pos - p.window + 1) / kPage;
+    const int sinks = (min(p.sinks, end) + kPage - 1) / kPage;
+    if (w0 <= sinks) return {total, 0, total};
+    return {sinks, w0 - sinks, total - (w0 - sinks)};
+}
+
+struct Entry {
+    int n, ql;  // keys cached, queries
+};
+__device__ __forceinline__ Entry entry_of(const BatchAttn& p, int b) {
+    const int n = p.n_cached[b], ql = p.q_lens ? p.q_lens[b] : p.S;
+    return {min(max(n, 0), p.capacity), min(max(ql, 0), p.S)};
+}
+
+// Row tiles and steps (of STEP pages) of an entry, for one kv head.
+template <int ROWS, int STEP>
+__device__ __forceinline__ void cost_of(const BatchAttn& p, const Entry& e, int& tiles, int& steps) {
+    tiles = (e.ql * p.G + ROWS - 1) / ROWS;
+    steps = tiles ? (span_of(p, p.causal ? e.n - e.ql : e.n - 1, e.n).pages + STEP - 1) / STEP : 0;
+}
+
+__device__ __forceinline__ int splits_of(const BatchAttn& p, int tiles, int steps, int quantum) {
+    return tiles == 0 ? 0 : p.can_split ? max(1, (steps + quantum - 1) / quantum) : 1;
+}
+
+// Steps per split: all of the batch's steps over p.target workgroups.  Every wave of the
+// split kernel and of the merge must come to the same number: the sums are whole numbers
+// below 2^53, exact in whatever order.
+template <int ROWS, int STEP>
+__device__ __forceinline__ int quantum_of(const BatchAttn& p) {
+    if (!p.can_split) return INT32_MAX;
+    const int lane = threadIdx.x & 63;
+    double sum = 0.0;
+    for (int b = lane; b < p.B; b += 64) {
+        int tiles, steps;
+        cost_of<ROWS, STEP>(p, entry_of(p, b), tiles, steps);
+        sum += double(int64_t(tiles) * steps);
+    }
+    for (int i = 1; i < 64 && i < p.B; i *= 2) sum += __shfl_xor(sum, i);
+    const int64_t all = int64_t(sum) * p.Hkv, q = (all + p.target - 1) / p.target;
+    return max(p.least, __builtin_amdgcn_readfirstlane(int(min(q, int64_t(INT32_MAX)))));
+}
+
+struct Work {
+    int b, tile, sp, h, ns;
+    int base;  // the entry's first workgroup
+    Entry e;
+};
+
+// What workgroup w does; false: nothing.  Entries lie one after the other, an entry's
+// workgroups as [tile][split][kv head]: with 8 kv heads those of one head run on one XCD.
+template <int ROWS, int STEP>
+__device__ __forceinline__ bool find_work(const BatchAttn& p, int w, Work& r) {
+    const int lane = threadIdx.x & 63;
+    const int quantum = quantum_of<ROWS, STEP>(p);
+    int base = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        int mine = 0, tiles = 0, steps = 0, ns = 0;
+        Entry e{0, 0};
+        if (b0 + lane < p.B) {
+            e = entry_of(p, b0 + lane);
+            cost_of<ROWS, STEP>(p, e, tiles, steps);
+            ns = splits_of(p, tiles, steps, quantum);
+            mine = tiles * ns * p.Hkv;
+        }
+        int upto = mine;
+        for (int i = 1; i < 64 && i < p.B; i *= 2) {
+            const int x = __shfl_up(upto, i);
+            if (lane >= i) upto += x;
+        }
+        const unsigned long long hit = __ballot(w >= base + upto - mine && w < base + upto);
+        if (hit) {
+            const int src = __builtin_ctzll(hit);
+            r.b = b0 + src;
+            r.base = base + __builtin_amdgcn_readlane(upto - mine, src);
+            r.ns = __builtin_amdgcn_readlane(ns, src);
+            r.e = {__builtin_amdgcn_readlane(e.n, src), __builtin_amdgcn_readlane(e.ql, src)};
+            const int all = __builtin_amdgcn_readlane(tiles, src);
+            const unsigned local = unsigned(w - r.base), rest = local / unsigned(p.Hkv);
+            r.h = __builtin_amdgcn_readfirstlane(int(local % unsigned(p.Hkv)));
+            r.sp = __builtin_amdgcn_readfirstlane(int(rest % unsigned(r.ns)));
+            // the last tiles have the most keys: first
+            r.tile = __builtin_amdgcn_readfirstlane(all - 1 - int(rest / unsigned(r.ns)));
+            return true;
+        }
+        base += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}
+
+// Where entry b's workgroups begin, and its splits.
+template <int ROWS, int STEP>
+__device__ __forceinline__ void find_entry(const BatchAttn& p, int b, int& base, int& ns, int& tiles, Entry& e) {
+    const int lane = threadIdx.x & 63;
+    const int quantum = quantum_of<ROWS, STEP>(p);
+    int before = 0;
+    for (int i = lane; i < b; i += 64) {
+        int t, s;
+        cost_of<ROWS, STEP>(p, entry_of(p, i), t, s);
+        before += t * splits_of(p, t, s, quantum) * p.Hkv;
+    }
+    for (int i = 1; i < 64 && i < b; i *= 2) before += __shfl_xor(before, i);
+    base = __builtin_amdgcn_readfirstlane(before);
+    e = entry_of(p, b);
+    int steps;
+    cost_of<ROWS, STEP>(p, e, tiles, steps);
+    ns = splits_of(p, tiles, steps, quantum);
+}
+
+// What a row sees: keys up to `pos`, of those from `from` on and those before p.sinks.
+struct Sight {
+    int pos, from;
+    bool any;  // the row has a key at all
+    __device__ __forceinline__ bool operator()(const BatchAttn& p, int t) const { return t <= pos && (t >= from || t < p.sinks); }
+};
+__device__ __forceinline__ Sight sight_of(const BatchAttn& p, const Entry& e, int query) {
+    const int pos = p.causal ? min(e.n - e.ql + query, e.n - 1) : e.n - 1;
+    return {pos, pos - p.window + 1, pos >= 0};
+}
+
+// 2^(byte - 127), NaN for 255
+__device__ __forceinline__ float scale_value(int byte) {
+    return byte == 255 ? __builtin_nanf("") : __uint_as_float(byte ? uint32_t(byte) << 23 : 0x00400000u);
+}
+// 2^e for e from -126 to 127, 2^-126 below
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(uint32_t(max(e, -126) + 127) << 23); }
+
+// A page as the lane that looked it up holds it.
+struct PageInfo {
+    int kid = -1, vid = -1;  // block ids, -1: no page
+    float kf = 0.0f;         // scores' factor in log2 units; NaN where an id or a scale is none
+    int ve = 0;              // exponent of V's scale
+};
+template <bool Q8>
+__device__ __forceinline__ PageInfo page_info(const BatchAttn& p, int b, int h, int page, bool there) {
+    PageInfo r;
+    r.kf = p.c;
+    if (there) {
+        r.kid = p.k_ids[b * p.k_ids_row + page];
+        r.vid = p.v_ids[b * p.v_ids_row + page];
+        const bool bad = unsigned(r.kid) >= unsigned(p.blocks) || unsigned(r.vid) >= unsigned(p.blocks);
+        if (bad) {
+            r.kid = r.vid = -1;
+            r.kf = __builtin_nanf("");
+        } else if constexpr (Q8) {
+            const int kb = p.k_scales[int64_t(r.kid) * p.Hkv + h], vb = p.v_scales[int64_t(r.vid) * p.Hkv + h];
+            const float f = scale_value(kb) * p.c;
+            r.kf = vb == 255 || f != f ? __builtin_nanf("") : fmaxf(f, __FLT_MIN__);
+            r.ve = vb - 127;
+        }
+    }
+    return r;
+}
+
+// Two e4m3 codes (the low or the high half of w) as a packed pair of elements
+template <bool F16, bool kHigh>
+__device__ __forceinline__ uint32_t f8_pair(uint32_t w, float scale) {
+    if constexpr (F16)
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, kHigh));
+    else
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, kHigh));
+}
+// eight codes as an MFMA operand
+template <bool F16>
+__device__ __forceinline__ uint4 f8_octet(uint32_t w0, uint32_t w1, float s0, float s1) {
+    return make_uint4(f8_pair<F16, false>(w0, s0), f8_pair<F16, true>(w0, s0), f8_pair<F16, false>(w1, s1), f8_pair<F16, true>(w1, s1));
+}
+
+// One key after another, in fp32, each row with only the keys it sees: what a wave runs
+// again whose tiles came out NaN or infinite.  (In the tiles a key that a row does not
+// see meets a probability of zero, and 0 x NaN is NaN.)  The lane's row is lane % 16;
+// acc: dims 16 db + 4 g + i, in V's own units; m in log2 units.  next(i): the i-th page
+// of the wave, or -1 at the end.
+template <int D, bool F16, bool Q8, typename Next>
+__device__ __forceinline__ void exact_keys(const BatchAttn& p, int b, int h, const uint16_t* qrow, const Sight& see, const Next& next,
+                                           f32x4_t (&acc)[D / 16], float& m, float& l) {
+    using E = Elem<F16>;
+    const int g = (threadIdx.x & 63) >> 4;
+    m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) acc[db] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0;; ++i) {
+        const int page = next(i);
+        if (page < 0) break;
+        const PageInfo info = page_info<Q8>(p, b, h, page, true);
+        const bool there = info.kid >= 0;
+        const char* const kb = p.k_pool + (there ? info.kid : 0) * p.k_block + int64_t(h) * p.k_head;
+        const char* const vb = p.v_pool + (there ? info.vid : 0) * p.v_block + int64_t(h) * p.v_head;
+        const float vs = Q8 ? scale_value(info.ve + 127) : 1.0f;
+        for (int j = 0; j < kPage; ++j) {
+            const int t = page * kPage + j;
+            const bool vis = see(p, t);
+            if (!__any(vis)) continue;
+            float x = 0.0f;
+#pragma unroll 1
+            for (int d = 8 * g; d < D; d += 32) {
+                const uint4 qq = *reinterpret_cast<const uint4*>(qrow + d);
+                const uint32_t qw[4] = {qq.x, qq.y, qq.z, qq.w};
+                uint32_t kw[4] = {0, 0, 0, 0};
+                if (there) {
+                    if constexpr (Q8) {
+                        const uint2 u = *reinterpret_cast<const uint2*>(kb + int64_t(j) * p.k_tok + d);
+                        const uint4 o = f8_octet<F16>(u.x, u.y, 1.0f, 1.0f);
+                        kw[0] = o.x, kw[1] = o.y, kw[2] = o.z, kw[3] = o.w;
+                    } else {
+                        const uint4 o = *reinterpret_cast<const uint4*>(kb + int64_t(j) * p.k_tok + 2 * d);
+                        kw[0] = o.x, kw[1] = o.y, kw[2] = o.z, kw[3] = o.w;
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    x = __builtin_fmaf(E::lo(qw[w]), E::lo(kw[w]), x);
+                    x = __builtin_fmaf(E::hi(qw[w]), E::hi(kw[w]), x);
+                }
+            }
+            x += __shfl_xor(x, 16);
+            x += __shfl_xor(x, 32);
+            x *= info.kf;
+            const float mn = vis ? __builtin_elementwise_maximum(m, x) : m;
+            const float alpha = m == -INFINITY ? 0.0f : mn == m ? 1.0f : exp2_fast(m - mn);
+            const float e = mn == -INFINITY ? 0.0f : exp2_fast(x - mn);
+            if (vis) l = __builtin_fmaf(l, alpha, e);
+#pragma unroll
+            for (int db = 0; db < D / 16; ++db) {
+                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (there) {
+                    if constexpr (Q8) {
+                        const uint32_t u = *reinterpret_cast<const uint32_t*>(vb + int64_t(j) * p.v_tok + 16 * db + 4 * g);
+                        // as read back, in fp16 (a code's value fits whole), then its scale
+                        const uint32_t lo = f8_pair<true, false>(u, 1.0f), hi = f8_pair<true, true>(u, 1.0f);
+                        v[0] = Elem<true>::lo(lo) * vs, v[1] = Elem<true>::hi(lo) * vs, v[2] = Elem<true>::lo(hi) * vs, v[3] = Elem<true>::hi(hi) * vs;
+                    } else {
+                        const uint2 u = *reinterpret_cast<const uint2*>(vb + int64_t(j) * p.v_tok + 2 * (16 * db + 4 * g));
+                        v[0] = E::lo(u.x), v[1] = E::hi(u.x), v[2] = E::lo(u.y), v[3] = E::hi(u.y);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[db][k] = vis ? __builtin_fmaf(e, v[k], acc[db][k] * alpha) : acc[db][k];
+            }
+            m = mn;
+        }
+    }
+}
+
+constexpr int kPrefillStep = 4;  // pages of a prefill step
+
+int launch_batch_decode(const BatchAttn& p, int head_dim, bool f16, hipStream_t stream);
+int launch_batch_prefill(const BatchAttn& p, int tile_rows, int head_dim, bool f16, hipStream_t stream);
+
+// Which kernel a call runs and how its work is divided at most.
+struct BatchPlan {
+    bool decode;
+    int rows;       // of a tile
+    int step;       // pages of a step
+    int64_t tiles;  // row tiles at most
+    int64_t slots;  // workgroups at most; as many partials where can_split
+    int target, least;
+    bool can_split;
+};
+
+}  // namespace genllm

@@ -489,6 +489,73 @@ def qk_norm_rope_axes(q, k, q_out, k_out, gamma_q, gamma_k, eps: float, cos, sin
         check(rc)
 
 
+# ------------------------------------------------ batches over a paged cache
+# Their arguments are checked and passed on in csrc/calls.cpp, too.
+
+
+def f8_pool(n_blocks: int, n_kv_heads: int, head_dim: int, device="cuda"):
+    """A pool of 8-bit pages, [n_blocks, 16, n_kv_heads, head_dim] float8_e4m3fn over memory in which a page of a head is
+    one piece, and its scales, [n_blocks, n_kv_heads] uint8 (E8M0: 2^(byte - 127)), both zeros."""
+    codes = torch.zeros((n_blocks, n_kv_heads, PAGE, head_dim), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+    return codes.transpose(1, 2), torch.zeros((n_blocks, n_kv_heads), dtype=torch.uint8, device=device)
+
+
+def kv_scatter_f8(k, v, k_pool, v_pool, k_scales, v_scales, k_ids, v_ids, start_pos, seq_lens=None, stream=None):
+    """genllm_kv_scatter_f8: a batch's new rows quantised into their 8-bit pages.
+
+    k, v [B, S, Hkv, D], bf16 or float16, any strides that keep rows dense and
+    16-byte aligned; k_pool, v_pool [n, 16, Hkv, D] float8_e4m3fn (or uint8), any
+    strides, and k_scales, v_scales [n, Hkv] uint8 (or float8_e8m0fnu), as f8_pool
+    makes them; k_ids, v_ids [B, P] int32: the block of each page of an entry;
+    start_pos, seq_lens [B] int32: the position of an entry's first row, its rows.
+    All on the GPU.  No page may be written by two entries of a call."""
+    rc = (_lib._calls or _lib.calls()).kv_scatter_f8(k, v, k_pool, v_pool, k_scales, v_scales, k_ids, v_ids, start_pos, seq_lens,
+                                                     None if stream is None else _stream(stream))
+    if rc:
+        check(rc)
+
+
+def kv_gather_f8(k_pool, v_pool, k_scales, v_scales, k_ids, v_ids, start_pos, k_out, v_out, seq_lens=None, stream=None):
+    """genllm_kv_gather_f8: rows of 8-bit pages read back as bf16 or float16; arguments as kv_scatter_f8's, k_out and
+    v_out in the place of k and v."""
+    rc = (_lib._calls or _lib.calls()).kv_gather_f8(k_out, v_out, k_pool, v_pool, k_scales, v_scales, k_ids, v_ids, start_pos, seq_lens,
+                                                    None if stream is None else _stream(stream))
+    if rc:
+        check(rc)
+
+
+@functools.lru_cache(maxsize=1024)
+def paged_attention_batch_workspace_bytes(batch: int, seq_len: int, n_q_heads: int, n_kv_heads: int, head_dim: int,
+                                          max_pages: int) -> int:
+    return lib().genllm_paged_attention_batch_workspace_bytes(batch, seq_len, n_q_heads, n_kv_heads, head_dim, max_pages)
+
+
+def paged_attention_batch(q, out, k_pool, v_pool, k_ids, v_ids, n_cached, scale: float, q_lens=None, k_scales=None, v_scales=None,
+                          causal: bool = True, window=None, sinks: int = 0, workspace=None, stream=None):
+    """genllm_paged_attention_batch: attention of a padded batch of queries over paged caches.
+
+    q, out [B, S, Hq, D], bf16 or float16, any strides that keep rows dense and
+    16-byte aligned (a head-major tensor comes in transposed; out may be q); k_pool,
+    v_pool [n, 16, Hkv, D] of q's type, any strides, or with k_scales and v_scales
+    8-bit pages as kv_scatter_f8 writes them; k_ids, v_ids [B, P] int32; n_cached
+    [B] int32: the tokens of each entry, the queries' own among them; q_lens [B]
+    int32: its queries (None: S each), the last of them at n_cached - 1.  window: a
+    query sees that many keys, itself the last, and the first `sinks` tokens (None:
+    all up to itself).  workspace: a device buffer of at least
+    paged_attention_batch_workspace_bytes(...) bytes when that is non-zero; None
+    takes one for this call from the pool of the stream that it runs on."""
+    if stream is not None:
+        if workspace is None and all(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == d for t, d in ((q, 4), (k_pool, 4), (k_ids, 2))):
+            need = paged_attention_batch_workspace_bytes(*q.shape[:3], k_pool.shape[2], q.shape[3], k_ids.shape[1])
+            if need:
+                workspace = _workspace(need, q.device, stream)
+        stream = _stream(stream)
+    rc = (_lib._calls or _lib.calls()).paged_attention_batch(q, out, k_pool, v_pool, k_ids, v_ids, n_cached, scale, q_lens, k_scales,
+                                                             v_scales, causal, window, sinks, workspace, stream)
+    if rc:
+        check(rc)
+
+
 def fill_normal_bf16(t: torch.Tensor, seed: int, offset: int = 0, stream=None):
     call("genllm_fill_normal_bf16", _ptr(t), t.numel(), seed, offset, _stream(stream))
 
@@ -520,7 +587,8 @@ def to_host_bits(t: torch.Tensor) -> np.ndarray:
 __all__ = [
     "PagedAttentionManager", "paged_attention", "qk_norm_rope_append", "rms_norm", "apply_rope", "rope_cache",
     "kv_scatter", "paged_decode", "paged_decode_noalloc", "paged_prefill", "flash_attention", "decode_workspace_bytes", "gated_delta_rule",
-    "gated_delta_workspace_bytes", "causal_conv", "qk_norm_rope_axes", "fill_normal_bf16", "fill_normal_f16",
+    "gated_delta_workspace_bytes", "causal_conv", "qk_norm_rope_axes", "f8_pool", "kv_scatter_f8", "kv_gather_f8",
+    "paged_attention_batch", "paged_attention_batch_workspace_bytes", "fill_normal_bf16", "fill_normal_f16",
     "selftest_mfma", "device_view", "to_device_bf16", "to_device_f16", "to_host_bits", "GenllmError", "PAGE",
     "DTYPE_BF16", "DTYPE_F16",
 ]

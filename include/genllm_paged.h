@@ -424,6 +424,76 @@ int genllm_qk_norm_rope_axes(const void *q, int64_t q_tok_stride, int64_t q_head
                              const int32_t *positions, int64_t pos_stride, int32_t n_axes, const int32_t *sections,
                              int32_t interleaved, int32_t seq_len, int32_t head_dim, int32_t dtype, void *stream);
 
+/* ------------------------------------------- batches over a paged cache
+ * No counterpart in the reference (one sequence per call, 16-bit pages): a
+ * server's batch, each entry with a row of block ids of its own, and pages in 8
+ * bits.  A pool is n_blocks blocks of 16 tokens x n_kv_heads rows of head_dim (64,
+ * 128 or 256) at any block, token and head strides (in pool elements, rows
+ * 16-byte aligned): [block][16][head][dim], as genllm_kv lays its pools out, or
+ * [block][head][16][dim], where a page of a head is one piece of memory, as
+ * is best for 8 bits.  k_ids, v_ids [batch][max_pages] (device, rows at a stride):
+ * page t / 16 of an entry holds its token t.  An id outside [0, n_blocks) is no page: nothing is
+ * written to it, and what reads it gives NaN.  No call allocates,
+ * copies or synchronises; all are kernel launches that a graph may capture.
+ *
+ * 8-bit pages: a page of 16 tokens and a head has one scale 2^e, in scales
+ * [n_blocks][n_kv_heads] as the byte e + 127 (E8M0), and codes e4m3(x / 2^e), of four significant bits,
+ * rounded to nearest even; e is the least, from -100 on, with |x| <= 448 * 2^e for all that was written.
+ *
+ * genllm_kv_scatter_f8 writes tokens start_pos[b] .. + seq_lens[b] - 1 (device;
+ * null: seq_len each) of k, v [batch][seq_len][n_kv_heads][head_dim].  Writing
+ * slot 0 of a page begins it anew; other slots join what the page holds: where
+ * they raise e, its other codes are rounded to the new scale, which is exact but
+ * for those that become e4m3 subnormals.  NaN and infinity are stored as NaN and leave e alone.  A negative
+ * start_pos is an idle entry; tokens past the table are dropped.  Two
+ * entries of a call must not write one page: what it holds then is not defined.
+ * genllm_kv_gather_f8 reads such tokens back into k_out, v_out, code * 2^e rounded once;
+ * rows past the table are NaN, rows behind seq_lens[b] left as they were. */
+int genllm_kv_scatter_f8(const void *k, int64_t k_batch_stride, int64_t k_tok_stride, int64_t k_head_stride,
+                         const void *v, int64_t v_batch_stride, int64_t v_tok_stride, int64_t v_head_stride,
+                         void *k_pool, int64_t kp_block_stride, int64_t kp_tok_stride, int64_t kp_head_stride,
+                         void *v_pool, int64_t vp_block_stride, int64_t vp_tok_stride, int64_t vp_head_stride,
+                         uint8_t *k_scales, uint8_t *v_scales, int32_t n_blocks, const int32_t *k_ids,
+                         int64_t k_ids_stride, const int32_t *v_ids, int64_t v_ids_stride, int32_t max_pages,
+                         const int32_t *start_pos, const int32_t *seq_lens, int32_t batch, int32_t seq_len,
+                         int32_t n_kv_heads, int32_t head_dim, int32_t dtype, void *stream);
+int genllm_kv_gather_f8(const void *k_pool, int64_t kp_block_stride, int64_t kp_tok_stride, int64_t kp_head_stride,
+                        const void *v_pool, int64_t vp_block_stride, int64_t vp_tok_stride, int64_t vp_head_stride,
+                        const uint8_t *k_scales, const uint8_t *v_scales, int32_t n_blocks, const int32_t *k_ids,
+                        int64_t k_ids_stride, const int32_t *v_ids, int64_t v_ids_stride, int32_t max_pages,
+                        const int32_t *start_pos, const int32_t *seq_lens, void *k_out, int64_t k_batch_stride,
+                        int64_t k_tok_stride, int64_t k_head_stride, void *v_out, int64_t v_batch_stride,
+                        int64_t v_tok_stride, int64_t v_head_stride, int32_t batch, int32_t seq_len,
+                        int32_t n_kv_heads, int32_t head_dim, int32_t dtype, void *stream);
+
+/* Attention of q [batch][seq_len][n_q_heads][head_dim] over the pages.  Entry b has
+ * n_cached[b] tokens (device; the new ones among them; at most the table's are read) and q_lens[b] queries (device;
+ * null: seq_len each), query i at position p = n_cached[b] - q_lens[b] + i.  It sees keys
+ * t <= p (causal; else all n_cached[b]) with t > p - window or t < sinks
+ * (window 0: no limit; a window needs causal).  Rows without a key are zeros, rows
+ * behind q_lens[b] are left as they were; NaN or infinity in a row's result comes only from
+ * keys that it sees.  Pools have dtype's elements, or, with k_scales and
+ * v_scales, 8-bit codes (strides in bytes).  scale is finite and >= 0; scores, maxima,
+ * sums and outputs are formed in fp32.  Probabilities are rounded to fp16 for
+ * 8-bit pages (V's codes then are fp16 values), to dtype for 16-bit ones; up to 16 rows per kv head over bf16
+ * pages keep 16 bits of them.  out may be q (the same address and strides), no other operand.
+ * workspace: genllm_paged_attention_batch_workspace_bytes (0: none is needed, or the sizes are
+ * refused), 16-byte aligned; its contents do not matter before or after the call;
+ * calls that share one must be ordered. */
+size_t genllm_paged_attention_batch_workspace_bytes(int32_t batch, int32_t seq_len, int32_t n_q_heads,
+                                                    int32_t n_kv_heads, int32_t head_dim, int32_t max_pages);
+int genllm_paged_attention_batch(const void *q, int64_t q_batch_stride, int64_t q_tok_stride, int64_t q_head_stride,
+                                 void *out, int64_t o_batch_stride, int64_t o_tok_stride, int64_t o_head_stride,
+                                 const void *k_pool, int64_t kp_block_stride, int64_t kp_tok_stride,
+                                 int64_t kp_head_stride, const void *v_pool, int64_t vp_block_stride,
+                                 int64_t vp_tok_stride, int64_t vp_head_stride, const uint8_t *k_scales,
+                                 const uint8_t *v_scales, int32_t n_blocks, const int32_t *k_ids,
+                                 int64_t k_ids_stride, const int32_t *v_ids, int64_t v_ids_stride,
+                                 int32_t max_pages, const int32_t *n_cached, const int32_t *q_lens, int32_t batch,
+                                 int32_t seq_len, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                 int32_t dtype, float scale, int32_t causal, int32_t window, int32_t sinks,
+                                 void *workspace, size_t workspace_bytes, void *stream);
+
 /* ------------------------------------------------------------ utilities
  * No counterpart in the reference: synthetic seeded inputs for tests and the
  * benchmark (counter-based hash -> Box-Muller -> RNE bf16, or RNE fp16 with
