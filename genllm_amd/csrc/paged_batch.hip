@@ -73,8 +73,9 @@ template <int D, bool Q8>
 struct Step {
     static constexpr int kLoads = D * (Q8 ? 1 : 2) / 64;  // 16-byte loads of a page and kind
     uint4 k[kStep][kLoads], v[kStep][kLoads];
-    float kf[kStep];
-    int ve[kStep], first[kStep];  // the pages' first tokens
+    int first[kStep];  // the pages' first tokens
+    int vid[kStep];
+    int at;  // the lane that knows the first page
 };
 
 template <int D, bool F16, bool Q8>
@@ -98,6 +99,7 @@ __global__ __launch_bounds__(kWaves * 64) void batch_decode_kernel(BatchAttn p) 
     const int n16 = lane & 15, g = lane >> 4;
     Work w;
     if (!find_work<kRows, kStep>(p, int(blockIdx.x), w)) return;
+    put_header(p, w);
     const int rows = w.e.ql * p.G;
     const int query = min(n16, rows - 1) / p.G, head = w.h * p.G + min(n16, rows - 1) % p.G;
     const uint16_t* const qrow = p.q + w.b * p.q_batch + query * p.q_tok + head * p.q_head;
@@ -136,13 +138,13 @@ __global__ __launch_bounds__(kWaves * 64) void batch_decode_kernel(BatchAttn p) 
         info = page_info<Q8>(p, w.b, w.h, span.page(j), there);
     };
     const auto load = [&](int i, int at, Step<D, Q8>& s) {  // step i of the wave; its pages are in lanes 2 at, 2 at + 1
+        s.at = 2 * at;
 #pragma unroll
         for (int pp = 0; pp < kStep; ++pp) {
             const int j = kStep * (s0 + wv + kWaves * i) + pp, from = 2 * at + pp;
             s.first[pp] = j < span.pages ? span.page(j) * kPage : 1 << 30;
-            s.kf[pp] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(info.kf), from));
-            s.ve[pp] = __builtin_amdgcn_readlane(info.ve, from);
             const int kid = __builtin_amdgcn_readlane(info.kid, from), vid = __builtin_amdgcn_readlane(info.vid, from);
+            s.vid[pp] = vid;
             const int valid = kid < 0 ? 0 : min(w.e.n - s.first[pp], kPage);  // rows behind the cache's end read as zeros
             const char* const kb = p.k_pool + (kid < 0 ? 0 : kid) * p.k_block + int64_t(w.h) * p.k_head;
             const char* const vb = p.v_pool + (kid < 0 ? 0 : vid) * p.v_block + int64_t(w.h) * p.v_head;
@@ -157,6 +159,15 @@ __global__ __launch_bounds__(kWaves * 64) void batch_decode_kernel(BatchAttn p) 
         }
     };
     const auto compute = [&](const Step<D, Q8>& s) {
+        // read here, not with the loads: the scales come after the ids, as K and V do
+        float kf[kStep];
+        int ve[kStep];
+#pragma unroll
+        for (int pp = 0; pp < kStep; ++pp) {
+            const int kb = __builtin_amdgcn_readlane(info.kb, s.at + pp), vb = __builtin_amdgcn_readlane(info.vb, s.at + pp);
+            kf[pp] = score_factor<Q8>(p, s.vid[pp], kb, vb);
+            ve[pp] = vb - 127;
+        }
         // V's rows to LDS, at [page][token][chunk ^ swizzle]
 #pragma unroll
         for (int pp = 0; pp < kStep; ++pp)
@@ -194,7 +205,7 @@ __global__ __launch_bounds__(kWaves * 64) void batch_decode_kernel(BatchAttn p) 
         for (int pp = 0; pp < kStep; ++pp) {
             const float a = __builtin_elementwise_maximum(__builtin_elementwise_maximum(x[pp][0], x[pp][1]),
                                                           __builtin_elementwise_maximum(x[pp][2], x[pp][3]));
-            mx = __builtin_elementwise_maximum(mx, a * s.kf[pp]);
+            mx = __builtin_elementwise_maximum(mx, a * kf[pp]);
         }
         if (__any(mx > th)) {
             mx = fmaxf(mx, __shfl_xor(mx, 16));
@@ -210,18 +221,18 @@ __global__ __launch_bounds__(kWaves * 64) void batch_decode_kernel(BatchAttn p) 
         }
         float vs[kStep] = {1.0f, 1.0f};
         if constexpr (Q8) {
-            const int most = max(s.ve[0], s.ve[1]);
+            const int most = max(ve[0], ve[1]);
             if (most > (vref == INT_MIN ? vref : vref + kScaleLead)) {  // wave-uniform
                 const float f = vref == INT_MIN ? 0.0f : power_of_two(vref - most);
 #pragma unroll
                 for (int db = 0; db < DB; ++db) acc[db] *= f;
                 vref = most;
             }
-            vs[0] = power_of_two(s.ve[0] - vref), vs[1] = power_of_two(s.ve[1] - vref);
+            vs[0] = power_of_two(ve[0] - vref), vs[1] = power_of_two(ve[1] - vref);
         }
         float e[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = exp2_fast(__builtin_fmaf(x[i >> 2][i & 3], s.kf[i >> 2], nm));
+        for (int i = 0; i < 8; ++i) e[i] = exp2_fast(__builtin_fmaf(x[i >> 2][i & 3], kf[i >> 2], nm));
         const uint4 pb = make_uint4(EV::pack_p(e[0], e[1]), EV::pack_p(e[2], e[3]), EV::pack_p(e[4], e[5]), EV::pack_p(e[6], e[7]));
         uint4 pl;  // what the first part leaves
         if constexpr (kTwoParts) {
@@ -322,10 +333,10 @@ __global__ __launch_bounds__(kWaves * 64) void batch_decode_kernel(BatchAttn p) 
     if (wv != 0 || n16 >= rows) return;
     if (w.ns > 1) {
         const int64_t at = int64_t(blockIdx.x) * kRows + n16;
-        float* const po = p.partial + at * D + 4 * g;
+        float* const po = partial_rows(p) + at * D + 4 * g;
 #pragma unroll
         for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4_t*>(po + 16 * db) = acc[db];
-        if (g == 0) *reinterpret_cast<float2*>(p.partial + int64_t(p.slots) * kRows * D + 2 * at) = make_float2(m, l);
+        if (g == 0) *reinterpret_cast<float2*>(partial_rows(p) + int64_t(p.slots) * kRows * D + 2 * at) = make_float2(m, l);
         return;
     }
     const float inv = see.any ? 1.0f / l : 0.0f;
@@ -341,33 +352,36 @@ __global__ __launch_bounds__(kWaves * 64) void batch_decode_kernel(BatchAttn p) 
 
 
 // Merge of the splits: M = max m_s, l = sum l_s 2^(m_s - M), o = sum o_s 2^(m_s - M) / l.
-// A lane has 4 dims of a row; SG groups of lanes share a row's splits (SG = 1: a row per
-// group).  Entries with one split were written by their workgroup.
-constexpr int kMergeThreads = 256, kMergeU = 8;
-template <int D, bool F16, int ROWS, int STEP, int SG>
-__global__ __launch_bounds__(kMergeThreads) void batch_merge_kernel(BatchAttn p, int tiles_max) {
+// A lane has 4 dims of a row; SG groups of D / 4 lanes share a row's splits (SG = 1: a row
+// per group).  Entries with one split were written by their workgroup.
+// A row's splits are shared by four waves where there are many of them on average.
+constexpr int kMergeU = 8, kMergeWide = 16;
+template <int D, bool F16, int ROWS, int SG, int THREADS>
+__global__ __launch_bounds__(THREADS) void batch_merge_kernel(BatchAttn p, int tiles_max, int row_blocks) {
     using E = Elem<F16>;
-    constexpr int LR = D / 4, GROUPS = kMergeThreads / LR, RPB = GROUPS / SG, NB = ROWS / RPB;
-    static_assert(GROUPS % SG == 0 && ROWS % RPB == 0, "whole rows");
+    constexpr int LR = D / 4, GROUPS = THREADS / LR, RPB = GROUPS / SG;
+    static_assert(GROUPS % SG == 0 && RPB >= 1, "whole rows");
     __shared__ float lds_o[SG > 1 ? GROUPS : 1][D], lds_ml[GROUPS][2];
-    prefetch_kernargs<sizeof(BatchAttn) + 4>();
-    const int rb = int(blockIdx.x) % NB;
-    unsigned rest = blockIdx.x / NB;
+    unsigned rest = blockIdx.x;
+    const int rb = int(rest % unsigned(row_blocks));
+    rest /= unsigned(row_blocks);
     const int h = int(rest % unsigned(p.Hkv));
     rest /= unsigned(p.Hkv);
     const int tile = int(rest % unsigned(tiles_max)), b = int(rest / unsigned(tiles_max));
-    int base, ns, tiles;
-    Entry e;
-    find_entry<ROWS, STEP>(p, b, base, ns, tiles, e);
-    if (ns < 2 || tile >= tiles) return;
+    const Header head_of = reinterpret_cast<const Header*>(p.partial)[b];
+    const Entry e = entry_of(p, b);
     const int group = int(threadIdx.x) / LR, d = 4 * (int(threadIdx.x) % LR);
     const int in_tile = rb * RPB + group / SG, sg = group % SG;
     const int row = tile * ROWS + in_tile;
-    const bool there = row < e.ql * p.G;
-    if (SG > 1 && !there) return;  // with RPB = 1, the whole workgroup
+    if (e.ql == 0) return;  // no header
+    const int base = head_of.base, ns = head_of.ns, tiles = head_of.tiles;
+    if (ns < 2 || tile >= tiles) return;
+    const bool there = in_tile < ROWS && row < e.ql * p.G;
+    if (SG > 1 && !there) return;  // RPB is 1 then: the whole workgroup
     float M = -INFINITY, L = 0.0f;
     f32x4_t o = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    const float2* const ml = reinterpret_cast<const float2*>(p.partial + int64_t(p.slots) * ROWS * D);
+    const float* const po = partial_rows(p);
+    const float2* const ml = reinterpret_cast<const float2*>(po + int64_t(p.slots) * ROWS * D);
     for (int s0 = sg; there && s0 < ns; s0 += SG * kMergeU) {
         f32x4_t x[kMergeU];
         float2 y[kMergeU];
@@ -375,7 +389,7 @@ __global__ __launch_bounds__(kMergeThreads) void batch_merge_kernel(BatchAttn p,
         for (int u = 0; u < kMergeU; ++u) {
             const int s = s0 + SG * u;
             const int64_t at = (int64_t(base) + (int64_t(tiles - 1 - tile) * ns + s) * p.Hkv + h) * ROWS + in_tile;
-            x[u] = s < ns ? *reinterpret_cast<const f32x4_t*>(p.partial + at * D + d) : f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            x[u] = s < ns ? *reinterpret_cast<const f32x4_t*>(po + at * D + d) : f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
             y[u] = s < ns ? ml[at] : make_float2(-INFINITY, 0.0f);
         }
         float mn = M;
@@ -431,14 +445,21 @@ int decode_of(const BatchAttn& p, int D, hipStream_t stream) {
 
 template <int D, bool F16>
 int merge_of(const BatchAttn& p, const BatchPlan& plan, hipStream_t stream) {
-    constexpr int G = kMergeThreads / (D / 4);
     const int tiles_max = int(plan.tiles / (int64_t(p.B) * p.Hkv));
-    if (plan.decode)
-        hipLaunchKernelGGL((batch_merge_kernel<D, F16, 16, kStep, G>), dim3(unsigned(plan.tiles * 16)), dim3(kMergeThreads), 0, stream, p, tiles_max);
+    const int rows = int(std::min<int64_t>(plan.rows, int64_t(p.S) * p.G));  // of a tile that may be there
+    const auto go = [&](auto kernel, int threads, int per_block) {
+        const int blocks = (rows + per_block - 1) / per_block;
+        hipLaunchKernelGGL(kernel, dim3(unsigned(plan.tiles * blocks)), dim3(threads), 0, stream, p, tiles_max, blocks);
+    };
+    constexpr int G64 = 64 / (D / 4), G256 = 256 / (D / 4);
+    if (plan.decode && plan.tiles * kMergeWide <= plan.target)
+        go(batch_merge_kernel<D, F16, 16, G256, 256>, 256, 1);
+    else if (plan.decode)
+        go(batch_merge_kernel<D, F16, 16, G64, 64>, 64, 1);
     else if (plan.rows == 64)
-        hipLaunchKernelGGL((batch_merge_kernel<D, F16, 64, kPrefillStep, 1>), dim3(unsigned(plan.tiles * (64 / G))), dim3(kMergeThreads), 0, stream, p, tiles_max);
+        go(batch_merge_kernel<D, F16, 64, 1, 256>, 256, G256);
     else
-        hipLaunchKernelGGL((batch_merge_kernel<D, F16, 128, kPrefillStep, 1>), dim3(unsigned(plan.tiles * (128 / G))), dim3(kMergeThreads), 0, stream, p, tiles_max);
+        go(batch_merge_kernel<D, F16, 128, 1, 256>, 256, G256);
     GENLLM_LAUNCH_CHECK("batch_merge_kernel");
     return GENLLM_OK;
 }
@@ -479,7 +500,7 @@ BatchPlan plan_of(const BatchSizes& z) {
     r.slots = r.tiles + (r.can_split ? r.target + 8 : 0);
     return r;
 }
-size_t workspace_of(const BatchPlan& r, int D) { return r.can_split ? size_t(r.slots) * r.rows * (D + 2) * 4 : 0; }
+size_t workspace_of(const BatchPlan& r, int batch, int D) { return r.can_split ? size_t(r.slots) * r.rows * (D + 2) * 4 + size_t(batch) * sizeof(Header) : 0; }
 constexpr int64_t kMostWorkgroups = INT_MAX / 256;
 
 }  // namespace
@@ -493,7 +514,7 @@ extern "C" size_t genllm_paged_attention_batch_workspace_bytes(int32_t batch, in
     const BatchSizes z{batch, seq_len, n_q_heads, n_kv_heads, head_dim, max_pages};
     if (z.refused() || z.empty() || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return 0;
     const BatchPlan plan = plan_of(z);
-    return plan.slots > kMostWorkgroups / 128 ? 0 : workspace_of(plan, head_dim);
+    return plan.slots > kMostWorkgroups / 128 ? 0 : workspace_of(plan, batch, head_dim);
 }
 
 extern "C" int genllm_paged_attention_batch(
@@ -508,6 +529,7 @@ extern "C" int genllm_paged_attention_batch(
     const BatchSizes z{batch, seq_len, n_q_heads, n_kv_heads, head_dim, max_pages};
     if (const char* why = z.refused()) return refuse(GENLLM_ERR_INVALID, why);
     if (n_blocks < 0) return refuse(GENLLM_ERR_INVALID, "negative size");
+    if (n_blocks == 0 && !z.empty()) return refuse(GENLLM_ERR_INVALID, "a pool without blocks");
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return refuse(GENLLM_ERR_UNSUPPORTED, "head_dim 64, 128 or 256");
     if (dtype != GENLLM_DTYPE_BF16 && dtype != GENLLM_DTYPE_F16) return refuse(GENLLM_ERR_UNSUPPORTED, "bf16 or fp16 elements");
     if (!(scale >= 0.0f) || !std::isfinite(scale)) return refuse(GENLLM_ERR_INVALID, "the scale must be finite and not negative");
@@ -540,7 +562,7 @@ extern "C" int genllm_paged_attention_batch(
 
     const BatchPlan plan = plan_of(z);
     if (plan.slots > kMostWorkgroups / 128) return refuse(GENLLM_ERR_INVALID, "more rows than one launch takes");
-    const size_t need = workspace_of(plan, head_dim);
+    const size_t need = workspace_of(plan, batch, head_dim);
     if (need && (!workspace || workspace_bytes < need || !aligned_to(workspace, 16)))
         return refuse(GENLLM_ERR_INVALID, "a 16-byte aligned workspace of " + std::to_string(need) + " bytes is needed");
 

@@ -36,7 +36,7 @@ struct BatchAttn {
     int32_t target = 1;    // workgroups to fill the GPU with
     int32_t least = 1;     // steps that a split takes at least
     int32_t can_split = 0; // else every row tile has one workgroup
-    float* partial = nullptr;  // o [workgroup][tile row][D], then {m, l} [workgroup][tile row]
+    float* partial = nullptr;  // headers [B], then o [workgroup][tile row][D], then {m, l} [workgroup][tile row]
     int32_t slots = 0;         // workgroups that the partials have room for
 };
 
@@ -142,24 +142,11 @@ __device__ __forceinline__ bool find_work(const BatchAttn& p, int w, Work& r) {
     return false;
 }
 
-// Where entry b's workgroups begin, and its splits.
-template <int ROWS, int STEP>
-__device__ __forceinline__ void find_entry(const BatchAttn& p, int b, int& base, int& ns, int& tiles, Entry& e) {
-    const int lane = threadIdx.x & 63;
-    const int quantum = quantum_of<ROWS, STEP>(p);
-    int before = 0;
-    for (int i = lane; i < b; i += 64) {
-        int t, s;
-        cost_of<ROWS, STEP>(p, entry_of(p, i), t, s);
-        before += t * splits_of(p, t, s, quantum) * p.Hkv;
-    }
-    for (int i = 1; i < 64 && i < b; i *= 2) before += __shfl_xor(before, i);
-    base = __builtin_amdgcn_readfirstlane(before);
-    e = entry_of(p, b);
-    int steps;
-    cost_of<ROWS, STEP>(p, e, tiles, steps);
-    ns = splits_of(p, tiles, steps, quantum);
-}
+// What the merge needs of an entry, left in the workspace by the entry's first workgroup
+// (an entry without queries has none, nor needs it).
+struct Header {
+    int base, ns, tiles, pad;
+};
 
 // What a row sees: keys up to `pos`, of those from `from` on and those before p.sinks.
 struct Sight {
@@ -179,31 +166,38 @@ __device__ __forceinline__ float scale_value(int byte) {
 // 2^e for e from -126 to 127, 2^-126 below
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(uint32_t(max(e, -126) + 127) << 23); }
 
-// A page as the lane that looked it up holds it.
+__device__ __forceinline__ float* partial_rows(const BatchAttn& p) { return p.partial + 4 * p.B; }
+
+__device__ __forceinline__ void put_header(const BatchAttn& p, const Work& w) {
+    if (p.can_split && int(blockIdx.x) == w.base && threadIdx.x == 0)
+        reinterpret_cast<Header*>(p.partial)[w.b] = {w.base, w.ns, w.tile + 1, 0};
+}
+
+// A page as the lane that looked it up holds it.  The scales' bytes are not looked at
+// before they are needed: they arrive with the page's rows, not ahead of them.
 struct PageInfo {
-    int kid = -1, vid = -1;  // block ids, -1: no page
-    float kf = 0.0f;         // scores' factor in log2 units; NaN where an id or a scale is none
-    int ve = 0;              // exponent of V's scale
+    int kid = -1, vid = -1;  // block ids; -1, -1: no page; -1, -2: an id that is none
+    int kb = 127, vb = 127;  // bytes of the scales
 };
 template <bool Q8>
 __device__ __forceinline__ PageInfo page_info(const BatchAttn& p, int b, int h, int page, bool there) {
     PageInfo r;
-    r.kf = p.c;
     if (there) {
         r.kid = p.k_ids[b * p.k_ids_row + page];
         r.vid = p.v_ids[b * p.v_ids_row + page];
-        const bool bad = unsigned(r.kid) >= unsigned(p.blocks) || unsigned(r.vid) >= unsigned(p.blocks);
-        if (bad) {
-            r.kid = r.vid = -1;
-            r.kf = __builtin_nanf("");
-        } else if constexpr (Q8) {
-            const int kb = p.k_scales[int64_t(r.kid) * p.Hkv + h], vb = p.v_scales[int64_t(r.vid) * p.Hkv + h];
-            const float f = scale_value(kb) * p.c;
-            r.kf = vb == 255 || f != f ? __builtin_nanf("") : fmaxf(f, __FLT_MIN__);
-            r.ve = vb - 127;
+        if (unsigned(r.kid) >= unsigned(p.blocks) || unsigned(r.vid) >= unsigned(p.blocks)) r.kid = -1, r.vid = -2;
+        if constexpr (Q8) {
+            r.kb = p.k_scales[int64_t(max(r.kid, 0)) * p.Hkv + h];
+            r.vb = p.v_scales[int64_t(max(r.vid, 0)) * p.Hkv + h];
         }
     }
     return r;
+}
+// What takes a page's scores to log2 units; NaN where an id or a scale is none.
+template <bool Q8>
+__device__ __forceinline__ float score_factor(const BatchAttn& p, int vid, int kb, int vb) {
+    if (vid == -2 || (Q8 && (kb == 255 || vb == 255))) return __builtin_nanf("");
+    return Q8 ? fmaxf(scale_value(kb) * p.c, __FLT_MIN__) : p.c;
 }
 
 // Two e4m3 codes (the low or the high half of w) as a packed pair of elements
@@ -240,7 +234,7 @@ __device__ __forceinline__ void exact_keys(const BatchAttn& p, int b, int h, con
         const bool there = info.kid >= 0;
         const char* const kb = p.k_pool + (there ? info.kid : 0) * p.k_block + int64_t(h) * p.k_head;
         const char* const vb = p.v_pool + (there ? info.vid : 0) * p.v_block + int64_t(h) * p.v_head;
-        const float vs = Q8 ? scale_value(info.ve + 127) : 1.0f;
+        const float kf = score_factor<Q8>(p, info.vid, info.kb, info.vb), vs = Q8 ? scale_value(info.vb) : 1.0f;
         for (int j = 0; j < kPage; ++j) {
             const int t = page * kPage + j;
             const bool vis = see(p, t);
@@ -269,7 +263,7 @@ __device__ __forceinline__ void exact_keys(const BatchAttn& p, int b, int h, con
             }
             x += __shfl_xor(x, 16);
             x += __shfl_xor(x, 32);
-            x *= info.kf;
+            x *= kf;
             const float mn = vis ? __builtin_elementwise_maximum(m, x) : m;
             const float alpha = m == -INFINITY ? 0.0f : mn == m ? 1.0f : exp2_fast(m - mn);
             const float e = mn == -INFINITY ? 0.0f : exp2_fast(x - mn);

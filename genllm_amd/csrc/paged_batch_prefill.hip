@@ -58,6 +58,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void batch_prefill_kernel(Ba
     const int n16 = lane & 15, g = lane >> 4;
     Work w;
     if (!find_work<ROWS, kPrefillStep>(p, int(blockIdx.x), w)) return;
+    put_header(p, w);
     const int rows = w.e.ql * p.G, row0 = w.tile * ROWS + 16 * RB * wv;  // of the entry; the wave's first
 
     uint4 qb[RB][KS];
@@ -122,13 +123,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void batch_prefill_kernel(Ba
         const int at = kPrefillStep * ((step - s0) % kBlock);
         float vs = 1.0f;
 #pragma unroll
-        for (int i = 0; i < kPrefillStep; ++i) kf_next[i] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(info.kf), at + i));
+        for (int i = 0; i < kPrefillStep; ++i)
+            kf_next[i] = score_factor<Q8>(p, __builtin_amdgcn_readlane(info.vid, at + i), __builtin_amdgcn_readlane(info.kb, at + i),
+                                          __builtin_amdgcn_readlane(info.vb, at + i));
         if constexpr (Q8) {
             int most = INT_MIN;
 #pragma unroll
-            for (int i = 0; i < kPrefillStep; ++i) most = max(most, __builtin_amdgcn_readlane(info.ve, at + i));
+            for (int i = 0; i < kPrefillStep; ++i) most = max(most, __builtin_amdgcn_readlane(info.vb, at + i) - 127);
             if (vref == INT_MIN || most > vref + kScaleLead) vref = most;
-            vs = power_of_two(__builtin_amdgcn_readlane(info.ve, at + wv) - vref);
+            vs = power_of_two(__builtin_amdgcn_readlane(info.vb, at + wv) - 127 - vref);
         }
 #pragma unroll
         for (int e = 0; e < LD; ++e) {
@@ -288,10 +291,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void batch_prefill_kernel(Ba
         if (row >= rows) continue;
         if (w.ns > 1) {
             const int64_t at = int64_t(blockIdx.x) * ROWS + (row - w.tile * ROWS);
-            float* const po = p.partial + at * D + 4 * g;
+            float* const po = partial_rows(p) + at * D + 4 * g;
 #pragma unroll
             for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4_t*>(po + 16 * db) = acc[rb][db];
-            if (g == 0) *reinterpret_cast<float2*>(p.partial + int64_t(p.slots) * ROWS * D + 2 * at) = make_float2(m[rb], l);
+            if (g == 0) *reinterpret_cast<float2*>(partial_rows(p) + int64_t(p.slots) * ROWS * D + 2 * at) = make_float2(m[rb], l);
             continue;
         }
         const float inv = 1.0f / l;
