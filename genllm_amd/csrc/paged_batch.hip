@@ -38,7 +38,8 @@ namespace {
 constexpr int kRows = 16;   // rows of a decode tile
 constexpr int kStep = 2;    // pages of a decode step
 constexpr int kWaves = 4;
-constexpr int kDecodeTarget = 1024, kDecodeLeast = 8;
+constexpr int kCus = 256;
+constexpr int kDecodeLeast = 1024;  // steps of a split at least, times head_dim
 constexpr int kPrefillTarget = 512, kPrefillLeast = 4;
 constexpr float kLazy = 8.0f;      // log2: a row's maximum may lag its scores by this much
 constexpr int kScaleLead = 6;      // a page's scale may be this many binades above the reference
@@ -78,8 +79,15 @@ struct Step {
     int at;  // the lane that knows the first page
 };
 
+// Workgroups that a CU holds.  Each is four waves, one on a SIMD: 512 registers over them.
+constexpr int resident(int D) { return D == 64 ? 4 : D == 128 ? 3 : 2; }
+// The next step's loads in flight beside this one's, where that leaves the registers for
+// the workgroups above.
+template <int D, bool Q8>
+constexpr bool kAheadOf = D * (Q8 ? 1 : 2) <= 128;
+
 template <int D, bool F16, bool Q8>
-__global__ __launch_bounds__(kWaves * 64) void batch_decode_kernel(BatchAttn p) {
+__global__ __launch_bounds__(kWaves * 64, resident(D)) void batch_decode_kernel(BatchAttn p) {
     using E = Elem<F16>;                 // q, out
     using EV = Elem<F16 || Q8>;          // P and V as the MFMA takes them
     constexpr int ES = Q8 ? 1 : 2;
@@ -87,7 +95,6 @@ __global__ __launch_bounds__(kWaves * 64) void batch_decode_kernel(BatchAttn p) 
     constexpr int ROWB = D * ES, RB = ROWB / 16;  // bytes and 16-byte chunks of a token's row
     constexpr int LD = Step<D, Q8>::kLoads;
     constexpr bool kTwoParts = !F16 && !Q8;
-    constexpr bool kAhead = ROWB <= 256;  // the next step's loads in flight beside this one's: what registers allow
     constexpr int VLDS = kStep * kPage * ROWB;
     constexpr int HAND = DB * 4 * 64 * 4;  // bytes of a wave's O^T
     constexpr int LDS = kWaves * VLDS > 2 * HAND ? kWaves * VLDS : 2 * HAND;
@@ -101,12 +108,18 @@ __global__ __launch_bounds__(kWaves * 64) void batch_decode_kernel(BatchAttn p) 
     if (!find_work<kRows, kStep>(p, int(blockIdx.x), w)) return;
     put_header(p, w);
     const int rows = w.e.ql * p.G;
-    const int query = min(n16, rows - 1) / p.G, head = w.h * p.G + min(n16, rows - 1) % p.G;
-    const uint16_t* const qrow = p.q + w.b * p.q_batch + query * p.q_tok + head * p.q_head;
-    const Sight see = sight_of(p, w.e, query);
+    // the row's query; its addresses are formed where they are used: held through the
+    // loop they cost the registers of a workgroup per CU
+    const int query = min(n16, rows - 1) / p.G;
+    const auto row_at = [&](int64_t batch, int64_t tok, int64_t head) {
+        int r = min(n16, rows - 1);
+        __asm__ volatile("" : "+v"(r));
+        return w.b * batch + query * tok + (w.h * p.G + r - query * p.G) * head;
+    };
 
     // Q^T operands: k-step 2 j + i of 8-bit keys is dims 64 j + 16 g + 8 i, of 16-bit ones 32 ks + 8 g
     uint4 qb[KS];
+    const uint16_t* const qrow = p.q + row_at(p.q_batch, p.q_tok, p.q_head);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
         const int d = Q8 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g;
@@ -196,6 +209,7 @@ __global__ __launch_bounds__(kWaves * 64) void batch_decode_kernel(BatchAttn p) 
         for (int pp = 0; pp < kStep; ++pp) {
             const int last = s.first[pp] + kPage - 1;
             if (last > first_pos || (s.first[pp] < clear_from && last >= p.sinks)) {  // some row does not see all of it
+                const Sight see = sight_of(p, w.e, query);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[pp][i] = see(p, s.first[pp] + 4 * g + i) ? x[pp][i] : -INFINITY;
             }
@@ -265,7 +279,7 @@ __global__ __launch_bounds__(kWaves * 64) void batch_decode_kernel(BatchAttn p) 
         look_up(block);
         const int end = min(mine - block, 32);
         Step<D, Q8> s;
-        if constexpr (kAhead) {
+        if constexpr (kAheadOf<D, Q8>) {
             load(block, 0, s);
             for (int i = 0; i + 1 < end; ++i) {
                 Step<D, Q8> next;
@@ -290,7 +304,7 @@ __global__ __launch_bounds__(kWaves * 64) void batch_decode_kernel(BatchAttn p) 
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum += acc[db][i];
         if (__any(n16 < rows && !(fabsf(sum) <= __FLT_MAX__))) {
-            exact_keys<D, F16, Q8>(p, w.b, w.h, qrow, see, [&](int i) {
+            exact_keys<D, F16, Q8>(p, w.b, w.h, p.q + row_at(p.q_batch, p.q_tok, p.q_head), sight_of(p, w.e, query), [&](int i) {
                 const int j = kStep * (s0 + wv + kWaves * (i >> 1)) + (i & 1);
                 return (i >> 1) < mine && j < span.pages ? span.page(j) : -1;
             }, acc, m, l);
@@ -339,13 +353,14 @@ __global__ __launch_bounds__(kWaves * 64) void batch_decode_kernel(BatchAttn p) 
         if (g == 0) *reinterpret_cast<float2*>(partial_rows(p) + int64_t(p.slots) * kRows * D + 2 * at) = make_float2(m, l);
         return;
     }
-    const float inv = see.any ? 1.0f / l : 0.0f;
-    uint16_t* const orow = p.out + w.b * p.o_batch + query * p.o_tok + head * p.o_head;
+    const bool any = sight_of(p, w.e, query).any;
+    const float inv = 1.0f / l;
+    uint16_t* const orow = p.out + row_at(p.o_batch, p.o_tok, p.o_head);
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
         float o[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = see.any ? acc[db][i] * inv : 0.0f;
+        for (int i = 0; i < 4; ++i) o[i] = any ? acc[db][i] * inv : 0.0f;
         *reinterpret_cast<uint2*>(orow + 16 * db + 4 * g) = make_uint2(E::pack_p(o[0], o[1]), E::pack_p(o[2], o[3]));
     }
 }
@@ -494,9 +509,13 @@ BatchPlan plan_of(const BatchSizes& z) {
     r.rows = r.decode ? kRows : rows <= 64 ? 64 : 128;
     r.step = r.decode ? kStep : kPrefillStep;
     r.tiles = (rows + r.rows - 1) / r.rows * z.batch * z.n_kv_heads;
-    r.target = r.decode ? kDecodeTarget : kPrefillTarget;
-    r.least = r.decode ? kDecodeLeast : kPrefillLeast;
-    r.can_split = (z.max_pages + r.step - 1) / r.step > r.least && (r.decode || r.tiles < r.target);
+    r.target = r.decode ? kCus * resident(z.head_dim) : kPrefillTarget;
+    r.least = r.decode ? kDecodeLeast / z.head_dim : kPrefillLeast;
+    // a merge is worth it for contexts of more than two such splits; where the tiles alone
+    // keep the workgroups busy in turn, for those that are long beside the others
+    const int64_t turns = std::max<int64_t>(1, std::min<int64_t>(r.tiles / r.target, 1 << 20));
+    r.can_split = (z.max_pages + r.step - 1) / r.step > 2 * r.least * turns && (r.decode || r.tiles < r.target);
+    r.least = int(r.least * turns);
     r.slots = r.tiles + (r.can_split ? r.target + 8 : 0);
     return r;
 }
