@@ -36,11 +36,12 @@ namespace genllm {
 namespace {
 
 constexpr int kRows = 16;   // rows of a decode tile
-constexpr int kStep = 2;    // pages of a decode step
+constexpr int kStep = kDecodeStep;
 constexpr int kWaves = 4;
 constexpr int kCus = 256;
 constexpr int kDecodeLeast = 1024;  // steps of a split at least, times head_dim
-constexpr int kPrefillTarget = 512, kPrefillLeast = 4;
+constexpr int kPrefillLeast = 4;
+constexpr int prefill_resident(int D) { return D == 256 ? 1 : 2; }
 constexpr float kLazy = 8.0f;      // log2: a row's maximum may lag its scores by this much
 constexpr int kScaleLead = 6;      // a page's scale may be this many binades above the reference
 constexpr int kNonTemporal = 2;
@@ -127,12 +128,13 @@ __global__ __launch_bounds__(kWaves * 64, resident(D)) void batch_decode_kernel(
         if (n16 >= rows) qb[ks] = make_uint4(0, 0, 0, 0);
     }
 
-    const Span span = span_of(p, p.causal ? w.e.n - w.e.ql : w.e.n - 1, w.e.n);
+    const TileKeys keys = tile_keys<kRows>(p, w.e, 0);
+    const Span span = span_of(p, keys.first, keys.end);
     const int steps = (span.pages + kStep - 1) / kStep;
     const int s0 = int(int64_t(steps) * w.sp / w.ns), s1 = int(int64_t(steps) * (w.sp + 1) / w.ns);
     const int mine = s1 - s0 - wv > 0 ? (s1 - s0 - wv + kWaves - 1) / kWaves : 0;  // this wave's steps
     // keys from clear_from on and below clear_to are seen by every row
-    const int first_pos = p.causal ? w.e.n - w.e.ql : w.e.n - 1, last_pos = w.e.n - 1;
+    const int first_pos = keys.first, last_pos = w.e.n - 1;
     const int clear_from = last_pos - p.window + 1;
 
     f32x4_t acc[DB], accl = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -372,7 +374,7 @@ __global__ __launch_bounds__(kWaves * 64, resident(D)) void batch_decode_kernel(
 // A row's splits are shared by four waves where there are many of them on average.
 constexpr int kMergeU = 8, kMergeWide = 16;
 template <int D, bool F16, int ROWS, int SG, int THREADS>
-__global__ __launch_bounds__(THREADS) void batch_merge_kernel(BatchAttn p, int tiles_max, int row_blocks) {
+__global__ __launch_bounds__(THREADS) void batch_merge_kernel(BatchAttn p, int row_blocks) {
     using E = Elem<F16>;
     constexpr int LR = D / 4, GROUPS = THREADS / LR, RPB = GROUPS / SG;
     static_assert(GROUPS % SG == 0 && RPB >= 1, "whole rows");
@@ -380,32 +382,29 @@ __global__ __launch_bounds__(THREADS) void batch_merge_kernel(BatchAttn p, int t
     unsigned rest = blockIdx.x;
     const int rb = int(rest % unsigned(row_blocks));
     rest /= unsigned(row_blocks);
-    const int h = int(rest % unsigned(p.Hkv));
-    rest /= unsigned(p.Hkv);
-    const int tile = int(rest % unsigned(tiles_max)), b = int(rest / unsigned(tiles_max));
-    const Header head_of = reinterpret_cast<const Header*>(p.partial)[b];
+    const int h = int(rest % unsigned(p.Hkv)), unit = int(rest / unsigned(p.Hkv));
+    const int b = unit / p.tiles_max, tile = unit - b * p.tiles_max;
+    const Header of = reinterpret_cast<const Header*>(p.partial)[unit];
     const Entry e = entry_of(p, b);
     const int group = int(threadIdx.x) / LR, d = 4 * (int(threadIdx.x) % LR);
     const int in_tile = rb * RPB + group / SG, sg = group % SG;
     const int row = tile * ROWS + in_tile;
-    if (e.ql == 0) return;  // no header
-    const int base = head_of.base, ns = head_of.ns, tiles = head_of.tiles;
-    if (ns < 2 || tile >= tiles) return;
+    if (tile * ROWS >= e.ql * p.G || of.ns < 2) return;  // no rows and no header, or one split
     const bool there = in_tile < ROWS && row < e.ql * p.G;
     if (SG > 1 && !there) return;  // RPB is 1 then: the whole workgroup
     float M = -INFINITY, L = 0.0f;
     f32x4_t o = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     const float* const po = partial_rows(p);
     const float2* const ml = reinterpret_cast<const float2*>(po + int64_t(p.slots) * ROWS * D);
-    for (int s0 = sg; there && s0 < ns; s0 += SG * kMergeU) {
+    for (int s0 = sg; there && s0 < of.ns; s0 += SG * kMergeU) {
         f32x4_t x[kMergeU];
         float2 y[kMergeU];
 #pragma unroll
         for (int u = 0; u < kMergeU; ++u) {
             const int s = s0 + SG * u;
-            const int64_t at = (int64_t(base) + (int64_t(tiles - 1 - tile) * ns + s) * p.Hkv + h) * ROWS + in_tile;
-            x[u] = s < ns ? *reinterpret_cast<const f32x4_t*>(po + at * D + d) : f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            y[u] = s < ns ? ml[at] : make_float2(-INFINITY, 0.0f);
+            const int64_t at = (int64_t(of.base) + int64_t(s) * p.Hkv + h) * ROWS + in_tile;
+            x[u] = s < of.ns ? *reinterpret_cast<const f32x4_t*>(po + at * D + d) : f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            y[u] = s < of.ns ? ml[at] : make_float2(-INFINITY, 0.0f);
         }
         float mn = M;
 #pragma unroll
@@ -460,11 +459,10 @@ int decode_of(const BatchAttn& p, int D, hipStream_t stream) {
 
 template <int D, bool F16>
 int merge_of(const BatchAttn& p, const BatchPlan& plan, hipStream_t stream) {
-    const int tiles_max = int(plan.tiles / (int64_t(p.B) * p.Hkv));
     const int rows = int(std::min<int64_t>(plan.rows, int64_t(p.S) * p.G));  // of a tile that may be there
     const auto go = [&](auto kernel, int threads, int per_block) {
         const int blocks = (rows + per_block - 1) / per_block;
-        hipLaunchKernelGGL(kernel, dim3(unsigned(plan.tiles * blocks)), dim3(threads), 0, stream, p, tiles_max, blocks);
+        hipLaunchKernelGGL(kernel, dim3(unsigned(plan.tiles * blocks)), dim3(threads), 0, stream, p, blocks);
     };
     constexpr int G64 = 64 / (D / 4), G256 = 256 / (D / 4);
     if (plan.decode && plan.tiles * kMergeWide <= plan.target)
@@ -508,18 +506,23 @@ BatchPlan plan_of(const BatchSizes& z) {
     r.decode = rows <= kRows;
     r.rows = r.decode ? kRows : rows <= 64 ? 64 : 128;
     r.step = r.decode ? kStep : kPrefillStep;
-    r.tiles = (rows + r.rows - 1) / r.rows * z.batch * z.n_kv_heads;
-    r.target = r.decode ? kCus * resident(z.head_dim) : kPrefillTarget;
+    r.tiles_max = (rows + r.rows - 1) / r.rows;
+    r.tiles = r.tiles_max * z.batch * z.n_kv_heads;
+    r.target = kCus * (r.decode ? resident(z.head_dim) : prefill_resident(z.head_dim));
     r.least = r.decode ? kDecodeLeast / z.head_dim : kPrefillLeast;
     // a merge is worth it for contexts of more than two such splits; where the tiles alone
-    // keep the workgroups busy in turn, for those that are long beside the others
+    // keep the workgroups busy in turn, for tokens that are long beside the others
     const int64_t turns = std::max<int64_t>(1, std::min<int64_t>(r.tiles / r.target, 1 << 20));
     r.can_split = (z.max_pages + r.step - 1) / r.step > 2 * r.least * turns && (r.decode || r.tiles < r.target);
     r.least = int(r.least * turns);
+    // all workgroups there at once, two to a CU: a long one beside a short one
+    r.paired = !r.decode && !r.can_split && prefill_resident(z.head_dim) == 2 && r.tiles > kCus && r.tiles <= 2 * kCus;
     r.slots = r.tiles + (r.can_split ? r.target + 8 : 0);
     return r;
 }
-size_t workspace_of(const BatchPlan& r, int batch, int D) { return r.can_split ? size_t(r.slots) * r.rows * (D + 2) * 4 + size_t(batch) * sizeof(Header) : 0; }
+size_t workspace_of(const BatchPlan& r, int batch, int D) {
+    return r.can_split ? size_t(r.slots) * r.rows * (D + 2) * 4 + (size_t(batch) * r.tiles_max * sizeof(Header) + 15 & ~size_t(15)) : 0;
+}
 constexpr int64_t kMostWorkgroups = INT_MAX / 256;
 
 }  // namespace
@@ -598,7 +601,7 @@ extern "C" int genllm_paged_attention_batch(
     p.blocks = n_blocks, p.capacity = max_pages * kPage;
     p.window = window > 0 ? std::min(window, kNoWindow) : kNoWindow, p.sinks = sinks, p.causal = causal != 0;
     p.c = std::max(scale * kLog2e, __FLT_MIN__);
-    p.target = plan.target, p.least = plan.least, p.can_split = plan.can_split, p.slots = int32_t(plan.slots);
+    p.tiles_max = int32_t(plan.tiles_max), p.target = plan.target, p.least = plan.least, p.can_split = plan.can_split, p.paired = plan.paired && causal, p.slots = int32_t(plan.slots);
     p.partial = need ? static_cast<float*>(workspace) : nullptr;
 
     const auto rows_of = [&](const void* at, int64_t b, int64_t t, int64_t h) {

@@ -33,14 +33,17 @@ struct BatchAttn {
     int32_t causal = 1;
     float c = 0.0f;        // scale * log2(e), at least FLT_MIN
     // division of the work
+    int32_t tiles_max = 1; // row tiles of an entry at most
     int32_t target = 1;    // workgroups to fill the GPU with
     int32_t least = 1;     // steps that a split takes at least
     int32_t can_split = 0; // else every row tile has one workgroup
-    float* partial = nullptr;  // headers [B], then o [workgroup][tile row][D], then {m, l} [workgroup][tile row]
+    int32_t paired = 0;    // row tiles in the order last, last but one, .., then first, second, ..
+    float* partial = nullptr;  // headers [unit], then o [workgroup][tile row][D], then {m, l} [workgroup][tile row]
     int32_t slots = 0;         // workgroups that the partials have room for
 };
 
 constexpr int32_t kNoWindow = 1 << 30;
+constexpr int kDecodeStep = 2, kPrefillStep = 4;  // pages of a step
 
 // Keys in pages: the first `sink_pages` of a sequence, then from sink_pages + skip on.
 struct Span {
@@ -66,75 +69,111 @@ __device__ __forceinline__ Entry entry_of(const BatchAttn& p, int b) {
     return {min(max(n, 0), p.capacity), min(max(ql, 0), p.S)};
 }
 
-// Row tiles and steps (of STEP pages) of an entry, for one kv head.
-template <int ROWS, int STEP>
-__device__ __forceinline__ void cost_of(const BatchAttn& p, const Entry& e, int& tiles, int& steps) {
-    tiles = (e.ql * p.G + ROWS - 1) / ROWS;
-    steps = tiles ? (span_of(p, p.causal ? e.n - e.ql : e.n - 1, e.n).pages + STEP - 1) / STEP : 0;
+// Positions of a row tile's first and last query, and how many keys it has: up to its last
+// query's own.
+struct TileKeys {
+    int first, end;
+};
+template <int ROWS>
+__device__ __forceinline__ TileKeys tile_keys(const BatchAttn& p, const Entry& e, int tile) {
+    if (!p.causal) return {e.n - 1, e.n};
+    const int rows = e.ql * p.G, at = e.n - e.ql;
+    return {at + tile * ROWS / p.G, max(min(at + (min((tile + 1) * ROWS, rows) - 1) / p.G + 1, e.n), 0)};
 }
 
-__device__ __forceinline__ int splits_of(const BatchAttn& p, int tiles, int steps, int quantum) {
-    return tiles == 0 ? 0 : p.can_split ? max(1, (steps + quantum - 1) / quantum) : 1;
-}
-
-// Steps per split: all of the batch's steps over p.target workgroups.  Every wave of the
-// split kernel and of the merge must come to the same number: the sums are whole numbers
-// below 2^53, exact in whatever order.
+// The work is divided by units, row tile `tile` of entry b being unit b * tiles_max + tile:
+// a unit has steps of STEP pages for each kv head, and its splits share them.
 template <int ROWS, int STEP>
-__device__ __forceinline__ int quantum_of(const BatchAttn& p) {
-    if (!p.can_split) return INT32_MAX;
-    const int lane = threadIdx.x & 63;
-    double sum = 0.0;
-    for (int b = lane; b < p.B; b += 64) {
-        int tiles, steps;
-        cost_of<ROWS, STEP>(p, entry_of(p, b), tiles, steps);
-        sum += double(int64_t(tiles) * steps);
-    }
-    for (int i = 1; i < 64 && i < p.B; i *= 2) sum += __shfl_xor(sum, i);
-    const int64_t all = int64_t(sum) * p.Hkv, q = (all + p.target - 1) / p.target;
-    return max(p.least, __builtin_amdgcn_readfirstlane(int(min(q, int64_t(INT32_MAX)))));
+__device__ __forceinline__ bool unit_steps(const BatchAttn& p, const Entry& e, int tile, int& steps) {
+    if (tile * ROWS >= e.ql * p.G) return false;  // no such tile
+    const TileKeys k = tile_keys<ROWS>(p, e, tile);
+    steps = (span_of(p, k.first, k.end).pages + STEP - 1) / STEP;
+    return true;
 }
 
 struct Work {
     int b, tile, sp, h, ns;
-    int base;  // the entry's first workgroup
+    int unit, base;  // the unit's first workgroup
     Entry e;
 };
 
-// What workgroup w does; false: nothing.  Entries lie one after the other, an entry's
-// workgroups as [tile][split][kv head]: with 8 kv heads those of one head run on one XCD.
+constexpr int kQuanta = 4;  // quanta tried: 1, 1 1/4, 1 1/2, 1 3/4 times the share
+
+// What workgroup w does; false: nothing.  Without splits, entry by entry, [tile][kv head],
+// the last tiles, which have the most keys, first.  With them all units of the batch are
+// cut into pieces of as many steps as a target of workgroups leaves for each: the waves of
+// every workgroup come to the same sum (a whole number below 2^53, exact in whatever
+// order), and find theirs by the pieces before it, [unit][split][kv head].  With 8 kv heads
+// those of one head run on one XCD.
 template <int ROWS, int STEP>
 __device__ __forceinline__ bool find_work(const BatchAttn& p, int w, Work& r) {
     const int lane = threadIdx.x & 63;
-    const int quantum = quantum_of<ROWS, STEP>(p);
-    int base = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-        int mine = 0, tiles = 0, steps = 0, ns = 0;
-        Entry e{0, 0};
-        if (b0 + lane < p.B) {
-            e = entry_of(p, b0 + lane);
-            cost_of<ROWS, STEP>(p, e, tiles, steps);
-            ns = splits_of(p, tiles, steps, quantum);
-            mine = tiles * ns * p.Hkv;
+    const unsigned rest = unsigned(w) / unsigned(p.Hkv);
+    r.h = __builtin_amdgcn_readfirstlane(int(unsigned(w) - rest * unsigned(p.Hkv)));
+    if (!p.can_split) {
+        const int b = int(rest / unsigned(p.tiles_max)), rank = int(rest - unsigned(b) * unsigned(p.tiles_max));
+        if (b >= p.B) return false;
+        r.b = __builtin_amdgcn_readfirstlane(b);
+        r.e = entry_of(p, r.b);
+        const int tiles = (r.e.ql * p.G + ROWS - 1) / ROWS, half = (tiles + 1) / 2;
+        if (rank >= tiles) return false;
+        r.tile = __builtin_amdgcn_readfirstlane(p.paired && rank >= half ? rank - half : tiles - 1 - rank);
+        r.ns = 1, r.sp = 0, r.unit = 0, r.base = w;
+        return true;
+    }
+    const int units = p.B * p.tiles_max;
+    double sum = 0.0;
+    for (int u = lane; u < units; u += 64) {
+        int steps = 0;
+        if (unit_steps<ROWS, STEP>(p, entry_of(p, u / p.tiles_max), u % p.tiles_max, steps)) sum += steps;
+    }
+    for (int i = 1; i < 64 && i < units; i *= 2) sum += __shfl_xor(sum, i);
+    const int64_t all = int64_t(sum) * p.Hkv, share = (all + p.target - 1) / p.target;
+    int quantum = max(p.least, __builtin_amdgcn_readfirstlane(int(min(share, int64_t(1 << 28)))));
+    // pieces that are no whole quantum may leave a few workgroups more than the target,
+    // which would run after all the others: up to twice the quantum where that avoids it
+    if (STEP == kPrefillStep && units * p.Hkv <= p.target) {
+        int pieces[kQuanta] = {};
+        for (int u = lane; u < units; u += 64) {
+            int steps = 0;
+            if (!unit_steps<ROWS, STEP>(p, entry_of(p, u / p.tiles_max), u % p.tiles_max, steps)) continue;
+#pragma unroll
+            for (int k = 0; k < kQuanta; ++k) pieces[k] += max(1, (steps + quantum * (kQuanta + k) / kQuanta - 1) / (quantum * (kQuanta + k) / kQuanta));
         }
-        int upto = mine;
-        for (int i = 1; i < 64 && i < p.B; i *= 2) {
+        for (int i = 1; i < 64 && i < units; i *= 2)
+#pragma unroll
+            for (int k = 0; k < kQuanta; ++k) pieces[k] += __shfl_xor(pieces[k], i);
+        int chosen = 2 * quantum;
+#pragma unroll
+        for (int k = kQuanta - 1; k >= 0; --k)
+            if (__builtin_amdgcn_readfirstlane(pieces[k]) * p.Hkv <= p.target) chosen = quantum * (kQuanta + k) / kQuanta;
+        quantum = chosen;
+    }
+    int base = 0;
+    for (int u0 = 0; u0 < units; u0 += 64) {
+        const int u = u0 + lane;
+        int ns = 0, steps = 0;
+        Entry e{0, 0};
+        if (u < units) {
+            e = entry_of(p, u / p.tiles_max);
+            if (unit_steps<ROWS, STEP>(p, e, u % p.tiles_max, steps)) ns = max(1, (steps + quantum - 1) / quantum);
+        }
+        int upto = ns * p.Hkv;
+        for (int i = 1; i < 64 && i < units; i *= 2) {
             const int x = __shfl_up(upto, i);
             if (lane >= i) upto += x;
         }
-        const unsigned long long hit = __ballot(w >= base + upto - mine && w < base + upto);
+        const unsigned long long hit = __ballot(w >= base + upto - ns * p.Hkv && w < base + upto);
         if (hit) {
             const int src = __builtin_ctzll(hit);
-            r.b = b0 + src;
-            r.base = base + __builtin_amdgcn_readlane(upto - mine, src);
+            r.unit = u0 + src;
+            r.b = r.unit / p.tiles_max, r.tile = r.unit % p.tiles_max;
             r.ns = __builtin_amdgcn_readlane(ns, src);
+            r.base = base + __builtin_amdgcn_readlane(upto, src) - r.ns * p.Hkv;
             r.e = {__builtin_amdgcn_readlane(e.n, src), __builtin_amdgcn_readlane(e.ql, src)};
-            const int all = __builtin_amdgcn_readlane(tiles, src);
-            const unsigned local = unsigned(w - r.base), rest = local / unsigned(p.Hkv);
-            r.h = __builtin_amdgcn_readfirstlane(int(local % unsigned(p.Hkv)));
-            r.sp = __builtin_amdgcn_readfirstlane(int(rest % unsigned(r.ns)));
-            // the last tiles have the most keys: first
-            r.tile = __builtin_amdgcn_readfirstlane(all - 1 - int(rest / unsigned(r.ns)));
+            const unsigned local = unsigned(w - r.base), sp = local / unsigned(p.Hkv);
+            r.sp = __builtin_amdgcn_readfirstlane(int(sp));
+            r.h = __builtin_amdgcn_readfirstlane(int(local - sp * unsigned(p.Hkv)));
             return true;
         }
         base += __builtin_amdgcn_readlane(upto, 63);
@@ -142,10 +181,10 @@ __device__ __forceinline__ bool find_work(const BatchAttn& p, int w, Work& r) {
     return false;
 }
 
-// What the merge needs of an entry, left in the workspace by the entry's first workgroup
-// (an entry without queries has none, nor needs it).
+// What the merge needs of a unit, left in the workspace by the unit's first workgroup (one
+// without rows has none, nor needs it).
 struct Header {
-    int base, ns, tiles, pad;
+    int base, ns;
 };
 
 // What a row sees: keys up to `pos`, of those from `from` on and those before p.sinks.
@@ -166,11 +205,11 @@ __device__ __forceinline__ float scale_value(int byte) {
 // 2^e for e from -126 to 127, 2^-126 below
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(uint32_t(max(e, -126) + 127) << 23); }
 
-__device__ __forceinline__ float* partial_rows(const BatchAttn& p) { return p.partial + 4 * p.B; }
+// behind the headers, two ints each, in whole 16 bytes
+__device__ __forceinline__ float* partial_rows(const BatchAttn& p) { return p.partial + (2 * int64_t(p.B) * p.tiles_max + 3 & ~int64_t(3)); }
 
 __device__ __forceinline__ void put_header(const BatchAttn& p, const Work& w) {
-    if (p.can_split && int(blockIdx.x) == w.base && threadIdx.x == 0)
-        reinterpret_cast<Header*>(p.partial)[w.b] = {w.base, w.ns, w.tile + 1, 0};
+    if (p.can_split && int(blockIdx.x) == w.base && threadIdx.x == 0) reinterpret_cast<Header*>(p.partial)[w.unit] = {w.base, w.ns};
 }
 
 // A page as the lane that looked it up holds it.  The scales' bytes are not looked at
@@ -199,6 +238,10 @@ __device__ __forceinline__ float score_factor(const BatchAttn& p, int vid, int k
     if (vid == -2 || (Q8 && (kb == 255 || vb == 255))) return __builtin_nanf("");
     return Q8 ? fmaxf(scale_value(kb) * p.c, __FLT_MIN__) : p.c;
 }
+
+// Waits for the loads of x and makes the compiler take it from here on as what it is: no
+// load's result, whose first use inside a loop would wait for the loads issued there.
+__device__ __forceinline__ void landed(uint4& x) { __asm__ volatile("" : "+v"(x.x), "+v"(x.y), "+v"(x.z), "+v"(x.w)); }
 
 // Two e4m3 codes (the low or the high half of w) as a packed pair of elements
 template <bool F16, bool kHigh>
@@ -290,20 +333,19 @@ __device__ __forceinline__ void exact_keys(const BatchAttn& p, int b, int h, con
     }
 }
 
-constexpr int kPrefillStep = 4;  // pages of a prefill step
-
 int launch_batch_decode(const BatchAttn& p, int head_dim, bool f16, hipStream_t stream);
-int launch_batch_prefill(const BatchAttn& p, int tile_rows, int head_dim, bool f16, hipStream_t stream);
+int launch_batch_prefill(const BatchAttn& p, int tile_rows, int head_dim, bool f16, hipStream_t stream);  // tiles of 64 or 128 rows
 
 // Which kernel a call runs and how its work is divided at most.
 struct BatchPlan {
     bool decode;
-    int rows;       // of a tile
-    int step;       // pages of a step
-    int64_t tiles;  // row tiles at most
+    int rows;           // of a tile
+    int step;           // pages of a step
+    int64_t tiles_max;  // row tiles of an entry and kv head at most
+    int64_t tiles;      // of the batch
     int64_t slots;  // workgroups at most; as many partials where can_split
     int target, least;
-    bool can_split;
+    bool can_split, paired;
 };
 
 }  // namespace genllm

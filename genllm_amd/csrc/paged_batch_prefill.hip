@@ -14,6 +14,8 @@
 //        by one more MFMA with ones, from the same rounded values
 // Lane (row, g) has the scores of keys 4g..4g+3 of each page: the running maximum and the
 // rescaling stay in the lane.  Two LDS buffers, one barrier a step.
+#include <type_traits>
+
 #include "paged_batch.hpp"
 
 namespace genllm {
@@ -32,26 +34,36 @@ __device__ __forceinline__ s16x4_t ds_read_tr16(const lds_char* p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(const_cast<lds_char*>(p)));
 }
 
-// Place of 16-byte chunk c in the LDS row of token r (of 16): K's reads (16 rows, one
-// chunk) and the halves of a transposing read (rows 0-3 and 8-11, or 4-7 and 12-15, two
-// neighbouring chunks) cover all banks once.
+// K in LDS: 16-byte chunk c of token r (of 16) at place c ^ f(r) of its row, so that the
+// reads of an operand (16 rows, one chunk) cover all banks once.
 template <int D>
-__device__ __forceinline__ int place(int r, int c) {
+__device__ __forceinline__ int k_place(int r, int c) {
     if constexpr (D == 64) return c ^ (((r >> 2) & 1) | ((r >> 1) & 1) << 1 | (r >> 3) << 2);
     return (c & ~15) | ((c & 15) ^ ((((r & 7) ^ ((r >> 1) & 4)) << 1) | (r >> 3)));
 }
+// V in LDS: rows apart by two chunks more than they have, those from the eighth on of a
+// page by eight more: the halves of a transposing read (rows 0-3 and 8-11, or 4-7 and 12-15,
+// two neighbouring chunks) cover all banks once, and the chunks of a row lie at fixed
+// distances: one address for all of them.
+template <int D>
+constexpr int kVRow = D == 64 ? 2 * D + 32 : 2 * D + 32;
+template <int D>
+constexpr int kVPage = kPage * kVRow<D> + 128;
+template <int D>
+__device__ __forceinline__ int v_row(int r) { return r * kVRow<D> + (r >> 3) * 128; }
 
-template <int D, bool F16, bool Q8, int RB>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void batch_prefill_kernel(BatchAttn p) {
+// KG groups of four waves share the keys of a step: 1 with 32 rows a wave (RB = 2), 2 with 16.
+template <int D, bool F16, bool Q8, int RB, int KG>
+__global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ? 1 : 2) void batch_prefill_kernel(BatchAttn p) {
     using E = Elem<F16>;
     using EV = Elem<F16 || Q8>;
     constexpr int ES = Q8 ? 1 : 2, KS = D / 32, DB = D / 16;
-    constexpr int ROWS = 64 * RB;
+    constexpr int ROWS = 64 * RB, NP = kPrefillStep / KG;  // pages of a step that are a wave's
     constexpr int ROWB = 2 * D;          // bytes of a token's row in LDS
     constexpr int SRC = D * ES / 16;     // 16-byte chunks of a token's row in memory
     constexpr int LD = SRC / 4;          // 16-byte loads of a lane for a page
     constexpr int TILE = kKeys * ROWB;
-    __shared__ __attribute__((aligned(16))) char lds_k0[TILE], lds_k1[TILE], lds_v0[TILE], lds_v1[TILE];
+    __shared__ __attribute__((aligned(16))) char lds_k0[TILE], lds_k1[TILE], lds_v0[kPrefillStep * kVPage<D>], lds_v1[kPrefillStep * kVPage<D>];
 
     prefetch_kernargs<sizeof(BatchAttn)>();
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -59,28 +71,31 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void batch_prefill_kernel(Ba
     Work w;
     if (!find_work<ROWS, kPrefillStep>(p, int(blockIdx.x), w)) return;
     put_header(p, w);
-    const int rows = w.e.ql * p.G, row0 = w.tile * ROWS + 16 * RB * wv;  // of the entry; the wave's first
+    const int rows = w.e.ql * p.G, row0 = w.tile * ROWS + 16 * RB * (wv & 3);  // of the entry; the wave's first
+    const int kg = KG == 1 ? 0 : wv >> 2, p0 = NP * kg;  // its group; the first of its pages in a step
 
     uint4 qb[RB][KS];
-    Sight see[RB];
-    const uint16_t* qrow[RB];
-    int64_t orow[RB];
+    int query[RB];
+    // addresses and sights of rows are formed where they are used
+    const auto row_at = [&](int rb, int64_t batch, int64_t tok, int64_t head) {
+        int row = min(row0 + 16 * rb + n16, rows - 1);
+        __asm__ volatile("" : "+v"(row));
+        return w.b * batch + query[rb] * tok + (w.h * p.G + row - query[rb] * p.G) * head;
+    };
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-        const int row = min(row0 + 16 * rb + n16, rows - 1), query = row / p.G, head = w.h * p.G + row - query * p.G;
-        see[rb] = sight_of(p, w.e, query);
-        qrow[rb] = p.q + w.b * p.q_batch + query * p.q_tok + head * p.q_head;
-        orow[rb] = w.b * p.o_batch + query * p.o_tok + head * p.o_head;
+        query[rb] = min(row0 + 16 * rb + n16, rows - 1) / p.G;
+        const uint16_t* const qrow = p.q + row_at(rb, p.q_batch, p.q_tok, p.q_head);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) qb[rb][ks] = *reinterpret_cast<const uint4*>(qrow[rb] + 32 * ks + 8 * g);
+        for (int ks = 0; ks < KS; ++ks) qb[rb][ks] = *reinterpret_cast<const uint4*>(qrow + 32 * ks + 8 * g);
     }
-    // positions of the tile's, and of the wave's, first and last row
+    // positions of the wave's first and last row
     const auto pos_of = [&](int row) { return p.causal ? w.e.n - w.e.ql + min(row, rows - 1) / p.G : w.e.n - 1; };
-    const int tile_first = pos_of(w.tile * ROWS), tile_last = pos_of(w.tile * ROWS + ROWS - 1);
     const bool has_rows = row0 < rows;
     const int pos_a = pos_of(row0), pos_b = pos_of(row0 + 16 * RB - 1);
 
-    const Span span = span_of(p, tile_first, min(tile_last + 1, w.e.n));
+    const TileKeys keys = tile_keys<ROWS>(p, w.e, w.tile);
+    const Span span = span_of(p, keys.first, keys.end);
     const int steps = (span.pages + kPrefillStep - 1) / kPrefillStep;
     const int s0 = int(int64_t(steps) * w.sp / w.ns), s1 = int(int64_t(steps) * (w.sp + 1) / w.ns);
 
@@ -102,87 +117,118 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void batch_prefill_kernel(Ba
         const int j = kPrefillStep * step + lane;
         info = page_info<Q8>(p, w.b, w.h, span.page(j), j < span.pages && step + lane / kPrefillStep < s1);
     };
-    uint4 kreg[LD], vreg[LD];
-    float kf[kPrefillStep], kf_next[kPrefillStep];
-    const int k_off = (lane / SRC) * p.k_tok + 16 * (lane % SRC), v_off = (lane / SRC) * p.v_tok + 16 * (lane % SRC);
+    float info_kf = 0.0f;  // of info, once its scales are needed
+    uint4 kreg[LD], vreg[KG == 1 ? LD : 1];  // two groups: one stages K (both in kreg), the other V
+    const int pg = wv & 3;
+    float kf[NP], kf_next[NP];
     const auto issue = [&](int step) {
-        const int at = kPrefillStep * ((step - s0) % kBlock) + wv, j = kPrefillStep * step + wv;
+        const int at = kPrefillStep * ((step - s0) % kBlock) + pg, j = kPrefillStep * step + pg;
         const int kid = __builtin_amdgcn_readlane(info.kid, at), vid = __builtin_amdgcn_readlane(info.vid, at);
         const int first = j < span.pages ? span.page(j) * kPage : 1 << 30;
         const int valid = kid < 0 ? 0 : min(w.e.n - first, kPage);  // rows behind the cache's end read as zeros
-        const char* const kb = p.k_pool + (kid < 0 ? 0 : kid) * p.k_block + int64_t(w.h) * p.k_head;
-        const char* const vb = p.v_pool + (kid < 0 ? 0 : vid) * p.v_block + int64_t(w.h) * p.v_head;
-        const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(kb), 0, valid > 0 ? (valid - 1) * p.k_tok + D * ES : 0, kBufferFlags);
-        const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(vb), 0, valid > 0 ? (valid - 1) * p.v_tok + D * ES : 0, kBufferFlags);
+        const auto rows_of = [&](const char* pool, int id, int64_t block, int head, int tok, uint4* reg) {
+            const char* const base = pool + (kid < 0 ? 0 : id) * block + int64_t(w.h) * head;
+            const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, valid > 0 ? (valid - 1) * tok + D * ES : 0, kBufferFlags);
+            const int off = (lane / SRC) * tok + 16 * (lane % SRC);
 #pragma unroll
-        for (int e = 0; e < LD; ++e) kreg[e] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off, e * (64 / SRC) * p.k_tok, 0));
-#pragma unroll
-        for (int e = 0; e < LD; ++e) vreg[e] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rv, v_off, e * (64 / SRC) * p.v_tok, 0));
+            for (int e = 0; e < LD; ++e) reg[e] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, e * (64 / SRC) * tok, 0));
+        };
+        if (KG == 1 || kg == 0) rows_of(p.k_pool, kid, p.k_block, p.k_head, p.k_tok, kreg);
+        if constexpr (KG == 1) rows_of(p.v_pool, vid, p.v_block, p.v_head, p.v_tok, vreg);
+        else if (kg == 1) rows_of(p.v_pool, vid, p.v_block, p.v_head, p.v_tok, kreg);
     };
     const auto stage = [&](int step, lds_char* kl, lds_char* vl) {
         const int at = kPrefillStep * ((step - s0) % kBlock);
         float vs = 1.0f;
+        if (at == 0) info_kf = score_factor<Q8>(p, info.vid, info.kb, info.vb);
 #pragma unroll
-        for (int i = 0; i < kPrefillStep; ++i)
-            kf_next[i] = score_factor<Q8>(p, __builtin_amdgcn_readlane(info.vid, at + i), __builtin_amdgcn_readlane(info.kb, at + i),
-                                          __builtin_amdgcn_readlane(info.vb, at + i));
+        for (int i = 0; i < NP; ++i) kf_next[i] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(info_kf), at + p0 + i));
         if constexpr (Q8) {
             int most = INT_MIN;
 #pragma unroll
             for (int i = 0; i < kPrefillStep; ++i) most = max(most, __builtin_amdgcn_readlane(info.vb, at + i) - 127);
             if (vref == INT_MIN || most > vref + kScaleLead) vref = most;
-            vs = power_of_two(__builtin_amdgcn_readlane(info.vb, at + wv) - 127 - vref);
+            vs = power_of_two(__builtin_amdgcn_readlane(info.vb, at + pg) - 127 - vref);
         }
+        const auto put = [](lds_char* at, const uint4& x) { *reinterpret_cast<lds_u32x4*>(at) = __builtin_bit_cast(u32x4_t, x); };
+        const auto put_k = [&](const uint4* reg) {
 #pragma unroll
-        for (int e = 0; e < LD; ++e) {
-            const int t = e * (64 / SRC) + lane / SRC, c = lane % SRC, row = (wv * kPage + t) * ROWB;
-            if constexpr (Q8) {
-                const auto put = [&](lds_char* l, int chunk, const uint4& x) {
-                    *reinterpret_cast<lds_u32x4*>(l + row + 16 * place<D>(t, chunk)) = __builtin_bit_cast(u32x4_t, x);
-                };
-                put(kl, 2 * c, f8_octet<F16>(kreg[e].x, kreg[e].y, 1.0f, 1.0f));
-                put(kl, 2 * c + 1, f8_octet<F16>(kreg[e].z, kreg[e].w, 1.0f, 1.0f));
-                put(vl, 2 * c, f8_octet<true>(vreg[e].x, vreg[e].y, vs, vs));
-                put(vl, 2 * c + 1, f8_octet<true>(vreg[e].z, vreg[e].w, vs, vs));
-            } else {
-                *reinterpret_cast<lds_u32x4*>(kl + row + 16 * place<D>(t, c)) = __builtin_bit_cast(u32x4_t, kreg[e]);
-                *reinterpret_cast<lds_u32x4*>(vl + row + 16 * place<D>(t, c)) = __builtin_bit_cast(u32x4_t, vreg[e]);
+            for (int e = 0; e < LD; ++e) {
+                const int t = e * (64 / SRC) + lane / SRC, c = lane % SRC;
+                lds_char* const to = kl + (pg * kPage + t) * ROWB;
+                if constexpr (Q8) {
+                    put(to + 16 * k_place<D>(t, 2 * c), f8_octet<F16>(reg[e].x, reg[e].y, 1.0f, 1.0f));
+                    put(to + 16 * k_place<D>(t, 2 * c + 1), f8_octet<F16>(reg[e].z, reg[e].w, 1.0f, 1.0f));
+                } else {
+                    put(to + 16 * k_place<D>(t, c), reg[e]);
+                }
             }
-        }
+        };
+        const auto put_v = [&](const uint4* reg) {
+#pragma unroll
+            for (int e = 0; e < LD; ++e) {
+                const int t = e * (64 / SRC) + lane / SRC, c = lane % SRC;
+                lds_char* const to = vl + pg * kVPage<D> + v_row<D>(t);
+                if constexpr (Q8) {
+                    put(to + 32 * c, f8_octet<true>(reg[e].x, reg[e].y, vs, vs));
+                    put(to + 32 * c + 16, f8_octet<true>(reg[e].z, reg[e].w, vs, vs));
+                } else {
+                    put(to + 16 * c, reg[e]);
+                }
+            }
+        };
+        if (KG == 1 || kg == 0) put_k(kreg);
+        if constexpr (KG == 1) put_v(vreg);
+        else if (kg == 1) put_v(kreg);
     };
 
-    const auto compute = [&](int step, const lds_char* kl, const lds_char* vl, int ref) {
-        int first[kPrefillStep];
-        bool some = false;
-#pragma unroll
-        for (int i = 0; i < kPrefillStep; ++i) {
-            const int j = kPrefillStep * step + i;
-            first[i] = j < span.pages ? span.page(j) * kPage : 1 << 30;
-            some |= first[i] <= pos_b && (first[i] + kPage - 1 > pos_a - p.window || first[i] < p.sinks);
+    // what the wave's rows see of its pages of a step: 0 nothing, 1 all of it, 2 some
+    const auto sight = [&](int step) {
+        if (!has_rows) return 0;
+        const int j = kPrefillStep * step + p0, first = span.page(j) * kPage;
+        if (j + NP <= span.pages) {
+            const int last = span.page(j + NP - 1) * kPage + kPage - 1;
+            if (last <= pos_a && (first > pos_b - p.window || last < p.sinks)) return 1;
         }
-        if (!some || !has_rows) return;  // wave-uniform
-        f32x4_t s[RB][kPrefillStep];
+        for (int i = 0; i < NP && j + i < span.pages; ++i) {
+            const int at = span.page(j + i) * kPage;
+            if (at <= pos_b && (at + kPage - 1 > pos_a - p.window || at < p.sinks)) return 2;
+        }
+        return 0;
+    };
+    const uint32_t one2 = EV::pack_p(1.0f, 1.0f);
+    const uint4 ones = make_uint4(one2, one2, one2, one2);
+    const auto compute = [&](int step, const lds_char* kl, const lds_char* vl, int ref) {
+        const int see_step = sight(step);
+        if (!see_step) return;  // wave-uniform
+        f32x4_t s[RB][NP];
 #pragma unroll
-        for (int i = 0; i < kPrefillStep; ++i) {
+        for (int i = 0; i < NP; ++i)
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) s[rb][i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        // two pages in turn: the MFMAs of a sum wait for each other
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const u32x4_t a = *reinterpret_cast<const lds_u32x4*>(kl + (i * kPage + n16) * ROWB + 16 * place<D>(n16, 4 * ks + g));
+        for (int i0 = 0; i0 < NP; i0 += 2)
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb) s[rb][i] = E::mma32(__builtin_bit_cast(uint4, a), qb[rb][ks], s[rb][i]);
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int i = i0; i < i0 + 2; ++i) {
+                    const u32x4_t a = *reinterpret_cast<const lds_u32x4*>(kl + ((p0 + i) * kPage + n16) * ROWB + 16 * k_place<D>(n16, 4 * ks + g));
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) s[rb][i] = E::mma32(__builtin_bit_cast(uint4, a), qb[rb][ks], s[rb][i]);
+                }
+        if (see_step == 2)
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int j = kPrefillStep * step + p0 + i, first = j < span.pages ? span.page(j) * kPage : 1 << 30, last = first + kPage - 1;
+                if (last <= pos_a && (first > pos_b - p.window || last < p.sinks)) continue;  // every row sees all of it
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    const Sight see = sight_of(p, w.e, query[rb]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s[rb][i][k] = see(p, first + 4 * g + k) ? s[rb][i][k] : -INFINITY;
+                }
             }
-        }
-#pragma unroll
-        for (int i = 0; i < kPrefillStep; ++i) {
-            const int last = first[i] + kPage - 1;
-            if (last > pos_a || (first[i] <= pos_b - p.window && last >= p.sinks)) {  // some row does not see all of it
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) s[rb][i][k] = see[rb](p, first[i] + 4 * g + k) ? s[rb][i][k] : -INFINITY;
-            }
-        }
         if constexpr (Q8) {
             if (vacc != ref) {  // wave-uniform
                 if (vacc != INT_MIN) {
@@ -195,12 +241,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void batch_prefill_kernel(Ba
                 vacc = ref;
             }
         }
-        uint4 pb[RB][kPrefillStep / 2];
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             float mx = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < kPrefillStep; ++i) {
+            for (int i = 0; i < NP; ++i) {
                 const float a = __builtin_elementwise_maximum(__builtin_elementwise_maximum(s[rb][i][0], s[rb][i][1]),
                                                               __builtin_elementwise_maximum(s[rb][i][2], s[rb][i][3]));
                 mx = __builtin_elementwise_maximum(mx, a * kf[i]);
@@ -217,27 +262,30 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void batch_prefill_kernel(Ba
 #pragma unroll
                 for (int db = 0; db < DB; ++db) acc[rb][db] *= alpha;
             }
-            uint32_t e2[2 * kPrefillStep];
-#pragma unroll
-            for (int i = 0; i < kPrefillStep; ++i)
-#pragma unroll
-                for (int k = 0; k < 4; k += 2)
-                    e2[2 * i + k / 2] = EV::pack_p(exp2_fast(__builtin_fmaf(s[rb][i][k], kf[i], nm[rb])),
-                                                   exp2_fast(__builtin_fmaf(s[rb][i][k + 1], kf[i], nm[rb])));
-#pragma unroll
-            for (int i = 0; i < kPrefillStep / 2; ++i) pb[rb][i] = make_uint4(e2[4 * i], e2[4 * i + 1], e2[4 * i + 2], e2[4 * i + 3]);
         }
-        const uint32_t one2 = EV::pack_p(1.0f, 1.0f);
-        const uint4 ones = make_uint4(one2, one2, one2, one2);
+        uint4 pb[RB][NP / 2];
 #pragma unroll
-        for (int i = 0; i < kPrefillStep / 2; ++i) {
+        for (int i = 0; i < NP / 2; ++i)
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                uint32_t e[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const f32x4_t& x = s[rb][2 * i + (k >> 1)];
+                    const float f = kf[2 * i + (k >> 1)];
+                    e[k] = EV::pack_p(exp2_fast(__builtin_fmaf(x[2 * (k & 1)], f, nm[rb])), exp2_fast(__builtin_fmaf(x[2 * (k & 1) + 1], f, nm[rb])));
+                }
+                pb[rb][i] = make_uint4(e[0], e[1], e[2], e[3]);
+            }
+        const int t = 4 * g + (n16 >> 2);
+        const lds_char* const vt = vl + p0 * kVPage<D> + v_row<D>(t) + 8 * (n16 & 3);
+#pragma unroll
+        for (int i = 0; i < NP / 2; ++i) {
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) accl[rb] = EV::mma32(ones, pb[rb][i], accl[rb]);
-            const int t = 4 * g + (n16 >> 2);
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
-                const lds_char* const at = vl + (32 * i + t) * ROWB + 16 * place<D>(t, 2 * db + ((n16 & 3) >> 1)) + 8 * (n16 & 1);
-                const s16x4_t u[2] = {ds_read_tr16(at), ds_read_tr16(at + kPage * ROWB)};
+                const s16x4_t u[2] = {ds_read_tr16(vt + 2 * i * kVPage<D> + 32 * db), ds_read_tr16(vt + (2 * i + 1) * kVPage<D> + 32 * db)};
                 const uint4 a = __builtin_bit_cast(uint4, u);
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) acc[rb][db] = EV::mma32(a, pb[rb][i], acc[rb][db]);
@@ -250,6 +298,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void batch_prefill_kernel(Ba
         issue(s0);
         stage(s0, (lds_char*)lds_k0, (lds_char*)lds_v0);
     }
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) landed(qb[rb][ks]);
     const auto turn = [&](int t, lds_char* kl, lds_char* vl, lds_char* kn, lds_char* vn) {
 #pragma unroll
         for (int i = 0; i < kPrefillStep; ++i) kf[i] = kf_next[i];
@@ -268,18 +320,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void batch_prefill_kernel(Ba
         if (t + 1 < s1) turn(t + 1, (lds_char*)lds_k1, (lds_char*)lds_v1, (lds_char*)lds_k0, (lds_char*)lds_v0);
     }
 
-    if (!has_rows) return;
+    float ls[RB];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
         const int row = row0 + 16 * rb + n16;
-        float l = accl[rb][0], sum = l;
+        float sum = accl[rb][0], &l = ls[rb];
+        l = sum;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum += acc[rb][db][i];
         if (__any(row < rows && !(fabsf(sum) <= __FLT_MAX__))) {
-            exact_keys<D, F16, Q8>(p, w.b, w.h, qrow[rb], see[rb], [&](int i) {
-                const int j = kPrefillStep * s0 + i;
+            exact_keys<D, F16, Q8>(p, w.b, w.h, p.q + row_at(rb, p.q_batch, p.q_tok, p.q_head), sight_of(p, w.e, query[rb]), [&](int i) {
+                const int j = kPrefillStep * (s0 + i / NP) + p0 + i % NP;
                 return j < kPrefillStep * s1 && j < span.pages ? span.page(j) : -1;
             }, acc[rb], m[rb], l);
         } else if (Q8 && vacc != INT_MIN) {
@@ -288,6 +341,37 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void batch_prefill_kernel(Ba
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[rb][db][i] = ldexpf(acc[rb][db][i], vacc);
         }
+    }
+    if constexpr (KG == 2) {
+        // the second group's state through LDS to the first's: m = max, l and O weighed by 2^(m_i - m)
+        constexpr int HAND = DB * 4 * 64 * 4;
+        static_assert(RB == 1 && 2 * HAND <= TILE, "two waves' O^T in a buffer of K");
+        __shared__ float lds_ml[4][2][64];
+        auto const x = (__attribute__((address_space(3))) float*)((lds_char*)(wv & 2 ? lds_k1 : lds_k0) + (wv & 1) * HAND) + lane;
+        __syncthreads();  // the buffers are free
+        if (kg == 1) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[(db * 4 + i) * 64] = acc[0][db][i];
+            lds_ml[wv & 3][0][lane] = m[0];
+            lds_ml[wv & 3][1][lane] = ls[0];
+        }
+        __syncthreads();
+        if (kg == 1) return;
+        const float m1 = lds_ml[wv][0][lane], l1 = lds_ml[wv][1][lane], mt = __builtin_elementwise_maximum(m[0], m1);
+        const float a0 = m[0] == -INFINITY ? 0.0f : exp2_fast(m[0] - mt), a1 = m1 == -INFINITY ? 0.0f : exp2_fast(m1 - mt);
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[0][db][i] = acc[0][db][i] * a0 + x[(db * 4 + i) * 64] * a1;
+        ls[0] = ls[0] * a0 + l1 * a1;
+        m[0] = mt;
+    }
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const int row = row0 + 16 * rb + n16;
+        const float l = ls[rb];
         if (row >= rows) continue;
         if (w.ns > 1) {
             const int64_t at = int64_t(blockIdx.x) * ROWS + (row - w.tile * ROWS);
@@ -298,35 +382,37 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void batch_prefill_kernel(Ba
             continue;
         }
         const float inv = 1.0f / l;
+        const bool any = sight_of(p, w.e, query[rb]).any;
+        uint16_t* const orow = p.out + row_at(rb, p.o_batch, p.o_tok, p.o_head);
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
             float o[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = see[rb].any ? acc[rb][db][i] * inv : 0.0f;
-            *reinterpret_cast<uint2*>(p.out + orow[rb] + 16 * db + 4 * g) = make_uint2(E::pack_p(o[0], o[1]), E::pack_p(o[2], o[3]));
+            for (int i = 0; i < 4; ++i) o[i] = any ? acc[rb][db][i] * inv : 0.0f;
+            *reinterpret_cast<uint2*>(orow + 16 * db + 4 * g) = make_uint2(E::pack_p(o[0], o[1]), E::pack_p(o[2], o[3]));
         }
     }
 }
 
-template <bool F16, bool Q8, int RB>
+template <bool F16, bool Q8, int RB, int KG>
 int prefill_of(const BatchAttn& p, int D, hipStream_t stream) {
-    const dim3 grid(unsigned(p.slots)), block(256);
-    if (D == 64) hipLaunchKernelGGL((batch_prefill_kernel<64, F16, Q8, RB>), grid, block, 0, stream, p);
-    else if (D == 128) hipLaunchKernelGGL((batch_prefill_kernel<128, F16, Q8, RB>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((batch_prefill_kernel<256, F16, Q8, RB>), grid, block, 0, stream, p);
+    const dim3 grid(unsigned(p.slots)), block(256 * KG);
+    if (D == 64) hipLaunchKernelGGL((batch_prefill_kernel<64, F16, Q8, RB, KG>), grid, block, 0, stream, p);
+    else if (D == 128) hipLaunchKernelGGL((batch_prefill_kernel<128, F16, Q8, RB, KG>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((batch_prefill_kernel<256, F16, Q8, RB, KG>), grid, block, 0, stream, p);
     GENLLM_LAUNCH_CHECK("batch_prefill_kernel");
     return GENLLM_OK;
 }
-template <int RB>
+template <int RB, int KG>
 int prefill_rows(const BatchAttn& p, int D, bool f16, hipStream_t s) {
-    return f16 ? p.k_scales ? prefill_of<true, true, RB>(p, D, s) : prefill_of<true, false, RB>(p, D, s)
-               : p.k_scales ? prefill_of<false, true, RB>(p, D, s) : prefill_of<false, false, RB>(p, D, s);
+    return f16 ? p.k_scales ? prefill_of<true, true, RB, KG>(p, D, s) : prefill_of<true, false, RB, KG>(p, D, s)
+               : p.k_scales ? prefill_of<false, true, RB, KG>(p, D, s) : prefill_of<false, false, RB, KG>(p, D, s);
 }
 
 }  // namespace
 
 int launch_batch_prefill(const BatchAttn& p, int tile_rows, int D, bool f16, hipStream_t stream) {
-    return tile_rows == 64 ? prefill_rows<1>(p, D, f16, stream) : prefill_rows<2>(p, D, f16, stream);
+    return tile_rows == 64 ? prefill_rows<1, 2>(p, D, f16, stream) : prefill_rows<2, 1>(p, D, f16, stream);
 }
 
 }  // namespace genllm
