@@ -282,6 +282,8 @@ __global__ __launch_bounds__(kWaves * 64, resident(D)) void batch_decode_kernel(
         const int end = min(mine - block, 32);
         Step<D, Q8> s;
         if constexpr (kAheadOf<D, Q8>) {
+            // not unrolled by two, which would save the copies: that took the registers of the
+            // third workgroup (64 sequences of 4096 tokens 57.0 -> 60.5 us)
             load(block, 0, s);
             for (int i = 0; i + 1 < end; ++i) {
                 Step<D, Q8> next;
@@ -504,16 +506,24 @@ BatchPlan plan_of(const BatchSizes& z) {
     BatchPlan r;
     const int64_t rows = int64_t(z.seq_len) * (z.n_q_heads / z.n_kv_heads);
     r.decode = rows <= kRows;
-    r.rows = r.decode ? kRows : rows <= 64 ? 64 : 128;
+    r.target = kCus * (r.decode ? resident(z.head_dim) : prefill_resident(z.head_dim));
+    // Prompts over little more than their own rows whose tiles of 64 are all there at once and
+    // leave few places: eight waves to each, a long tile beside a short one, no split (16 q and
+    // 8 kv heads of 128, 2048 tokens: 44 us, with tiles of 128 in splits 49.5; 1800: 37.4 and
+    // 44.4).  Not for short ones (4 x 512: 21.9 and 20.0), nor for chunks on a long context,
+    // which splits divide evenly (2048 on 8192: 182 and 150).
+    const int64_t fine = (rows + 63) / 64 * z.batch * z.n_kv_heads;
+    const bool fits = !r.decode && rows > 64 && z.seq_len >= 1024 && int64_t(z.max_pages) * kPage < 2 * int64_t(z.seq_len) && fine <= r.target &&
+                      fine >= r.target / 4 * 3;
+    r.rows = r.decode ? kRows : rows <= 64 || fits ? 64 : 128;
     r.step = r.decode ? kStep : kPrefillStep;
     r.tiles_max = (rows + r.rows - 1) / r.rows;
     r.tiles = r.tiles_max * z.batch * z.n_kv_heads;
-    r.target = kCus * (r.decode ? resident(z.head_dim) : prefill_resident(z.head_dim));
     r.least = r.decode ? kDecodeLeast / z.head_dim : kPrefillLeast;
     // a merge is worth it for contexts of more than two such splits; where the tiles alone
     // keep the workgroups busy in turn, for tokens that are long beside the others
     const int64_t turns = std::max<int64_t>(1, std::min<int64_t>(r.tiles / r.target, 1 << 20));
-    r.can_split = (z.max_pages + r.step - 1) / r.step > 2 * r.least * turns && (r.decode || r.tiles < r.target);
+    r.can_split = (z.max_pages + r.step - 1) / r.step > 2 * r.least * turns && (r.decode || r.tiles < r.target) && !fits;
     r.least = int(r.least * turns);
     // all workgroups there at once, two to a CU: a long one beside a short one
     r.paired = !r.decode && !r.can_split && prefill_resident(z.head_dim) == 2 && r.tiles > kCus && r.tiles <= 2 * kCus;
@@ -523,7 +533,7 @@ BatchPlan plan_of(const BatchSizes& z) {
 size_t workspace_of(const BatchPlan& r, int batch, int D) {
     return r.can_split ? size_t(r.slots) * r.rows * (D + 2) * 4 + (size_t(batch) * r.tiles_max * sizeof(Header) + 15 & ~size_t(15)) : 0;
 }
-constexpr int64_t kMostWorkgroups = INT_MAX / 256;
+constexpr int64_t kMostWorkgroups = INT_MAX / 512;  // of 512 threads, in a launch of fewer than 2^32; a merge has up to 16 of 64 for each
 
 }  // namespace
 
@@ -536,7 +546,7 @@ extern "C" size_t genllm_paged_attention_batch_workspace_bytes(int32_t batch, in
     const BatchSizes z{batch, seq_len, n_q_heads, n_kv_heads, head_dim, max_pages};
     if (z.refused() || z.empty() || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return 0;
     const BatchPlan plan = plan_of(z);
-    return plan.slots > kMostWorkgroups / 128 ? 0 : workspace_of(plan, batch, head_dim);
+    return plan.slots > kMostWorkgroups ? 0 : workspace_of(plan, batch, head_dim);
 }
 
 extern "C" int genllm_paged_attention_batch(
@@ -583,7 +593,7 @@ extern "C" int genllm_paged_attention_batch(
         return refuse(GENLLM_ERR_INVALID, "a pool's token rows must follow each other within less than 2^26 bytes, a block's heads within 2^31");
 
     const BatchPlan plan = plan_of(z);
-    if (plan.slots > kMostWorkgroups / 128) return refuse(GENLLM_ERR_INVALID, "more rows than one launch takes");
+    if (plan.slots > kMostWorkgroups) return refuse(GENLLM_ERR_INVALID, "more rows than one launch takes");
     const size_t need = workspace_of(plan, batch, head_dim);
     if (need && (!workspace || workspace_bytes < need || !aligned_to(workspace, 16)))
         return refuse(GENLLM_ERR_INVALID, "a 16-byte aligned workspace of " + std::to_string(need) + " bytes is needed");

@@ -61,6 +61,22 @@ __device__ __forceinline__ Span span_of(const BatchAttn& p, int first_pos, int e
     return {sinks, w0 - sinks, total - (w0 - sinks)};
 }
 
+// Quotients of numbers from 0 on, rounded down, by a divisor that the lanes have in common:
+// by its reciprocal in fp32, once more for what the first (within 2^-21 of itself) leaves,
+// and a step up or down.  (The compiler's integer division takes about 40 instructions; a
+// plan of 32 row tiles took 8800 cycles with it.)
+struct Divisor {
+    int d;
+    float r;
+    __device__ __forceinline__ explicit Divisor(int d_) : d(d_), r(__builtin_amdgcn_rcpf(float(d_))) {}
+    __device__ __forceinline__ int operator()(int x) const {
+        int q = int(float(x) * r), rest = x - q * d;
+        const int more = int(float(rest) * r);
+        q += more, rest -= more * d;
+        return q + (rest >= d ? 1 : 0) - (rest < 0 ? 1 : 0);
+    }
+};
+
 struct Entry {
     int n, ql;  // keys cached, queries
 };
@@ -78,7 +94,8 @@ template <int ROWS>
 __device__ __forceinline__ TileKeys tile_keys(const BatchAttn& p, const Entry& e, int tile) {
     if (!p.causal) return {e.n - 1, e.n};
     const int rows = e.ql * p.G, at = e.n - e.ql;
-    return {at + tile * ROWS / p.G, max(min(at + (min((tile + 1) * ROWS, rows) - 1) / p.G + 1, e.n), 0)};
+    const Divisor by_g(p.G);
+    return {at + by_g(tile * ROWS), max(min(at + by_g(min((tile + 1) * ROWS, rows) - 1) + 1, e.n), 0)};
 }
 
 // The work is divided by units, row tile `tile` of entry b being unit b * tiles_max + tile:
@@ -108,13 +125,13 @@ constexpr int kQuanta = 4;  // quanta tried: 1, 1 1/4, 1 1/2, 1 3/4 times the sh
 template <int ROWS, int STEP>
 __device__ __forceinline__ bool find_work(const BatchAttn& p, int w, Work& r) {
     const int lane = threadIdx.x & 63;
-    const unsigned rest = unsigned(w) / unsigned(p.Hkv);
-    r.h = __builtin_amdgcn_readfirstlane(int(unsigned(w) - rest * unsigned(p.Hkv)));
+    const Divisor by_heads(p.Hkv), by_tiles(p.tiles_max);
     if (!p.can_split) {
-        const int b = int(rest / unsigned(p.tiles_max)), rank = int(rest - unsigned(b) * unsigned(p.tiles_max));
+        const int rest = by_heads(w), b = by_tiles(rest), rank = rest - b * p.tiles_max;
         if (b >= p.B) return false;
         r.b = __builtin_amdgcn_readfirstlane(b);
         r.e = entry_of(p, r.b);
+        r.h = __builtin_amdgcn_readfirstlane(w - rest * p.Hkv);
         const int tiles = (r.e.ql * p.G + ROWS - 1) / ROWS, half = (tiles + 1) / 2;
         if (rank >= tiles) return false;
         r.tile = __builtin_amdgcn_readfirstlane(p.paired && rank >= half ? rank - half : tiles - 1 - rank);
@@ -124,21 +141,26 @@ __device__ __forceinline__ bool find_work(const BatchAttn& p, int w, Work& r) {
     const int units = p.B * p.tiles_max;
     double sum = 0.0;
     for (int u = lane; u < units; u += 64) {
+        const int b = by_tiles(u);
         int steps = 0;
-        if (unit_steps<ROWS, STEP>(p, entry_of(p, u / p.tiles_max), u % p.tiles_max, steps)) sum += steps;
+        if (unit_steps<ROWS, STEP>(p, entry_of(p, b), u - b * p.tiles_max, steps)) sum += steps;
     }
     for (int i = 1; i < 64 && i < units; i *= 2) sum += __shfl_xor(sum, i);
-    const int64_t all = int64_t(sum) * p.Hkv, share = (all + p.target - 1) / p.target;
-    int quantum = max(p.least, __builtin_amdgcn_readfirstlane(int(min(share, int64_t(1 << 28)))));
+    const double share = ceil(sum * p.Hkv * (1.0 / p.target));  // every workgroup's the same, whatever the last bit is
+    int quantum = max(p.least, __builtin_amdgcn_readfirstlane(int(fmin(share, double(1 << 28)))));
     // pieces that are no whole quantum may leave a few workgroups more than the target,
     // which would run after all the others: up to twice the quantum where that avoids it
     if (STEP == kPrefillStep && units * p.Hkv <= p.target) {
         int pieces[kQuanta] = {};
         for (int u = lane; u < units; u += 64) {
+            const int b = by_tiles(u);
             int steps = 0;
-            if (!unit_steps<ROWS, STEP>(p, entry_of(p, u / p.tiles_max), u % p.tiles_max, steps)) continue;
+            if (!unit_steps<ROWS, STEP>(p, entry_of(p, b), u - b * p.tiles_max, steps)) continue;
 #pragma unroll
-            for (int k = 0; k < kQuanta; ++k) pieces[k] += max(1, (steps + quantum * (kQuanta + k) / kQuanta - 1) / (quantum * (kQuanta + k) / kQuanta));
+            for (int k = 0; k < kQuanta; ++k) {
+                const int q = quantum * (kQuanta + k) / kQuanta;
+                pieces[k] += max(1, Divisor(q)(steps + q - 1));
+            }
         }
         for (int i = 1; i < 64 && i < units; i *= 2)
 #pragma unroll
@@ -149,14 +171,16 @@ __device__ __forceinline__ bool find_work(const BatchAttn& p, int w, Work& r) {
             if (__builtin_amdgcn_readfirstlane(pieces[k]) * p.Hkv <= p.target) chosen = quantum * (kQuanta + k) / kQuanta;
         quantum = chosen;
     }
+    const Divisor by_quantum(quantum);
     int base = 0;
     for (int u0 = 0; u0 < units; u0 += 64) {
         const int u = u0 + lane;
         int ns = 0, steps = 0;
         Entry e{0, 0};
         if (u < units) {
-            e = entry_of(p, u / p.tiles_max);
-            if (unit_steps<ROWS, STEP>(p, e, u % p.tiles_max, steps)) ns = max(1, (steps + quantum - 1) / quantum);
+            const int b = by_tiles(u);
+            e = entry_of(p, b);
+            if (unit_steps<ROWS, STEP>(p, e, u - b * p.tiles_max, steps)) ns = max(1, by_quantum(steps + quantum - 1));
         }
         int upto = ns * p.Hkv;
         for (int i = 1; i < 64 && i < units; i *= 2) {
@@ -167,13 +191,12 @@ __device__ __forceinline__ bool find_work(const BatchAttn& p, int w, Work& r) {
         if (hit) {
             const int src = __builtin_ctzll(hit);
             r.unit = u0 + src;
-            r.b = r.unit / p.tiles_max, r.tile = r.unit % p.tiles_max;
+            r.b = __builtin_amdgcn_readfirstlane(by_tiles(r.unit)), r.tile = r.unit - r.b * p.tiles_max;
             r.ns = __builtin_amdgcn_readlane(ns, src);
             r.base = base + __builtin_amdgcn_readlane(upto, src) - r.ns * p.Hkv;
             r.e = {__builtin_amdgcn_readlane(e.n, src), __builtin_amdgcn_readlane(e.ql, src)};
-            const unsigned local = unsigned(w - r.base), sp = local / unsigned(p.Hkv);
-            r.sp = __builtin_amdgcn_readfirstlane(int(sp));
-            r.h = __builtin_amdgcn_readfirstlane(int(local - sp * unsigned(p.Hkv)));
+            r.sp = __builtin_amdgcn_readfirstlane(by_heads(w - r.base));
+            r.h = w - r.base - r.sp * p.Hkv;
             return true;
         }
         base += __builtin_amdgcn_readlane(upto, 63);

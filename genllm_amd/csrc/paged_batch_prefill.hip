@@ -74,6 +74,7 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
     const int rows = w.e.ql * p.G, row0 = w.tile * ROWS + 16 * RB * (wv & 3);  // of the entry; the wave's first
     const int kg = KG == 1 ? 0 : wv >> 2, p0 = NP * kg;  // its group; the first of its pages in a step
 
+    const Divisor by_g(p.G);
     uint4 qb[RB][KS];
     int query[RB];
     // addresses and sights of rows are formed where they are used
@@ -84,15 +85,15 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
     };
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-        query[rb] = min(row0 + 16 * rb + n16, rows - 1) / p.G;
+        query[rb] = by_g(min(row0 + 16 * rb + n16, rows - 1));
         const uint16_t* const qrow = p.q + row_at(rb, p.q_batch, p.q_tok, p.q_head);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) qb[rb][ks] = *reinterpret_cast<const uint4*>(qrow + 32 * ks + 8 * g);
     }
     // positions of the wave's first and last row
-    const auto pos_of = [&](int row) { return p.causal ? w.e.n - w.e.ql + min(row, rows - 1) / p.G : w.e.n - 1; };
+    const auto pos_of = [&](int row) { return p.causal ? w.e.n - w.e.ql + by_g(min(row, rows - 1)) : w.e.n - 1; };
     const bool has_rows = row0 < rows;
-    const int pos_a = pos_of(row0), pos_b = pos_of(row0 + 16 * RB - 1);
+    const int pos_a = __builtin_amdgcn_readfirstlane(pos_of(row0)), pos_b = __builtin_amdgcn_readfirstlane(pos_of(row0 + 16 * RB - 1));
 
     const TileKeys keys = tile_keys<ROWS>(p, w.e, w.tile);
     const Span span = span_of(p, keys.first, keys.end);
@@ -113,29 +114,35 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
     // ---- staging: lane i of every wave knows page i of 16 steps
     constexpr int kBlock = 64 / kPrefillStep;
     PageInfo info;
+    // where its rows are that this wave stages (64 bits; K's, or V's in the second of two
+    // groups), and how many: formed by the lanes, taken by `issue`
+    int info_k[2], info_v[KG == 1 ? 2 : 1], info_n;
     const auto look_up = [&](int step) {
         const int j = kPrefillStep * step + lane;
         info = page_info<Q8>(p, w.b, w.h, span.page(j), j < span.pages && step + lane / kPrefillStep < s1);
+        const char* const k = p.k_pool + max(info.kid, 0) * p.k_block + int64_t(w.h) * p.k_head;
+        const char* const v = p.v_pool + max(info.vid, 0) * p.v_block + int64_t(w.h) * p.v_head;
+        const uintptr_t one = uintptr_t(KG == 1 || kg == 0 ? k : v);
+        info_k[0] = int(one), info_k[1] = int(one >> 32);
+        if constexpr (KG == 1) info_v[0] = int(uintptr_t(v)), info_v[1] = int(uintptr_t(v) >> 32);
+        info_n = info.kid < 0 ? 0 : min(w.e.n - span.page(j) * kPage, kPage);  // rows behind the cache's end read as zeros
     };
     float info_kf = 0.0f;  // of info, once its scales are needed
     uint4 kreg[LD], vreg[KG == 1 ? LD : 1];  // two groups: one stages K (both in kreg), the other V
     const int pg = wv & 3;
     float kf[NP], kf_next[NP];
     const auto issue = [&](int step) {
-        const int at = kPrefillStep * ((step - s0) % kBlock) + pg, j = kPrefillStep * step + pg;
-        const int kid = __builtin_amdgcn_readlane(info.kid, at), vid = __builtin_amdgcn_readlane(info.vid, at);
-        const int first = j < span.pages ? span.page(j) * kPage : 1 << 30;
-        const int valid = kid < 0 ? 0 : min(w.e.n - first, kPage);  // rows behind the cache's end read as zeros
-        const auto rows_of = [&](const char* pool, int id, int64_t block, int head, int tok, uint4* reg) {
-            const char* const base = pool + (kid < 0 ? 0 : id) * block + int64_t(w.h) * head;
-            const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, valid > 0 ? (valid - 1) * tok + D * ES : 0, kBufferFlags);
+        const int at = kPrefillStep * ((step - s0) % kBlock) + pg;
+        const int n = __builtin_amdgcn_readlane(info_n, at);
+        const auto rows_of = [&](const int (&place)[2], int tok, uint4* reg) {
+            const uint64_t base = uint32_t(__builtin_amdgcn_readlane(place[0], at)) | uint64_t(uint32_t(__builtin_amdgcn_readlane(place[1], at))) << 32;
+            const auto r = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base), 0, n > 0 ? (n - 1) * tok + D * ES : 0, kBufferFlags);
             const int off = (lane / SRC) * tok + 16 * (lane % SRC);
 #pragma unroll
             for (int e = 0; e < LD; ++e) reg[e] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, e * (64 / SRC) * tok, 0));
         };
-        if (KG == 1 || kg == 0) rows_of(p.k_pool, kid, p.k_block, p.k_head, p.k_tok, kreg);
-        if constexpr (KG == 1) rows_of(p.v_pool, vid, p.v_block, p.v_head, p.v_tok, vreg);
-        else if (kg == 1) rows_of(p.v_pool, vid, p.v_block, p.v_head, p.v_tok, kreg);
+        rows_of(info_k, KG == 1 || kg == 0 ? p.k_tok : p.v_tok, kreg);
+        if constexpr (KG == 1) rows_of(info_v, p.v_tok, vreg);
     };
     const auto stage = [&](int step, lds_char* kl, lds_char* vl) {
         const int at = kPrefillStep * ((step - s0) % kBlock);
@@ -157,8 +164,11 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
                 const int t = e * (64 / SRC) + lane / SRC, c = lane % SRC;
                 lds_char* const to = kl + (pg * kPage + t) * ROWB;
                 if constexpr (Q8) {
-                    put(to + 16 * k_place<D>(t, 2 * c), f8_octet<F16>(reg[e].x, reg[e].y, 1.0f, 1.0f));
-                    put(to + 16 * k_place<D>(t, 2 * c + 1), f8_octet<F16>(reg[e].z, reg[e].w, 1.0f, 1.0f));
+                    // every other row its second chunk first: a row's even places, then its odd
+                    // ones, are half the banks
+                    const bool odd = t & 1;
+                    put(to + 16 * k_place<D>(t, 2 * c + odd), f8_octet<F16>(odd ? reg[e].z : reg[e].x, odd ? reg[e].w : reg[e].y, 1.0f, 1.0f));
+                    put(to + 16 * k_place<D>(t, 2 * c + !odd), f8_octet<F16>(odd ? reg[e].x : reg[e].z, odd ? reg[e].y : reg[e].w, 1.0f, 1.0f));
                 } else {
                     put(to + 16 * k_place<D>(t, c), reg[e]);
                 }
@@ -170,8 +180,9 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
                 const int t = e * (64 / SRC) + lane / SRC, c = lane % SRC;
                 lds_char* const to = vl + pg * kVPage<D> + v_row<D>(t);
                 if constexpr (Q8) {
-                    put(to + 32 * c, f8_octet<true>(reg[e].x, reg[e].y, vs, vs));
-                    put(to + 32 * c + 16, f8_octet<true>(reg[e].z, reg[e].w, vs, vs));
+                    const bool odd = t & 1;
+                    put(to + 32 * c + 16 * odd, f8_octet<true>(odd ? reg[e].z : reg[e].x, odd ? reg[e].w : reg[e].y, vs, vs));
+                    put(to + 32 * c + 16 * !odd, f8_octet<true>(odd ? reg[e].x : reg[e].z, odd ? reg[e].y : reg[e].w, vs, vs));
                 } else {
                     put(to + 16 * c, reg[e]);
                 }
@@ -206,17 +217,26 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
         for (int i = 0; i < NP; ++i)
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) s[rb][i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        // two pages in turn: the MFMAs of a sum wait for each other
+        // Two pages in turn: the MFMAs of a sum wait for each other.  kAheadK operands on
+        // their way from LDS while one is used: a read takes as long as six MFMAs or more, and
+        // two waves to a SIMD do not hide that (2 x 512 queries on 8192 keys 170 -> 157 us).
+        constexpr int NK = NP * KS, kAheadK = KG == 1 && NK >= 4 ? 4 : 2;
+        u32x4_t ka[kAheadK];
+        const auto k_operand = [&](int x) {  // x: page pair, k-step, page of the pair
+            const int i = 2 * (x / (2 * KS)) + (x & 1), ks = x / 2 % KS;
+            return *reinterpret_cast<const lds_u32x4*>(kl + ((p0 + i) * kPage + n16) * ROWB + 16 * k_place<D>(n16, 4 * ks + g));
+        };
 #pragma unroll
-        for (int i0 = 0; i0 < NP; i0 += 2)
+        for (int x = 0; x < kAheadK; ++x) ka[x] = k_operand(x);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
+        for (int x = 0; x < NK; ++x) {
+            const int i = 2 * (x / (2 * KS)) + (x & 1), ks = x / 2 % KS;
 #pragma unroll
-                for (int i = i0; i < i0 + 2; ++i) {
-                    const u32x4_t a = *reinterpret_cast<const lds_u32x4*>(kl + ((p0 + i) * kPage + n16) * ROWB + 16 * k_place<D>(n16, 4 * ks + g));
-#pragma unroll
-                    for (int rb = 0; rb < RB; ++rb) s[rb][i] = E::mma32(__builtin_bit_cast(uint4, a), qb[rb][ks], s[rb][i]);
-                }
+            for (int rb = 0; rb < RB; ++rb) s[rb][i] = E::mma32(__builtin_bit_cast(uint4, ka[x % kAheadK]), qb[rb][ks], s[rb][i]);
+            if (x + kAheadK < NK) ka[x % kAheadK] = k_operand(x + kAheadK);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if (see_step == 2)
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
@@ -263,6 +283,18 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
                 for (int db = 0; db < DB; ++db) acc[rb][db] *= alpha;
             }
         }
+        // V's first operands come while the probabilities are formed
+        constexpr int NV = NP / 2 * DB, kAheadV = KG == 1 ? 4 : 2;
+        const int t = 4 * g + (n16 >> 2);
+        const lds_char* const vt = vl + p0 * kVPage<D> + v_row<D>(t) + 8 * (n16 & 3);
+        s16x4_t va[kAheadV][2];
+        const auto v_operand = [&](int x, s16x4_t (&to)[2]) {
+            const int i = x / DB, db = x % DB;
+            to[0] = ds_read_tr16(vt + 2 * i * kVPage<D> + 32 * db), to[1] = ds_read_tr16(vt + (2 * i + 1) * kVPage<D> + 32 * db);
+        };
+#pragma unroll
+        for (int x = 0; x < kAheadV; ++x) v_operand(x, va[x]);
+        __builtin_amdgcn_sched_barrier(0);
         uint4 pb[RB][NP / 2];
 #pragma unroll
         for (int i = 0; i < NP / 2; ++i)
@@ -276,20 +308,16 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
                     e[k] = EV::pack_p(exp2_fast(__builtin_fmaf(x[2 * (k & 1)], f, nm[rb])), exp2_fast(__builtin_fmaf(x[2 * (k & 1) + 1], f, nm[rb])));
                 }
                 pb[rb][i] = make_uint4(e[0], e[1], e[2], e[3]);
+                accl[rb] = EV::mma32(ones, pb[rb][i], accl[rb]);
             }
-        const int t = 4 * g + (n16 >> 2);
-        const lds_char* const vt = vl + p0 * kVPage<D> + v_row<D>(t) + 8 * (n16 & 3);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < NP / 2; ++i) {
+        for (int x = 0; x < NV; ++x) {
+            const uint4 a = __builtin_bit_cast(uint4, va[x % kAheadV]);
 #pragma unroll
-            for (int rb = 0; rb < RB; ++rb) accl[rb] = EV::mma32(ones, pb[rb][i], accl[rb]);
-#pragma unroll
-            for (int db = 0; db < DB; ++db) {
-                const s16x4_t u[2] = {ds_read_tr16(vt + 2 * i * kVPage<D> + 32 * db), ds_read_tr16(vt + (2 * i + 1) * kVPage<D> + 32 * db)};
-                const uint4 a = __builtin_bit_cast(uint4, u);
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) acc[rb][db] = EV::mma32(a, pb[rb][i], acc[rb][db]);
-            }
+            for (int rb = 0; rb < RB; ++rb) acc[rb][x % DB] = EV::mma32(a, pb[rb][x / DB], acc[rb][x % DB]);
+            if (x + kAheadV < NV) v_operand(x + kAheadV, va[x % kAheadV]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
@@ -304,7 +332,7 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
         for (int ks = 0; ks < KS; ++ks) landed(qb[rb][ks]);
     const auto turn = [&](int t, lds_char* kl, lds_char* vl, lds_char* kn, lds_char* vn) {
 #pragma unroll
-        for (int i = 0; i < kPrefillStep; ++i) kf[i] = kf_next[i];
+        for (int i = 0; i < NP; ++i) kf[i] = kf_next[i];
         const int ref = vref;
         __syncthreads();  // step t is staged; the other buffer is free
         const bool more = t + 1 < s1;

@@ -100,6 +100,26 @@ def test_prompts(Hq, H, D, S, dtype, f8):
     c.check("prompts")
 
 
+@pytest.mark.parametrize("f8,window", [(True, None), (False, 300)])
+@pytest.mark.parametrize("Hq,H,D", [(6, 3, 64), (8, 8, 128), (6, 3, 256)])
+def test_whole_prompts(Hq, H, D, f8, window):
+    """Prompts of a thousand tokens whose tiles are all there at once, a long tile beside a short one."""
+    S = 1030
+    B = {64: 4, 128: 3, 256: 2}[D]
+    n = [S, S + 900, 700, S - 1][:B]
+    c = Case(Hq, H, D, BF, f8, n, S, [S, S, 650, S - 1][:B])
+    c.run(window=window)
+    c.check("whole prompts", window=window)
+
+
+def test_many_tiles():
+    """More tiles than 16 bits count, most of them of an entry that has few rows."""
+    n = [i % 17 for i in range(1100)]
+    c = Case(64, 64, 64, BF, True, n, 17, [min(i % 5, x) for i, x in enumerate(n)])
+    c.run()
+    c.check("many tiles")
+
+
 @pytest.mark.parametrize("f8", [True, False])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (5, 4), (16, 0), (16, 16), (100, 20), (33, 300), (2 ** 31 - 1, 3)])
 @pytest.mark.parametrize("S", [1, 3, 40, 130])
