@@ -511,9 +511,10 @@ BatchPlan plan_of(const BatchSizes& z) {
     // leave few places: eight waves to each, a long tile beside a short one, no split (16 q and
     // 8 kv heads of 128, 2048 tokens: 44 us, with tiles of 128 in splits 49.5; 1800: 37.4 and
     // 44.4).  Not for short ones (4 x 512: 21.9 and 20.0), nor for chunks on a long context,
-    // which splits divide evenly (2048 on 8192: 182 and 150).
+    // which splits divide evenly (2048 on 8192: 182 and 150), nor at head_dim 256, one workgroup
+    // to a CU (8 and 2 heads, 2048 tokens: 56 and 52).
     const int64_t fine = (rows + 63) / 64 * z.batch * z.n_kv_heads;
-    const bool fits = !r.decode && rows > 64 && z.seq_len >= 1024 && int64_t(z.max_pages) * kPage < 2 * int64_t(z.seq_len) && fine <= r.target &&
+    const bool fits = !r.decode && rows > 64 && z.head_dim <= 128 && z.seq_len >= 1024 && int64_t(z.max_pages) * kPage < 2 * int64_t(z.seq_len) && fine <= r.target &&
                       fine >= r.target / 4 * 3;
     r.rows = r.decode ? kRows : rows <= 64 || fits ? 64 : 128;
     r.step = r.decode ? kStep : kPrefillStep;

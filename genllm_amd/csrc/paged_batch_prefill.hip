@@ -24,6 +24,10 @@ namespace {
 
 constexpr float kLazy = 8.0f;  // log2: a row's maximum may lag its scores by this much
 constexpr int kScaleLead = 6;  // a page's scale may be this many binades above the reference
+// The two waves of a SIMD: one whose MFMA waits for the matrix core keeps the other's vector
+// instructions from being issued, unless those come first (8192 tokens, 16 and 8 heads of 128:
+// 298 us without priorities, 289 with both at 3, 268 so).
+constexpr int kSoftmaxPrio = 2, kStagePrio = 3;
 constexpr int kKeys = kPrefillStep * kPage;
 
 typedef __attribute__((address_space(3))) char lds_char;
@@ -92,7 +96,6 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
     }
     // positions of the wave's first and last row
     const auto pos_of = [&](int row) { return p.causal ? w.e.n - w.e.ql + by_g(min(row, rows - 1)) : w.e.n - 1; };
-    const bool has_rows = row0 < rows;
     const int pos_a = __builtin_amdgcn_readfirstlane(pos_of(row0)), pos_b = __builtin_amdgcn_readfirstlane(pos_of(row0 + 16 * RB - 1));
 
     const TileKeys keys = tile_keys<ROWS>(p, w.e, w.tile);
@@ -131,18 +134,27 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
     uint4 kreg[LD], vreg[KG == 1 ? LD : 1];  // two groups: one stages K (both in kreg), the other V
     const int pg = wv & 3;
     float kf[NP], kf_next[NP];
-    const auto issue = [&](int step) {
+    // the next step's loads: `aim` finds the rows, `load` brings one of kLoads 16-byte parts
+    struct Rows { __amdgpu_buffer_rsrc_t at; int tok, off; } from[KG == 1 ? 2 : 1];
+    constexpr int kLoads = KG == 1 ? 2 * LD : LD;
+    // many loads at once hold the wave up (16 of 16 bytes to a lane, 1200 cycles of a step's
+    // 5900 at D = 256): they are issued between the MFMAs of the scores (a window of 512 on 4096
+    // tokens 34.0 -> 32.6 us); four or eight are not (8 at D = 128: no difference)
+    constexpr bool kSpread = kLoads >= 16;
+    const auto aim = [&](int step) {
         const int at = kPrefillStep * ((step - s0) % kBlock) + pg;
-        const int n = __builtin_amdgcn_readlane(info_n, at);
-        const auto rows_of = [&](const int (&place)[2], int tok, uint4* reg) {
+        const int n = step < s1 ? __builtin_amdgcn_readlane(info_n, at) : 0;
+        const auto rows_of = [&](const int (&place)[2], int tok) {
             const uint64_t base = uint32_t(__builtin_amdgcn_readlane(place[0], at)) | uint64_t(uint32_t(__builtin_amdgcn_readlane(place[1], at))) << 32;
-            const auto r = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base), 0, n > 0 ? (n - 1) * tok + D * ES : 0, kBufferFlags);
-            const int off = (lane / SRC) * tok + 16 * (lane % SRC);
-#pragma unroll
-            for (int e = 0; e < LD; ++e) reg[e] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, e * (64 / SRC) * tok, 0));
+            return Rows{__builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base), 0, n > 0 ? (n - 1) * tok + D * ES : 0, kBufferFlags), tok,
+                        (lane / SRC) * tok + 16 * (lane % SRC)};
         };
-        rows_of(info_k, KG == 1 || kg == 0 ? p.k_tok : p.v_tok, kreg);
-        if constexpr (KG == 1) rows_of(info_v, p.v_tok, vreg);
+        from[0] = rows_of(info_k, KG == 1 || kg == 0 ? p.k_tok : p.v_tok);
+        if constexpr (KG == 1) from[1] = rows_of(info_v, p.v_tok);
+    };
+    const auto load = [&](int l) {
+        const Rows& f = from[KG == 1 ? l / LD : 0];
+        (KG == 2 || l < LD ? kreg : vreg)[l % LD] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(f.at, f.off, l % LD * (64 / SRC) * f.tok, 0));
     };
     const auto stage = [&](int step, lds_char* kl, lds_char* vl) {
         const int at = kPrefillStep * ((step - s0) % kBlock);
@@ -193,25 +205,16 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
         else if (kg == 1) put_v(kreg);
     };
 
-    // what the wave's rows see of its pages of a step: 0 nothing, 1 all of it, 2 some
-    const auto sight = [&](int step) {
-        if (!has_rows) return 0;
+    // whether the wave's rows see all of its pages of a step
+    const auto sees_all = [&](int step) {
         const int j = kPrefillStep * step + p0, first = span.page(j) * kPage;
-        if (j + NP <= span.pages) {
-            const int last = span.page(j + NP - 1) * kPage + kPage - 1;
-            if (last <= pos_a && (first > pos_b - p.window || last < p.sinks)) return 1;
-        }
-        for (int i = 0; i < NP && j + i < span.pages; ++i) {
-            const int at = span.page(j + i) * kPage;
-            if (at <= pos_b && (at + kPage - 1 > pos_a - p.window || at < p.sinks)) return 2;
-        }
-        return 0;
+        if (j + NP > span.pages) return false;
+        const int last = span.page(j + NP - 1) * kPage + kPage - 1;
+        return last <= pos_a && (first > pos_b - p.window || last < p.sinks);
     };
     const uint32_t one2 = EV::pack_p(1.0f, 1.0f);
     const uint4 ones = make_uint4(one2, one2, one2, one2);
     const auto compute = [&](int step, const lds_char* kl, const lds_char* vl, int ref) {
-        const int see_step = sight(step);
-        if (!see_step) return;  // wave-uniform
         f32x4_t s[RB][NP];
 #pragma unroll
         for (int i = 0; i < NP; ++i)
@@ -235,9 +238,12 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) s[rb][i] = E::mma32(__builtin_bit_cast(uint4, ka[x % kAheadK]), qb[rb][ks], s[rb][i]);
             if (x + kAheadK < NK) ka[x % kAheadK] = k_operand(x + kAheadK);
+#pragma unroll
+            for (int l = (x * kLoads + NK - 1) / NK; kSpread && l < ((x + 1) * kLoads + NK - 1) / NK; ++l) load(l);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (see_step == 2)
+        __builtin_amdgcn_s_setprio(kSoftmaxPrio);
+        if (!sees_all(step))  // wave-uniform
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const int j = kPrefillStep * step + p0 + i, first = j < span.pages ? span.page(j) * kPage : 1 << 30, last = first + kPage - 1;
@@ -311,6 +317,7 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
                 accl[rb] = EV::mma32(ones, pb[rb][i], accl[rb]);
             }
         __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(0);
 #pragma unroll
         for (int x = 0; x < NV; ++x) {
             const uint4 a = __builtin_bit_cast(uint4, va[x % kAheadV]);
@@ -323,7 +330,9 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
 
     if (s0 < s1) {
         look_up(s0);
-        issue(s0);
+        aim(s0);
+#pragma unroll
+        for (int l = 0; l < kLoads; ++l) load(l);
         stage(s0, (lds_char*)lds_k0, (lds_char*)lds_v0);
     }
 #pragma unroll
@@ -336,12 +345,14 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
         const int ref = vref;
         __syncthreads();  // step t is staged; the other buffer is free
         const bool more = t + 1 < s1;
-        if (more) {
-            if ((t + 1 - s0) % kBlock == 0) look_up(t + 1);
-            issue(t + 1);
-        }
+        if (more && (t + 1 - s0) % kBlock == 0) look_up(t + 1);
+        aim(t + 1);
+#pragma unroll
+        for (int l = 0; !kSpread && l < kLoads; ++l) load(l);
         compute(t, kl, vl, ref);
+        __builtin_amdgcn_s_setprio(kStagePrio);
         if (more) stage(t + 1, kn, vn);
+        __builtin_amdgcn_s_setprio(0);
     };
     for (int t = s0; t < s1; t += 2) {
         turn(t, (lds_char*)lds_k0, (lds_char*)lds_v0, (lds_char*)lds_k1, (lds_char*)lds_v1);
