@@ -114,6 +114,17 @@ struct Work {
     Entry e;
 };
 
+// The sums of x over the lanes up to this one, all of them active
+__device__ __forceinline__ int wave_sums(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // from the lanes 1, 2, 4, 8 before in a row of 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // a row's last to the next row
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // the second row's last to the last two
+    return x;
+}
+
 constexpr int kQuanta = 4;  // quanta tried: 1, 1 1/4, 1 1/2, 1 3/4 times the share
 
 // What workgroup w does; false: nothing.  Without splits, entry by entry, [tile][kv head],
@@ -139,54 +150,52 @@ __device__ __forceinline__ bool find_work(const BatchAttn& p, int w, Work& r) {
         return true;
     }
     const int units = p.B * p.tiles_max;
-    double sum = 0.0;
-    for (int u = lane; u < units; u += 64) {
-        const int b = by_tiles(u);
-        int steps = 0;
-        if (unit_steps<ROWS, STEP>(p, entry_of(p, b), u - b * p.tiles_max, steps)) sum += steps;
-    }
-    for (int i = 1; i < 64 && i < units; i *= 2) sum += __shfl_xor(sum, i);
+    // what lane u % 64 knows of unit u, the first 64 once and for all
+    struct Unit {
+        int steps = -1;  // none: the entry has no such tile
+        Entry e{0, 0};
+    };
+    const auto unit = [&](int u) {
+        Unit r;
+        if (u < units) {
+            const int b = by_tiles(u);
+            r.e = entry_of(p, b);
+            if (!unit_steps<ROWS, STEP>(p, r.e, u - b * p.tiles_max, r.steps)) r.steps = -1;
+        }
+        return r;
+    };
+    const Unit first = unit(lane);
+    int64_t mine = max(first.steps, 0);
+    for (int u = lane + 64; u < units; u += 64) mine += max(unit(u).steps, 0);
+    // of at most 2^48 in a lane, exact
+    const double sum = double(__builtin_amdgcn_readlane(wave_sums(int(mine & 0xffffff)), 63)) +
+                       (units > 64 ? double(__builtin_amdgcn_readlane(wave_sums(int(mine >> 24)), 63)) * (1 << 24) : 0.0);
     const double share = ceil(sum * p.Hkv * (1.0 / p.target));  // every workgroup's the same, whatever the last bit is
     int quantum = max(p.least, __builtin_amdgcn_readfirstlane(int(fmin(share, double(1 << 28)))));
     // pieces that are no whole quantum may leave a few workgroups more than the target,
     // which would run after all the others: up to twice the quantum where that avoids it
     if (STEP == kPrefillStep && units * p.Hkv <= p.target) {
-        int pieces[kQuanta] = {};
-        for (int u = lane; u < units; u += 64) {
-            const int b = by_tiles(u);
-            int steps = 0;
-            if (!unit_steps<ROWS, STEP>(p, entry_of(p, b), u - b * p.tiles_max, steps)) continue;
-#pragma unroll
-            for (int k = 0; k < kQuanta; ++k) {
-                const int q = quantum * (kQuanta + k) / kQuanta;
-                pieces[k] += max(1, Divisor(q)(steps + q - 1));
-            }
-        }
-        for (int i = 1; i < 64 && i < units; i *= 2)
-#pragma unroll
-            for (int k = 0; k < kQuanta; ++k) pieces[k] += __shfl_xor(pieces[k], i);
         int chosen = 2 * quantum;
 #pragma unroll
-        for (int k = kQuanta - 1; k >= 0; --k)
-            if (__builtin_amdgcn_readfirstlane(pieces[k]) * p.Hkv <= p.target) chosen = quantum * (kQuanta + k) / kQuanta;
+        for (int k = kQuanta - 1; k >= 0; --k) {
+            const int q = quantum * (kQuanta + k) / kQuanta;
+            const Divisor by(q);
+            int pieces = first.steps < 0 ? 0 : max(1, by(first.steps + q - 1));
+            for (int u = lane + 64; u < units; u += 64) {
+                const int steps = unit(u).steps;
+                pieces += steps < 0 ? 0 : max(1, by(steps + q - 1));
+            }
+            if (__builtin_amdgcn_readlane(wave_sums(pieces), 63) * p.Hkv <= p.target) chosen = q;
+        }
         quantum = chosen;
     }
     const Divisor by_quantum(quantum);
     int base = 0;
     for (int u0 = 0; u0 < units; u0 += 64) {
-        const int u = u0 + lane;
-        int ns = 0, steps = 0;
-        Entry e{0, 0};
-        if (u < units) {
-            const int b = by_tiles(u);
-            e = entry_of(p, b);
-            if (unit_steps<ROWS, STEP>(p, e, u - b * p.tiles_max, steps)) ns = max(1, by_quantum(steps + quantum - 1));
-        }
-        int upto = ns * p.Hkv;
-        for (int i = 1; i < 64 && i < units; i *= 2) {
-            const int x = __shfl_up(upto, i);
-            if (lane >= i) upto += x;
-        }
+        const Unit at = u0 == 0 ? first : unit(u0 + lane);
+        const Entry e = at.e;
+        const int ns = at.steps < 0 ? 0 : max(1, by_quantum(at.steps + quantum - 1));
+        const int upto = wave_sums(ns * p.Hkv);
         const unsigned long long hit = __ballot(w >= base + upto - ns * p.Hkv && w < base + upto);
         if (hit) {
             const int src = __builtin_ctzll(hit);
