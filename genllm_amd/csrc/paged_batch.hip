@@ -521,10 +521,12 @@ BatchPlan plan_of(const BatchSizes& z) {
     r.tiles_max = (rows + r.rows - 1) / r.rows;
     r.tiles = r.tiles_max * z.batch * z.n_kv_heads;
     r.least = r.decode ? kDecodeLeast / z.head_dim : kPrefillLeast;
-    // a merge is worth it for contexts of more than two such splits; where the tiles alone
-    // keep the workgroups busy in turn, for tokens that are long beside the others
+    // a merge is worth it for contexts of more than two such splits, three of one tile (one
+    // token, 32 and 8 heads of 128, after 600: 9.2 us in one launch, 11.4 split; after 800:
+    // 10.6 and 10.7; after 2000: 13 and 11.8); where the tiles alone keep the workgroups busy
+    // in turn, for contexts that are long beside the others
     const int64_t turns = std::max<int64_t>(1, std::min<int64_t>(r.tiles / r.target, 1 << 20));
-    r.can_split = (z.max_pages + r.step - 1) / r.step > 2 * r.least * turns && (r.decode || r.tiles < r.target) && !fits;
+    r.can_split = (z.max_pages + r.step - 1) / r.step > (r.decode ? 3 : 2) * r.least * turns && (r.decode || r.tiles < r.target) && !fits;
     r.least = int(r.least * turns);
     // all workgroups there at once, two to a CU: a long one beside a short one
     r.paired = !r.decode && !r.can_split && prefill_resident(z.head_dim) == 2 && r.tiles > kCus && r.tiles <= 2 * kCus;
