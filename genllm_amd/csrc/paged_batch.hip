@@ -142,6 +142,7 @@ __global__ __launch_bounds__(kWaves * 64, resident(D)) void batch_decode_kernel(
     for (int db = 0; db < DB; ++db) acc[db] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, nm = 0.0f, th = -INFINITY;  // row maximum, its negative (0 while there is none), where it grows
     int vref = INT_MIN;
+    ScaleRange range;
     lds_char* const vt = (lds_char*)lds + wv * VLDS;
 
     const int k_off = n16 * p.k_tok + 16 * g;
@@ -298,6 +299,7 @@ __global__ __launch_bounds__(kWaves * 64, resident(D)) void batch_decode_kernel(
                 compute(s);
             }
         }
+        if constexpr (Q8) range.add(info);
     }
 
     float l = accl[0];
@@ -307,11 +309,12 @@ __global__ __launch_bounds__(kWaves * 64, resident(D)) void batch_decode_kernel(
         for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum += acc[db][i];
-        if (__any(n16 < rows && !(fabsf(sum) <= __FLT_MAX__))) {
-            exact_keys<D, F16, Q8>(p, w.b, w.h, p.q + row_at(p.q_batch, p.q_tok, p.q_head), sight_of(p, w.e, query), [&](int i) {
-                const int j = kStep * (s0 + wv + kWaves * (i >> 1)) + (i & 1);
-                return (i >> 1) < mine && j < span.pages ? span.page(j) : -1;
-            }, acc, m, l);
+        const auto page_of = [&](int i) {
+            const int j = kStep * (s0 + wv + kWaves * (i >> 1)) + (i & 1);
+            return (i >> 1) < mine && j < span.pages ? span.page(j) : -1;
+        };
+        if (__any(n16 < rows && !(fabsf(sum) <= __FLT_MAX__)) || (Q8 && range.left<D>(p, w.b, w.h, vref, page_of))) {
+            exact_keys<D, F16, Q8>(p, w.b, w.h, p.q + row_at(p.q_batch, p.q_tok, p.q_head), sight_of(p, w.e, query), page_of, acc, m, l);
         } else if (Q8 && vref != INT_MIN) {
 #pragma unroll
             for (int db = 0; db < DB; ++db)

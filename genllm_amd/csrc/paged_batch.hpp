@@ -248,7 +248,7 @@ __device__ __forceinline__ void put_header(const BatchAttn& p, const Work& w) {
 // before they are needed: they arrive with the page's rows, not ahead of them.
 struct PageInfo {
     int kid = -1, vid = -1;  // block ids; -1, -1: no page; -1, -2: an id that is none
-    int kb = 127, vb = 127;  // bytes of the scales
+    int kb = 127, vb = 0;    // bytes of the scales; no page: the least, which raises no reference
 };
 template <bool Q8>
 __device__ __forceinline__ PageInfo page_info(const BatchAttn& p, int b, int h, int page, bool there) {
@@ -288,6 +288,39 @@ template <bool F16>
 __device__ __forceinline__ uint4 f8_octet(uint32_t w0, uint32_t w1, float s0, float s1) {
     return make_uint4(f8_pair<F16, false>(w0, s0), f8_pair<F16, true>(w0, s0), f8_pair<F16, false>(w1, s1), f8_pair<F16, true>(w1, s1));
 }
+
+// V's pages are taken relative to a reference scale 2^ref, at least a 64th of the largest so
+// far.  That is exact for a page at most 15 binades below it: a code's last bit, 2^-9, is
+// fp16's, 2^-24.  Where there are lower ones, or sums might leave fp32's range, rows are
+// computed by exact_keys in the end: the scale of another page, of keys that a row may not
+// even see, costs no row its precision.  Pages of zeros alone, which have the least scale, do
+// not count.  low: a lane's least; next(i): the i-th page, -1 behind the last.
+constexpr int kScaleReach = 15, kMostScale = 90;
+struct ScaleRange {
+    int low = 1 << 20;
+    __device__ __forceinline__ void add(const PageInfo& info) { low = info.kid >= 0 ? min(low, info.vb - 127) : low; }
+    template <int D, class Next>
+    __device__ __forceinline__ bool left(const BatchAttn& p, int b, int h, int ref, const Next& next) const {
+        if (ref == INT_MIN) return false;
+        if (ref > kMostScale) return true;
+        if (!__any(low < ref - kScaleReach)) return false;
+        const int lane = threadIdx.x & 63;
+        for (int i = 0;; ++i) {
+            const int page = next(i);
+            if (page < 0) return false;
+            const PageInfo info = page_info<true>(p, b, h, page, true);
+            if (info.kid < 0 || info.vb - 127 >= ref - kScaleReach) continue;
+            if (info.vb - 127 > -100) return true;
+            uint32_t any = 0;
+            const char* const row = p.v_pool + info.vid * p.v_block + int64_t(h) * p.v_head + int64_t(lane >> 2) * p.v_tok;
+            for (int d = 16 * (lane & 3); d < D; d += 64) {
+                const uint4 u = *reinterpret_cast<const uint4*>(row + d);
+                any |= u.x | u.y | u.z | u.w;
+            }
+            if (__any((any & 0x7f7f7f7f) != 0)) return true;
+        }
+    }
+};
 
 // One key after another, in fp32, each row with only the keys it sees: what a wave runs
 // again whose tiles came out NaN or infinite.  (In the tiles a key that a row does not

@@ -113,6 +113,7 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
         m[rb] = -INFINITY, nm[rb] = 0.0f, th[rb] = -INFINITY;
     }
     int vref = INT_MIN, vacc = INT_MIN;  // reference scale of the staged step, and of acc
+    ScaleRange range;
 
     // ---- staging: lane i of every wave knows page i of 16 steps
     constexpr int kBlock = 64 / kPrefillStep;
@@ -159,7 +160,10 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
     const auto stage = [&](int step, lds_char* kl, lds_char* vl) {
         const int at = kPrefillStep * ((step - s0) % kBlock);
         float vs = 1.0f;
-        if (at == 0) info_kf = score_factor<Q8>(p, info.vid, info.kb, info.vb);
+        if (at == 0) {
+            info_kf = score_factor<Q8>(p, info.vid, info.kb, info.vb);
+            if constexpr (Q8) range.add(info);
+        }
 #pragma unroll
         for (int i = 0; i < NP; ++i) kf_next[i] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(info_kf), at + p0 + i));
         if constexpr (Q8) {
@@ -359,6 +363,11 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
         if (t + 1 < s1) turn(t + 1, (lds_char*)lds_k1, (lds_char*)lds_v1, (lds_char*)lds_k0, (lds_char*)lds_v0);
     }
 
+    const auto page_of = [&](int i) {
+        const int j = kPrefillStep * (s0 + i / NP) + p0 + i % NP;
+        return j < kPrefillStep * s1 && j < span.pages ? span.page(j) : -1;
+    };
+    const bool left = Q8 && range.left<D>(p, w.b, w.h, vref, page_of);
     float ls[RB];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
@@ -369,11 +378,8 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
         for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum += acc[rb][db][i];
-        if (__any(row < rows && !(fabsf(sum) <= __FLT_MAX__))) {
-            exact_keys<D, F16, Q8>(p, w.b, w.h, p.q + row_at(rb, p.q_batch, p.q_tok, p.q_head), sight_of(p, w.e, query[rb]), [&](int i) {
-                const int j = kPrefillStep * (s0 + i / NP) + p0 + i % NP;
-                return j < kPrefillStep * s1 && j < span.pages ? span.page(j) : -1;
-            }, acc[rb], m[rb], l);
+        if (__any(row < rows && !(fabsf(sum) <= __FLT_MAX__)) || left) {
+            exact_keys<D, F16, Q8>(p, w.b, w.h, p.q + row_at(rb, p.q_batch, p.q_tok, p.q_head), sight_of(p, w.e, query[rb]), page_of, acc[rb], m[rb], l);
         } else if (Q8 && vacc != INT_MIN) {
 #pragma unroll
             for (int db = 0; db < DB; ++db)

@@ -228,6 +228,59 @@ def test_scales_far_apart(S):
     c.check("scales")
 
 
+def scaled(c, exponents):
+    """V's pages, in the order of each entry's table, with these exponents in turn."""
+    for ids in c.ids[1]:
+        e = torch.tensor([exponents[i % len(exponents)] for i in range(len(ids))], dtype=torch.int32)
+        c.scales[1][ids.long().cuda()] = (e + 127).to(torch.uint8)[:, None].expand(-1, c.H).cuda()
+
+
+@pytest.mark.parametrize("e", [-90, -40, 25, 100])
+@pytest.mark.parametrize("S", [1, 7, 40, 130])
+def test_one_scale(S, e):
+    """Values of any one size, also where a step has fewer pages than it takes."""
+    c = Case(8, 2, 128, BF, True, [S, S + 17, 900, S + 40], S)
+    scaled(c, [e])
+    c.run()
+    c.check("one scale")
+
+
+@pytest.mark.parametrize("exponents", [(-60, -20, 20, 60), (60, 20, -20, -60), (-30, -30, 0), (0, -14, -30), (-9, 6)])
+@pytest.mark.parametrize("S", [1, 3, 33, 150])
+def test_scales_of_unseen_pages(S, exponents):
+    """A query's result has its own keys' precision, whatever the pages behind it hold (bf16: 2^60 is no fp16 value)."""
+    c = Case(4, 2, 128, BF, True, [S, S + 20, 400], S)
+    scaled(c, exponents)
+    c.run()
+    c.check("unseen scales")
+
+
+@pytest.mark.parametrize("S", [1, 3, 33, 150])
+def test_pages_of_zeros(S):
+    """Pages of zeros, which have the least scale, among others."""
+    c = Case(4, 2, 128, BF, True, [S, S + 20, 400], S)
+    for ids in c.ids[1]:
+        at = ids.long().cuda()[::2]
+        c.pools[1].view(torch.uint8)[at] = 0
+        c.scales[1][at] = 27
+    c.run()
+    c.check("zeros")
+
+
+@pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** -12])
+@pytest.mark.parametrize("S", [1, 3, 33, 150])
+def test_small_elements(S, size):
+    """fp16's subnormal values, as keys, values and queries."""
+    c = Case(4, 2, 128, HF, False, [S, S + 20, 400], S)
+    for pool in c.pools:
+        pool.mul_(size)
+    c.run()
+    c.check("small")
+    c.q.mul_(size)
+    c.run()
+    c.check("small q")
+
+
 @pytest.mark.parametrize("f8", [True, False])
 def test_many_entries(f8):
     """More entries than a wave has lanes, most of them empty, one long."""
