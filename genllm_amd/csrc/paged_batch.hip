@@ -570,7 +570,7 @@ extern "C" int genllm_paged_attention_batch(
     if (n_blocks == 0 && !z.empty()) return refuse(GENLLM_ERR_INVALID, "a pool without blocks");
     if (head_dim != 64 && head_dim != 128 && head_dim != 256) return refuse(GENLLM_ERR_UNSUPPORTED, "head_dim 64, 128 or 256");
     if (dtype != GENLLM_DTYPE_BF16 && dtype != GENLLM_DTYPE_F16) return refuse(GENLLM_ERR_UNSUPPORTED, "bf16 or fp16 elements");
-    if (!(scale >= 0.0f) || !std::isfinite(scale)) return refuse(GENLLM_ERR_INVALID, "the scale must be finite and not negative");
+    if (!(scale >= 0.0f) || !std::isfinite(scale * kLog2e)) return refuse(GENLLM_ERR_INVALID, "the scale must be finite and not negative");
     if (window < 0 || sinks < 0) return refuse(GENLLM_ERR_INVALID, "negative window or sinks");
     if (window > 0 && !causal) return refuse(GENLLM_ERR_INVALID, "a window goes with causal attention");
     if ((k_scales != nullptr) != (v_scales != nullptr)) return refuse(GENLLM_ERR_INVALID, "k_scales and v_scales go together");

@@ -72,7 +72,7 @@ def test_gather_refuses_what_it_would_write_over(kw, msg):
     *[({x: None}, INV, b"null pointer") for x in ("q", "out", "kp", "vp", "ki", "vi", "nc")],
     *[({x: -1}, INV, b"negative") for x in ("B", "S", "n", "P", "window", "sinks")], (dict(H=-2), INV, b"negative"),
     (dict(D=192), UNS, b"64, 128 or 256"), (dict(dtype=2), UNS, b"bf16 or fp16"), (dict(Hq=7), INV, b"multiple of n_kv_heads"),
-    (dict(H=0), INV, b"multiple of n_kv_heads"), (dict(scale=NAN), INV, b"finite"), (dict(scale=INF), INV, b"finite"),
+    (dict(H=0), INV, b"multiple of n_kv_heads"), (dict(scale=NAN), INV, b"finite"), (dict(scale=INF), INV, b"finite"), (dict(scale=3e38), INV, b"finite"),
     (dict(scale=-0.1), INV, b"not negative"), (dict(window=4, causal=0), INV, b"causal"), (dict(ks=5 * GB), INV, b"go together"),
     (dict(vs=5 * GB), INV, b"go together"), (dict(P=(1 << 26) + 1), INV, b"2^26"), (dict(S=1 << 29), INV, b"2^30"),
     (dict(q=GB + 8), INV, b"16-byte aligned"), (dict(out=2 * GB + 4), INV, b"16-byte aligned"), (dict(qt=1028), INV, b"16-byte aligned"),

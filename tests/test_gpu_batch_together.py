@@ -114,6 +114,47 @@ def test_captured(S):
         at = now if turn < 2 else [a - 3 for a in now]  # drafts taken back
 
 
+@pytest.mark.parametrize("S", [1, 40])
+def test_captured_splits(S):
+    """Contexts that are split over workgroups: two graphs with a workspace in common, replayed in order while lengths
+    change, eager calls in that workspace between them."""
+    g = torch.Generator().manual_seed(S)
+    pages, n = 120, [1900, 300]
+    pools = [torch.randn(2 * pages, PAGE, H, D, generator=g).to(BF) for _ in "kv"]
+    ids = torch.randperm(2 * pages, generator=g).view(2, pages).int()
+    dev, dev_ids = [x.cuda() for x in pools], ids.cuda()
+    q = torch.randn(2, S, HQ, D, generator=g).to(BF)
+    dev_q = q.cuda()
+    need = paged.paged_attention_batch_workspace_bytes(2, S, HQ, H, D, pages)
+    assert need > 0
+    room = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    lens, outs = ints(n), [torch.zeros_like(dev_q) for _ in range(3)]
+    how = [dict(), dict(window=700, sinks=5)]
+
+    def run(out, **kw):
+        paged.paged_attention_batch(dev_q, out, *dev, dev_ids, dev_ids, lens, SCALE, workspace=room, **kw)
+
+    run(outs[0])
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in how]
+    for graph, out, kw in zip(graphs, outs, how):
+        with torch.cuda.graph(graph):
+            run(out, **kw)
+    for turn, n in enumerate([n, [S, 1920], [1000, 0], [1920, 1919]]):
+        lens.copy_(ints(n))
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for out, kw in zip(outs, how):
+            outs[2].zero_()
+            run(outs[2], **kw)
+            torch.cuda.synchronize()
+            assert torch.equal(out, outs[2]), f"replay {turn}"
+            for b in range(2):
+                k, v = (x[ids[b].long()].reshape(-1, H, D)[: n[b]].double() for x in pools)
+                assert_attended(out[b], *attend(q[b], k, v, n[b] - S, SCALE, **kw), max(1, n[b]), 2.0 ** -8, f"replay {turn} entry {b}")
+
+
 def test_streams():
     """Two streams at once, each with workspaces of its own; streams given as objects and as handles."""
     s = Server(9)
