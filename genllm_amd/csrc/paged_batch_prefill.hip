@@ -1,11 +1,15 @@
 // paged_batch_prefill.hip -- attention of a padded batch over paged caches, for more than
 // 16 rows per kv head: prompts, chunks on top of a cache, drafts of many heads.
 //
-// Rows are the (query, q head) pairs of a kv head, q heads fastest, in tiles of 64 or 128;
-// wave w of four has 16 or 32 of them, as columns of the MFMA tiles (RB blocks of 16), and
-// all keys of a step: four pages, 64 keys.  Wave w stages page w of the next step: 16-byte
-// loads into registers while this step is computed, then to LDS as 16-bit rows whose
-// 16-byte chunks are swizzled.  8-bit codes are converted once here, for all waves: K's to
+// Rows are the (query, q head) pairs of a kv head, q heads fastest; a step is four pages, 64
+// keys.  Two forms:
+//   tiles of 128 rows, four waves of 32 (RB = 2 blocks of 16) that take all keys of a step:
+//     an operand read from LDS feeds two MFMAs, as long as its read takes the four waves;
+//   tiles of 64 rows, eight waves of 16 in two groups (KG = 2) with half of a step's keys
+//     each, joined through LDS in the end: more waves for few rows (the rule is plan_of's).
+// Waves stage the pages of the next step: 16-byte loads into registers while this step is
+// computed, then to LDS as 16-bit rows, two buffers, one barrier a step.  K's 16-byte chunks
+// are swizzled, V's rows padded.  8-bit codes are converted once here, for all waves: K's to
 // q's type (without loss; the page's scale is in the factor of the scores), V's to fp16
 // relative to a reference scale that follows the largest, so that P is rounded to fp16 (11
 // bits) whatever q's type is.  From 16-bit pages P has the elements' type.  Per step:
@@ -13,7 +17,14 @@
 //   O^T += V^T P^T  with V^T by transposing LDS reads; the sum of a row's probabilities
 //        by one more MFMA with ones, from the same rounded values
 // Lane (row, g) has the scores of keys 4g..4g+3 of each page: the running maximum and the
-// rescaling stay in the lane.  Two LDS buffers, one barrier a step.
+// rescaling stay in the lane.
+//
+// Bound by a wave's chain where two waves share a SIMD: of a step's 4,400 cycles for both
+// (D = 128, 8-bit) the matrix core is busy in 2,180, vector instructions and exponentials
+// take about as many and overlap it in part.  2 x 512 queries on 8192 tokens, 32 and 8 heads
+// of 128: 148 us, 900 TFLOP/s (a large library product reaches 1,184); 8192 tokens, 16 and 8
+// heads, causal: 268 us.  Also tried: staging between the MFMAs of P V (no gain), loads two
+// steps ahead (none), Q and the output through LDS as whole rows (2 % slower).
 #include <type_traits>
 
 #include "paged_batch.hpp"
@@ -50,7 +61,7 @@ __device__ __forceinline__ int k_place(int r, int c) {
 // two neighbouring chunks) cover all banks once, and the chunks of a row lie at fixed
 // distances: one address for all of them.
 template <int D>
-constexpr int kVRow = D == 64 ? 2 * D + 32 : 2 * D + 32;
+constexpr int kVRow = 2 * D + 32;
 template <int D>
 constexpr int kVPage = kPage * kVRow<D> + 128;
 template <int D>

@@ -9,7 +9,11 @@
 // whether its tokens came at once or one by one, but for such.
 //
 // One wave per (K or V, page, head): lane l has token l / 4 and, of each 64 dims, 16 from
-// 16 (l % 4) on: two 16-byte loads to one 16-byte store.  Bound by memory.
+// 16 (l % 4) on: two 16-byte loads to one 16-byte store, 64 bytes of a row together.
+//
+// Bound by memory where there are many rows, else by the launch (8 heads of 128: 8192 tokens
+// read back in 11.0 us, 91 % of a large copy's rate; 2048 written in 4.5 us, and one token of
+// each of 64 entries in 4.4, of which the launch is 4.3).
 #include <algorithm>
 #include <climits>
 #include <string>
