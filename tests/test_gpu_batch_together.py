@@ -176,6 +176,33 @@ def test_streams():
         s.check(q, outs[i], lens, [q.shape[1]] * B, f"call {i}")
 
 
+def test_streams_that_split():
+    """Split contexts on two streams at once, the workspaces taken for each call: a stream as an object, as a handle, and
+    the current one."""
+    g = torch.Generator().manual_seed(5)
+    pages, n = 100, [1600, 900]
+    pools = [torch.randn(2 * pages, PAGE, H, D, generator=g).to(BF) for _ in "kv"]
+    ids = torch.randperm(2 * pages, generator=g).view(2, pages).int()
+    dev, dev_ids, lens = [x.cuda() for x in pools], ids.cuda(), ints(n)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    qs = [torch.randn(2, S, HQ, D, generator=g).to(BF) for S in (1, 30, 1, 30, 1, 30)]
+    dev_q = [q.cuda() for q in qs]
+    outs = [torch.zeros_like(q) for q in dev_q]
+    for q in qs:
+        assert paged.paged_attention_batch_workspace_bytes(2, q.shape[1], HQ, H, D, pages) > 0
+    torch.cuda.synchronize()
+    for i, (q, out) in enumerate(zip(dev_q, outs)):
+        on = [streams[i % 2], streams[i % 2].cuda_stream, None][i // 2]
+        with torch.cuda.stream(streams[i % 2] if on is None else torch.cuda.current_stream()):
+            paged.paged_attention_batch(q, out, *dev, dev_ids, dev_ids, lens, SCALE, stream=on)
+    torch.cuda.synchronize()
+    for i, q in enumerate(qs):
+        for b in range(2):
+            k, v = (x[ids[b].long()].reshape(-1, H, D)[: n[b]].double() for x in pools)
+            step = 2.0 ** -16 if q.shape[1] == 1 else 2.0 ** -8
+            assert_attended(outs[i][b], *attend(q[b], k, v, n[b] - q.shape[1], SCALE), n[b], step, f"call {i} entry {b}")
+
+
 def test_managed_pools():
     """The pages of a PagedAttentionManager's layer, attended as a batch of one: the op's own result but for its rounding."""
     mgr = paged.PagedAttentionManager(8 << 20)
