@@ -537,10 +537,12 @@ BatchPlan plan_of(const BatchSizes& z) {
     r.least = r.decode ? kDecodeLeast / z.head_dim : kPrefillLeast;
     // a merge is worth it for contexts of more than two such splits, three of one tile (one
     // token, 32 and 8 heads of 128, after 600: 9.2 us in one launch, 11.4 split; after 800:
-    // 10.6 and 10.7; after 2000: 13 and 11.8); where the tiles alone keep the workgroups busy
-    // in turn, for contexts that are long beside the others
+    // 10.6 and 10.7; after 2000: 13 and 11.8).  Where the tiles alone keep the workgroups busy
+    // in turn, only for contexts that are long beside the others: every workgroup looks through
+    // all units to find its own (one token each, ragged, unsplit and split: 1024 entries of up
+    // to 2048 tokens, 8 and 2 heads, 90 and 136 us; 256 of up to 4096, 32 and 8, 173 and 180)
     const int64_t turns = std::max<int64_t>(1, std::min<int64_t>(r.tiles / r.target, 1 << 20));
-    r.can_split = (z.max_pages + r.step - 1) / r.step > (r.decode ? 3 : 2) * r.least * turns && (r.decode || r.tiles < r.target) && !fits;
+    r.can_split = (z.max_pages + r.step - 1) / r.step > (!r.decode ? 2 : turns > 1 ? 12 : 3) * r.least * turns && (r.decode || r.tiles < r.target) && !fits;
     r.least = int(r.least * turns);
     // all workgroups there at once, two to a CU: a long one beside a short one
     r.paired = !r.decode && !r.can_split && prefill_resident(z.head_dim) == 2 && r.tiles > kCus && r.tiles <= 2 * kCus;

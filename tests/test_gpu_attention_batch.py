@@ -291,6 +291,19 @@ def test_many_entries(f8):
     c.check("many")
 
 
+@pytest.mark.parametrize("pages", [12, 400])
+def test_more_entries_than_workgroups(pages):
+    """Enough entries for several turns of the workgroups there are, with short tables and with long ones."""
+    n = [(i * 37) % 90 for i in range(1100)]
+    n[3], n[1050] = 16 * pages, 16 * pages - 5
+    c = Case(4, 2, 128, BF, True, [1] * 1100, 1, P=1)
+    blocks = c.scales[0].shape[0]
+    g = torch.Generator().manual_seed(pages)
+    c.n, c.ids = n, [torch.randint(0, blocks, (1100, pages), generator=g).int() for _ in "kv"]
+    c.run()
+    c.check("more entries")
+
+
 @pytest.mark.parametrize("S", [1, 30])
 def test_more_tokens_than_the_table(S):
     """n_cached past the table: the table's tokens alone, the last query at their end."""
