@@ -41,15 +41,9 @@ namespace genllm {
 
 namespace {
 
-constexpr int kRows = 16;   // rows of a decode tile
+constexpr int kRows = kDecodeRows;
 constexpr int kStep = kDecodeStep;
 constexpr int kWaves = 4;
-constexpr int kCus = 256;
-// steps of a split at least, times head_dim (8192 tokens, 32 and 8 heads of 128: 12.4 us with
-// 8 steps, 13.2 with 12, 13.9 with 16)
-constexpr int kDecodeLeast = 1024;
-constexpr int kPrefillLeast = 4;
-constexpr int prefill_resident(int D) { return D == 256 ? 1 : 2; }
 constexpr float kLazy = 8.0f;      // log2: a row's maximum may lag its scores by this much
 constexpr int kScaleLead = 6;      // a page's scale may be this many binades above the reference
 constexpr int kNonTemporal = 2;
@@ -88,9 +82,6 @@ struct Step {
     int at;  // the lane that knows the first page
 };
 
-// Workgroups that a CU holds.  Each is four waves, one on a SIMD: 512 registers over them.
-// Three at D = 128 in place of two: 32 windows of 1024 tokens, 16-bit, 50.5 -> 34 us.
-constexpr int resident(int D) { return D == 64 ? 4 : D == 128 ? 3 : 2; }
 // The next step's loads in flight beside this one's, where that leaves the registers for
 // the workgroups above.
 template <int D, bool Q8>
@@ -499,62 +490,6 @@ int launch_batch_decode(const BatchAttn& p, int D, bool f16, hipStream_t stream)
     return f16 ? p.k_scales ? decode_of<true, true>(p, D, stream) : decode_of<true, false>(p, D, stream)
                : p.k_scales ? decode_of<false, true>(p, D, stream) : decode_of<false, false>(p, D, stream);
 }
-
-namespace {
-
-// The sizes of a call: which kernel, how its work is divided at most.
-struct BatchSizes {
-    int32_t batch, seq_len, n_q_heads, n_kv_heads, head_dim, max_pages;
-    bool empty() const { return batch <= 0 || seq_len <= 0 || n_q_heads <= 0 || n_kv_heads <= 0; }
-    const char* refused() const {
-        if (batch < 0 || seq_len < 0 || n_q_heads < 0 || n_kv_heads < 0 || max_pages < 0) return "negative size";
-        if (n_kv_heads == 0 ? n_q_heads != 0 : n_q_heads % n_kv_heads != 0) return "n_q_heads must be a multiple of n_kv_heads";
-        if (max_pages > 1 << 26) return "tables of up to 2^26 pages";
-        if (int64_t(seq_len) * (n_kv_heads ? n_q_heads / n_kv_heads : 1) > 1 << 30) return "up to 2^30 rows for a kv head";
-        return nullptr;
-    }
-};
-
-// Decode rows: one 16-row tile.  More rows: tiles of 64 or 128.
-BatchPlan plan_of(const BatchSizes& z) {
-    BatchPlan r;
-    const int64_t rows = int64_t(z.seq_len) * (z.n_q_heads / z.n_kv_heads);
-    r.decode = rows <= kRows;
-    r.target = kCus * (r.decode ? resident(z.head_dim) : prefill_resident(z.head_dim));
-    // Prompts over little more than their own rows whose tiles of 64 are all there at once and
-    // leave few places: eight waves to each, a long tile beside a short one, no split (16 q and
-    // 8 kv heads of 128, 2048 tokens: 44 us, with tiles of 128 in splits 49.5; 1800: 37.4 and
-    // 44.4).  Not for short ones (4 x 512: 21.9 and 20.0), nor for chunks on a long context,
-    // which splits divide evenly (2048 on 8192: 182 and 150), nor at head_dim 256, one workgroup
-    // to a CU (8 and 2 heads, 2048 tokens: 56 and 52).
-    const int64_t fine = (rows + 63) / 64 * z.batch * z.n_kv_heads;
-    const bool fits = !r.decode && rows > 64 && z.head_dim <= 128 && z.seq_len >= 1024 && int64_t(z.max_pages) * kPage < 2 * int64_t(z.seq_len) && fine <= r.target &&
-                      fine >= r.target / 4 * 3;
-    r.rows = r.decode ? kRows : rows <= 64 || fits ? 64 : 128;
-    r.step = r.decode ? kStep : kPrefillStep;
-    r.tiles_max = (rows + r.rows - 1) / r.rows;
-    r.tiles = r.tiles_max * z.batch * z.n_kv_heads;
-    r.least = r.decode ? kDecodeLeast / z.head_dim : kPrefillLeast;
-    // a merge is worth it for contexts of more than two such splits, three of one tile (one
-    // token, 32 and 8 heads of 128, after 600: 9.2 us in one launch, 11.4 split; after 800:
-    // 10.6 and 10.7; after 2000: 13 and 11.8).  Where the tiles alone keep the workgroups busy
-    // in turn, only for contexts that are long beside the others: every workgroup looks through
-    // all units to find its own (one token each, ragged, unsplit and split: 1024 entries of up
-    // to 2048 tokens, 8 and 2 heads, 90 and 136 us; 256 of up to 4096, 32 and 8, 173 and 180)
-    const int64_t turns = std::max<int64_t>(1, std::min<int64_t>(r.tiles / r.target, 1 << 20));
-    r.can_split = (z.max_pages + r.step - 1) / r.step > (!r.decode ? 2 : turns > 1 ? 12 : 3) * r.least * turns && (r.decode || r.tiles < r.target) && !fits;
-    r.least = int(r.least * turns);
-    // all workgroups there at once, two to a CU: a long one beside a short one
-    r.paired = !r.decode && !r.can_split && prefill_resident(z.head_dim) == 2 && r.tiles > kCus && r.tiles <= 2 * kCus;
-    r.slots = r.tiles + (r.can_split ? r.target + 8 : 0);
-    return r;
-}
-size_t workspace_of(const BatchPlan& r, int batch, int D) {
-    return r.can_split ? size_t(r.slots) * r.rows * (D + 2) * 4 + (size_t(batch) * r.tiles_max * sizeof(Header) + 15 & ~size_t(15)) : 0;
-}
-constexpr int64_t kMostWorkgroups = INT_MAX / 512;  // of 512 threads, in a launch of fewer than 2^32; a merge has up to 16 of 64 for each
-
-}  // namespace
 
 }  // namespace genllm
 
