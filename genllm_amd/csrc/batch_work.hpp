@@ -174,9 +174,9 @@ __device__ __forceinline__ bool find_work(const BatchAttn& p, int w, Work& r) {
     const Unit first = unit(lane);
     int64_t mine = max(first.steps, 0);
     for (int u = lane + 64; u < units; u += 64) mine += max(unit(u).steps, 0);
-    // of at most 2^48 in a lane, exact
+    // in halves: with few rows one unit alone has up to 2^25 steps, a lane's share of the units up to 2^41
     const double sum = double(__builtin_amdgcn_readlane(wave_sums(int(mine & 0xffffff)), 63)) +
-                       (units > 64 ? double(__builtin_amdgcn_readlane(wave_sums(int(mine >> 24)), 63)) * (1 << 24) : 0.0);
+                       double(__builtin_amdgcn_readlane(wave_sums(int(mine >> 24)), 63)) * (1 << 24);
     const double share = ceil(sum * p.Hkv * (1.0 / p.target));  // every workgroup's the same, whatever the last bit is
     int quantum = max(p.least, __builtin_amdgcn_readfirstlane(int(fmin(share, double(1 << 28)))));
     // pieces that are no whole quantum may leave a few workgroups more than the target,

@@ -273,3 +273,9 @@ pytestmark = pytest.mark.skipif(shutil.which("g++") is None, reason="g++ builds 
 
 def test_batches(program):
     run(program, "batches")
+
+
+def test_tables_of_many_pages(program):
+    """Contexts up to the 2^30 tokens that a table holds: the sum of the steps keeps all its bits, so that the pieces
+    stay in the workspace."""
+    run(program, "long")
