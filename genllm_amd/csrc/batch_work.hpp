@@ -265,6 +265,9 @@ struct BatchSizes {
 inline BatchPlan plan_of(const BatchSizes& z) {
     BatchPlan r;
     const int64_t rows = int64_t(z.seq_len) * (z.n_q_heads / z.n_kv_heads);
+    // no more than 2^31, so that 2^30 rows of each make no product of more than 64 bits: above
+    // kMostWorkgroups the call is refused
+    const int64_t heads = std::min<int64_t>(int64_t(z.batch) * z.n_kv_heads, int64_t(1) << 31);
     r.decode = rows <= kDecodeRows;
     r.target = kCus * (r.decode ? resident(z.head_dim) : prefill_resident(z.head_dim));
     // Prompts over little more than their own rows whose tiles of 64 are all there at once and
@@ -273,13 +276,13 @@ inline BatchPlan plan_of(const BatchSizes& z) {
     // 44.4).  Not for short ones (4 x 512: 21.9 and 20.0), nor for chunks on a long context,
     // which splits divide evenly (2048 on 8192: 182 and 150), nor at head_dim 256, one workgroup
     // to a CU (8 and 2 heads, 2048 tokens: 56 and 52).
-    const int64_t fine = (rows + 63) / 64 * z.batch * z.n_kv_heads;
+    const int64_t fine = (rows + 63) / 64 * heads;
     const bool fits = !r.decode && rows > 64 && z.head_dim <= 128 && z.seq_len >= 1024 && int64_t(z.max_pages) * kPage < 2 * int64_t(z.seq_len) && fine <= r.target &&
                       fine >= r.target / 4 * 3;
     r.rows = r.decode ? kDecodeRows : rows <= 64 || fits ? 64 : 128;
     r.step = r.decode ? kDecodeStep : kPrefillStep;
     r.tiles_max = (rows + r.rows - 1) / r.rows;
-    r.tiles = r.tiles_max * z.batch * z.n_kv_heads;
+    r.tiles = r.tiles_max * heads;
     r.least = r.decode ? kDecodeLeast / z.head_dim : kPrefillLeast;
     // a merge is worth it for contexts of more than two such splits, three of one tile (one
     // token, 32 and 8 heads of 128, after 600: 9.2 us in one launch, 11.4 split; after 800:

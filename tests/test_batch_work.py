@@ -263,6 +263,12 @@ def program(tmp_path_factory):
     return str(at / "work")
 
 
+def workspace(*sizes):
+    from genllm_amd import _lib
+
+    return _lib.lib().genllm_paged_attention_batch_workspace_bytes(*sizes)
+
+
 def run(program, what):
     r = subprocess.run([program, what], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and r.stdout.endswith("as counted\n"), (r.returncode, r.stdout[-2000:], r.stderr[-500:])
@@ -279,3 +285,20 @@ def test_tables_of_many_pages(program):
     """Contexts up to the 2^30 tokens that a table holds: the sum of the steps keeps all its bits, so that the pieces
     stay in the workspace."""
     run(program, "long")
+
+
+@pytest.mark.parametrize("Hq,H", [(2 ** 31 - 1, 2 ** 31 - 1), (2 ** 30, 2 ** 30), (2 ** 31 - 2, 2 ** 30 - 1)])
+@pytest.mark.parametrize("B,S", [(2 ** 31 - 1, 300), (2 ** 31 - 1, 5), (2 ** 31 - 1, 1), (2 ** 30, 33), (2 ** 24, 2 ** 20)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("P", [0, 100, 1 << 26])
+def test_more_tiles_than_64_bits_count(B, S, Hq, H, D, P):
+    """Sizes whose product leaves 64 bits are refused like others of more rows than a launch takes: no workspace."""
+    assert workspace(B, S, Hq, H, D, P) == 0
+
+
+def test_attention_refuses_more_tiles_than_64_bits_count():
+    from test_batch_refusals import attend, refused, INV
+
+    big = 2 ** 31 - 1
+    for B, S in ((big, 300), (big, 1), (2 ** 30, 300)):
+        refused(attend(B=B, S=S, Hq=big, H=big, qb=0, ob=0, kis=0, vis=0, kph=0, vph=0), INV, b"one launch")
