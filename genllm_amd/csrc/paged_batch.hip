@@ -44,7 +44,6 @@ namespace {
 constexpr int kRows = kDecodeRows;
 constexpr int kStep = kDecodeStep;
 constexpr int kWaves = 4;
-constexpr float kLazy = 8.0f;      // log2: a row's maximum may lag its scores by this much
 constexpr int kScaleLead = 6;      // a page's scale may be this many binades above the reference
 constexpr int kNonTemporal = 2;
 
@@ -308,12 +307,12 @@ __global__ __launch_bounds__(kWaves * 64, resident(D)) void batch_decode_kernel(
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum += acc[db][i];
+            for (int i = 0; i < 4; ++i) sum += fabsf(acc[db][i]);
         const auto page_of = [&](int i) {
             const int j = kStep * (s0 + wv + kWaves * (i >> 1)) + (i & 1);
             return (i >> 1) < mine && j < span.pages ? span.page(j) : -1;
         };
-        if (__any(n16 < rows && !(fabsf(sum) <= __FLT_MAX__)) || (Q8 && range.left<D>(p, w.b, w.h, vref, page_of))) {
+        if (__any(n16 < rows && !(sum <= kMostSum)) || (Q8 && range.left<D>(p, w.b, w.h, vref, page_of))) {
             exact_keys<D, F16, Q8>(p, w.b, w.h, p.q + row_at(p.q_batch, p.q_tok, p.q_head), sight_of(p, w.e, query), page_of, acc, m, l);
         } else if (Q8 && vref != INT_MIN) {
 #pragma unroll

@@ -86,7 +86,14 @@ __device__ __forceinline__ uint4 f8_octet(uint32_t w0, uint32_t w1, float s0, fl
 // computed by exact_keys in the end: the scale of another page, of keys that a row may not
 // even see, costs no row its precision.  Pages of zeros alone, which have the least scale, do
 // not count.  low: a lane's least; next(i): the i-th page, -1 behind the last.
-constexpr int kScaleReach = 15, kMostScale = 90;
+constexpr int kScaleReach = 15, kMostScale = 64;
+
+// A row's maximum may lag its scores by kLazy (log2), so a wave's sums may be 2^kLazy times
+// those of probabilities of at most one.  Where all waves and splits (at most 2^13) might not add up
+// within fp32's range, exact_keys takes its keys, with probabilities of at most one: sums of
+// products above kMostSum, and 8-bit pages whose reference is above kMostScale (2^15 of a
+// code and its lead, 2^8, 2^30 keys: sums of up to 2^(53 + 64)).
+constexpr float kLazy = 8.0f, kMostSum = 0x1p100f;
 struct ScaleRange {
     int low = 1 << 20;
     __device__ __forceinline__ void add(const PageInfo& info) { low = info.kid >= 0 ? min(low, info.vb - 127) : low; }

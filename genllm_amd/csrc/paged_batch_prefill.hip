@@ -33,7 +33,6 @@ namespace genllm {
 
 namespace {
 
-constexpr float kLazy = 8.0f;  // log2: a row's maximum may lag its scores by this much
 constexpr int kScaleLead = 6;  // a page's scale may be this many binades above the reference
 // The two waves of a SIMD: one whose MFMA waits for the matrix core keeps the other's vector
 // instructions from being issued, unless those come first (8192 tokens, 16 and 8 heads of 128:
@@ -388,8 +387,8 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum += acc[rb][db][i];
-        if (__any(row < rows && !(fabsf(sum) <= __FLT_MAX__)) || left) {
+            for (int i = 0; i < 4; ++i) sum += fabsf(acc[rb][db][i]);
+        if (__any(row < rows && !(sum <= kMostSum)) || left) {
             exact_keys<D, F16, Q8>(p, w.b, w.h, p.q + row_at(rb, p.q_batch, p.q_tok, p.q_head), sight_of(p, w.e, query[rb]), page_of, acc[rb], m[rb], l);
         } else if (Q8 && vacc != INT_MIN) {
 #pragma unroll
