@@ -139,7 +139,8 @@ __global__ __launch_bounds__(kWaves * 64, resident(D)) void batch_decode_kernel(
     f32x4_t acc[DB], accl = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int db = 0; db < DB; ++db) acc[db] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, nm = 0.0f, th = -INFINITY;  // row maximum, its negative (0 while there is none), where it grows
+    constexpr float kBelow = kHead<F16 || Q8>;
+    float m = -INFINITY, nm = 0.0f, th = -INFINITY;  // kBelow under the row's maximum, its negative (0 while there is none), where it grows
     int vref = INT_MIN;
     ScaleRange range;
     lds_char* const vt = (lds_char*)lds + wv * VLDS;
@@ -227,10 +228,10 @@ __global__ __launch_bounds__(kWaves * 64, resident(D)) void batch_decode_kernel(
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
             const bool grow = mx > th;
-            const float mn = grow ? mx : m, alpha = grow ? exp2_fast(m - mn) : 1.0f;
+            const float mn = grow ? mx - kBelow : m, alpha = grow ? exp2_fast(m - mn) : 1.0f;
             m = mn;
             nm = grow ? -mn : nm;
-            th = grow ? mn + kLazy : th;
+            th = grow ? mn + (kBelow + kLazy) : th;
             accl *= alpha;
 #pragma unroll
             for (int db = 0; db < DB; ++db) acc[db] *= alpha;

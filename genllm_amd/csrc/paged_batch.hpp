@@ -92,8 +92,16 @@ constexpr int kScaleReach = 15, kMostScale = 64;
 // those of probabilities of at most one.  Where all waves and splits (at most 2^13) might not add up
 // within fp32's range, exact_keys takes its keys, with probabilities of at most one: sums of
 // products above kMostSum, and 8-bit pages whose reference is above kMostScale (2^15 of a
-// code and its lead, 2^8, 2^30 keys: sums of up to 2^(53 + 64)).
+// code and its lead, 2^15 of a probability, 2^30 keys: sums of up to 2^(60 + 64)).
 constexpr float kLazy = 8.0f, kMostSum = 0x1p100f;
+
+// A row's probabilities are formed relative to a reference, this much (log2) below its maximum.
+// Relative to the maximum itself fp16, whose last bit is 2^-24, would make zeros of all keys
+// 25 binades below it, which at the end of a long context can be 0.4 % of the weight (131072
+// keys).  7 is what fp16's range leaves: 2^(kLazy + 7); the last bit is 2^-31 of the maximum.  bf16 has
+// fp32's range.
+template <bool kFp16>
+constexpr float kHead = kFp16 ? 7.0f : 0.0f;
 struct ScaleRange {
     int low = 1 << 20;
     __device__ __forceinline__ void add(const PageInfo& info) { low = info.kid >= 0 ? min(low, info.vb - 127) : low; }

@@ -114,7 +114,8 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
     const int s0 = int(int64_t(steps) * w.sp / w.ns), s1 = int(int64_t(steps) * (w.sp + 1) / w.ns);
 
     f32x4_t acc[RB][DB], accl[RB];
-    float m[RB], nm[RB], th[RB];
+    constexpr float kBelow = kHead<F16 || Q8>;
+    float m[RB], nm[RB], th[RB];  // kBelow under a row's maximum, its negative (0 while there is none), where it grows
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
         accl[rb] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -294,10 +295,10 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
                 mx = fmaxf(mx, __shfl_xor(mx, 16));
                 mx = fmaxf(mx, __shfl_xor(mx, 32));
                 const bool grow = mx > th[rb];
-                const float mn = grow ? mx : m[rb], alpha = grow ? exp2_fast(m[rb] - mn) : 1.0f;
+                const float mn = grow ? mx - kBelow : m[rb], alpha = grow ? exp2_fast(m[rb] - mn) : 1.0f;
                 m[rb] = mn;
                 nm[rb] = grow ? -mn : nm[rb];
-                th[rb] = grow ? mn + kLazy : th[rb];
+                th[rb] = grow ? mn + (kBelow + kLazy) : th[rb];
                 accl[rb] *= alpha;
 #pragma unroll
                 for (int db = 0; db < DB; ++db) acc[rb][db] *= alpha;

@@ -475,8 +475,8 @@ int genllm_kv_gather_f8(const void *k_pool, int64_t kp_block_stride, int64_t kp_
  * keys that it sees.  Pools have dtype's elements, or, with k_scales and
  * v_scales, 8-bit codes (strides in bytes).  scale is finite and >= 0; scores, maxima,
  * sums and outputs are formed in fp32 (whose range the sum of |v| over the keys must not leave).  Probabilities are rounded to fp16 for
- * 8-bit pages (V's codes then are fp16 values), to dtype for 16-bit ones; up to 16 rows per kv head over bf16
- * pages keep 16 bits of them.  out may be q (the same address and strides), no other operand.
+ * 8-bit pages (V's codes then are fp16 values), to dtype for 16-bit ones (fp16's least step is 2^-31 of a row's
+ * largest); up to 16 rows per kv head over bf16 pages keep 16 bits of them.  out may be q (the same address and strides), no other operand.
  * workspace: genllm_paged_attention_batch_workspace_bytes (0: none is needed, or the sizes are
  * refused), 16-byte aligned; its contents do not matter before or after the call;
  * calls that share one must be ordered. */

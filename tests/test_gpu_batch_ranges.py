@@ -6,6 +6,7 @@ import torch
 
 from genllm_amd import paged
 from batch import PAGE, assert_attended, attend
+from hybrid import half_step
 
 pytestmark = pytest.mark.gpu
 
@@ -13,8 +14,8 @@ BF, HF = torch.bfloat16, torch.float16
 
 
 class Keys:
-    """An entry of n tokens whose pages come from a pool of a few kinds of page, each a K row, a V row and V's exponent
-    (8-bit pages); `kinds` gives the kind of each page.  D = 64, H kv heads with the same rows.  Other entries have a token
+    """An entry of n tokens whose pages come from a pool of a few kinds of page, each a row of K and one of V (or
+    [16, 64] of them) and V's exponent (8-bit pages); `kinds` gives the kind of each page.  D = 64, H kv heads with the same rows.  Other entries have a token
     each: with enough of them the long one's tiles are not split."""
 
     D = 64
@@ -24,7 +25,7 @@ class Keys:
         self.n, self.S, self.dtype, self.f8, self.H, self.G = n or len(kinds) * PAGE, S, dtype, f8, H, G
         self.kinds = torch.tensor(kinds)
         element = torch.float8_e4m3fn if f8 else dtype
-        self.k, self.v = (x.to(element)[:, None, None, :].expand(m, PAGE, H, self.D) for x in (k, v))
+        self.k, self.v = ((x if x.dim() == 3 else x[:, None]).to(element)[:, :, None].expand(m, PAGE, H, self.D) for x in (k, v))
         self.pools = [x.contiguous().cuda() for x in (self.k, self.v)]
         self.scales = [None, None]
         self.two = torch.ones(m).double()
@@ -100,3 +101,36 @@ def test_large_scales(S, G, entries):
             want = attend(q.to(BF).expand(1, G, 64), kk[:, :1], vv[:, :1], c.n - S + s, 1.0)
             for h in (0, H - 1):
                 assert_attended(got[s : s + 1, G * h : G * h + G], *want, c.n, 2.0 ** -11, f"scales of 2^{e}, query {s}, head {h}")
+
+
+def assert_small_weights(got, want, weight, plain, size, n, label):
+    """assert_attended's bound with a probability's least step 2^-31 of the largest: they are formed relative to 2^-7 of
+    it or less, so that fp16's step of 2^-24, off by up to 2^-25, leaves 2^-32."""
+    g, w, a, b, z = (x.detach().cpu().double() for x in (got, want, weight, plain, size))
+    part = 2.0 ** -11 + (264 * z + 2 * n) * 2.0 ** -24
+    bound = half_step(got.dtype) * (1 + 2.0 ** -6) * w.abs() + part * (a + w.abs()) + torch.finfo(got.dtype).smallest_normal + 2.0 ** -32 * (b + n * w.abs())
+    worst = ((g - w).abs() / bound).max().item()
+    print(f"[{label}] worst error {worst:.3f} of its bound", flush=True)
+    assert worst <= 1.0, f"{label}: {worst} times the bound"
+
+
+@pytest.mark.parametrize("f8,dtype", [(True, BF), (True, HF), (False, HF)])
+@pytest.mark.parametrize("below", [-22.0, -25.0, -28.0, -31.0])
+@pytest.mark.parametrize("S,G,entries,pages", [(1, 1, 1, 40), (5, 3, 1, 40), (20, 1, 1, 30), (40, 4, 1, 30), (1, 1, 1408, 4096), (20, 1, 64, 4096), (40, 4, 64, 4096)])
+def test_tail_behind_one_key(S, G, entries, pages, below, f8, dtype):
+    """A first key that has almost all the weight, on a value of zero, and a long tail of keys that each have less than
+    2^-21 of it, on values of one: the result is the tail's weight alone."""
+    H = 8 if entries > 1 else 1
+    q, k = scored(-below / 2, below / 2)
+    k = k[1].expand(2, PAGE, 64).clone()
+    k[0, 0] *= -1
+    v = torch.ones(2, PAGE, 64)
+    v[:, :, 1::2] = -1.0
+    v[0, 0] = 0.0
+    c = Keys([0] + [1] * (pages - 1), k, v, S, dtype, f8, H, G)
+    kk, vv = c.rows()
+    got = c.run(q, entries)
+    for s in {0, S - 1}:
+        want = attend(q.to(dtype).expand(1, G, 64), kk[:, :1], vv[:, :1], c.n - S + s, 1.0)
+        for h in {0, H - 1}:
+            assert_small_weights(got[s : s + 1, G * h : G * h + G], *want, c.n, f"tail at 2^{below}, query {s}, head {h}")
