@@ -523,7 +523,7 @@ extern "C" int genllm_paged_attention_batch(
     if (window > 0 && !causal) return refuse(GENLLM_ERR_INVALID, "a window goes with causal attention");
     if ((k_scales != nullptr) != (v_scales != nullptr)) return refuse(GENLLM_ERR_INVALID, "k_scales and v_scales go together");
     if (z.empty()) return GENLLM_OK;
-    if (!q || !out || !k_pool || !v_pool || !k_ids || !v_ids || !n_cached) return refuse(GENLLM_ERR_INVALID, "null pointer");
+    if (!q || !out || !k_pool || !v_pool || (max_pages > 0 && (!k_ids || !v_ids)) || !n_cached) return refuse(GENLLM_ERR_INVALID, "null pointer");
     const bool q8 = k_scales != nullptr;
     const int64_t es = q8 ? 1 : 2, row = head_dim * es;
     const auto one = [](int64_t stride, int64_t n) { return n > 1 ? stride : 0; };  // the stride of a dim of one never matters

@@ -248,7 +248,7 @@ int run(const Call& c) {
     if (c.max_pages > 1 << 26) return refuse(GENLLM_ERR_INVALID, "tables of up to 2^26 pages");
     if (c.seq_len > 1 << 30) return refuse(GENLLM_ERR_INVALID, "up to 2^30 tokens");
     if (c.batch == 0 || c.seq_len == 0 || c.n_kv_heads == 0) return GENLLM_OK;
-    if (!c.k || !c.v || !c.k_pool || !c.v_pool || !c.k_scales || !c.v_scales || !c.k_ids || !c.v_ids || !c.start_pos)
+    if (!c.k || !c.v || !c.k_pool || !c.v_pool || !c.k_scales || !c.v_scales || (c.max_pages > 0 && (!c.k_ids || !c.v_ids)) || !c.start_pos)
         return refuse(GENLLM_ERR_INVALID, "null pointer");
     if (!aligned_to(c.k, 16) || !aligned_to(c.v, 16) || !aligned_to(c.k_pool, 16) || !aligned_to(c.v_pool, 16) ||
         ((c.k_batch | c.k_tok | c.k_head | c.v_batch | c.v_tok | c.v_head) & 7) ||

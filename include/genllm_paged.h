@@ -432,7 +432,7 @@ int genllm_qk_norm_rope_axes(const void *q, int64_t q_tok_stride, int64_t q_head
  * 16-byte aligned): [block][16][head][dim], as genllm_kv lays its pools out, or
  * [block][head][16][dim], where a page of a head is one piece of memory, as
  * is best for 8 bits.  k_ids, v_ids [batch][max_pages] (device, rows at a stride):
- * page t / 16 of an entry holds its token t.  An id outside [0, n_blocks) is no page: nothing is
+ * page t / 16 of an entry holds its token t (they may be null where max_pages is 0).  An id outside [0, n_blocks) is no page: nothing is
  * written to it, and what reads it gives NaN.  No call allocates,
  * copies or synchronises; all are kernel launches that a graph may capture.
  *
