@@ -44,16 +44,10 @@ namespace {
 constexpr int kRows = kDecodeRows;
 constexpr int kStep = kDecodeStep;
 constexpr int kWaves = 4;
-constexpr int kScaleLead = 6;      // a page's scale may be this many binades above the reference
 constexpr int kNonTemporal = 2;
 
-typedef __attribute__((address_space(3))) char lds_char;
-typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x2_t __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ s16x4_t ds_read_tr16(const lds_char* p) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(const_cast<lds_char*>(p)));
-}
 __device__ __forceinline__ i32x2_t ds_read_tr8(const lds_char* p) {
     return __builtin_amdgcn_ds_read_tr8_b64_v2i32(reinterpret_cast<__attribute__((address_space(3))) i32x2_t*>(const_cast<lds_char*>(p)));
 }

@@ -80,13 +80,21 @@ __device__ __forceinline__ uint4 f8_octet(uint32_t w0, uint32_t w1, float s0, fl
     return make_uint4(f8_pair<F16, false>(w0, s0), f8_pair<F16, true>(w0, s0), f8_pair<F16, false>(w1, s1), f8_pair<F16, true>(w1, s1));
 }
 
+typedef __attribute__((address_space(3))) char lds_char;
+typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ s16x4_t ds_read_tr16(const lds_char* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(const_cast<lds_char*>(p)));
+}
+
 // V's pages are taken relative to a reference scale 2^ref, at least a 64th of the largest so
 // far.  That is exact for a page at most 15 binades below it: a code's last bit, 2^-9, is
 // fp16's, 2^-24.  Where there are lower ones, or sums might leave fp32's range, rows are
 // computed by exact_keys in the end: the scale of another page, of keys that a row may not
 // even see, costs no row its precision.  Pages of zeros alone, which have the least scale, do
 // not count.  low: a lane's least; next(i): the i-th page, -1 behind the last.
-constexpr int kScaleReach = 15, kMostScale = 64;
+// kScaleLead: how far a page may be above the reference.
+constexpr int kScaleReach = 15, kScaleLead = 6, kMostScale = 64;
 
 // A row's maximum may lag its scores by kLazy (log2), so a wave's sums may be 2^kLazy times
 // those of probabilities of at most one.  Where all waves and splits (at most 2^13) might not add up

@@ -33,20 +33,13 @@ namespace genllm {
 
 namespace {
 
-constexpr int kScaleLead = 6;  // a page's scale may be this many binades above the reference
 // The two waves of a SIMD: one whose MFMA waits for the matrix core keeps the other's vector
 // instructions from being issued, unless those come first (8192 tokens, 16 and 8 heads of 128:
 // 298 us without priorities, 289 with both at 3, 268 so).
 constexpr int kSoftmaxPrio = 2, kStagePrio = 3;
 constexpr int kKeys = kPrefillStep * kPage;
 
-typedef __attribute__((address_space(3))) char lds_char;
-typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) u32x4_t lds_u32x4;
-
-__device__ __forceinline__ s16x4_t ds_read_tr16(const lds_char* p) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4_t*>(const_cast<lds_char*>(p)));
-}
 
 // K in LDS: 16-byte chunk c of token r (of 16) at place c ^ f(r) of its row, so that the
 // reads of an operand (16 rows, one chunk) cover all banks once.
