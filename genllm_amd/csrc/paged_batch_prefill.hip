@@ -184,11 +184,10 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
                 const int t = e * (64 / SRC) + lane / SRC, c = lane % SRC;
                 lds_char* const to = kl + (pg * kPage + t) * ROWB;
                 if constexpr (Q8) {
-                    // every other row its second chunk first: a row's even places, then its odd
-                    // ones, are half the banks
-                    const bool odd = t & 1;
-                    put(to + 16 * k_place<D>(t, 2 * c + odd), f8_octet<F16>(odd ? reg[e].z : reg[e].x, odd ? reg[e].w : reg[e].y, 1.0f, 1.0f));
-                    put(to + 16 * k_place<D>(t, 2 * c + !odd), f8_octet<F16>(odd ? reg[e].x : reg[e].z, odd ? reg[e].y : reg[e].w, 1.0f, 1.0f));
+                    // chunks 32 bytes apart over the lanes: a step's writes (32 KB at D = 128) take 256 cycles
+                    // of bank conflicts; the two in turn from row to row take as many
+                    put(to + 16 * k_place<D>(t, 2 * c), f8_octet<F16>(reg[e].x, reg[e].y, 1.0f, 1.0f));
+                    put(to + 16 * k_place<D>(t, 2 * c + 1), f8_octet<F16>(reg[e].z, reg[e].w, 1.0f, 1.0f));
                 } else {
                     put(to + 16 * k_place<D>(t, c), reg[e]);
                 }
@@ -200,9 +199,8 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
                 const int t = e * (64 / SRC) + lane / SRC, c = lane % SRC;
                 lds_char* const to = vl + pg * kVPage<D> + v_row<D>(t);
                 if constexpr (Q8) {
-                    const bool odd = t & 1;
-                    put(to + 32 * c + 16 * odd, f8_octet<true>(odd ? reg[e].z : reg[e].x, odd ? reg[e].w : reg[e].y, vs, vs));
-                    put(to + 32 * c + 16 * !odd, f8_octet<true>(odd ? reg[e].x : reg[e].z, odd ? reg[e].y : reg[e].w, vs, vs));
+                    put(to + 32 * c, f8_octet<true>(reg[e].x, reg[e].y, vs, vs));
+                    put(to + 32 * c + 16, f8_octet<true>(reg[e].z, reg[e].w, vs, vs));
                 } else {
                     put(to + 16 * c, reg[e]);
                 }
