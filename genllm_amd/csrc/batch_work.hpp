@@ -227,13 +227,16 @@ struct Header {
 };
 
 constexpr int kCus = 256;
-// steps of a split at least, times head_dim (8192 tokens, 32 and 8 heads of 128: 12.4 us with
-// 8 steps, 13.2 with 12, 13.9 with 16)
+// The times beside the rules below are of whole calls over three sets of inputs in turn, both sides on one GPU.
+// steps of a split at least, times head_dim (one token, 32 and 8 heads of 128, 8-bit pages: after
+// 8192 12.8 us with 8 steps, 13.4 with 12, 14.4 with 16; after 1500 11.9, 12.8 and 15.6)
 constexpr int kDecodeLeast = 1024;
 constexpr int kPrefillLeast = 4;
 constexpr int prefill_resident(int D) { return D == 256 ? 1 : 2; }
 // Workgroups that a CU holds.  Each is four waves, one on a SIMD: 512 registers over them.
-// Three at D = 128 in place of two: 32 windows of 1024 tokens, 16-bit, 50.5 -> 34 us.
+// Three at D = 128 in place of two, 8-bit pages: 64 sequences of up to 4096 tokens 63.4 -> 55.3 us,
+// 200 of up to 500 31.8 -> 27.4 (32 windows of 1024 tokens over 16-bit pages 32.8 both ways, one
+// sequence of 32768 34.9 -> 36.1).
 constexpr int resident(int D) { return D == 64 ? 4 : D == 128 ? 3 : 2; }
 
 // Which kernel a call runs and how its work is divided at most.
@@ -272,10 +275,10 @@ inline BatchPlan plan_of(const BatchSizes& z) {
     r.target = kCus * (r.decode ? resident(z.head_dim) : prefill_resident(z.head_dim));
     // Prompts over little more than their own rows whose tiles of 64 are all there at once and
     // leave few places: eight waves to each, a long tile beside a short one, no split (16 q and
-    // 8 kv heads of 128, 2048 tokens: 44 us, with tiles of 128 in splits 49.5; 1800: 37.4 and
-    // 44.4).  Not for short ones (4 x 512: 21.9 and 20.0), nor for chunks on a long context,
-    // which splits divide evenly (2048 on 8192: 182 and 150), nor at head_dim 256, one workgroup
-    // to a CU (8 and 2 heads, 2048 tokens: 56 and 52).
+    // 8 kv heads of 128, 2048 tokens: 43.5 us, with tiles of 128 in splits 45.0; 1800: 37.6 and
+    // 41.4; 2 x 1024: 31.2 and 34.0).  Not for short ones (4 x 512: 22.0 and 20.5), nor for chunks on a long
+    // context, which splits divide evenly (2048 on 8192: 167 and 144), nor at head_dim 256, one workgroup
+    // to a CU (8 and 2 heads, 2048 tokens: 56.6 and 48.6).
     const int64_t fine = (rows + 63) / 64 * heads;
     const bool fits = !r.decode && rows > 64 && z.head_dim <= 128 && z.seq_len >= 1024 && int64_t(z.max_pages) * kPage < 2 * int64_t(z.seq_len) && fine <= r.target &&
                       fine >= r.target / 4 * 3;
@@ -285,11 +288,14 @@ inline BatchPlan plan_of(const BatchSizes& z) {
     r.tiles = r.tiles_max * heads;
     r.least = r.decode ? kDecodeLeast / z.head_dim : kPrefillLeast;
     // a merge is worth it for contexts of more than two such splits, three of one tile (one
-    // token, 32 and 8 heads of 128, after 600: 9.2 us in one launch, 11.4 split; after 800:
-    // 10.6 and 10.7; after 2000: 13 and 11.8).  Where the tiles alone keep the workgroups busy
+    // token, 32 and 8 heads of 128, after 600: 9.3 us in one launch, 11.7 split; after 800:
+    // 10.9 and 11.2; after 2048: 19.2 and 11.4).  Where the tiles alone keep the workgroups busy
     // in turn, only for contexts that are long beside the others: every workgroup looks through
     // all units to find its own (one token each, ragged, unsplit and split: 1024 entries of up
-    // to 2048 tokens, 8 and 2 heads, 90 and 136 us; 256 of up to 4096, 32 and 8, 173 and 180)
+    // to 2048 tokens, 8 and 2 heads, 90 and 135 us; 256 of up to 4096, 32 and 8, 173 and 179).
+    // A long entry among many then is one workgroup for each kv head, and takes as long as its tokens
+    // after each other.  So it does with more rows as soon as the padded tiles fill the GPU, whatever rows
+    // are there: a token at the end of a long context is better off in a call of few rows each.
     const int64_t turns = std::max<int64_t>(1, std::min<int64_t>(r.tiles / r.target, 1 << 20));
     r.can_split = (z.max_pages + r.step - 1) / r.step > (!r.decode ? 2 : turns > 1 ? 12 : 3) * r.least * turns && (r.decode || r.tiles < r.target) && !fits;
     r.least = int(r.least * turns);

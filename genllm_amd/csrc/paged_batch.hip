@@ -16,7 +16,10 @@
 // From 8-bit pages V's codes are fp16 values and P is rounded to fp16 (11 bits), whatever
 // q's type is: the scale of a page is taken relative to a reference of the wave, which
 // follows the largest as the running maximum does.  From bf16 pages P is split into two
-// bf16 parts (16 bits; a second MFMA costs nothing here).  The sum of a row's
+// bf16 parts (16 bits).  fp16 in two parts as well would leave bf16 results as far from 64-bit ones
+// as they are, by their own rounding (relative 1.7e-3), fp16 ones 2.1e-4 in place of 2.4e-4,
+// and takes time: 64 sequences of up to 4096 tokens 55.0 -> 57.6 us, six drafts of 4 queries
+// 10.4 -> 12.0, one token after 300 7.7 -> 8.5.  The sum of a row's
 // probabilities comes from one more MFMA with ones, so from the same rounded values.
 //
 // Sequences of a batch are unlike in length, so workgroups are given equal numbers of
@@ -24,10 +27,12 @@
 // (find_work).
 //
 // Long contexts are bound by memory: one token each of 64 sequences of up to 4096 tokens (8 kv heads
-// of 128, 8-bit pages) 55 us, 5.0 TB/s, as a large copy; one of 131072 tokens 50 us, 5.3 TB/s.
+// of 128, 8-bit pages) 55 us a call, 5.0 TB/s, as a large copy; one of 131072 tokens 51 us, 5.3 TB/s.
 // Short ones are bound by launches and by loads after each other (lengths, ids, rows): 300
-// tokens 7.7 us, 8192 in a split and a merge launch 11.5.  Eight waves to a workgroup in place
-// of four made no difference there (600 tokens 9.2 us both ways).
+// tokens 7.7 us, 8192 in a split and a merge launch 11.2 (among other calls of its own; 12.5 to 13 over
+// three sets of inputs in turn).  Eight waves to a workgroup in place
+// of four made no difference there (600 tokens 9.2 us both ways).  At D = 256 over fp16 pages two
+// registers go to scratch memory.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -371,8 +376,8 @@ __global__ __launch_bounds__(kWaves * 64, resident(D)) void batch_decode_kernel(
 // A lane has 4 dims of a row; SG groups of D / 4 lanes share a row's splits (SG = 1: a row
 // per group).  Entries with one split were written by their workgroup.
 // A row's splits are shared by four waves where there are many of them on average.
-// kMergeU splits at once (8 of them: 2 x 512 queries on 8192 tokens 147.5 us in all, 4: 145.8; 131072 tokens of
-// one sequence 54.0, 54.1, with 2 55.1).
+// kMergeU splits at once (whole calls with 8 of them, 4, 2: 2 x 512 queries on 8192 tokens 151.1 us,
+// 149.7, 149.0; one token after 131072 50.6, 50.7, 51.6).
 constexpr int kMergeU = 4, kMergeWide = 16;
 template <int D, bool F16, int ROWS, int SG, int THREADS>
 __global__ __launch_bounds__(THREADS) void batch_merge_kernel(BatchAttn p, int row_blocks) {

@@ -12,7 +12,11 @@
 // are swizzled, V's rows padded.  8-bit codes are converted once here, for all waves: K's to
 // q's type (without loss; the page's scale is in the factor of the scores), V's to fp16
 // relative to a reference scale that follows the largest, so that P is rounded to fp16 (11
-// bits) whatever q's type is.  From 16-bit pages P has the elements' type.  Per step:
+// bits) whatever q's type is.  From 16-bit pages P has the elements' type, as the MFMA takes it:
+// over bf16 pages results are off by 2.1e-3 (relative, against 64 bits) where their own rounding
+// alone leaves 1.7e-3.  In two parts, as for few rows, P V takes twice the MFMAs, where a wave's
+// chain is the bound: 4096 tokens in windows of 512 35.1 -> 40.9 us, 2 x 512 queries on 8192 tokens 159 ->
+// 203, over 8-bit pages 148 -> 197.  Per step:
 //   S^T = K Q^T   v_mfma 16x16x32, K's operand read once for the RB row blocks
 //   O^T += V^T P^T  with V^T by transposing LDS reads; the sum of a row's probabilities
 //        by one more MFMA with ones, from the same rounded values
@@ -22,8 +26,12 @@
 // Bound by a wave's chain where two waves share a SIMD: of a step's 4,400 cycles for both
 // (D = 128, 8-bit) the matrix core is busy in 2,180, vector instructions and exponentials
 // take about as many and overlap it in part.  2 x 512 queries on 8192 tokens, 32 and 8 heads
-// of 128: 148 us, 900 TFLOP/s (a large library product reaches 1,184); 8192 tokens, 16 and 8
-// heads, causal: 268 us.  Also tried: staging between the MFMAs of P V (no gain), loads two
+// of 128: 145 us, 920 TFLOP/s (a large library product reaches 1,184); 8192 tokens, 16 and 8
+// heads, causal: 268 us.  2048 tokens, 16 and 8 heads: 40.7 us, where the kernel for one sequence over 16-bit
+// pages (paged_prefill.hip) takes 30: this one issues 1.6 times its vector and twice its scalar instructions and
+// LDS cycles (pages found and descriptors formed anew each step, conversion, conflicts of the
+// staging writes).  At D = 128 registers go to scratch memory: 2 of the form with 64 rows over
+// 8-bit pages, 12 over 16-bit ones, 4 of the form with 128 rows over 16-bit ones.  Also tried: staging between the MFMAs of P V (no gain), loads two
 // steps ahead (none), Q and the output through LDS as whole rows (2 % slower).
 #include <type_traits>
 
@@ -35,7 +43,7 @@ namespace {
 
 // The two waves of a SIMD: one whose MFMA waits for the matrix core keeps the other's vector
 // instructions from being issued, unless those come first (8192 tokens, 16 and 8 heads of 128:
-// 298 us without priorities, 289 with both at 3, 268 so).
+// 309 us without priorities, 295 with both at 3, 275 so; 2 x 512 queries on 8192 158, 154, 150).
 constexpr int kSoftmaxPrio = 2, kStagePrio = 3;
 constexpr int kKeys = kPrefillStep * kPage;
 
@@ -144,7 +152,7 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? (D == 256 ? 2 : 4) : D == 256 ?
     constexpr int kLoads = KG == 1 ? 2 * LD : LD;
     // many loads at once hold the wave up (16 of 16 bytes to a lane, 1200 cycles of a step's
     // 5900 at D = 256): they are issued between the MFMAs of the scores (a window of 512 on 4096
-    // tokens 34.0 -> 32.6 us); four or eight are not (8 at D = 128: no difference)
+    // tokens 36.1 -> 35.1 us); four or eight are not (8 at D = 128: 2 x 512 on 8192 160 and 158 us)
     constexpr bool kSpread = kLoads >= 16;
     const auto aim = [&](int step) {
         const int at = kPrefillStep * ((step - s0) % kBlock) + pg;
