@@ -28,7 +28,7 @@
 // take about as many and overlap it in part.  2 x 512 queries on 8192 tokens, 32 and 8 heads
 // of 128: 145 us, 920 TFLOP/s (a large library product reaches 1,184); 8192 tokens, 16 and 8
 // heads, causal: 268 us.  2048 tokens, 16 and 8 heads: 40.7 us, where the kernel for one sequence over 16-bit
-// pages (paged_prefill.hip) takes 30: this one issues 1.6 times its vector and twice its scalar instructions and
+// pages (paged_prefill.hip) takes 30: this one issues 1.5 times its vector and twice its scalar instructions and
 // LDS cycles (pages found and descriptors formed anew each step, conversion, conflicts of the
 // staging writes).  At D = 128 registers go to scratch memory: 2 of the form with 64 rows over
 // 8-bit pages, 12 over 16-bit ones, 4 of the form with 128 rows over 16-bit ones.  Also tried: staging between the MFMAs of P V (no gain), loads two
