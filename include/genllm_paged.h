@@ -474,7 +474,8 @@ int genllm_kv_gather_f8(const void *k_pool, int64_t kp_block_stride, int64_t kp_
  * (window 0: no limit; a window needs causal).  Rows without a key are zeros, rows
  * behind q_lens[b] are left as they were; NaN or infinity in a row's result comes only from
  * keys that it sees.  Pools have dtype's elements, or, with k_scales and
- * v_scales, 8-bit codes (strides in bytes).  scale is finite and >= 0; scores, maxima,
+ * v_scales, 8-bit codes (strides in bytes); a block's token rows lie less than 2^26 bytes apart, its heads
+ * within 2^31.  scale is finite and >= 0; scores, maxima,
  * sums and outputs are formed in fp32 (whose range the sum of |v| over the keys must not leave).  Probabilities are rounded to fp16 for
  * 8-bit pages (V's codes then are fp16 values), to dtype for 16-bit ones (fp16's least step is 2^-31 of a row's
  * largest); up to 16 rows per kv head over bf16 pages keep 16 bits of them.  out may be q (the same address and strides), no other operand.

@@ -249,6 +249,26 @@ int main(int argc, char** argv) {
         if (check("tiles of 64", batch(2, 20, 1, 1, 64, all, {1 << 30, 90}))) return 1;
         if (check("tiles of 128", batch(1, 600, 1, 1, 128, all, {1 << 30}))) return 1;
     }
+    if (what == "quotients") {
+        // x up to 2^30 and a tile, by any divisor, the reciprocal off by a unit in the last place either way
+        std::mt19937 g(2);
+        const auto one = [](int64_t x, int64_t d) {
+            if (x < 0 || x > (int64_t(1) << 30) + 128 || d < 1 || d > 1 << 30) return 0;
+            for (float r : {1.0f / float(d), std::nextafterf(1.0f / float(d), 0.0f), std::nextafterf(1.0f / float(d), 2.0f)}) {
+                Divisor by{int(d)};
+                by.r = r;
+                if (by(int(x)) != x / d) return printf("%ld / %ld is not %d\n", long(x), long(d), by(int(x))), 1;
+            }
+            return 0;
+        };
+        for (int i = 0; i < 3000000; ++i) {
+            const int64_t d = 1 + (g() & ((1u << (1 + g() % 30)) - 1)), x = int64_t(g() & ((1u << (1 + g() % 31)) - 1));
+            if (one(x, d) || one(x / d * d, d) || one(x / d * d - 1, d) || one(x / d * d + d - 1, d)) return 1;
+        }
+        for (int64_t d = 1; d < 5000; ++d)
+            for (int64_t x : {int64_t(1) << 30, (int64_t(1) << 30) + 128, (int64_t(1) << 30) / d * d, (int64_t(1) << 30) / d * d - 1, d - 1, d, d + 1})
+                if (one(x, d)) return 1;
+    }
     puts("as counted");
 }
 '''
@@ -279,6 +299,10 @@ pytestmark = pytest.mark.skipif(shutil.which("g++") is None, reason="g++ builds 
 
 def test_batches(program):
     run(program, "batches")
+
+
+def test_quotients(program):
+    run(program, "quotients")
 
 
 def test_tables_of_many_pages(program):
