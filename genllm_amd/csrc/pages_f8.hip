@@ -292,7 +292,10 @@ int run(const Call& c) {
     const char *a, *b;
     const auto never = [](const Rows&, const Rows&) { return false; };
     if constexpr (kScatter) {
-        const NamedRows written[] = {{"k_pool", as_pool[0]}, {"v_pool", as_pool[1]}, {"k_scales", scales[0]}, {"v_scales", scales[1]}};
+        // one pool, with one or two arrays of scales, may hold K's and V's blocks: the tables then name different ones
+        const bool one_pool = as_pool[1].same_as(as_pool[0]), one_scales = one_pool && scales[1].same_as(scales[0]);
+        const NamedRows written[] = {{"k_pool", as_pool[0]}, {"v_pool", one_pool ? Rows() : as_pool[1]},
+                                     {"k_scales", scales[0]}, {"v_scales", one_scales ? Rows() : scales[1]}};
         const NamedRows read[] = {{"k", as_rows[0]}, {"v", as_rows[1]}, {"k_ids", as_ids[0]}, {"v_ids", as_ids[1]}, {"start_pos", start}, {"seq_lens", lens}};
         if (find_overlap(written, read, never, a, b)) return refuse(GENLLM_ERR_INVALID, std::string(a) + " overlaps " + b);
         for (int i = 0; i < 2; ++i)

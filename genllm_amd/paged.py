@@ -508,7 +508,8 @@ def kv_scatter_f8(k, v, k_pool, v_pool, k_scales, v_scales, k_ids, v_ids, start_
     strides, and k_scales, v_scales [n, Hkv] uint8 (or float8_e8m0fnu), as f8_pool
     makes them; k_ids, v_ids [B, P] int32: the block of each page of an entry;
     start_pos, seq_lens [B] int32: the position of an entry's first row, its rows.
-    All on the GPU.  No page may be written twice in a call; K's and V's pools and scales are different memory."""
+    All on the GPU.  No page may be written twice in a call; k_pool and v_pool may be one pool (as their
+    scales may then be one tensor) whose blocks are K's or V's."""
     rc = (_lib._calls or _lib.calls()).kv_scatter_f8(k, v, k_pool, v_pool, k_scales, v_scales, k_ids, v_ids, start_pos, seq_lens,
                                                      None if stream is None else _stream(stream))
     if rc:

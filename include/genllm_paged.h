@@ -446,8 +446,9 @@ int genllm_qk_norm_rope_axes(const void *q, int64_t q_tok_stride, int64_t q_head
  * they raise e, its other codes are rounded to the new scale, which is exact but
  * for those that become e4m3 subnormals.  NaN and infinity are stored as NaN and leave e alone.  A negative
  * start_pos is an idle entry; tokens past the table are dropped.  A page must not be
- * written twice in a call, by two entries or as two pages of one: what it holds then is not
- * defined.  K's and V's pools and scales must be different memory (the call refuses what they share).
+ * written twice in a call, by two entries, as two pages of one or for both K and V: what it holds then is not
+ * defined.  k_pool and v_pool may be one pool (with the same strides, and the same scales or others); pools that overlap
+ * otherwise are refused.
  * genllm_kv_gather_f8 reads such tokens back into k_out, v_out, code * 2^e rounded once;
  * rows past the table are NaN, rows behind seq_lens[b] left as they were. */
 int genllm_kv_scatter_f8(const void *k, int64_t k_batch_stride, int64_t k_tok_stride, int64_t k_head_stride,
